@@ -95,6 +95,31 @@ class PrologueArgs(ctypes.Structure):
                 ("dhead", ctypes.c_int32), ("dconv", ctypes.c_int32), ("eps", ctypes.c_float),
                 ("profile", ctypes.c_void_p)]
 
+
+class LatentArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("tq", ctypes.c_int32), ("tk", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("dn", ctypes.c_int32), ("dr", ctypes.c_int32), ("dv", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("q_stride", ctypes.c_int64 * 3),
+                ("kv_stride", ctypes.c_int64 * 3), ("kpe_stride", ctypes.c_int64 * 2),
+                ("do_stride", ctypes.c_int64 * 3), ("profile", ctypes.c_void_p)]
+
+
+class LatentAppendArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("dn", ctypes.c_int32), ("dr", ctypes.c_int32),
+                ("dc", ctypes.c_int32), ("dtype", ctypes.c_int32), ("page", ctypes.c_int32),
+                ("pages", ctypes.c_int32), ("rope_rows", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("c_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("q_stride", ctypes.c_int64 * 2),
+                ("profile", ctypes.c_void_p)]
+
+
+class LatentDecodeArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("dn", ctypes.c_int32), ("dr", ctypes.c_int32), ("dv", ctypes.c_int32), ("dc", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("page", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("table_pages", ctypes.c_int32), ("rope_rows", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("q_stride", ctypes.c_int64 * 3), ("profile", ctypes.c_void_p)]
+
+
 PROFILE_MAX = 16
 
 
@@ -244,6 +269,12 @@ _SIGS = {
     "atomic_mamba2_proj_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(Mamba2ProjArgs), ctypes.c_int]),
     "atomic_mamba2_proj_fwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 16 + [_P, ctypes.c_size_t, _P]),
     "atomic_mamba2_proj_bwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 24 + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_fwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 7 + [_P]),
+    "atomic_latent_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentArgs)]),
+    "atomic_latent_bwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 11 + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_append": (ctypes.c_int, [ctypes.POINTER(LatentAppendArgs)] + [_P] * 10 + [_P]),
+    "atomic_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentDecodeArgs)]),
+    "atomic_latent_decode": (ctypes.c_int, [ctypes.POINTER(LatentDecodeArgs)] + [_P] * 8 + [_P, ctypes.c_size_t, _P]),
 }
 
 _lib = None

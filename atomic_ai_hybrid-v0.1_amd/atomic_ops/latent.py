@@ -1,0 +1,283 @@
+"""PyTorch host side of latent attention: attention whose keys and values come
+from one latent vector a token.  Every computation runs in libatomic_hybrid.so;
+there is no fallback.
+
+Sizes: H heads; dn, the key width without position; dr, the rotated key width
+(shared by all heads); dv, the value width; dc, the latent width.  ``w_kv``
+[H, dn + dv, dc] is the up-projection, as a Linear layer from dc to H (dn + dv)
+holds it.  Operands are bfloat16 or float32 (one dtype).
+
+Expanded form (prompts and training): ``kv`` [B, S, H, dn + dv] is the
+up-projection's output and ``k_pe`` [B, S, dr] the rotated key.
+  ``attention``           differentiable in q, kv and k_pe
+  ``forward``/``backward``  the two directions by themselves
+Absorbed form (single tokens, or a few a sequence), over the latents of a paged
+cache [pages, page, dc + dr] whose rows are [latent | rotated key]:
+  ``append``   writes tokens into the cache and rotates keys and queries
+  ``decode``   reads it
+The two forms of the same weights and tokens give the same outputs up to rounding.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DT = {torch.float32: _lib.ATOMIC_F32, torch.bfloat16: _lib.ATOMIC_BF16}
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _strided(t, n):
+    """``(tensor, strides)``: t as the library reads it, with its first n
+    strides (0 for a dimension of one).  The last dimension has to be dense and
+    the strides and the address whole 16-byte pieces; anything else is copied.
+    Every other order of the first dimensions is read in place."""
+    piece = 16 // t.element_size()
+    for _ in range(2):
+        shape, st = t.shape, t.stride()
+        s = [st[i] if shape[i] > 1 else 0 for i in range(n)]
+        if (shape[-1] == 1 or st[-1] == 1) and not any(x % piece for x in s) and t.data_ptr() % 16 == 0:
+            return t, s
+        t = t.clone() if t.is_contiguous() else t.contiguous()
+    raise ValueError("latent attention: rows have to be whole 16-byte pieces (dimensions that are multiples of 8)")
+
+
+def _operands(what, *named):
+    """Checks that the operands are on one HIP device and of one supported dtype."""
+    first = named[0][1]
+    if not first.is_cuda:
+        raise ValueError(f"{what}: inputs must be HIP device tensors")
+    if first.dtype not in _DT:
+        raise TypeError(f"{what}: {named[0][0]} must be bfloat16 or float32")
+    for name, t in named[1:]:
+        if t.device != first.device:
+            raise ValueError(f"{what}: {name} must be on {named[0][0]}'s device")
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what}: {name} must have {named[0][0]}'s dtype")
+
+
+def _index(what, name, t, shape, dtype, device):
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{what}: {name} must be {str(dtype)[6:]} {list(shape)} on the inputs' device")
+    return t.contiguous()
+
+
+# ------------------------------------------------------------ expanded form
+def _check(q, kv, k_pe, q_lens, kv_lens):
+    _operands("latent attention", ("q", q), ("kv", kv), ("k_pe", k_pe))
+    if q.dim() != 4 or kv.dim() != 4 or k_pe.dim() != 3:
+        raise ValueError("q must be [B, T, H, dn + dr], kv [B, S, H, dn + dv] and k_pe [B, S, dr]")
+    B, T, H, d = q.shape
+    S, dr = k_pe.shape[1:]
+    if kv.shape[:3] != (B, S, H) or k_pe.shape[0] != B or not 0 < dr < d or kv.shape[3] <= d - dr:
+        raise ValueError("q must be [B, T, H, dn + dr], kv [B, S, H, dn + dv] and k_pe [B, S, dr]")
+    lens = [None if t is None else _index("latent attention", n, t, (B,), torch.int32, q.device)
+            for n, t in (("q_lens", q_lens), ("kv_lens", kv_lens))]
+    return lens
+
+
+def make_args(q, kv, k_pe, scale, causal, dout=None):
+    """``(args, operands)``: the args struct and the operands as the library reads them."""
+    B, T, H, d = q.shape
+    S, dr = k_pe.shape[1:]
+    q, qs = _strided(q, 3)
+    kv, ks = _strided(kv, 3)
+    k_pe, ps = _strided(k_pe, 2)
+    gs = (0, 0, 0)
+    if dout is not None:
+        dout, gs = _strided(dout, 3)
+    args = _lib.LatentArgs(B, T, S, H, d - dr, dr, kv.shape[3] - (d - dr), _DT[q.dtype], 1 if causal else 0, scale,
+                           tuple(qs), tuple(ks), tuple(ps), tuple(gs))
+    return args, (q, kv, k_pe, dout)
+
+
+def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, timer=None):
+    """``(o, lse)``: o [B, T, H, dv] in q's dtype and lse [B, H, T] float32.
+
+    Query i of batch row b sees the keys j < kv_lens[b]; with ``causal`` those
+    with j <= i + kv_lens[b] - q_lens[b] (queries stand at the end of the keys).
+    ``q_lens`` / ``kv_lens`` are int32 [B] on the device (the whole T / S without
+    them).  A query that sees no key, and one past its length, has o = 0 and
+    lse = -inf.  Inputs of any batch, token and head strides are read in place."""
+    q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
+    lib = _lib.load()
+    args, (q, kv, k_pe, _) = make_args(q, kv, k_pe, scale, causal)
+    if timer is not None:
+        args.profile = timer.arm()
+    B, T, H = q.shape[:3]
+    o = torch.empty(B, T, H, args.dv, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
+    rc = lib.atomic_latent_fwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
+                               _ptr(o), _ptr(lse), _stream(q.device))
+    _lib.check(rc, "atomic_latent_fwd")
+    return o, lse
+
+
+def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_lens=None, workspace=None, timer=None):
+    """``(dq, dkv, dk_pe)`` in the inputs' shapes and dtype from the forward's
+    ``o`` and ``lse``; k_pe's gradient is summed over the heads.  The same
+    inputs give the same bits."""
+    q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
+    B, T, H, d = q.shape
+    dv = kv.shape[3] - (d - k_pe.shape[2])
+    _operands("latent attention", ("q", q), ("o", o), ("dout", dout))
+    if o.shape != (B, T, H, dv) or dout.shape != o.shape:
+        raise ValueError("o and dout must be [B, T, H, dv]")
+    if lse.shape != (B, H, T) or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be float32 [B, H, T] on q's device")
+    lib = _lib.load()
+    args, (q, kv, k_pe, dout) = make_args(q, kv, k_pe, scale, causal, dout)
+    if timer is not None:
+        args.profile = timer.arm()
+    nbytes = lib.atomic_latent_bwd_workspace_size(ctypes.byref(args))
+    if nbytes == 0:
+        raise _lib.AtomicError("atomic_latent_bwd_workspace_size: unsupported shape")
+    if workspace is None or workspace.numel() < nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    o, lse = o.contiguous(), lse.contiguous()
+    dq, dkv, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, kv, k_pe))
+    rc = lib.atomic_latent_bwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
+                               _ptr(o), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dkv), _ptr(dk), _ptr(workspace),
+                               workspace.numel(), _stream(q.device))
+    _lib.check(rc, "atomic_latent_bwd")
+    return dq, dkv, dk
+
+
+class LatentAttention(torch.autograd.Function):
+    """``forward`` with ``backward`` as its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, kv, k_pe, scale, causal, q_lens, kv_lens):
+        o, lse = forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)
+        ctx.save_for_backward(q, kv, k_pe, o, lse)
+        ctx.scale, ctx.causal, ctx.lens = scale, causal, (q_lens, kv_lens)
+        return o
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, kv, k_pe, o, lse = ctx.saved_tensors
+        dq, dkv, dk = backward(q, kv, k_pe, o, lse, dout.to(q.dtype), ctx.scale, causal=ctx.causal,
+                               q_lens=ctx.lens[0], kv_lens=ctx.lens[1])
+        return dq, dkv, dk, None, None, None, None
+
+
+def attention(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None):
+    """o [B, T, H, dv] of ``forward``, differentiable in q, kv and k_pe."""
+    return LatentAttention.apply(q, kv, k_pe, scale, causal, q_lens, kv_lens)
+
+
+# ------------------------------------------------------------ paged cache
+def _tables(what, cos, sin, dr, device):
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != dr // 2 or \
+            cos.shape[0] < 1 or sin.shape != cos.shape or cos.device != device or sin.device != device:
+        raise ValueError(f"{what}: cos and sin must be float32 [positions, dr / 2] on the inputs' device")
+    return cos.contiguous(), sin.contiguous()
+
+
+def _cache(what, cache, width):
+    if cache.dim() != 3 or cache.shape[2] != width or not cache.is_contiguous() or cache.data_ptr() % 16:
+        raise ValueError(f"{what}: cache must be a dense [pages, page, dc + dr]")
+
+
+def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved=False, timer=None):
+    """Appends N tokens to the cache and rotates by position on the way.
+
+    Row ``slots[t]`` (page slots[t] // page, row slots[t] % page; int64 [N])
+    becomes [c_kv[t] | rotate(k_pe[t])]; a negative slot, or one past the cache,
+    leaves it as it is.  ``positions`` int32 [N] choose the rows of the float32
+    tables ``cos`` / ``sin`` [positions, dr / 2]; the rotation turns the pairs
+    (i, i + dr / 2), or (2 i, 2 i + 1) with ``interleaved``.  Returns
+    ``(k, q)``: the rotated keys [N, dr] and, where ``q`` [N, H, dn + dr] is
+    given, q with its last dr elements rotated (else None).  ``cache`` None
+    (with c_kv and slots None) only rotates."""
+    named = [("k_pe", k_pe)] + [(n, t) for n, t in (("c_kv", c_kv), ("cache", cache), ("q", q)) if t is not None]
+    _operands("latent append", *named)
+    if k_pe.dim() != 2:
+        raise ValueError("latent append: k_pe must be [N, dr]")
+    N, dr = k_pe.shape
+    pages, page, dc, cs = 1, 1, 8, (0,)
+    if cache is not None:
+        if c_kv is None or slots is None or c_kv.dim() != 2 or c_kv.shape[0] != N:
+            raise ValueError("latent append: c_kv must be [N, dc], with a slot for each token")
+        dc = c_kv.shape[1]
+        _cache("latent append", cache, dc + dr)
+        pages, page = cache.shape[:2]
+        slots = _index("latent append", "slots", slots, (N,), torch.int64, k_pe.device)
+        c_kv, cs = _strided(c_kv, 1)
+    positions = _index("latent append", "positions", positions, (N,), torch.int32, k_pe.device)
+    cos, sin = _tables("latent append", cos, sin, dr, k_pe.device)
+    k_pe, ks = _strided(k_pe, 1)
+    H, dn, qs, q_out = 1, 8, (0, 0), None
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != N or q.shape[2] <= dr:
+            raise ValueError("latent append: q must be [N, H, dn + dr]")
+        q, qs = _strided(q, 2)
+        H, dn = q.shape[1], q.shape[2] - dr
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(N, dr, dtype=k_pe.dtype, device=k_pe.device)
+    args = _lib.LatentAppendArgs(N, H, dn, dr, dc, _DT[k_pe.dtype], page, pages, cos.shape[0], 1 if interleaved else 0,
+                                 cs[0], ks[0], tuple(qs))
+    if timer is not None:
+        args.profile = timer.arm()
+    rc = _lib.load().atomic_latent_append(ctypes.byref(args), _ptr(c_kv), _ptr(k_pe), _ptr(slots), _ptr(positions),
+                                          _ptr(cos), _ptr(sin), _ptr(q), _ptr(cache), _ptr(k_out), _ptr(q_out),
+                                          _stream(k_pe.device))
+    _lib.check(rc, "atomic_latent_append")
+    return k_out, q_out
+
+
+def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, interleaved=False, workspace=None,
+           timer=None):
+    """o [B, n, H, dv]: n query tokens a sequence over its cached latents.
+
+    ``q`` [B, n, H, dn + dr]; ``page_table`` int32 [B, pages of the longest];
+    ``kv_lens`` int32 [B], the appended tokens counted in.  Query t of sequence
+    b stands at position kv_lens[b] - n + t and sees the tokens up to and with
+    its own; one before the sequence's start (as in an empty sequence) has
+    o = 0.  With ``cos`` / ``sin`` the last dr elements of q are rotated by that
+    position on the way, without them they are taken as rotated already."""
+    _operands("latent decode", ("q", q), ("w_kv", w_kv), ("cache", cache))
+    if q.dim() != 4 or w_kv.dim() != 3 or w_kv.shape[0] != q.shape[2]:
+        raise ValueError("latent decode: q must be [B, n, H, dn + dr] and w_kv [H, dn + dv, dc]")
+    B, n, H, d = q.shape
+    dc = w_kv.shape[2]
+    if cache.dim() != 3 or not 0 < cache.shape[2] - dc < d or w_kv.shape[1] <= d - (cache.shape[2] - dc):
+        raise ValueError("latent decode: cache must be [pages, page, dc + dr], w_kv [H, dn + dv, dc]")
+    dr = cache.shape[2] - dc
+    _cache("latent decode", cache, dc + dr)
+    if page_table.dim() != 2:
+        raise ValueError("latent decode: page_table must be int32 [B, pages]")
+    page_table = _index("latent decode", "page_table", page_table, (B, page_table.shape[1]), torch.int32, q.device)
+    kv_lens = _index("latent decode", "kv_lens", kv_lens, (B,), torch.int32, q.device)
+    if (cos is None) != (sin is None):
+        raise ValueError("latent decode: cos and sin come together")
+    if cos is not None:
+        cos, sin = _tables("latent decode", cos, sin, dr, q.device)
+    q, qs = _strided(q, 3)
+    w_kv, _ = _strided(w_kv.contiguous(), 2)
+    lib = _lib.load()
+    args = _lib.LatentDecodeArgs(B, n, H, d - dr, dr, w_kv.shape[1] - (d - dr), dc, _DT[q.dtype], cache.shape[1],
+                                 cache.shape[0], page_table.shape[1], 0 if cos is None else cos.shape[0],
+                                 1 if interleaved else 0, scale, tuple(qs))
+    if timer is not None:
+        args.profile = timer.arm()
+    nbytes = lib.atomic_latent_decode_workspace_size(ctypes.byref(args))
+    if nbytes == 0:
+        raise _lib.AtomicError("atomic_latent_decode_workspace_size: unsupported shape")
+    if workspace is None or workspace.numel() < nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    o = torch.empty(B, n, H, args.dv, dtype=q.dtype, device=q.device)
+    rc = lib.atomic_latent_decode(ctypes.byref(args), _ptr(q), _ptr(w_kv), _ptr(cache), _ptr(page_table),
+                                  _ptr(kv_lens), _ptr(cos), _ptr(sin), _ptr(o), _ptr(workspace), workspace.numel(),
+                                  _stream(q.device))
+    _lib.check(rc, "atomic_latent_decode")
+    return o

@@ -1,0 +1,126 @@
+// Shared pieces of the latent-attention kernels: 32 x 32 MFMA fragments, the
+// LDS tile layout and the host checks.
+//
+// Every product is arranged so that the softmax's row (a query) runs along the
+// columns of an MFMA result: S^T = K Q^T gives lane l (query l % 32) the scores
+// of tokens 8 (r / 4) + 4 (l / 32) + r % 4, and registers 8 s .. 8 s + 7 of it
+// are, as they stand, the B operand of the next product over the 16 tokens of
+// step s (its k order is the same permutation on both sides).  So probabilities
+// and score gradients never leave the registers.
+#pragma once
+#include "common.hpp"
+#include "launch.hpp"
+#include "ws_tag.hpp"
+
+namespace ah {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// v_log_f32 flushes subnormals; the arguments here are sums of at least one 1.0
+__device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
+
+template <typename T> struct M32;
+template <> struct M32<bf16> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+// fp32: the same eight k values a lane, as eight instructions of two k values
+// (one from each half of the wave)
+template <> struct M32<float> {
+  typedef f32x8 frag;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Eight consecutive elements as a fragment (zeros where !ok: the padding of a width).
+__device__ __forceinline__ bf16x8 ld_frag(const bf16* p) { return *reinterpret_cast<const bf16x8*>(p); }
+__device__ __forceinline__ f32x8 ld_frag(const float* p) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <typename T> __device__ __forceinline__ typename M32<T>::frag zero_frag() {
+  typename M32<T>::frag z;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = (T)0.f;
+  return z;
+}
+// registers 8 s .. 8 s + 7 of a result as the next product's operand
+template <typename T> __device__ __forceinline__ typename M32<T>::frag pack_frag(const f32x16& x, int s) {
+  typename M32<T>::frag z;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = (T)x[8 * s + j];
+  return z;
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) z[j] = 0.f;
+  return z;
+}
+
+// A tile of rows of W elements in LDS as 16-byte pieces, piece c of row r at
+// place c ^ swz(r): eight consecutive rows read at one piece, and four
+// consecutive rows read at a pair of pieces (the transposed reads), fall on
+// distinct banks.
+template <typename T, int W>
+struct LTile {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  static constexpr int NC = (W / VEC + 7) / 8 * 8;
+  static constexpr int ROWB = NC * 16;
+  static __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+  static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
+  // row operand: lane (l % 32) holds row r0 + l % 32, elements k0 + 8 (l / 32) .. + 7
+  static __device__ __forceinline__ typename M32<T>::frag row(const char* s, int r0, int k0) {
+    const int l = lane_id(), r = r0 + (l & 31), k = k0 + 8 * (l >> 5);
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const bf16x8*>(s + off(r, k / 8));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(s + off(r, k / 4));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(s + off(r, k / 4 + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // column operand: lane (l % 32) holds column c0 + l % 32 of the 16 rows from r0, in the order that
+  // a result's registers have: rows r0 + 4 (l / 32) + j and r0 + 8 + 4 (l / 32) + j
+  static __device__ __forceinline__ typename M32<T>::frag col(const char* s, int r0, int c0) {
+    const int l = lane_id(), h = l >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int t = l & 15, r = r0 + 4 * h + (t >> 2), c = c0 + 16 * ((l >> 4) & 1) + 4 * (t & 3);
+      typedef __attribute__((address_space(3))) bf16x4* lds_p;
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + off(r, c / 8) + 2 * (c & 7)));
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + off(r + 8, c / 8) + 2 * (c & 7)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const int c = c0 + (l & 31);
+      f32x8 z;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
+        z[j] = *reinterpret_cast<const float*>(s + off(r, c / 4) + 4 * (c & 3));
+      }
+      return z;
+    }
+  }
+};
+
+inline int latent_widths_check(int dn, int dr, int dtype) {
+  if (dtype != ATOMIC_F32 && dtype != ATOMIC_BF16) return ATOMIC_ERR_DTYPE;
+  if (dn < 8 || dn > 128 || dn % 8 || dr < 8 || dr > 64 || dr % 8) return ATOMIC_ERR_SHAPE;
+  return ATOMIC_OK;
+}
+inline bool whole_pieces(std::initializer_list<int64_t> strides, int dtype) {
+  const int64_t v = dtype == ATOMIC_BF16 ? 8 : 4;
+  for (int64_t s : strides)
+    if (s < 0 || s % v || s > INT64_MAX / 16) return false;
+  return true;
+}
+
+}  // namespace ah

@@ -1,0 +1,521 @@
+// Latent attention in its expanded form for gfx950: forward and backward over
+// k_nope and v as the up-projection leaves them ([.., H, dn + dv]) and the
+// rotated key that all heads share.
+//
+//   s_ij = scale (q_nope_i . k_nope_j + q_pe_i . k_pe_j)     visible j only
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i)
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dk_pe_j summed over the heads
+//
+// Scores and their gradients live in registers only (latent.hpp).  p and ds are
+// rounded to the operand type for the second product, as its MFMA takes them;
+// everything else (scores, the running maximum and sum, lse, delta, every
+// accumulator) is fp32.
+#include "latent.hpp"
+
+namespace ah {
+
+struct LatDims {
+  int B, T, S, H, dn, dr, dv, causal, blocks;  // blocks: row (or token) blocks of a head
+  float scale;
+  int64_t qs[3], ks[3], ps[2], gs[3];  // strides of q, kv, k_pe, do
+};
+
+// Block x of the grid -> (head of the batch, block of its rows): the blocks of a
+// head share an XCD's L2, which then holds the head's other operand once.
+__device__ __forceinline__ void lat_map(const LatDims& d, int& b, int& h, int& blk) {
+  int bh;
+  xcd_group_map(blockIdx.x, d.B * d.H, d.blocks, bh, blk);
+  b = bh / d.H;
+  h = bh % d.H;
+}
+__device__ __forceinline__ int clamp_len(const int32_t* p, int b, int most) {
+  return p ? min(max(p[b], 0), most) : most;
+}
+
+// Rows [r0, r0 + R) of a matrix as two spans of pieces (w0 elements from src0,
+// then at column W0 w1 elements from src1) into an LDS tile; rows past `last`
+// repeat it (their products are masked, and padding rows are never read), the
+// padding of the widths is zero.
+template <typename T, int R, int W0, int W1, int NTH>
+__device__ __forceinline__ void stage_tile(char* dst, int r0, int last, const T* src0, int64_t ld0, int w0,
+                                           const T* src1, int64_t ld1, int w1) {
+  typedef LTile<T, W0 + W1> L;
+  constexpr int V = L::VEC, PR = (W0 + W1) / V, NP = R * PR, IT = (NP + NTH - 1) / NTH;
+  u32x4 tmp[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int e = threadIdx.x + NTH * i, r = e / PR, c = (e % PR) * V;
+    u32x4 x = {0, 0, 0, 0};
+    if (NP % NTH == 0 || e < NP) {
+      const int64_t row = min(r0 + r, last);
+      if (W1 == 0 || c < W0) {
+        if (c < w0) x = *reinterpret_cast<const u32x4*>(src0 + row * ld0 + c);
+      } else if (c - W0 < w1) {
+        x = *reinterpret_cast<const u32x4*>(src1 + row * ld1 + c - W0);
+      }
+    }
+    tmp[i] = x;
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int e = threadIdx.x + NTH * i;
+    if (NP % NTH == 0 || e < NP) *reinterpret_cast<u32x4*>(dst + L::off(e / PR, e % PR)) = tmp[i];
+  }
+}
+
+// The same split row as register fragments: this lane's row at src0 / src1.
+template <typename T, int W0, int W1>
+__device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) / 16], const T* src0, int w0,
+                                          const T* src1, int w1) {
+  const int h8 = 8 * (lane_id() >> 5);
+#pragma unroll
+  for (int s = 0; s < (W0 + W1) / 16; ++s) {
+    const int k = 16 * s + h8;
+    f[s] = zero_frag<T>();
+    if (16 * s < W0) {
+      if (k < w0) f[s] = ld_frag(src0 + k);
+    } else if (k - W0 < w1) {
+      f[s] = ld_frag(src1 + k - W0);
+    }
+  }
+}
+
+// Token of register r of a score tile (from its first token).
+__device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3); }
+
+// ------------------------------------------------------------------ forward
+// 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens.
+template <typename T, int DN, int DR, int DV>
+__global__ __launch_bounds__(256) void latent_fwd(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
+                                                  const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
+                                                  const int32_t* __restrict__ kv_lens, T* __restrict__ o,
+                                                  float* __restrict__ lse) {
+  constexpr int D = DN + DR, KS = D / 16, NT = DV / 32, TK = 64;
+  typedef LTile<T, D> LK;
+  typedef LTile<T, DV> LV;
+  typedef typename M32<T>::frag frag;
+  __shared__ __attribute__((aligned(1024))) char sk[TK * LK::ROWB];
+  __shared__ __attribute__((aligned(1024))) char sv[TK * LV::ROWB];
+  int b, h, blk;
+  lat_map(d, b, h, blk);
+  blk = d.blocks - 1 - blk;  // with causal the long rows first
+  const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
+  const int w0 = 128 * blk + 32 * wave_id();  // this wave's first row
+  const int row = w0 + (lane_id() & 31);
+  const int last = min(128 * blk + 127, ql - 1);  // the workgroup's last row
+  int end = kl;                                   // keys that any row sees
+  if (d.causal) end = min(end, last + off + 1);
+  if (last < 128 * blk) end = 0;
+  const T* qr = q + b * d.qs[0] + (int64_t)max(min(row, ql - 1), 0) * d.qs[1] + h * d.qs[2];
+  const T* kb = kv + b * d.ks[0] + h * d.ks[2];
+  const T* pb = kpe + b * d.ps[0];
+  frag qf[KS];
+  row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
+  f32x16 acc[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) acc[n] = zero16();
+  const float c2 = d.scale * kLog2e;
+  float m = -INFINITY, sum = 0.f;  // running maximum (of c2 times the scores) and this lane's part of the sum
+  for (int k0 = 0; k0 < end; k0 += TK) {
+    __syncthreads();
+    stage_tile<T, TK, DN, DR, 256>(sk, k0, kl - 1, kb, d.ks[1], d.dn, pb, d.ps[1], d.dr);
+    stage_tile<T, TK, DV, 0, 256>(sv, k0, kl - 1, kb + d.dn, d.ks[1], d.dv, (const T*)nullptr, 0, 0);
+    __syncthreads();
+    if (w0 >= ql || (d.causal && k0 > w0 + 31 + off)) continue;  // nothing visible to this wave
+    f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      s[0] = M32<T>::mma(LK::row(sk, 0, 16 * t), qf[t], s[0]);
+      s[1] = M32<T>::mma(LK::row(sk, 32, 16 * t), qf[t], s[1]);
+    }
+    if (k0 + TK > kl || (d.causal && k0 + TK - 1 > w0 + off)) {
+      const int seen = min(kl, d.causal ? row + off + 1 : kl) - k0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * i + reg_row(r) >= seen) s[i][r] = -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r] * c2);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float mn = fmaxf(m, top);
+    const float ref = mn == -INFINITY ? 0.f : mn;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
+    const float fade = fast_exp2(m - ref);
+    m = mn;
+    sum *= fade;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][r] *= fade;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[i][r] = fast_exp2(s[i][r] * c2 - ref);
+        sum += s[i][r];
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const frag p = pack_frag<T>(s[i], t);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n] = M32<T>::mma(LV::col(sv, 32 * i + 16 * t, 32 * n), p, acc[n]);
+      }
+  }
+  if (row >= d.T) return;
+  sum += __shfl_xor(sum, 32);
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  T* orow = o + (((int64_t)b * d.T + row) * d.H + h) * d.dv;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c = 32 * n + reg_row(r);
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] * inv : 0.f;
+      if (c < d.dv) store4(orow + c, v);
+    }
+  if (lane_id() < 32)
+    lse[((int64_t)b * d.H + h) * d.T + row] = row < ql && sum != 0.f ? m * kLn2 + fast_log2(sum) * kLn2 : -INFINITY;
+}
+
+// ----------------------------------------------------------------- backward
+// delta [B, H, T]: sixteen lanes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restrict__ o, const T* __restrict__ dout,
+                                                    float* __restrict__ delta) {
+  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, t, h)
+  if (i >= (int64_t)d.B * d.T * d.H) return;
+  const int h = (int)(i % d.H), t = (int)(i / d.H % d.T), b = (int)(i / d.H / d.T);
+  const T* g = dout + b * d.gs[0] + t * d.gs[1] + h * d.gs[2];
+  float s = 0.f;
+  for (int c = 8 * (threadIdx.x & 15); c < d.dv; c += 128) {
+    float x[8], y[8];
+    load8(o + i * d.dv + c, x);
+    load8(g + c, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += x[j] * y[j];
+  }
+#pragma unroll
+  for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
+  if ((threadIdx.x & 15) == 0) delta[((int64_t)b * d.H + h) * d.T + t] = s;
+}
+
+// dq: 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens.
+template <typename T, int DN, int DR, int DV>
+__global__ __launch_bounds__(256) void latent_bwd_dq(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
+                                                     const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
+                                                     const int32_t* __restrict__ kv_lens,
+                                                     const float* __restrict__ lse, const float* __restrict__ delta,
+                                                     const T* __restrict__ dout, T* __restrict__ dq) {
+  constexpr int D = DN + DR, KS = D / 16, VS = DV / 16, NT = D / 32, TK = 64;
+  typedef LTile<T, D> LK;
+  typedef LTile<T, DV> LV;
+  typedef typename M32<T>::frag frag;
+  __shared__ __attribute__((aligned(1024))) char sk[TK * LK::ROWB];
+  __shared__ __attribute__((aligned(1024))) char sv[TK * LV::ROWB];
+  int b, h, blk;
+  lat_map(d, b, h, blk);
+  blk = d.blocks - 1 - blk;
+  const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
+  const int w0 = 128 * blk + 32 * wave_id();
+  const int row = w0 + (lane_id() & 31);
+  const int last = min(128 * blk + 127, ql - 1);
+  int end = kl;
+  if (d.causal) end = min(end, last + off + 1);
+  if (last < 128 * blk) end = 0;
+  const int rowc = max(min(row, ql - 1), 0);
+  const T* qr = q + b * d.qs[0] + (int64_t)rowc * d.qs[1] + h * d.qs[2];
+  const T* kb = kv + b * d.ks[0] + h * d.ks[2];
+  const T* pb = kpe + b * d.ps[0];
+  frag qf[KS], gf[VS];
+  row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
+  row_frags<T, DV, 0>(gf, dout + b * d.gs[0] + (int64_t)rowc * d.gs[1] + h * d.gs[2], d.dv, (const T*)nullptr, 0);
+  const float l2 = lse[((int64_t)b * d.H + h) * d.T + rowc] * kLog2e;
+  const float dl = delta[((int64_t)b * d.H + h) * d.T + rowc];
+  f32x16 acc[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) acc[n] = zero16();
+  const float c2 = d.scale * kLog2e;
+  for (int k0 = 0; k0 < end; k0 += TK) {
+    __syncthreads();
+    stage_tile<T, TK, DN, DR, 256>(sk, k0, kl - 1, kb, d.ks[1], d.dn, pb, d.ps[1], d.dr);
+    stage_tile<T, TK, DV, 0, 256>(sv, k0, kl - 1, kb + d.dn, d.ks[1], d.dv, (const T*)nullptr, 0, 0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t0 = k0 + 32 * i;
+      if (w0 >= ql || t0 >= kl || (d.causal && t0 > w0 + 31 + off)) break;
+      f32x16 s = zero16(), g = zero16();
+#pragma unroll
+      for (int t = 0; t < KS; ++t) s = M32<T>::mma(LK::row(sk, 32 * i, 16 * t), qf[t], s);
+#pragma unroll
+      for (int t = 0; t < VS; ++t) g = M32<T>::mma(LV::row(sv, 32 * i, 16 * t), gf[t], g);
+      const int seen = min(kl, d.causal ? row + off + 1 : kl) - t0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = fast_exp2(s[r] * c2 - l2);
+        s[r] = reg_row(r) < seen ? p * (g[r] - dl) : 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const frag ds = pack_frag<T>(s, t);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n] = M32<T>::mma(LK::col(sk, 32 * i + 16 * t, 32 * n), ds, acc[n]);
+      }
+    }
+  }
+  if (row >= d.T) return;
+  T* out = dq + (((int64_t)b * d.T + row) * d.H + h) * (d.dn + d.dr);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c = 32 * n + reg_row(r);
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] * d.scale : 0.f;
+      if (32 * n < DN) {
+        if (c < d.dn) store4(out + c, v);
+      } else if (c - DN < d.dr) {
+        store4(out + d.dn + c - DN, v);
+      }
+    }
+}
+
+// dk, dv: 128 tokens of a head a workgroup, 32 a wave (their keys, values and
+// gradient accumulators in registers), against tiles of 32 query rows.  The
+// rotated key's gradient leaves as this head's part, fp32 [B, H, S, dr].
+template <typename T, int DN, int DR, int DV>
+__global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
+                                                         const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
+                                                         const int32_t* __restrict__ kv_lens,
+                                                         const float* __restrict__ lse,
+                                                         const float* __restrict__ delta, const T* __restrict__ dout,
+                                                         T* __restrict__ dkv, float* __restrict__ dkp) {
+  constexpr int D = DN + DR, KS = D / 16, VS = DV / 16, NK = D / 32, NV = DV / 32, TQ = 32;
+  typedef LTile<T, D> LQ;
+  typedef LTile<T, DV> LG;
+  typedef typename M32<T>::frag frag;
+  __shared__ __attribute__((aligned(1024))) char sq[TQ * LQ::ROWB];
+  __shared__ __attribute__((aligned(1024))) char sg[TQ * LG::ROWB];
+  __shared__ __attribute__((aligned(16))) float sl[TQ], sd[TQ];
+  int b, h, blk;
+  lat_map(d, b, h, blk);
+  const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
+  const int w0 = 128 * blk + 32 * wave_id();  // this wave's first token
+  const int tok = w0 + (lane_id() & 31);
+  const int tokc = max(min(tok, kl - 1), 0);
+  int first = 0;  // the first query that sees any of the workgroup's tokens
+  if (d.causal) first = max(0, 128 * blk - off);
+  if (128 * blk >= kl) first = ql;
+  const T* qb = q + b * d.qs[0] + h * d.qs[2];
+  const T* gb = dout + b * d.gs[0] + h * d.gs[2];
+  const T* kr = kv + b * d.ks[0] + (int64_t)tokc * d.ks[1] + h * d.ks[2];
+  const float* lb = lse + ((int64_t)b * d.H + h) * d.T;
+  const float* db = delta + ((int64_t)b * d.H + h) * d.T;
+  frag kf[KS], vf[VS];
+  row_frags<T, DN, DR>(kf, kr, d.dn, kpe + b * d.ps[0] + (int64_t)tokc * d.ps[1], d.dr);
+  row_frags<T, DV, 0>(vf, kr + d.dn, d.dv, (const T*)nullptr, 0);
+  f32x16 ak[NK], av[NV];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) ak[n] = zero16();
+#pragma unroll
+  for (int n = 0; n < NV; ++n) av[n] = zero16();
+  const float c2 = d.scale * kLog2e;
+  for (int r0 = first & ~(TQ - 1); r0 < ql; r0 += TQ) {
+    __syncthreads();
+    stage_tile<T, TQ, DN, DR, 256>(sq, r0, ql - 1, qb, d.qs[1], d.dn, qb + d.dn, d.qs[1], d.dr);
+    stage_tile<T, TQ, DV, 0, 256>(sg, r0, ql - 1, gb, d.gs[1], d.dv, (const T*)nullptr, 0, 0);
+    if (threadIdx.x < TQ) {
+      sl[threadIdx.x] = lb[min(r0 + (int)threadIdx.x, ql - 1)] * kLog2e;
+      sd[threadIdx.x] = db[min(r0 + (int)threadIdx.x, ql - 1)];
+    }
+    __syncthreads();
+    if (w0 >= kl || (d.causal && w0 > r0 + TQ - 1 + off)) continue;
+    f32x16 s = zero16(), g = zero16();
+#pragma unroll
+    for (int t = 0; t < KS; ++t) s = M32<T>::mma(LQ::row(sq, 0, 16 * t), kf[t], s);
+#pragma unroll
+    for (int t = 0; t < VS; ++t) g = M32<T>::mma(LG::row(sg, 0, 16 * t), vf[t], g);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = reg_row(r), at = r0 + i;
+      const bool ok = at < ql && tok < kl && (!d.causal || tok <= at + off);
+      const float p = fast_exp2(s[r] * c2 - sl[i]);
+      s[r] = ok ? p : 0.f;
+      g[r] = ok ? p * (g[r] - sd[i]) : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const frag p = pack_frag<T>(s, t), ds = pack_frag<T>(g, t);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) av[n] = M32<T>::mma(LG::col(sg, 16 * t, 32 * n), p, av[n]);
+#pragma unroll
+      for (int n = 0; n < NK; ++n) ak[n] = M32<T>::mma(LQ::col(sq, 16 * t, 32 * n), ds, ak[n]);
+    }
+  }
+  if (tok >= d.S) return;
+  T* out = dkv + (((int64_t)b * d.S + tok) * d.H + h) * (d.dn + d.dv);
+  float* op = dkp + (((int64_t)b * d.H + h) * d.S + tok) * d.dr;
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c = 32 * n + reg_row(r);
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = tok < kl ? ak[n][r + j] * d.scale : 0.f;
+      if (32 * n < DN) {
+        if (c < d.dn) store4(out + c, v);
+      } else if (c - DN < d.dr) {
+        store4(op + c - DN, v);
+      }
+    }
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c = 32 * n + reg_row(r);
+      f32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = tok < kl ? av[n][r + j] : 0.f;
+      if (c < d.dv) store4(out + d.dn + c, v);
+    }
+}
+
+// dk_pe = the heads' parts summed in their order: four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void latent_bwd_dkpe(LatDims d, const float* __restrict__ dkp, T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, per = (int64_t)d.S * d.dr;
+  if (i >= d.B * per) return;
+  const float* p = dkp + i / per * d.H * per + i % per;
+  f32x4 s = zero4();
+  for (int h = 0; h < d.H; ++h) s += *reinterpret_cast<const f32x4*>(p + h * per);
+  store4(out + i, s);
+}
+
+// ------------------------------------------------------------------ host
+static int lat_check(const atomic_latent_args* a) {
+  if (!a) return ATOMIC_ERR_NULL;
+  if (int rc = latent_widths_check(a->dn, a->dr, a->dtype)) return rc;
+  if (a->dv < 8 || a->dv > 128 || a->dv % 8 || a->batch < 1 || a->tq < 1 || a->tk < 1 || a->heads < 1 ||
+      (a->causal != 0 && a->causal != 1))
+    return ATOMIC_ERR_SHAPE;
+  // row numbers and lengths stay in 31 bits with room for a block; grids in 31 bits
+  if (a->tq > (1 << 30) || a->tk > (1 << 30)) return ATOMIC_ERR_SHAPE;
+  const int64_t most = (int64_t)(a->tq > a->tk ? a->tq : a->tk), bh = (int64_t)a->batch * a->heads;
+  if (bh > INT32_MAX || bh * ((most + 127) / 128) > INT32_MAX || bh * ((most + 15) / 16) > INT32_MAX ||
+      (int64_t)a->batch * ((a->tk + 15) / 16) * a->dr > INT32_MAX)
+    return ATOMIC_ERR_SHAPE;
+  if (!whole_pieces({a->q_stride[0], a->q_stride[1], a->q_stride[2], a->kv_stride[0], a->kv_stride[1],
+                     a->kv_stride[2], a->kpe_stride[0], a->kpe_stride[1], a->do_stride[0], a->do_stride[1],
+                     a->do_stride[2]}, a->dtype))
+    return ATOMIC_ERR_SHAPE;
+  return ATOMIC_OK;
+}
+
+static LatDims lat_dims(const atomic_latent_args* a) {
+  LatDims d{a->batch, a->tq, a->tk, a->heads, a->dn, a->dr, a->dv, a->causal, 0, a->scale, {}, {}, {}, {}};
+  for (int i = 0; i < 3; ++i) {
+    d.qs[i] = a->q_stride[i];
+    d.ks[i] = a->kv_stride[i];
+    d.gs[i] = a->do_stride[i];
+  }
+  d.ps[0] = a->kpe_stride[0];
+  d.ps[1] = a->kpe_stride[1];
+  return d;
+}
+
+// f(type, widths): the two sets of widths that are built; others run in the next larger, padded with zeros
+template <int N, int R, int V> struct Widths { static constexpr int DN = N, DR = R, DV = V; };
+template <typename F>
+static int lat_dispatch(const atomic_latent_args* a, F&& f) {
+  const bool small = a->dn <= 64 && a->dr <= 32 && a->dv <= 64;
+  if (a->dtype == ATOMIC_BF16) return small ? f(bf16(), Widths<64, 32, 64>()) : f(bf16(), Widths<128, 64, 128>());
+  return small ? f(float(), Widths<64, 32, 64>()) : f(float(), Widths<128, 64, 128>());
+}
+
+static size_t lat_delta_bytes(const atomic_latent_args* a) {
+  return ((size_t)a->batch * a->heads * a->tq * sizeof(float) + 255) / 256 * 256;
+}
+
+}  // namespace ah
+
+using namespace ah;
+
+extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
+                                 const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* stream) {
+  if (int rc = lat_check(a)) return rc;
+  if (!q || !kv || !k_pe || !o || !lse) return ATOMIC_ERR_NULL;
+  if (!aligned16({q, kv, k_pe, o})) return ATOMIC_ERR_SHAPE;
+  LatDims d = lat_dims(a);
+  d.blocks = (d.T + 127) / 128;
+  const hipStream_t st = (hipStream_t)stream;
+  Launch L{a->profile, st};
+  return lat_dispatch(a, [&](auto t, auto w) {
+    typedef decltype(t) T;
+    typedef decltype(w) W;
+    return L("latent_fwd", [&] {
+      hipLaunchKernelGGL((latent_fwd<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256), 0,
+                         st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, (T*)o, lse);
+    });
+  });
+}
+
+extern "C" size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a) {
+  if (lat_check(a) != ATOMIC_OK) return 0;
+  return lat_delta_bytes(a) + (size_t)a->batch * a->heads * a->tk * a->dr * sizeof(float);
+}
+
+extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
+                                 const int32_t* q_lens, const int32_t* kv_lens, const void* o, const float* lse,
+                                 const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  if (int rc = lat_check(a)) return rc;
+  if (!q || !kv || !k_pe || !o || !lse || !dout || !dq || !dkv || !dk_pe) return ATOMIC_ERR_NULL;
+  if (!aligned16({q, kv, k_pe, o, dout, dq, dkv, dk_pe})) return ATOMIC_ERR_SHAPE;
+  if (!workspace || workspace_bytes < atomic_latent_bwd_workspace_size(a) || !aligned16({workspace}))
+    return ATOMIC_ERR_WORKSPACE;
+  ws_tag_clobber(workspace, atomic_latent_bwd_workspace_size(a));
+  float* delta = (float*)workspace;
+  float* dkp = (float*)((char*)workspace + lat_delta_bytes(a));
+  const hipStream_t st = (hipStream_t)stream;
+  Launch L{a->profile, st};
+  return lat_dispatch(a, [&](auto t, auto w) {
+    typedef decltype(t) T;
+    typedef decltype(w) W;
+    LatDims d = lat_dims(a);
+    const int64_t rows = (int64_t)d.B * d.T * d.H;
+    int rc = L("latent_delta", [&] {
+      hipLaunchKernelGGL((latent_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, d, (const T*)o,
+                         (const T*)dout, delta);
+    });
+    if (rc) return rc;
+    d.blocks = (d.S + 127) / 128;
+    rc = L("latent_bwd_dkv", [&] {
+      hipLaunchKernelGGL((latent_bwd_dkv<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
+                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, lse, delta,
+                         (const T*)dout, (T*)dkv, dkp);
+    });
+    if (rc) return rc;
+    d.blocks = (d.T + 127) / 128;
+    rc = L("latent_bwd_dq", [&] {
+      hipLaunchKernelGGL((latent_bwd_dq<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
+                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, lse, delta,
+                         (const T*)dout, (T*)dq);
+    });
+    if (rc) return rc;
+    return L("latent_bwd_dkpe", [&] {
+      hipLaunchKernelGGL((latent_bwd_dkpe<T>), dim3((unsigned)(((int64_t)d.B * d.S * d.dr / 4 + 255) / 256)),
+                         dim3(256), 0, st, d, dkp, (T*)dk_pe);
+    });
+  });
+}

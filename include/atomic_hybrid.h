@@ -761,6 +761,138 @@ int atomic_mamba2_proj_bwd(const atomic_mamba2_proj_args* a, const void* x_bc, c
                            float* db_dt, float* dw_b, float* dw_c, float* da_log, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Latent attention: keys and values from one latent vector a token.
+ *
+ * Sizes: H heads; dn, the key width without position; dr, the rotated key
+ * width, shared by all heads; dv, the value width; dc, the latent width.  With
+ * the up-projection w_kv [H, dn + dv, dc] a token's latent c gives each head
+ *   k_nope = w_kv[h, :dn] c,   v = w_kv[h, dn:] c
+ * and a query scores it scale * (q_nope . k_nope + q_pe . k_pe), a query row
+ * being [q_nope | q_pe].  Two forms: expanded, over k_nope and v as they stand
+ * (prompts and training), and absorbed, over the latents of a paged cache.
+ *
+ * dtype is ATOMIC_BF16 or ATOMIC_F32 for every operand named "dtype"; sums,
+ * softmax statistics and accumulators are fp32.  Strides are in elements.
+ * "Piece": 16 bytes (8 bf16 or 4 fp32 elements).  Operand pointers that a
+ * stride belongs to are 16-byte aligned and their strides whole pieces.
+ */
+
+/* Expanded form.  Query i of batch row b (i < ql = q_lens[b], or tq) sees the
+ * keys j < kl = kv_lens[b] (or tk), with causal only those with
+ * j <= i + kl - ql.  Lengths outside [0, tq] / [0, tk] are taken to the nearer
+ * end.  A query that sees no key has o = 0, lse = -inf and zero gradients, and
+ * so have the rows past the lengths; what the inputs hold past the lengths
+ * does not matter. */
+typedef struct atomic_latent_args {
+  int32_t batch;      /* B                                                  */
+  int32_t tq;         /* query rows of the padded batch, >= 1               */
+  int32_t tk;         /* key rows of the padded batch, >= 1                 */
+  int32_t heads;      /* H                                                  */
+  int32_t dn;         /* a multiple of 8, 8 .. 128                          */
+  int32_t dr;         /* a multiple of 8, 8 .. 64                           */
+  int32_t dv;         /* a multiple of 8, 8 .. 128                          */
+  int32_t dtype;      /* ATOMIC_F32 / ATOMIC_BF16                           */
+  int32_t causal;     /* 0 or 1                                             */
+  float scale;        /* of the scores                                      */
+  /* strides of q [B, tq, H, dn + dr], kv [B, tk, H, dn + dv] (k_nope | v) and
+     do [B, tq, H, dv]: batch row, token, head; of k_pe [B, tk, dr]: batch row,
+     token.  The last dimension is dense. */
+  int64_t q_stride[3];
+  int64_t kv_stride[3];
+  int64_t kpe_stride[2];
+  int64_t do_stride[3];
+  atomic_profile* profile;  /* optional per-kernel event timing, or NULL */
+} atomic_latent_args;
+
+/* Forward: o [B, tq, H, dv] dtype and lse [B, H, tq] fp32 (the natural log of
+ * the sum of the scores' exponentials), both dense.  q_lens and kv_lens are
+ * int32 [B] device arrays, or NULL. */
+int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
+                      const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* stream);
+
+/* Bytes of workspace the backward needs; 0 for unsupported args. */
+size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a);
+
+/* Backward from the forward's o and lse and the upstream gradient do: dq
+ * [B, tq, H, dn + dr], dkv [B, tk, H, dn + dv], dk_pe [B, tk, dr] (summed over
+ * the heads), dense, dtype.  The same inputs give the same bits. */
+int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
+                      const int32_t* q_lens, const int32_t* kv_lens, const void* o, const float* lse,
+                      const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The paged cache: [pages, page, dc + dr] dtype, dense; a token's row holds its
+ * latent and its rotated key.  Rotation by position p turns each pair (a, b) of
+ * the last dr elements into (a cos - b sin, b cos + a sin) with the row p of the
+ * fp32 tables cos / sin [rope_rows, dr / 2]: pairs (i, i + dr / 2), or
+ * (2 i, 2 i + 1) with interleaved.  The rotation is computed in fp32 and
+ * rounded once. */
+typedef struct atomic_latent_append_args {
+  int32_t tokens;      /* N                                                 */
+  int32_t heads;       /* H of q (any value >= 0 with q NULL)               */
+  int32_t dn;          /* a multiple of 8, 8 .. 128                         */
+  int32_t dr;          /* a multiple of 8, 8 .. 64                          */
+  int32_t dc;          /* a multiple of 8, 8 .. 512                         */
+  int32_t dtype;       /* ATOMIC_F32 / ATOMIC_BF16                          */
+  int32_t page;        /* tokens a page                                     */
+  int32_t pages;       /* pages of the cache                                */
+  int32_t rope_rows;   /* rows of the cos / sin tables                      */
+  int32_t interleaved; /* 0 or 1                                            */
+  int64_t c_stride;    /* of c_kv's rows                                    */
+  int64_t k_stride;    /* of k_pe's rows                                    */
+  int64_t q_stride[2]; /* of q: token, head                                 */
+  atomic_profile* profile;
+} atomic_latent_append_args;
+
+/* Appends N tokens: row slots[t] of the cache (page slots[t] / page, row
+ * slots[t] % page) becomes [c_kv[t] | rotate(k_pe[t], positions[t])]; a slot
+ * outside the cache (-1 by custom) leaves it as it is.  Slots that occur twice
+ * in a call hold either token's row.  k_out [N, dr] receives the rotated keys
+ * and, where q [N, H, dn + dr] is given, q_out (dense) q with its last dr
+ * elements rotated.  cache or k_out may be NULL (not written).  Positions
+ * outside the tables are taken to the nearer end. */
+int atomic_latent_append(const atomic_latent_append_args* a, const void* c_kv, const void* k_pe,
+                         const int64_t* slots, const int32_t* positions, const float* cos, const float* sin,
+                         const void* q, void* cache, void* k_out, void* q_out, void* stream);
+
+/* Absorbed form: n query tokens a sequence against its cached latents.  Query t
+ * of sequence b stands at position kv_lens[b] - n + t and sees the cached
+ * tokens up to and with that one; a position below zero sees nothing (o = 0).
+ * Token j of sequence b lies in page page_table[b][j / page], row j % page;
+ * entries past the last needed one are not used, page numbers outside the
+ * cache and lengths outside [0, table_pages * page] are taken to the nearer end. */
+typedef struct atomic_latent_decode_args {
+  int32_t batch;       /* B                                                 */
+  int32_t tokens;      /* n                                                 */
+  int32_t heads;       /* H; n H <= 4096                                    */
+  int32_t dn;          /* a multiple of 8, 8 .. 128                         */
+  int32_t dr;          /* a multiple of 8, 8 .. 64                          */
+  int32_t dv;          /* a multiple of 8, 8 .. 128                         */
+  int32_t dc;          /* a multiple of 8, 8 .. 512                         */
+  int32_t dtype;       /* ATOMIC_F32 / ATOMIC_BF16                          */
+  int32_t page;        /* tokens a page                                     */
+  int32_t pages;       /* pages of the cache                                */
+  int32_t table_pages; /* entries of a page_table row                       */
+  int32_t rope_rows;   /* rows of the cos / sin tables                      */
+  int32_t interleaved; /* 0 or 1                                            */
+  float scale;         /* of the scores                                     */
+  int64_t q_stride[3]; /* of q [B, n, H, dn + dr]: sequence, token, head    */
+  atomic_profile* profile;
+} atomic_latent_decode_args;
+
+/* Bytes of workspace the decode needs; 0 for unsupported args. */
+size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a);
+
+/* w_kv [H, dn + dv, dc] dtype, dense; page_table int32 [B, table_pages];
+ * kv_lens int32 [B] (the appended tokens counted in).  q's last dr elements are
+ * rotated by the query's position on the way; with cos and sin NULL they are
+ * taken as rotated already.  o [B, n, H, dv] dtype. */
+int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
+                         const void* cache, const int32_t* page_table, const int32_t* kv_lens,
+                         const float* cos, const float* sin, void* o, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
