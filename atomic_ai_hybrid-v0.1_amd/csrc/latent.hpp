@@ -17,6 +17,10 @@ namespace ah {
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// A row's reference may lag its true maximum by this many powers of two before the
+// accumulators are rescaled: p stays below 2^8, and most tiles need neither the
+// maximum across lanes nor a rescale.
+constexpr float kLag = 8.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // v_log_f32 flushes subnormals; the arguments here are sums of at least one 1.0
@@ -76,7 +80,10 @@ struct LTile {
   static constexpr int NC = (W / VEC + 7) / 8 * 8;
   static constexpr int ROWB = NC * 16;
   static __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-  static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
+  // (the piece's upper bits apart: they become the read's immediate offset)
+  static __device__ __forceinline__ int off(int r, int c) {
+    return r * ROWB + (((c & 7) ^ swz(r)) << 4) + ((c & ~7) << 4);
+  }
   // row operand: lane (l % 32) holds row r0 + l % 32, elements k0 + 8 (l / 32) .. + 7
   static __device__ __forceinline__ typename M32<T>::frag row(const char* s, int r0, int k0) {
     const int l = lane_id(), r = r0 + (l & 31), k = k0 + 8 * (l >> 5);
@@ -110,6 +117,27 @@ struct LTile {
     }
   }
 };
+
+// use(i, load(i)) for i in [0, N), G loads ahead of their uses: the reads of a
+// group are issued before the previous group is used (left alone, the compiler
+// reads each LDS fragment right before its MFMA and waits for it there).
+template <int N, int G, typename F, typename L, typename U>
+__device__ __forceinline__ void in_groups(L&& load, U&& use) {
+  F f[2][G];
+#pragma unroll
+  for (int j = 0; j < G && j < N; ++j) f[0][j] = load(j);
+#pragma unroll
+  for (int i = 0; i < N; i += G) {
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+      if (i + G + j < N) f[(i / G + 1) & 1][j] = load(i + G + j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+      if (i + j < N) use(i + j, f[(i / G) & 1][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 inline int latent_widths_check(int dn, int dr, int dtype) {
   if (dtype != ATOMIC_F32 && dtype != ATOMIC_BF16) return ATOMIC_ERR_DTYPE;

@@ -105,6 +105,7 @@ struct DecDims {
   float scale;
   int64_t qs[3];
 };
+constexpr int kDecChunk = 1024, kDecPages = kDecChunk + 1;  // tokens of a split, pages that they can lie in
 __device__ __forceinline__ int dec_len(const DecDims& d, const int32_t* kv_lens, int b) {
   return (int)min((int64_t)max(kv_lens[b], 0), (int64_t)d.table * d.page);
 }
@@ -215,105 +216,181 @@ struct DTile : LTile<T, W> {
   }
 };
 
-// One split of one sequence against 16 MT of its query rows (row t H + h): tiles
-// of 64 tokens, wave w taking the 16 rows w % MT and MT of the tile's four groups
-// of 16 tokens.  The waves of a row group join at the end.
-template <typename T, int DC, int MT>
-__global__ __launch_bounds__(256) void latent_split(DecDims d, const T* __restrict__ qa, const T* __restrict__ cache,
-                                                    const int32_t* __restrict__ table,
-                                                    const int32_t* __restrict__ kv_lens, float* __restrict__ part,
-                                                    float* __restrict__ stat) {
-  constexpr int DR = 64, W = DC + DR, KS = W / 32, NT = DC / 16, TK = 64, TW = 4 / MT, V = 16 / (int)sizeof(T);
-  typedef DTile<T, W> L;
+// Eight zeros: the source of the padding of a latent narrower than its tile.
+__device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+
+// One split of one sequence against 16 MT of its query rows (row t H + h).  NW
+// waves go over tiles of 16 NW tokens: wave w loads 16 tokens of each tile and
+// computes with the 16 rows w % MT and the tokens of MT waves.  The waves of a
+// row group join at the end.
+//
+// Bound by the cache's bytes: 16 heads need 30 operations a byte.  So the tiles go
+// straight to LDS, two of them (147 KB with 512 bf16 latents), and a wave that has
+// its rows to itself (MT = 1) never meets a barrier: it loads what it reads.  The
+// split's page numbers lie in LDS, so no wait for an index drains the tiles in flight.
+template <typename T, int DC, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
+                                                        const T* __restrict__ cache, const int32_t* __restrict__ table,
+                                                        const int32_t* __restrict__ kv_lens, float* __restrict__ part,
+                                                        float* __restrict__ stat, float* __restrict__ olat) {
+  constexpr int DR = 64, W = DC + DR, KS = W / 32, NT = DC / 16, TK = 16 * NW, TW = NW / MT, V = 16 / (int)sizeof(T);
+  constexpr int PC = DC / V, PR = DR / V;       // pieces of a row's latent and rotated key
+  constexpr int IC = PC * 16 / 64, IR = PR * 16 / 64;  // loads of one wave for its 16 tokens
+  typedef DTile<T, DC> LC;
+  typedef DTile<T, DR> LR;
   typedef typename M16<T>::frag frag;
   typedef typename M16<T>::half half;
-  __shared__ __attribute__((aligned(1024))) char sk[TK * L::ROWB];
-  __shared__ float sm[4][16], ss[4][16];
-  const int sp = blockIdx.x, b = blockIdx.z, wv = wave_id(), rw = wv % MT, tw = wv / MT;
+  constexpr int SC = 16 * LC::ROWB, SR = 16 * LR::ROWB;  // one wave's tokens of a tile
+  __shared__ __attribute__((aligned(1024))) char sk[2 * NW * (SC + SR)];
+  __shared__ int32_t spt[kDecPages];
+  __shared__ float sm[NW][16], ss[NW][16];
+  const int sp = blockIdx.x, b = blockIdx.z, wv = wave_id(), lane = lane_id(), rw = wv % MT, tw = wv / MT;
   const int len = dec_len(d, kv_lens, b), rows = d.n * d.H, wide = d.dc + d.dr;
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
-  if (first >= len) return;
-  const int row = 16 * (blockIdx.y * MT + rw) + (lane_id() & 15);
+  if (first >= len && (sp > 0 || d.splits > 1)) return;  // (one split only: it writes the empty sequence's zeros)
+  const int page0 = first / d.page;
+  for (int i = threadIdx.x; first < end && i <= (end - 1) / d.page - page0; i += 64 * NW)
+    spt[i] = min(max(table[(int64_t)b * d.table + page0 + i], 0), d.pages - 1);
+  const int row = 16 * (blockIdx.y * MT + rw) + (lane & 15);
   const int seen = len - d.n + min(row, rows - 1) / d.H + 1;  // tokens that this lane's row sees
+  const int least = len - d.n + 1;                            // and that every row sees
   const T* qr = qa + ((int64_t)b * rows + min(row, rows - 1)) * wide;
   frag qf[KS];
 #pragma unroll
   for (int t = 0; t < KS; ++t) {
-    const int k = 32 * t + 8 * (lane_id() >> 4);
-    qf[t] = zero_frag<T>();
-    if (32 * t < DC) {
-      if (k < d.dc) qf[t] = ld_frag(qr + k);
-    } else if (k - DC < d.dr) {
-      qf[t] = ld_frag(qr + d.dc + k - DC);
-    }
+    const int k = 32 * t + 8 * (lane >> 4);
+    if (32 * t < DC) qf[t] = ld_frag(k < d.dc ? qr + k : (const T*)lat_zeros);
+    else qf[t] = ld_frag(k - DC < d.dr ? qr + d.dc + k - DC : (const T*)lat_zeros);
   }
+  __syncthreads();  // the page numbers are there
+  const uint32_t lds0 = lds_addr(sk);
+  // Byte offsets of this lane's piece in a row, by the row's swizzle.  The padding
+  // of a width reads the row's first piece instead: the query has zeros there.
+  constexpr int RL = PC >= 64 ? PC / 64 : 1;  // loads a row
+  uint32_t oc[RL][8];
+#pragma unroll
+  for (int l = 0; l < RL; ++l)
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      const int c = 64 * l + (lane ^ z);
+      oc[l][z] = c * V < d.dc ? 16 * c : 0;
+    }
+  // this wave's 16 tokens of the tile at k0 into buffer `buf`; tokens past the end repeat the last one (masked below)
+  auto load = [&](int k0, int buf) {
+    const int j = min(k0 + 16 * wv + (lane & 15), end - 1), pg = j / d.page;
+    const uint64_t at = (uint64_t)(cache + ((int64_t)spt[pg - page0] * d.page + (j - pg * d.page)) * wide);
+    const uint32_t lo = (uint32_t)at, hi = (uint32_t)(at >> 32);
+    const uint32_t dst = lds0 + (buf * NW + wv) * (SC + SR);
+#pragma unroll
+    for (int i = 0; i < IC; ++i) {  // 64 pieces of the 16 rows of PC
+      if constexpr (PC >= 64) {
+        const int r = i / RL;
+        const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, r) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane(lo, r);
+        dma16_raw_s(row, oc[i % RL][LC::swz(r)], dst + 1024 * i);
+      } else {
+        const int r = (64 * i + lane) / PC;
+        const uint64_t row = (uint64_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r);
+        const int c = (lane % PC) ^ LC::swz(r);
+        dma16_raw((const void*)(row + (c * V < d.dc ? 16 * c : 0)), dst + 1024 * i);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < IR; ++i) {
+      const int e = 64 * i + lane, r = e / PR, c = (e % PR) ^ LR::swz(r);
+      const uint64_t row = (uint64_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r);
+      dma16_raw((const void*)(row + d.dc * sizeof(T) + (c * V < d.dr ? 16 * c : 0)), dst + SC + 1024 * i);
+    }
+  };
   f32x4 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero4();
   const float c2 = d.scale * kLog2e;
   float m = -INFINITY, sum = 0.f;
-  for (int k0 = first; k0 < end; k0 += TK) {
-    __syncthreads();
-    constexpr int PR = W / V;
-    for (int e = threadIdx.x; e < TK * PR; e += 256) {
-      const int c = e % PR * V, j = min(k0 + e / PR, end - 1);  // rows past the end repeat the last one, masked below
-      const int64_t pg = min(max(table[(int64_t)b * d.table + j / d.page], 0), d.pages - 1);
-      const T* src = cache + (pg * d.page + j % d.page) * wide;
-      u32x4 x = {0, 0, 0, 0};
-      if (c < DC) {
-        if (c < d.dc) x = *reinterpret_cast<const u32x4*>(src + c);
-      } else if (c - DC < d.dr) {
-        x = *reinterpret_cast<const u32x4*>(src + d.dc + c - DC);
-      }
-      *reinterpret_cast<u32x4*>(sk + L::off(e / PR, e % PR)) = x;
-    }
-    __syncthreads();
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the query fragments: no later wait for them drains the tiles
+  if (first < end) load(first, 0);
+  if (first + TK < end) load(first + TK, 1);
+  int buf = 0;
+  for (int k0 = first; k0 < end; k0 += TK, buf ^= 1) {
+    if (k0 + TK < end) vm_wait<IC + IR>();  // this tile is there, the next one in flight
+    else vm_wait<0>();
+    if constexpr (MT > 1) bare_barrier();
     f32x4 s[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) s[i] = zero4();
+    for (int i = 0; i < MT; ++i) {
+      const char* kc = sk + (buf * NW + MT * tw + i) * (SC + SR);
+      f32x4 x[2] = {zero4(), zero4()};  // two chains: each waits for its own result only
+      in_groups<KS, 24 / (int)sizeof(T) / 2, frag>(
+          [&](int t) { return 32 * t < DC ? LC::row16(kc, 0, 32 * t) : LR::row16(kc + SC, 0, 32 * t - DC); },
+          [&](int t, frag a) { x[t & 1] = M16<T>::mma(a, qf[t], x[t & 1]); });
+      s[i] = x[0] + x[1];
+    }
 #pragma unroll
-    for (int t = 0; t < KS; ++t)
+    for (int i = 0; i < MT; ++i) s[i] *= c2;
+    if (k0 + TK > min(end, least)) {
+      const int lim = min(end, seen) - k0 - 16 * MT * tw;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) s[i] = M16<T>::mma(L::row16(sk, 16 * (MT * tw + i), 32 * t), qf[t], s[i]);
-    const int lim = min(end, seen) - k0 - 16 * MT * tw;
-    float top = -INFINITY;
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + tile_row(r) >= lim) s[i][r] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
+    if (__any(top > m + kLag)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      sum *= fade;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n] *= fade;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
+    half p[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[i][r] = 16 * i + tile_row(r) < lim ? s[i][r] * c2 : -INFINITY;
-        top = fmaxf(top, s[i][r]);
-      }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, fade = fast_exp2(m - ref);
-    m = mn;
-    sum *= fade;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n] *= fade;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      half p;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
         const float e = fast_exp2(s[i][r] - ref);
         sum += e;
-        p[r] = (T)e;
+        p[i][r] = (T)e;
       }
+    const char* kc = sk + (buf * NW + MT * tw) * (SC + SR);
+    if constexpr (MT == 1) {
+      in_groups<NT, 16 / (int)sizeof(T), half>([&](int n) { return LC::col16(kc, 0, 16 * n); },
+                                               [&](int n, half a) { acc[n] = M16<T>::mma4(a, p[0], acc[n]); });
+    } else {  // 32 tokens an instruction
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n] = M16<T>::mma4(L::col16(sk, 16 * (MT * tw + i), 16 * n), p, acc[n]);
+      for (int i = 0; i < MT; i += 2) {
+        const frag pp = __builtin_shufflevector(p[i], p[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const char* ka = kc + i * (SC + SR);
+        in_groups<NT, 8 / (int)sizeof(T), frag>(
+            [&](int n) {
+              return __builtin_shufflevector(LC::col16(ka, 0, 16 * n), LC::col16(ka + SC + SR, 0, 16 * n), 0, 1, 2, 3,
+                                             4, 5, 6, 7);
+            },
+            [&](int n, frag a) { acc[n] = M16<T>::mma(a, pp, acc[n]); });
+      }
     }
+    // every read of this buffer has returned before it is loaded again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (MT > 1) bare_barrier();
+    if (k0 + 2 * TK < end) load(k0 + 2 * TK, buf);
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
   // the TW waves of a row group: a common maximum, then sums pairwise through LDS
   if constexpr (TW > 1) {
-    if (lane_id() < 16) {
-      sm[wv][lane_id()] = m;
-      ss[wv][lane_id()] = sum;
+    if (lane < 16) {
+      sm[wv][lane] = m;
+      ss[wv][lane] = sum;
     }
     __syncthreads();
-    const int col = lane_id() & 15;
+    const int col = lane & 15;
     float mm = -INFINITY;
 #pragma unroll
     for (int t = 0; t < TW; ++t) mm = fmaxf(mm, sm[t * MT + rw][col]);
@@ -331,75 +408,119 @@ __global__ __launch_bounds__(256) void latent_split(DecDims d, const T* __restri
       __syncthreads();
       if (tw >= hw && tw < 2 * hw) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[(((tw - hw) * MT + rw) * NT + n) * 64 + lane_id()] = acc[n];
+        for (int n = 0; n < NT; ++n) x[(((tw - hw) * MT + rw) * NT + n) * 64 + lane] = acc[n];
       }
       __syncthreads();
       if (tw < hw) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n] += x[((tw * MT + rw) * NT + n) * 64 + lane_id()];
+        for (int n = 0; n < NT; ++n) acc[n] += x[((tw * MT + rw) * NT + n) * 64 + lane];
       }
     }
   }
   if (tw != 0 || row >= rows) return;
-  const int64_t at = ((int64_t)b * d.splits + sp) * rows + row;
+  float* dst = part + (((int64_t)b * d.splits + sp) * rows + row) * d.dc;
+  float by = 1.f;
+  if (d.splits == 1) {  // nothing to join
+    by = sum == 0.f ? 0.f : 1.f / sum;
+    dst = olat + ((int64_t)b * rows + row) * d.dc;
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int c = 16 * n + tile_row(0);
-    if (c < d.dc) store4(part + at * d.dc + c, acc[n]);
+    if (c < d.dc) store4(dst + c, acc[n] * by);
   }
-  if (lane_id() < 16) {
+  if (lane < 16 && d.splits > 1) {
+    const int64_t at = ((int64_t)b * d.splits + sp) * rows + row;
     stat[2 * at] = m;
     stat[2 * at + 1] = sum;
   }
 }
 
-// o: joins the splits of 16 query tokens of a head and multiplies with the
-// head's value projection, 64 value columns a workgroup.
-template <typename T>
-__global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict__ w_kv, const float* __restrict__ part,
-                                                 const float* __restrict__ stat, const int32_t* __restrict__ kv_lens,
-                                                 T* __restrict__ o) {
-  constexpr int V = 16 / (int)sizeof(T), LD = 512 + V, KS = 32, PARTS = sizeof(T) == 2 ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) T so[PARTS][16 * LD];
-  const int h = blockIdx.x, v0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, rows = d.n * d.H;
-  {
-    const int r = min(r0 + (int)(threadIdx.x >> 4), R - 1), b = r / d.n, rr = r % d.n * d.H + h;
-    const int len = dec_len(d, kv_lens, b), ns = (len + d.chunk - 1) / d.chunk;
-    const int64_t at = (int64_t)b * d.splits * rows + rr;
-    float m = -INFINITY;
-    for (int s = 0; s < ns; ++s) m = fmaxf(m, stat[2 * (at + (int64_t)s * rows)]);
+// o_lat [B n H, dc]: the splits of a row joined.  16 `ways` threads take 64
+// columns of a row, thread group g the splits g, g + ways, ...; the groups join
+// through LDS.  (With few rows and many splits the parts are spread over the card
+// this way: 4 sequences of 32768 tokens, 16 heads: 16 MB of parts.)
+__global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const float* __restrict__ part,
+                                                   const float* __restrict__ stat,
+                                                   const int32_t* __restrict__ kv_lens, float* __restrict__ olat) {
+  __shared__ f32x4 sa[256];
+  __shared__ float sm[256], ss[256];
+  const int per = 16 * ways, cb = (d.dc + 63) / 64, rows = d.n * d.H, tid = threadIdx.x;
+  const int64_t u = (int64_t)blockIdx.x * (256 / per) + tid / per;  // (row, block of columns)
+  const int g = tid % per / 16, c = (int)(u % cb) * 64 + 4 * (tid & 15);
+  const int64_t row = u / cb;
+  const bool ok = row < (int64_t)d.B * rows && c < d.dc;
+  float m = -INFINITY, sum = 0.f;
+  f32x4 x = zero4();
+  if (ok) {
+    const int b = (int)(row / rows);
+    const int ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
+    const int64_t at = (int64_t)b * d.splits * rows + row % rows;
+    for (int s = g; s < ns; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)s * rows)]);
     const float ref = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
-    for (int s = 0; s < ns; ++s)
-      sum += stat[2 * (at + (int64_t)s * rows) + 1] * fast_exp2(stat[2 * (at + (int64_t)s * rows)] - ref);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int c = 4 * (threadIdx.x & 15); c < (d.dc + 31) / 32 * 32; c += 64) {
-      f32x4 x = zero4();
-      if (c < d.dc)
-        for (int s = 0; s < ns; ++s) {
-          const int64_t a = at + (int64_t)s * rows;
-          const float w = fast_exp2(stat[2 * a] - ref) * inv;
-          x += w * *reinterpret_cast<const f32x4*>(part + a * d.dc + c);
-        }
-      store4(&so[0][(threadIdx.x >> 4) * LD + c], x);
-      if constexpr (PARTS == 2) {
+#pragma unroll 4
+    for (int s = g; s < ns; s += ways) {
+      const int64_t a = at + (int64_t)s * rows;
+      const float w = fast_exp2(stat[2 * a] - ref);
+      sum += w * stat[2 * a + 1];
+      x += w * *reinterpret_cast<const f32x4*>(part + a * d.dc + c);
+    }
+  }
+  sa[tid] = x;
+  sm[tid] = m;
+  ss[tid] = sum;
+  __syncthreads();
+  if (!ok || g) return;
+  for (int i = 1; i < ways; ++i) m = fmaxf(m, sm[tid + 16 * i]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  x = zero4();
+  sum = 0.f;
+  for (int i = 0; i < ways; ++i) {
+    const float w = fast_exp2(sm[tid + 16 * i] - ref);
+    sum += w * ss[tid + 16 * i];
+    x += w * sa[tid + 16 * i];
+  }
+  store4(olat + row * d.dc + c, x * (sum == 0.f ? 0.f : 1.f / sum));
+}
+
+// o: 16 query tokens of a head times 64 rows of its value projection a
+// workgroup, 16 a wave.
+template <typename T>
+__global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict__ w_kv, const float* __restrict__ olat,
+                                                 T* __restrict__ o) {
+  constexpr int V = 16 / (int)sizeof(T), LD = 512 + V, PARTS = sizeof(T) == 2 ? 2 : 1, KS = 16;
+  __shared__ __attribute__((aligned(16))) T so[PARTS][16 * LD];
+  const int h = blockIdx.x, v0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, KP = (d.dc + 31) / 32 * 32;
+  const int vr = v0 + 16 * wave_id();
+  const T* w = w_kv + ((int64_t)h * (d.dn + d.dv) + d.dn + min(vr + (lane_id() & 15), d.dv - 1)) * d.dc;
+  typename M16<T>::frag wf[KS];  // all of this wave's weights in flight before the rows are waited for
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] -= (float)(T)x[j];
-        store4(&so[PARTS - 1][(threadIdx.x >> 4) * LD + c], x);
-      }
+  for (int t = 0; t < KS; ++t) {
+    const int k = 32 * t + 8 * (lane_id() >> 4);
+    wf[t] = ld_frag(k < d.dc ? w + k : (const T*)lat_zeros);
+  }
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 16 * (KP / 4); e += 256) {
+    const int r = e / (KP / 4), c = e % (KP / 4) * 4;
+    f32x4 x = zero4();
+    if (c < d.dc && r0 + r < R) x = *reinterpret_cast<const f32x4*>(olat + ((int64_t)(r0 + r) * d.H + h) * d.dc + c);
+    store4(&so[0][r * LD + c], x);
+    if constexpr (PARTS == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] -= (float)(T)x[j];
+      store4(&so[PARTS - 1][r * LD + c], x);
     }
   }
   __syncthreads();
-  const int vr = v0 + 16 * wave_id();
   if (vr >= d.dv) return;
-  const T* w = w_kv + ((int64_t)h * (d.dn + d.dv) + d.dn + min(vr + (lane_id() & 15), d.dv - 1)) * d.dc;
   f32x4 acc = zero4();
-#pragma unroll 4
-  for (int k0 = 0; k0 < d.dc; k0 += KS) {
-    const int k = k0 + 8 * (lane_id() >> 4);
-    const typename M16<T>::frag a = k < d.dc ? ld_frag(w + k) : zero_frag<T>();
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) acc = M16<T>::mma(a, ld_frag(&so[p][(lane_id() & 15) * LD + k]), acc);
+  for (int t = 0; t < KS; ++t) {
+    if (32 * t < KP) {
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p)
+        acc = M16<T>::mma(wf[t], ld_frag(&so[p][(lane_id() & 15) * LD + 32 * t + 8 * (lane_id() >> 4)]), acc);
+    }
   }
   const int r = r0 + tile_col(), v = vr + tile_row(0);
   if (r < R && v < d.dv) store4(o + ((int64_t)r * d.H + h) * d.dv + v, acc);
@@ -437,21 +558,26 @@ static int dec_check(const atomic_latent_decode_args* a) {
   return ATOMIC_OK;
 }
 
-// rows a workgroup of latent_split takes, in tiles of 16
+// Rows a workgroup of latent_split takes, in tiles of 16.
 static int dec_row_tiles(const atomic_latent_decode_args* a) {
   const int rows = a->tokens * a->heads;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 || a->dtype != ATOMIC_BF16 ? 2 : 4;
 }
 
 static DecDims dec_dims(const atomic_latent_decode_args* a) {
   DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, a->table_pages,
             a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]}};
-  const int rt = 16 * dec_row_tiles(a);
+  const int mt = dec_row_tiles(a), rt = 16 * mt, tile = mt == 4 ? 64 : 32;
   d.groups = (d.n * d.H + rt - 1) / rt;
-  // about 512 workgroups if every sequence were as long as its table
-  const int64_t most = (int64_t)d.table * d.page, want = most * d.B * d.groups / 512;
-  const int64_t chunk = want < 64 ? 64 : want > 2048 ? 2048 : want;
-  d.chunk = (int)((chunk + 63) / 64 * 64);
+  // As many workgroups as the card holds at once if every sequence were as long as
+  // its table: two a CU with two waves each in bf16, else one (the tiles' LDS).
+  // Split and join together, us: 64 sequences of up to 8192 tokens, 16 heads: 116 in
+  // splits of 512, 103 of 1024; 4 of 32768: 42 of 256 or 512, 56 of 128; 8 of 4096
+  // with 64 rows: 33 of 128, 36 of 256, 46 of 64; one of 777: 18 of 32, 22 of 128.
+  const int64_t slots = mt == 4 || a->dtype != ATOMIC_BF16 ? 256 : 512;
+  const int64_t most = (int64_t)d.table * d.page, want = (most * d.B * d.groups + slots - 1) / slots;
+  const int64_t chunk = want < tile ? tile : want > kDecChunk ? kDecChunk : want;
+  d.chunk = (int)((chunk + tile - 1) / tile * tile);
   d.splits = (int)((most + d.chunk - 1) / d.chunk);
   return d;
 }
@@ -459,7 +585,11 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 static size_t dec_qa_bytes(const DecDims& d, int dtype) {
   return up256((size_t)d.B * d.n * d.H * (d.dc + d.dr) * (dtype == ATOMIC_BF16 ? 2 : 4));
 }
-static size_t dec_part_rows(const DecDims& d) { return (size_t)d.B * d.splits * d.n * d.H; }
+static size_t dec_olat_bytes(const DecDims& d) { return up256((size_t)d.B * d.n * d.H * d.dc * sizeof(float)); }
+// one split needs no parts
+static size_t dec_part_rows(const DecDims& d) { return d.splits > 1 ? (size_t)d.B * d.splits * d.n * d.H : 0; }
+static size_t dec_stat_bytes(const DecDims& d) { return up256(dec_part_rows(d) * 2 * sizeof(float)); }
+static size_t dec_part_bytes(const DecDims& d) { return dec_part_rows(d) * d.dc * sizeof(float); }
 
 }  // namespace ah
 
@@ -495,22 +625,21 @@ extern "C" int atomic_latent_append(const atomic_latent_append_args* a, const vo
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
   const DecDims d = dec_dims(a);
-  return dec_qa_bytes(d, a->dtype) + up256(dec_part_rows(d) * 8) + dec_part_rows(d) * d.dc * sizeof(float);
+  return dec_qa_bytes(d, a->dtype) + dec_olat_bytes(d) + dec_stat_bytes(d) + dec_part_bytes(d);
 }
 
 template <typename T, int DC>
 static void launch_split(const DecDims& d, int mt, hipStream_t st, const T* qa, const void* cache, const int32_t* table,
-                         const int32_t* kv_lens, float* part, float* stat) {
+                         const int32_t* kv_lens, float* part, float* stat, float* olat) {
   const dim3 grid((unsigned)d.splits, (unsigned)d.groups, (unsigned)d.B);
-  if (mt == 1)
-    hipLaunchKernelGGL((latent_split<T, DC, 1>), grid, dim3(256), 0, st, d, qa, (const T*)cache, table, kv_lens, part,
-                       stat);
-  else if (mt == 2)
-    hipLaunchKernelGGL((latent_split<T, DC, 2>), grid, dim3(256), 0, st, d, qa, (const T*)cache, table, kv_lens, part,
-                       stat);
-  else
-    hipLaunchKernelGGL((latent_split<T, DC, 4>), grid, dim3(256), 0, st, d, qa, (const T*)cache, table, kv_lens, part,
-                       stat);
+  auto go = [&](auto m) {
+    constexpr int NW = decltype(m)::value == 4 ? 4 : 2;
+    hipLaunchKernelGGL((latent_split<T, DC, decltype(m)::value, NW>), grid, dim3(64 * NW), 0, st, d, qa,
+                       (const T*)cache, table, kv_lens, part, stat, olat);
+  };
+  if (mt == 1) go(IntC<1>());
+  else if (mt == 2) go(IntC<2>());
+  else if constexpr (sizeof(T) == 2) go(IntC<4>());
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -530,8 +659,9 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
   auto go = [&](auto t) {
     typedef decltype(t) T;
     T* qa = (T*)workspace;
-    float* stat = (float*)((char*)workspace + dec_qa_bytes(d, a->dtype));
-    float* part = (float*)((char*)stat + up256(dec_part_rows(d) * 8));
+    float* olat = (float*)((char*)workspace + dec_qa_bytes(d, a->dtype));
+    float* stat = (float*)((char*)olat + dec_olat_bytes(d));
+    float* part = (float*)((char*)stat + dec_stat_bytes(d));
     const unsigned rt = (unsigned)((d.B * d.n + 15) / 16);
     int rc = L("latent_absorb", [&] {
       hipLaunchKernelGGL((latent_absorb<T>), dim3((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt), dim3(256), 0,
@@ -540,14 +670,24 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
     if (rc) return rc;
     rc = L("latent_split", [&] {
       if (d.dc <= 256)
-        launch_split<T, 256>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat);
+        launch_split<T, 256>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat, olat);
       else
-        launch_split<T, 512>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat);
+        launch_split<T, 512>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat, olat);
     });
     if (rc) return rc;
+    if (d.splits > 1) {
+      int ways = 1;  // about four splits a thread
+      while (ways < 16 && 4 * ways < d.splits) ways *= 2;
+      const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
+      rc = L("latent_join", [&] {
+        hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, part,
+                           stat, kv_lens, olat);
+      });
+      if (rc) return rc;
+    }
     return L("latent_up", [&] {
       hipLaunchKernelGGL((latent_up<T>), dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
-                         (const T*)w_kv, part, stat, kv_lens, (T*)o);
+                         (const T*)w_kv, olat, (T*)o);
     });
   };
   return a->dtype == ATOMIC_BF16 ? go(bf16()) : go(float());
