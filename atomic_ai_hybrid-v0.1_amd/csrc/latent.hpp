@@ -139,6 +139,42 @@ __device__ __forceinline__ void in_groups(L&& load, U&& use) {
   }
 }
 
+// Rows of a matrix (W elements, `width` of them real) straight to an LTile of ROWS
+// rows, NW waves taking 1 KB each in turn.  The lane's place is fixed: wave w's
+// i-th load covers rows RPI (w + NW i) .. + RPI - 1, which share their swizzle.
+// Rows past `last` repeat it (what lies there is never read and the products are
+// masked); the padding of the width reads the row's first piece (the other operand
+// is zero there, or the product's column is not stored).
+template <typename T, int W, int ROWS, int NW>
+struct RowDma {
+  typedef LTile<T, W> L;
+  static constexpr int RPI = 64 / L::NC, N = ROWS / RPI / NW;
+  static_assert(RPI * L::NC == 64 && N * RPI * NW == ROWS && NW * RPI % 8 == 0, "whole loads");
+  const char* base;  // uniform: row 0
+  int64_t ld;        // bytes a row
+  int r0, cb;        // this lane's row in the first load, byte in the row
+  __device__ __forceinline__ void init(const T* p, int64_t stride, int width) {
+    base = (const char*)p;
+    ld = stride * (int64_t)sizeof(T);
+    r0 = RPI * wave_id() + lane_id() / L::NC;
+    const int c = (lane_id() % L::NC) ^ L::swz(r0);
+    cb = c * L::VEC < width ? 16 * c : 0;
+  }
+  // `dst`: the tile's LDS address
+  __device__ __forceinline__ void load(int k0, int last, uint32_t dst) const {
+    dst += 1024 * wave_id();
+    if (k0 + ROWS - 1 <= last) {
+      const char* p = base + k0 * ld + ((int64_t)r0 * ld + cb);
+#pragma unroll
+      for (int i = 0; i < N; ++i) dma16_raw(p + (int64_t)(i * NW * RPI) * ld, dst + 1024 * NW * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        dma16_raw(base + (int64_t)min(k0 + r0 + i * NW * RPI, last) * ld + cb, dst + 1024 * NW * i);
+    }
+  }
+};
+
 inline int latent_widths_check(int dn, int dr, int dtype) {
   if (dtype != ATOMIC_F32 && dtype != ATOMIC_BF16) return ATOMIC_ERR_DTYPE;
   if (dn < 8 || dn > 128 || dn % 8 || dr < 8 || dr > 64 || dr % 8) return ATOMIC_ERR_SHAPE;

@@ -11,6 +11,8 @@
 // rounded to the operand type for the second product, as its MFMA takes them;
 // everything else (scores, the running maximum and sum, lse, delta, every
 // accumulator) is fp32.
+#include <cfloat>
+
 #include "latent.hpp"
 
 namespace ah {
@@ -85,18 +87,22 @@ __device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) /
 __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3); }
 
 // ------------------------------------------------------------------ forward
-// 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens.
+// 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens (32
+// in fp32).  Two tiles in LDS: while one is computed with, the next is loaded
+// straight to LDS; one barrier a tile.  Two workgroups a CU (80 KB of LDS and 256
+// registers a lane each), so that one's MFMAs run beside the other's softmax.
 template <typename T, int DN, int DR, int DV>
-__global__ __launch_bounds__(256) void latent_fwd(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
-                                                  const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
-                                                  const int32_t* __restrict__ kv_lens, T* __restrict__ o,
-                                                  float* __restrict__ lse) {
-  constexpr int D = DN + DR, KS = D / 16, NT = DV / 32, TK = 64;
-  typedef LTile<T, D> LK;
+__global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
+                                                     const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
+                                                     const int32_t* __restrict__ kv_lens, T* __restrict__ o,
+                                                     float* __restrict__ lse) {
+  constexpr int KN = DN / 16, KS = (DN + DR) / 16, NT = DV / 32, TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
+  typedef LTile<T, DN> LN;
+  typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LV;
   typedef typename M32<T>::frag frag;
-  __shared__ __attribute__((aligned(1024))) char sk[TK * LK::ROWB];
-  __shared__ __attribute__((aligned(1024))) char sv[TK * LV::ROWB];
+  constexpr int OR = TK * LN::ROWB, OV = OR + TK * LR::ROWB, STAGE = OV + TK * LV::ROWB;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
   blk = d.blocks - 1 - blk;  // with causal the long rows first
@@ -109,64 +115,82 @@ __global__ __launch_bounds__(256) void latent_fwd(LatDims d, const T* __restrict
   if (last < 128 * blk) end = 0;
   const T* qr = q + b * d.qs[0] + (int64_t)max(min(row, ql - 1), 0) * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
-  const T* pb = kpe + b * d.ps[0];
+  RowDma<T, DN, TK, 4> dn;
+  RowDma<T, DR, TK, 4> dr;
+  RowDma<T, DV, TK, 4> dv;
+  dn.init(kb, d.ks[1], d.dn);
+  dr.init(kpe + b * d.ps[0], d.ps[1], d.dr);
+  dv.init(kb + d.dn, d.ks[1], d.dv);
   frag qf[KS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   f32x16 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
-  const float c2 = d.scale * kLog2e;
-  float m = -INFINITY, sum = 0.f;  // running maximum (of c2 times the scores) and this lane's part of the sum
-  for (int k0 = 0; k0 < end; k0 += TK) {
-    __syncthreads();
-    stage_tile<T, TK, DN, DR, 256>(sk, k0, kl - 1, kb, d.ks[1], d.dn, pb, d.ps[1], d.dr);
-    stage_tile<T, TK, DV, 0, 256>(sv, k0, kl - 1, kb + d.dn, d.ks[1], d.dv, (const T*)nullptr, 0, 0);
-    __syncthreads();
+  // (a scale of zero as the smallest number: a masked score stays infinite)
+  const float c2 = d.scale == 0.f ? FLT_MIN : d.scale * kLog2e;
+  float m = -INFINITY, sum = 0.f;  // reference (of c2 times the scores, see kLag) and this lane's part of the sum
+  const uint32_t l0 = lds_addr(lds);
+  auto load = [&](int k0, int buf) {
+    const uint32_t at = l0 + buf * STAGE;
+    dn.load(k0, kl - 1, at);
+    dr.load(k0, kl - 1, at + OR);
+    dv.load(k0, kl - 1, at + OV);
+  };
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the query: no later wait for it drains the tiles
+  if (end > 0) load(0, 0);
+  int buf = 0;
+  for (int k0 = 0; k0 < end; k0 += TK, buf ^= 1) {
+    vm_wait<0>();
+    bare_barrier();  // the tile is there, and nobody reads the other one any more
+    if (k0 + TK < end) load(k0 + TK, buf ^ 1);
     if (w0 >= ql || (d.causal && k0 > w0 + 31 + off)) continue;  // nothing visible to this wave
-    f32x16 s[2] = {zero16(), zero16()};
+    const char* sk = lds + buf * STAGE;
+    f32x16 s[NS];
 #pragma unroll
-    for (int t = 0; t < KS; ++t) {
-      s[0] = M32<T>::mma(LK::row(sk, 0, 16 * t), qf[t], s[0]);
-      s[1] = M32<T>::mma(LK::row(sk, 32, 16 * t), qf[t], s[1]);
-    }
+    for (int i = 0; i < NS; ++i) s[i] = zero16();
+    in_groups<KS * NS, 4, frag>(
+        [&](int j) {
+          const int t = j / NS, i = j % NS;
+          return t < KN ? LN::row(sk, 32 * i, 16 * t) : LR::row(sk + OR, 32 * i, 16 * (t - KN));
+        },
+        [&](int j, frag a) { s[j % NS] = M32<T>::mma(a, qf[j / NS], s[j % NS]); });
     if (k0 + TK > kl || (d.causal && k0 + TK - 1 > w0 + off)) {
       const int seen = min(kl, d.causal ? row + off + 1 : kl) - k0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (32 * i + reg_row(r) >= seen) s[i][r] = -INFINITY;
+          if (32 * i + reg_row(r) >= seen) s[i][r] = c2 < 0.f ? INFINITY : -INFINITY;
     }
-    float top = -INFINITY;
+    float top = s[0][0] * c2;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r] * c2);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float mn = fmaxf(m, top);
-    const float ref = mn == -INFINITY ? 0.f : mn;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
-    const float fade = fast_exp2(m - ref);
-    m = mn;
-    sum *= fade;
+    if (__any(top > m + kLag)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      sum *= fade;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[n][r] *= fade;
+        for (int r = 0; r < 16; ++r) acc[n][r] *= fade;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
+    frag p[2 * NS];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NS; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[i][r] = fast_exp2(s[i][r] * c2 - ref);
         sum += s[i][r];
       }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const frag p = pack_frag<T>(s[i], t);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n] = M32<T>::mma(LV::col(sv, 32 * i + 16 * t, 32 * n), p, acc[n]);
-      }
+      p[2 * i] = pack_frag<T>(s[i], 0);
+      p[2 * i + 1] = pack_frag<T>(s[i], 1);
+    }
+    in_groups<2 * NS * NT, 4, frag>([&](int j) { return LV::col(sk + OV, 16 * (j / NT), 32 * (j % NT)); },
+                                    [&](int j, frag a) { acc[j % NT] = M32<T>::mma(a, p[j / NT], acc[j % NT]); });
   }
   if (row >= d.T) return;
   sum += __shfl_xor(sum, 32);
