@@ -35,38 +35,8 @@ __device__ __forceinline__ int clamp_len(const int32_t* p, int b, int most) {
   return p ? min(max(p[b], 0), most) : most;
 }
 
-// Rows [r0, r0 + R) of a matrix as two spans of pieces (w0 elements from src0,
-// then at column W0 w1 elements from src1) into an LDS tile; rows past `last`
-// repeat it (their products are masked, and padding rows are never read), the
-// padding of the widths is zero.
-template <typename T, int R, int W0, int W1, int NTH>
-__device__ __forceinline__ void stage_tile(char* dst, int r0, int last, const T* src0, int64_t ld0, int w0,
-                                           const T* src1, int64_t ld1, int w1) {
-  typedef LTile<T, W0 + W1> L;
-  constexpr int V = L::VEC, PR = (W0 + W1) / V, NP = R * PR, IT = (NP + NTH - 1) / NTH;
-  u32x4 tmp[IT];
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int e = threadIdx.x + NTH * i, r = e / PR, c = (e % PR) * V;
-    u32x4 x = {0, 0, 0, 0};
-    if (NP % NTH == 0 || e < NP) {
-      const int64_t row = min(r0 + r, last);
-      if (W1 == 0 || c < W0) {
-        if (c < w0) x = *reinterpret_cast<const u32x4*>(src0 + row * ld0 + c);
-      } else if (c - W0 < w1) {
-        x = *reinterpret_cast<const u32x4*>(src1 + row * ld1 + c - W0);
-      }
-    }
-    tmp[i] = x;
-  }
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int e = threadIdx.x + NTH * i;
-    if (NP % NTH == 0 || e < NP) *reinterpret_cast<u32x4*>(dst + L::off(e / PR, e % PR)) = tmp[i];
-  }
-}
-
-// The same split row as register fragments: this lane's row at src0 / src1.
+// A row of two spans (w0 elements from src0, then from element W0 on w1 from src1)
+// as register fragments, padded with zeros: this lane's row at src0 / src1.
 template <typename T, int W0, int W1>
 __device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) / 16], const T* src0, int w0,
                                           const T* src1, int w1) {
@@ -211,12 +181,12 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
 }
 
 // ----------------------------------------------------------------- backward
-// delta [B, H, T]: sixteen lanes a row.
+// stat: delta and lse in powers of two, each [B, H, T]: sixteen lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restrict__ o, const T* __restrict__ dout,
-                                                    float* __restrict__ delta) {
-  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, t, h)
-  if (i >= (int64_t)d.B * d.T * d.H) return;
+                                                    const float* __restrict__ lse, float* __restrict__ stat) {
+  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)d.B * d.T * d.H;  // (b, t, h)
+  if (i >= rows) return;
   const int h = (int)(i % d.H), t = (int)(i / d.H % d.T), b = (int)(i / d.H / d.T);
   const T* g = dout + b * d.gs[0] + t * d.gs[1] + h * d.gs[2];
   float s = 0.f;
@@ -229,22 +199,28 @@ __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restri
   }
 #pragma unroll
   for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
-  if ((threadIdx.x & 15) == 0) delta[((int64_t)b * d.H + h) * d.T + t] = s;
+  if ((threadIdx.x & 15) == 0) {
+    const int64_t at = ((int64_t)b * d.H + h) * d.T + t;
+    stat[at] = s;
+    stat[rows + at] = lse[at] * kLog2e;
+  }
 }
 
-// dq: 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens.
+// dq: 128 query rows of a head a workgroup, 32 a wave, against tiles of tokens,
+// staged as in the forward.
 template <typename T, int DN, int DR, int DV>
-__global__ __launch_bounds__(256) void latent_bwd_dq(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
-                                                     const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
-                                                     const int32_t* __restrict__ kv_lens,
-                                                     const float* __restrict__ lse, const float* __restrict__ delta,
-                                                     const T* __restrict__ dout, T* __restrict__ dq) {
-  constexpr int D = DN + DR, KS = D / 16, VS = DV / 16, NT = D / 32, TK = 64;
-  typedef LTile<T, D> LK;
+__global__ __launch_bounds__(256, 1) void latent_bwd_dq(
+    LatDims d, const T* __restrict__ q, const T* __restrict__ kv, const T* __restrict__ kpe,
+    const int32_t* __restrict__ q_lens, const int32_t* __restrict__ kv_lens, const float* __restrict__ stat,
+    const T* __restrict__ dout, T* __restrict__ dq) {
+  constexpr int KN = DN / 16, KS = (DN + DR) / 16, VS = DV / 16, NN = DN / 32, NT = (DN + DR) / 32;
+  constexpr int TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
+  typedef LTile<T, DN> LN;
+  typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LV;
   typedef typename M32<T>::frag frag;
-  __shared__ __attribute__((aligned(1024))) char sk[TK * LK::ROWB];
-  __shared__ __attribute__((aligned(1024))) char sv[TK * LV::ROWB];
+  constexpr int OR = TK * LN::ROWB, OV = OR + TK * LR::ROWB, STAGE = OV + TK * LV::ROWB;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
   blk = d.blocks - 1 - blk;
@@ -258,42 +234,65 @@ __global__ __launch_bounds__(256) void latent_bwd_dq(LatDims d, const T* __restr
   const int rowc = max(min(row, ql - 1), 0);
   const T* qr = q + b * d.qs[0] + (int64_t)rowc * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
-  const T* pb = kpe + b * d.ps[0];
+  RowDma<T, DN, TK, 4> dn;
+  RowDma<T, DR, TK, 4> dr;
+  RowDma<T, DV, TK, 4> dv;
+  dn.init(kb, d.ks[1], d.dn);
+  dr.init(kpe + b * d.ps[0], d.ps[1], d.dr);
+  dv.init(kb + d.dn, d.ks[1], d.dv);
   frag qf[KS], gf[VS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   row_frags<T, DV, 0>(gf, dout + b * d.gs[0] + (int64_t)rowc * d.gs[1] + h * d.gs[2], d.dv, (const T*)nullptr, 0);
-  const float l2 = lse[((int64_t)b * d.H + h) * d.T + rowc] * kLog2e;
-  const float dl = delta[((int64_t)b * d.H + h) * d.T + rowc];
+  const int64_t at = ((int64_t)b * d.H + h) * d.T + rowc;
+  const float dl = stat[at], l2 = stat[(int64_t)d.B * d.H * d.T + at];
   f32x16 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
   const float c2 = d.scale * kLog2e;
-  for (int k0 = 0; k0 < end; k0 += TK) {
-    __syncthreads();
-    stage_tile<T, TK, DN, DR, 256>(sk, k0, kl - 1, kb, d.ks[1], d.dn, pb, d.ps[1], d.dr);
-    stage_tile<T, TK, DV, 0, 256>(sv, k0, kl - 1, kb + d.dn, d.ks[1], d.dv, (const T*)nullptr, 0, 0);
-    __syncthreads();
+  const uint32_t l0 = lds_addr(lds);
+  auto load = [&](int k0, int buf) {
+    const uint32_t at = l0 + buf * STAGE;
+    dn.load(k0, kl - 1, at);
+    dr.load(k0, kl - 1, at + OR);
+    dv.load(k0, kl - 1, at + OV);
+  };
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  if (end > 0) load(0, 0);
+  int buf = 0;
+  for (int k0 = 0; k0 < end; k0 += TK, buf ^= 1) {
+    vm_wait<0>();
+    bare_barrier();
+    if (k0 + TK < end) load(k0 + TK, buf ^ 1);
+    const char* sk = lds + buf * STAGE;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NS; ++i) {
       const int t0 = k0 + 32 * i;
       if (w0 >= ql || t0 >= kl || (d.causal && t0 > w0 + 31 + off)) break;
       f32x16 s = zero16(), g = zero16();
+      in_groups<KS + VS, 4, frag>(
+          [&](int j) {
+            return j < KN ? LN::row(sk, 32 * i, 16 * j)
+                          : j < KS ? LR::row(sk + OR, 32 * i, 16 * (j - KN)) : LV::row(sk + OV, 32 * i, 16 * (j - KS));
+          },
+          [&](int j, frag a) {
+            if (j < KS) s = M32<T>::mma(a, qf[j], s);
+            else g = M32<T>::mma(a, gf[j - KS], g);
+          });
 #pragma unroll
-      for (int t = 0; t < KS; ++t) s = M32<T>::mma(LK::row(sk, 32 * i, 16 * t), qf[t], s);
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(s[r] * c2 - l2) * (g[r] - dl);
+      if (t0 + 32 > kl || (d.causal && t0 + 31 > w0 + off)) {
+        const int seen = min(kl, d.causal ? row + off + 1 : kl) - t0;
 #pragma unroll
-      for (int t = 0; t < VS; ++t) g = M32<T>::mma(LV::row(sv, 32 * i, 16 * t), gf[t], g);
-      const int seen = min(kl, d.causal ? row + off + 1 : kl) - t0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = fast_exp2(s[r] * c2 - l2);
-        s[r] = reg_row(r) < seen ? p * (g[r] - dl) : 0.f;
+        for (int r = 0; r < 16; ++r)
+          if (reg_row(r) >= seen) s[r] = 0.f;
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const frag ds = pack_frag<T>(s, t);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n] = M32<T>::mma(LK::col(sk, 32 * i + 16 * t, 32 * n), ds, acc[n]);
-      }
+      const frag ds[2] = {pack_frag<T>(s, 0), pack_frag<T>(s, 1)};
+      in_groups<2 * NT, 4, frag>(
+          [&](int j) {
+            const int t = j / NT, n = j % NT;
+            return n < NN ? LN::col(sk, 32 * i + 16 * t, 32 * n) : LR::col(sk + OR, 32 * i + 16 * t, 32 * (n - NN));
+          },
+          [&](int j, frag a) { acc[j % NT] = M32<T>::mma(a, ds[j / NT], acc[j % NT]); });
     }
   }
   if (row >= d.T) return;
@@ -315,22 +314,23 @@ __global__ __launch_bounds__(256) void latent_bwd_dq(LatDims d, const T* __restr
 }
 
 // dk, dv: 128 tokens of a head a workgroup, 32 a wave (their keys, values and
-// gradient accumulators in registers), against tiles of 32 query rows.  The
+// gradient accumulators in registers: one wave a SIMD), against tiles of query
+// rows staged as the forward's tokens are, with delta and lse beside them.  The
 // rotated key's gradient leaves as this head's part, fp32 [B, H, S, dr].
 template <typename T, int DN, int DR, int DV>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
                                                          const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
                                                          const int32_t* __restrict__ kv_lens,
-                                                         const float* __restrict__ lse,
-                                                         const float* __restrict__ delta, const T* __restrict__ dout,
+                                                         const float* __restrict__ stat, const T* __restrict__ dout,
                                                          T* __restrict__ dkv, float* __restrict__ dkp) {
-  constexpr int D = DN + DR, KS = D / 16, VS = DV / 16, NK = D / 32, NV = DV / 32, TQ = 32;
-  typedef LTile<T, D> LQ;
+  constexpr int KN = DN / 16, KS = (DN + DR) / 16, VS = DV / 16, NN = DN / 32, NK = (DN + DR) / 32, NV = DV / 32;
+  constexpr int TQ = sizeof(T) == 2 ? 64 : 32, NS = TQ / 32;
+  typedef LTile<T, DN> LN;
+  typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LG;
   typedef typename M32<T>::frag frag;
-  __shared__ __attribute__((aligned(1024))) char sq[TQ * LQ::ROWB];
-  __shared__ __attribute__((aligned(1024))) char sg[TQ * LG::ROWB];
-  __shared__ __attribute__((aligned(16))) float sl[TQ], sd[TQ];
+  constexpr int OR = TQ * LN::ROWB, OG = OR + TQ * LR::ROWB, OS = OG + TQ * LG::ROWB, STAGE = OS + 512;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
   const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
@@ -340,11 +340,26 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   int first = 0;  // the first query that sees any of the workgroup's tokens
   if (d.causal) first = max(0, 128 * blk - off);
   if (128 * blk >= kl) first = ql;
+  first &= ~(TQ - 1);
   const T* qb = q + b * d.qs[0] + h * d.qs[2];
   const T* gb = dout + b * d.gs[0] + h * d.gs[2];
   const T* kr = kv + b * d.ks[0] + (int64_t)tokc * d.ks[1] + h * d.ks[2];
-  const float* lb = lse + ((int64_t)b * d.H + h) * d.T;
-  const float* db = delta + ((int64_t)b * d.H + h) * d.T;
+  RowDma<T, DN, TQ, 4> dn;
+  RowDma<T, DR, TQ, 4> dr;
+  RowDma<T, DV, TQ, 4> dg;
+  dn.init(qb, d.qs[1], d.dn);
+  dr.init(qb + d.dn, d.qs[1], d.dr);
+  dg.init(gb, d.gs[1], d.dv);
+  // wave 0 brings delta, wave 1 lse (64 rows; an fp32 tile uses half of them)
+  const float* sb = stat + (wave_id() & 1 ? (int64_t)d.B * d.H * d.T : 0) + ((int64_t)b * d.H + h) * d.T;
+  const uint32_t l0 = lds_addr(lds);
+  auto load = [&](int r0, int buf) {
+    const uint32_t at = l0 + buf * STAGE;
+    dn.load(r0, ql - 1, at);
+    dr.load(r0, ql - 1, at + OR);
+    dg.load(r0, ql - 1, at + OG);
+    if (wave_id() < 2) dma4_raw(sb + min(r0 + lane_id(), ql - 1), at + OS + 256 * wave_id());
+  };
   frag kf[KS], vf[VS];
   row_frags<T, DN, DR>(kf, kr, d.dn, kpe + b * d.ps[0] + (int64_t)tokc * d.ps[1], d.dr);
   row_frags<T, DV, 0>(vf, kr + d.dn, d.dv, (const T*)nullptr, 0);
@@ -354,36 +369,59 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
 #pragma unroll
   for (int n = 0; n < NV; ++n) av[n] = zero16();
   const float c2 = d.scale * kLog2e;
-  for (int r0 = first & ~(TQ - 1); r0 < ql; r0 += TQ) {
-    __syncthreads();
-    stage_tile<T, TQ, DN, DR, 256>(sq, r0, ql - 1, qb, d.qs[1], d.dn, qb + d.dn, d.qs[1], d.dr);
-    stage_tile<T, TQ, DV, 0, 256>(sg, r0, ql - 1, gb, d.gs[1], d.dv, (const T*)nullptr, 0, 0);
-    if (threadIdx.x < TQ) {
-      sl[threadIdx.x] = lb[min(r0 + (int)threadIdx.x, ql - 1)] * kLog2e;
-      sd[threadIdx.x] = db[min(r0 + (int)threadIdx.x, ql - 1)];
-    }
-    __syncthreads();
-    if (w0 >= kl || (d.causal && w0 > r0 + TQ - 1 + off)) continue;
-    f32x16 s = zero16(), g = zero16();
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  if (first < ql) load(first, 0);
+  int buf = 0;
+  for (int q0 = first; q0 < ql; q0 += TQ, buf ^= 1) {
+    vm_wait<0>();
+    bare_barrier();
+    if (q0 + TQ < ql) load(q0 + TQ, buf ^ 1);
+    const char* sq = lds + buf * STAGE;
+    const float *sd = (const float*)(sq + OS), *sl = sd + 64;
 #pragma unroll
-    for (int t = 0; t < KS; ++t) s = M32<T>::mma(LQ::row(sq, 0, 16 * t), kf[t], s);
+    for (int i = 0; i < NS; ++i) {
+      const int r0 = q0 + 32 * i;
+      if (w0 >= kl || r0 >= ql || (d.causal && w0 > r0 + 31 + off)) continue;
+      f32x16 s = zero16(), g = zero16();
+      in_groups<KS + VS, 4, frag>(
+          [&](int j) {
+            return j < KN ? LN::row(sq, 32 * i, 16 * j)
+                          : j < KS ? LR::row(sq + OR, 32 * i, 16 * (j - KN)) : LG::row(sq + OG, 32 * i, 16 * (j - KS));
+          },
+          [&](int j, frag a) {
+            if (j < KS) s = M32<T>::mma(a, kf[j], s);
+            else g = M32<T>::mma(a, vf[j - KS], g);
+          });
 #pragma unroll
-    for (int t = 0; t < VS; ++t) g = M32<T>::mma(LG::row(sg, 0, 16 * t), vf[t], g);
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(sl + 32 * i + reg_row(r));
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + 32 * i + reg_row(r));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int i = reg_row(r), at = r0 + i;
-      const bool ok = at < ql && tok < kl && (!d.causal || tok <= at + off);
-      const float p = fast_exp2(s[r] * c2 - sl[i]);
-      s[r] = ok ? p : 0.f;
-      g[r] = ok ? p * (g[r] - sd[i]) : 0.f;
-    }
+        for (int j = 0; j < 4; ++j) {
+          const float p = fast_exp2(s[r + j] * c2 - l4[j]);
+          s[r + j] = p;
+          g[r + j] = p * (g[r + j] - d4[j]);
+        }
+      }
+      if (r0 + 32 > ql || w0 + 32 > kl || (d.causal && w0 + 31 > r0 + off)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const frag p = pack_frag<T>(s, t), ds = pack_frag<T>(g, t);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) av[n] = M32<T>::mma(LG::col(sg, 16 * t, 32 * n), p, av[n]);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) ak[n] = M32<T>::mma(LQ::col(sq, 16 * t, 32 * n), ds, ak[n]);
+        for (int r = 0; r < 16; ++r) {
+          const int at = r0 + reg_row(r);
+          if (at >= ql || tok >= kl || (d.causal && tok > at + off)) s[r] = g[r] = 0.f;
+        }
+      }
+      const frag p[2] = {pack_frag<T>(s, 0), pack_frag<T>(s, 1)}, ds[2] = {pack_frag<T>(g, 0), pack_frag<T>(g, 1)};
+      in_groups<2 * (NV + NK), 4, frag>(
+          [&](int j) {
+            const int t = j / (NV + NK), n = j % (NV + NK), r = 32 * i + 16 * t;
+            return n < NV ? LG::col(sq + OG, r, 32 * n)
+                          : n < NV + NN ? LN::col(sq, r, 32 * (n - NV)) : LR::col(sq + OR, r, 32 * (n - NV - NN));
+          },
+          [&](int j, frag a) {
+            const int t = j / (NV + NK), n = j % (NV + NK);
+            if (n < NV) av[n] = M32<T>::mma(a, p[t], av[n]);
+            else ak[n - NV] = M32<T>::mma(a, ds[t], ak[n - NV]);
+          });
     }
   }
   if (tok >= d.S) return;
@@ -467,8 +505,8 @@ static int lat_dispatch(const atomic_latent_args* a, F&& f) {
   return small ? f(float(), Widths<64, 32, 64>()) : f(float(), Widths<128, 64, 128>());
 }
 
-static size_t lat_delta_bytes(const atomic_latent_args* a) {
-  return ((size_t)a->batch * a->heads * a->tq * sizeof(float) + 255) / 256 * 256;
+static size_t lat_stat_bytes(const atomic_latent_args* a) {
+  return ((size_t)a->batch * a->heads * a->tq * 2 * sizeof(float) + 255) / 256 * 256;
 }
 
 }  // namespace ah
@@ -496,7 +534,7 @@ extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, con
 
 extern "C" size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a) {
   if (lat_check(a) != ATOMIC_OK) return 0;
-  return lat_delta_bytes(a) + (size_t)a->batch * a->heads * a->tk * a->dr * sizeof(float);
+  return lat_stat_bytes(a) + (size_t)a->batch * a->heads * a->tk * a->dr * sizeof(float);
 }
 
 extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
@@ -509,8 +547,8 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
   if (!workspace || workspace_bytes < atomic_latent_bwd_workspace_size(a) || !aligned16({workspace}))
     return ATOMIC_ERR_WORKSPACE;
   ws_tag_clobber(workspace, atomic_latent_bwd_workspace_size(a));
-  float* delta = (float*)workspace;
-  float* dkp = (float*)((char*)workspace + lat_delta_bytes(a));
+  float* stat = (float*)workspace;
+  float* dkp = (float*)((char*)workspace + lat_stat_bytes(a));
   const hipStream_t st = (hipStream_t)stream;
   Launch L{a->profile, st};
   return lat_dispatch(a, [&](auto t, auto w) {
@@ -520,20 +558,20 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
     const int64_t rows = (int64_t)d.B * d.T * d.H;
     int rc = L("latent_delta", [&] {
       hipLaunchKernelGGL((latent_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, d, (const T*)o,
-                         (const T*)dout, delta);
+                         (const T*)dout, lse, stat);
     });
     if (rc) return rc;
     d.blocks = (d.S + 127) / 128;
     rc = L("latent_bwd_dkv", [&] {
       hipLaunchKernelGGL((latent_bwd_dkv<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
-                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, lse, delta,
+                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
                          (const T*)dout, (T*)dkv, dkp);
     });
     if (rc) return rc;
     d.blocks = (d.T + 127) / 128;
     rc = L("latent_bwd_dq", [&] {
       hipLaunchKernelGGL((latent_bwd_dq<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
-                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, lse, delta,
+                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
                          (const T*)dout, (T*)dq);
     });
     if (rc) return rc;
