@@ -71,18 +71,23 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // A tile of rows of W elements in LDS as 16-byte pieces, piece c of row r at
-// place c ^ swz(r): eight consecutive rows read at one piece, and four
-// consecutive rows read at a pair of pieces (the transposed reads), fall on
-// distinct banks.
-template <typename T, int W>
+// place c ^ swz(r).  With FR rows a fragment (32 or 16), the row reads (16 bytes a
+// lane) and the transposed reads (8 bytes a lane) both run without bank conflicts
+// (256 bytes a clock over 64 banks; measured one wave's pattern each: rows of 256
+// bytes and more want all four bits, 16-row fragments in their own order; with
+// only 128 bytes swizzled the row reads took twice as long).
+template <typename T, int W, int FR = 32>
 struct LTile {
   static constexpr int VEC = 16 / (int)sizeof(T);
   static constexpr int NC = (W / VEC + 7) / 8 * 8;
   static constexpr int ROWB = NC * 16;
-  static __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+  static __device__ __forceinline__ int swz(int r) {
+    return NC == 8 ? (r >> 1) & 7 : FR == 16 ? r & 15 : ((r & 3) << 2) | ((r >> 2) & 3);
+  }
   // (the piece's upper bits apart: they become the read's immediate offset)
   static __device__ __forceinline__ int off(int r, int c) {
-    return r * ROWB + (((c & 7) ^ swz(r)) << 4) + ((c & ~7) << 4);
+    constexpr int M = NC == 8 ? 7 : 15;
+    return r * ROWB + (((c & M) ^ swz(r)) << 4) + ((c & ~M) << 4);
   }
   // row operand: lane (l % 32) holds row r0 + l % 32, elements k0 + 8 (l / 32) .. + 7
   static __device__ __forceinline__ typename M32<T>::frag row(const char* s, int r0, int k0) {
@@ -140,37 +145,40 @@ __device__ __forceinline__ void in_groups(L&& load, U&& use) {
 }
 
 // Rows of a matrix (W elements, `width` of them real) straight to an LTile of ROWS
-// rows, NW waves taking 1 KB each in turn.  The lane's place is fixed: wave w's
-// i-th load covers rows RPI (w + NW i) .. + RPI - 1, which share their swizzle.
-// Rows past `last` repeat it (what lies there is never read and the products are
-// masked); the padding of the width reads the row's first piece (the other operand
-// is zero there, or the product's column is not stored).
+// rows, NW waves taking 1 KB each in turn: wave w's i-th load covers the rows
+// RPI (w + NW i) .. + RPI - 1.  Rows past `last` repeat it (what lies there is never
+// read and the products are masked); the padding of the width reads the row's first
+// piece (the other operand is zero there, or the product's column is not stored).
 template <typename T, int W, int ROWS, int NW>
 struct RowDma {
   typedef LTile<T, W> L;
-  static constexpr int RPI = 64 / L::NC, N = ROWS / RPI / NW;
-  static_assert(RPI * L::NC == 64 && N * RPI * NW == ROWS && NW * RPI % 8 == 0, "whole loads");
+  static constexpr int RPI = 64 / L::NC, N = ROWS / RPI / NW, STEP = NW * RPI;
+  static constexpr int NZ = STEP >= 16 ? 1 : 16 / STEP;  // the swizzle repeats every 16 rows
+  static_assert(RPI * L::NC == 64 && N * STEP == ROWS && (STEP >= 16 || 16 % STEP == 0), "whole loads");
   const char* base;  // uniform: row 0
   int64_t ld;        // bytes a row
-  int r0, cb;        // this lane's row in the first load, byte in the row
+  int r0, cb[NZ];    // this lane's row in the first load, byte in the row
   __device__ __forceinline__ void init(const T* p, int64_t stride, int width) {
     base = (const char*)p;
     ld = stride * (int64_t)sizeof(T);
     r0 = RPI * wave_id() + lane_id() / L::NC;
-    const int c = (lane_id() % L::NC) ^ L::swz(r0);
-    cb = c * L::VEC < width ? 16 * c : 0;
+#pragma unroll
+    for (int z = 0; z < NZ; ++z) {
+      const int c = (lane_id() % L::NC) ^ L::swz(r0 + z * STEP);
+      cb[z] = c * L::VEC < width ? 16 * c : 0;
+    }
   }
   // `dst`: the tile's LDS address
   __device__ __forceinline__ void load(int k0, int last, uint32_t dst) const {
     dst += 1024 * wave_id();
     if (k0 + ROWS - 1 <= last) {
-      const char* p = base + k0 * ld + ((int64_t)r0 * ld + cb);
+      const char* p = base + k0 * ld + (int64_t)r0 * ld;
 #pragma unroll
-      for (int i = 0; i < N; ++i) dma16_raw(p + (int64_t)(i * NW * RPI) * ld, dst + 1024 * NW * i);
+      for (int i = 0; i < N; ++i) dma16_raw(p + ((int64_t)(i * STEP) * ld + cb[i % NZ]), dst + 1024 * NW * i);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        dma16_raw(base + (int64_t)min(k0 + r0 + i * NW * RPI, last) * ld + cb, dst + 1024 * NW * i);
+        dma16_raw(base + ((int64_t)min(k0 + r0 + i * STEP, last) * ld + cb[i % NZ]), dst + 1024 * NW * i);
     }
   }
 };

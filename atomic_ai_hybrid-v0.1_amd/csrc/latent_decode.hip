@@ -187,8 +187,8 @@ template <> struct M16<float> {
   }
 };
 template <typename T, int W>
-struct DTile : LTile<T, W> {
-  typedef LTile<T, W> L;
+struct DTile : LTile<T, W, 16> {
+  typedef LTile<T, W, 16> L;
   static __device__ __forceinline__ typename M16<T>::frag row16(const char* s, int r0, int k0) {
     const int l = lane_id(), r = r0 + (l & 15), k = k0 + 8 * (l >> 4);
     if constexpr (sizeof(T) == 2) {
@@ -264,17 +264,18 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
   }
   __syncthreads();  // the page numbers are there
   const uint32_t lds0 = lds_addr(sk);
-  // Byte offsets of this lane's piece in a row, by the row's swizzle.  The padding
-  // of a width reads the row's first piece instead: the query has zeros there.
   constexpr int RL = PC >= 64 ? PC / 64 : 1;  // loads a row
-  uint32_t oc[RL][8];
+  // Byte offset of this lane's piece in load l of a row with swizzle z.  The padding
+  // of a width reads the row's first piece instead: the query has zeros there.
+  auto piece = [&](int l, int z) {
+    const int c = 64 * l + (lane ^ z);
+    return c * V < d.dc ? 16 * c : 0;
+  };
+  uint32_t oc[16];
+  if constexpr (RL == 1) {
 #pragma unroll
-  for (int l = 0; l < RL; ++l)
-#pragma unroll
-    for (int z = 0; z < 8; ++z) {
-      const int c = 64 * l + (lane ^ z);
-      oc[l][z] = c * V < d.dc ? 16 * c : 0;
-    }
+    for (int z = 0; z < 16; ++z) oc[z] = piece(0, z);
+  }
   // this wave's 16 tokens of the tile at k0 into buffer `buf`; tokens past the end repeat the last one (masked below)
   auto load = [&](int k0, int buf) {
     const int j = min(k0 + 16 * wv + (lane & 15), end - 1), pg = j / d.page;
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
         const int r = i / RL;
         const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, r) << 32 |
                              (uint32_t)__builtin_amdgcn_readlane(lo, r);
-        dma16_raw_s(row, oc[i % RL][LC::swz(r)], dst + 1024 * i);
+        dma16_raw_s(row, RL == 1 ? oc[r] : piece(i % RL, r), dst + 1024 * i);  // (swz(r) = r)
       } else {
         const int r = (64 * i + lane) / PC;
         const uint64_t row = (uint64_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r);
