@@ -181,13 +181,27 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
 }
 
 // ----------------------------------------------------------------- backward
-// stat: delta and lse in powers of two, each [B, H, T]: sixteen lanes a row.
+// Rows of delta and lse a head: whole tiles, so that the rows past the last query
+// can hold an lse of infinity (every p of theirs is zero).
+__host__ __device__ inline int64_t stat_rows(int T) { return (int64_t)(T + 63) / 64 * 64; }
+
+// stat: delta and lse in powers of two, each [B, H, stat_rows]: sixteen lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restrict__ o, const T* __restrict__ dout,
-                                                    const float* __restrict__ lse, float* __restrict__ stat) {
-  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)d.B * d.T * d.H;  // (b, t, h)
-  if (i >= rows) return;
-  const int h = (int)(i % d.H), t = (int)(i / d.H % d.T), b = (int)(i / d.H / d.T);
+                                                    const float* __restrict__ lse, const int32_t* __restrict__ q_lens,
+                                                    float* __restrict__ stat) {
+  const int64_t TP = stat_rows(d.T), j = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, t, h)
+  if (j >= d.B * TP * d.H) return;
+  const int h = (int)(j % d.H), t = (int)(j / d.H % TP), b = (int)(j / d.H / TP);
+  const int64_t at = ((int64_t)b * d.H + h) * TP + t, half = d.B * TP * d.H;
+  if (t >= clamp_len(q_lens, b, d.T)) {
+    if ((threadIdx.x & 15) == 0) {
+      stat[at] = 0.f;
+      stat[half + at] = INFINITY;
+    }
+    return;
+  }
+  const int64_t i = ((int64_t)b * d.T + t) * d.H + h;
   const T* g = dout + b * d.gs[0] + t * d.gs[1] + h * d.gs[2];
   float s = 0.f;
   for (int c = 8 * (threadIdx.x & 15); c < d.dv; c += 128) {
@@ -200,9 +214,9 @@ __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restri
 #pragma unroll
   for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
   if ((threadIdx.x & 15) == 0) {
-    const int64_t at = ((int64_t)b * d.H + h) * d.T + t;
+    // (a query that sees nothing has lse = -infinity; all of its places are masked)
     stat[at] = s;
-    stat[rows + at] = lse[at] * kLog2e;
+    stat[half + at] = lse[((int64_t)b * d.H + h) * d.T + t] * kLog2e;
   }
 }
 
@@ -243,8 +257,8 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   frag qf[KS], gf[VS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   row_frags<T, DV, 0>(gf, dout + b * d.gs[0] + (int64_t)rowc * d.gs[1] + h * d.gs[2], d.dv, (const T*)nullptr, 0);
-  const int64_t at = ((int64_t)b * d.H + h) * d.T + rowc;
-  const float dl = stat[at], l2 = stat[(int64_t)d.B * d.H * d.T + at];
+  const int64_t at = ((int64_t)b * d.H + h) * stat_rows(d.T) + rowc;
+  const float dl = stat[at], l2 = stat[(int64_t)d.B * d.H * stat_rows(d.T) + at];
   f32x16 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
@@ -351,14 +365,14 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   dr.init(qb + d.dn, d.qs[1], d.dr);
   dg.init(gb, d.gs[1], d.dv);
   // wave 0 brings delta, wave 1 lse (64 rows; an fp32 tile uses half of them)
-  const float* sb = stat + (wave_id() & 1 ? (int64_t)d.B * d.H * d.T : 0) + ((int64_t)b * d.H + h) * d.T;
+  const float* sb = stat + ((wave_id() & 1 ? (int64_t)d.B * d.H : 0) + (int64_t)b * d.H + h) * stat_rows(d.T);
   const uint32_t l0 = lds_addr(lds);
   auto load = [&](int r0, int buf) {
     const uint32_t at = l0 + buf * STAGE;
     dn.load(r0, ql - 1, at);
     dr.load(r0, ql - 1, at + OR);
     dg.load(r0, ql - 1, at + OG);
-    if (wave_id() < 2) dma4_raw(sb + min(r0 + lane_id(), ql - 1), at + OS + 256 * wave_id());
+    if (wave_id() < 2) dma4_raw(sb + (r0 & ~63) + lane_id(), at + OS + 256 * wave_id());
   };
   frag kf[KS], vf[VS];
   row_frags<T, DN, DR>(kf, kr, d.dn, kpe + b * d.ps[0] + (int64_t)tokc * d.ps[1], d.dr);
@@ -371,58 +385,91 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   const float c2 = d.scale * kLog2e;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   if (first < ql) load(first, 0);
-  int buf = 0;
-  for (int q0 = first; q0 < ql; q0 += TQ, buf ^= 1) {
+  int q0 = first, buf = 0;
+  auto stage = [&] {  // this tile is there, the next one on its way
     vm_wait<0>();
     bare_barrier();
     if (q0 + TQ < ql) load(q0 + TQ, buf ^ 1);
+  };
+  // One tile.  Its two halves follow each other by a phase: the scores of the
+  // second half run beside the first half's exponentials, the gradients of the
+  // first beside the second's.  Only the diagonal needs a mask: rows past the last
+  // query have an lse of infinity, tokens past the last key are not stored.
+  auto step = [&](auto masked) {
     const char* sq = lds + buf * STAGE;
-    const float *sd = (const float*)(sq + OS), *sl = sd + 64;
+    const float *sd = (const float*)(sq + OS) + (q0 & 63), *sl = sd + 64;
+    f32x16 s[NS], g[NS];
+    frag p[NS][2], ds[NS][2];
+    constexpr int M1 = KS + VS, M2 = 2 * (NV + NK);
+    auto row_at = [&](int i, int j) {
+      return j < KN ? LN::row(sq, 32 * i, 16 * j)
+                    : j < KS ? LR::row(sq + OR, 32 * i, 16 * (j - KN)) : LG::row(sq + OG, 32 * i, 16 * (j - KS));
+    };
+    auto score = [&](int i, int j, frag a) {
+      if (j == 0) s[i] = zero16();
+      if (j == KS) g[i] = zero16();
+      if (j < KS) s[i] = M32<T>::mma(a, kf[j], s[i]);
+      else g[i] = M32<T>::mma(a, vf[j - KS], g[i]);
+    };
+    auto col_at = [&](int i, int j) {
+      const int t = j / (NV + NK), n = j % (NV + NK), r = 32 * i + 16 * t;
+      return n < NV ? LG::col(sq + OG, r, 32 * n)
+                    : n < NV + NN ? LN::col(sq, r, 32 * (n - NV)) : LR::col(sq + OR, r, 32 * (n - NV - NN));
+    };
+    auto grad = [&](int i, int j, frag a) {
+      const int t = j / (NV + NK), n = j % (NV + NK);
+      if (n < NV) av[n] = M32<T>::mma(a, p[i][t], av[n]);
+      else ak[n - NV] = M32<T>::mma(a, ds[i][t], ak[n - NV]);
+    };
+    auto prob = [&](int i, int k) {  // four rows
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(sl + 32 * i + reg_row(4 * k));
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + 32 * i + reg_row(4 * k));
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int r0 = q0 + 32 * i;
-      if (w0 >= kl || r0 >= ql || (d.causal && w0 > r0 + 31 + off)) continue;
-      f32x16 s = zero16(), g = zero16();
-      in_groups<KS + VS, 4, frag>(
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * k + j;
+        float x = fast_exp2(s[i][r] * c2 - l4[j]), y = x * (g[i][r] - d4[j]);
+        if constexpr (decltype(masked)::value) {
+          const bool ok = tok <= q0 + 32 * i + reg_row(r) + off;
+          x = ok ? x : 0.f;
+          y = ok ? y : 0.f;
+        }
+        p[i][k / 2][4 * (k & 1) + j] = (T)x;
+        ds[i][k / 2][4 * (k & 1) + j] = (T)y;
+      }
+    };
+    if constexpr (NS == 2) {
+      constexpr int G = M1 % 4 || M2 % 4 ? 5 : 4;  // whole groups a phase: a phase's work starts after the one before
+      static_assert(M1 % G == 0 && M2 % G == 0, "whole groups");
+      in_groups<2 * M1 + 2 * M2, G, 6, frag>(
           [&](int j) {
-            return j < KN ? LN::row(sq, 32 * i, 16 * j)
-                          : j < KS ? LR::row(sq + OR, 32 * i, 16 * (j - KN)) : LG::row(sq + OG, 32 * i, 16 * (j - KS));
+            return j < 2 * M1 ? row_at(j / M1, j % M1) : col_at((j - 2 * M1) / M2, (j - 2 * M1) % M2);
           },
           [&](int j, frag a) {
-            if (j < KS) s = M32<T>::mma(a, kf[j], s);
-            else g = M32<T>::mma(a, vf[j - KS], g);
-          });
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(sl + 32 * i + reg_row(r));
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + 32 * i + reg_row(r));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = fast_exp2(s[r + j] * c2 - l4[j]);
-          s[r + j] = p;
-          g[r + j] = p * (g[r + j] - d4[j]);
-        }
-      }
-      if (r0 + 32 > ql || w0 + 32 > kl || (d.causal && w0 + 31 > r0 + off)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = r0 + reg_row(r);
-          if (at >= ql || tok >= kl || (d.causal && tok > at + off)) s[r] = g[r] = 0.f;
-        }
-      }
-      const frag p[2] = {pack_frag<T>(s, 0), pack_frag<T>(s, 1)}, ds[2] = {pack_frag<T>(g, 0), pack_frag<T>(g, 1)};
-      in_groups<2 * (NV + NK), 4, frag>(
-          [&](int j) {
-            const int t = j / (NV + NK), n = j % (NV + NK), r = 32 * i + 16 * t;
-            return n < NV ? LG::col(sq + OG, r, 32 * n)
-                          : n < NV + NN ? LN::col(sq, r, 32 * (n - NV)) : LR::col(sq + OR, r, 32 * (n - NV - NN));
+            if (j < 2 * M1) score(j / M1, j % M1, a);
+            else grad((j - 2 * M1) / M2, (j - 2 * M1) % M2, a);
           },
-          [&](int j, frag a) {
-            const int t = j / (NV + NK), n = j % (NV + NK);
-            if (n < NV) av[n] = M32<T>::mma(a, p[t], av[n]);
-            else ak[n - NV] = M32<T>::mma(a, ds[t], ak[n - NV]);
+          [&](int j) {
+            if (j >= M1 && j < 2 * M1 && (j - M1) % (M1 / 4) == 1 && (j - M1) / (M1 / 4) < 4) prob(0, (j - M1) / (M1 / 4));
+            if (j >= 2 * M1 && j < 2 * M1 + M2 && (j - 2 * M1) % (M2 / 4) == 1 && (j - 2 * M1) / (M2 / 4) < 4)
+              prob(1, (j - 2 * M1) / (M2 / 4));
           });
+    } else {
+      in_groups<M1, 4, frag>([&](int j) { return row_at(0, j); }, [&](int j, frag a) { score(0, j, a); });
+#pragma unroll
+      for (int k = 0; k < 4; ++k) prob(0, k);
+      in_groups<M2, 4, frag>([&](int j) { return col_at(0, j); }, [&](int j, frag a) { grad(0, j, a); });
     }
+  };
+  // tiles that this wave's tokens are not visible to, those on the diagonal, the rest
+  // (a wave without tokens only keeps the others company)
+  for (; q0 < ql && (w0 >= kl || (d.causal && w0 > q0 + TQ - 1 + off)); q0 += TQ, buf ^= 1) stage();
+  for (; q0 < ql && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
+    stage();
+    step(IntC<1>());
+  }
+  for (; q0 < ql; q0 += TQ, buf ^= 1) {
+    stage();
+    step(IntC<0>());
   }
   if (tok >= d.S) return;
   T* out = dkv + (((int64_t)b * d.S + tok) * d.H + h) * (d.dn + d.dv);
@@ -474,7 +521,7 @@ static int lat_check(const atomic_latent_args* a) {
   // row numbers and lengths stay in 31 bits with room for a block; grids in 31 bits
   if (a->tq > (1 << 30) || a->tk > (1 << 30)) return ATOMIC_ERR_SHAPE;
   const int64_t most = (int64_t)(a->tq > a->tk ? a->tq : a->tk), bh = (int64_t)a->batch * a->heads;
-  if (bh > INT32_MAX || bh * ((most + 127) / 128) > INT32_MAX || bh * ((most + 15) / 16) > INT32_MAX ||
+  if (bh > INT32_MAX || bh * ((most + 127) / 128) > INT32_MAX || bh * (stat_rows((int)most) / 16) > INT32_MAX ||
       (int64_t)a->batch * ((a->tk + 15) / 16) * a->dr > INT32_MAX)
     return ATOMIC_ERR_SHAPE;
   if (!whole_pieces({a->q_stride[0], a->q_stride[1], a->q_stride[2], a->kv_stride[0], a->kv_stride[1],
@@ -506,7 +553,7 @@ static int lat_dispatch(const atomic_latent_args* a, F&& f) {
 }
 
 static size_t lat_stat_bytes(const atomic_latent_args* a) {
-  return ((size_t)a->batch * a->heads * a->tq * 2 * sizeof(float) + 255) / 256 * 256;
+  return (size_t)a->batch * a->heads * stat_rows(a->tq) * 2 * sizeof(float);
 }
 
 }  // namespace ah
@@ -555,10 +602,10 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
     typedef decltype(t) T;
     typedef decltype(w) W;
     LatDims d = lat_dims(a);
-    const int64_t rows = (int64_t)d.B * d.T * d.H;
+    const int64_t rows = (int64_t)d.B * stat_rows(d.T) * d.H;
     int rc = L("latent_delta", [&] {
       hipLaunchKernelGGL((latent_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, d, (const T*)o,
-                         (const T*)dout, lse, stat);
+                         (const T*)dout, lse, q_lens, stat);
     });
     if (rc) return rc;
     d.blocks = (d.S + 127) / 128;
