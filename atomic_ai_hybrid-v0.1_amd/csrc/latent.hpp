@@ -123,43 +123,42 @@ struct LTile {
   }
 };
 
-// use(i, load(i)) for i in [0, N), each use one MFMA, with its operand read from
-// LDS a group of G uses ahead (left alone, the compiler reads each fragment right
-// before its MFMA and waits for it there).  work(i) is other work done at slot i;
-// VN > 0 spreads a group's vector instructions over its MFMAs, VN after each,
-// where they run while the matrix pipe is busy.
-template <int N, int G, int VN, typename F, typename L, typename U, typename K>
+// use(i, load(i)) for i in [0, N), each use one MFMA, in groups of G, with its
+// operand read from LDS `LA` groups ahead (left alone, the compiler reads each
+// fragment right before its MFMA and waits for it there).  work(i) is other work
+// done at slot i; VN > 0 spreads a group's vector instructions over its MFMAs, VN
+// after each, where they run while the matrix pipe is busy.
+template <int N, int G, int LA, int VN, typename F, typename L, typename U, typename K>
 __device__ __forceinline__ void in_groups(L&& load, U&& use, K&& work) {
-  F f[2][G];
-#pragma unroll
-  for (int j = 0; j < G && j < N; ++j) f[0][j] = load(j);
+  F f[LA + 1][G];
+  static_for<(LA * G < N ? LA * G : N)>([&](auto j) { f[j.value / G][j.value % G] = load(j.value); });
   __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int i = 0; i < N; i += G) {
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (i + G + j < N) f[(i / G + 1) & 1][j] = load(i + G + j);
+  static_for<(N + G - 1) / G>([&](auto gr) {
+    constexpr int g = decltype(gr)::value;
+    static_for<G>([&](auto j) {
+      constexpr int at = (g + LA) * G + decltype(j)::value;
+      if constexpr (at < N) f[(g + LA) % (LA + 1)][j.value] = load(at);
+    });
     if constexpr (VN == 0) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (i + j < N) work(i + j);
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-      if (i + j < N) use(i + j, f[(i / G) & 1][j]);
+    static_for<G>([&](auto j) {
+      if constexpr (g * G + decltype(j)::value < N) work(g * G + j.value);
+    });
+    static_for<G>([&](auto j) {
+      if constexpr (g * G + decltype(j)::value < N) use(g * G + j.value, f[g % (LA + 1)][j.value]);
+    });
     if constexpr (VN > 0) {
       __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
+      static_for<G>([&](auto) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
         __builtin_amdgcn_sched_group_barrier(0x002, VN, 0);  // vector
-      }
+      });
     }
     __builtin_amdgcn_sched_barrier(0);
-  }
+  });
 }
 template <int N, int G, typename F, typename L, typename U>
 __device__ __forceinline__ void in_groups(L&& load, U&& use) {
-  in_groups<N, G, 0, F>(load, use, [](int) {});
+  in_groups<N, G, 1, 0, F>(load, use, [](int) {});
 }
 
 // Rows of a matrix (W elements, `width` of them real) straight to an LTile of ROWS

@@ -17,6 +17,10 @@
 
 namespace ah {
 
+#ifndef KA
+#define KA 2
+#endif
+constexpr int kAhead = KA;
 struct LatDims {
   int B, T, S, H, dn, dr, dv, causal, blocks;  // blocks: row (or token) blocks of a head
   float scale;
@@ -272,43 +276,79 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   if (end > 0) load(0, 0);
-  int buf = 0;
-  for (int k0 = 0; k0 < end; k0 += TK, buf ^= 1) {
+  int k0 = 0, buf = 0;
+  auto stage = [&] {  // this tile is there, the next one on its way
     vm_wait<0>();
     bare_barrier();
     if (k0 + TK < end) load(k0 + TK, buf ^ 1);
+  };
+  // one tile, its halves a phase apart as in latent_bwd_dkv
+  auto step = [&](auto masked) {
     const char* sk = lds + buf * STAGE;
+    const int seen = min(kl, d.causal ? row + off + 1 : kl) - k0;
+    f32x16 s[NS], g[NS];
+    frag ds[NS][2];
+    constexpr int M1 = KS + VS, M2 = 2 * NT;
+    auto row_at = [&](int i, int j) {
+      return j < KN ? LN::row(sk, 32 * i, 16 * j)
+                    : j < KS ? LR::row(sk + OR, 32 * i, 16 * (j - KN)) : LV::row(sk + OV, 32 * i, 16 * (j - KS));
+    };
+    auto score = [&](int i, int j, frag a) {
+      if (j == 0) s[i] = zero16();
+      if (j == KS) g[i] = zero16();
+      if (j < KS) s[i] = M32<T>::mma(a, qf[j], s[i]);
+      else g[i] = M32<T>::mma(a, gf[j - KS], g[i]);
+    };
+    auto col_at = [&](int i, int j) {
+      const int t = j / NT, n = j % NT, r = 32 * i + 16 * t;
+      return n < NN ? LN::col(sk, r, 32 * n) : LR::col(sk + OR, r, 32 * (n - NN));
+    };
+    auto grad = [&](int i, int j, frag a) { acc[j % NT] = M32<T>::mma(a, ds[i][j / NT], acc[j % NT]); };
+    auto prob = [&](int i, int k) {  // four tokens
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int t0 = k0 + 32 * i;
-      if (w0 >= ql || t0 >= kl || (d.causal && t0 > w0 + 31 + off)) break;
-      f32x16 s = zero16(), g = zero16();
-      in_groups<KS + VS, 4, frag>(
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * k + j;
+        float y = fast_exp2(s[i][r] * c2 - l2) * (g[i][r] - dl);
+        if constexpr (decltype(masked)::value) y = 32 * i + reg_row(r) < seen ? y : 0.f;
+        ds[i][k / 2][4 * (k & 1) + j] = (T)y;
+      }
+    };
+    if constexpr (NS == 2) {
+      constexpr int G = M1 % 4 || M2 % 4 ? (M1 % 5 || M2 % 5 ? 2 : 5) : 4;
+      static_assert(M1 % G == 0 && M2 % G == 0, "whole groups");
+      in_groups<2 * M1 + 2 * M2, G, kAhead, 6, frag>(
           [&](int j) {
-            return j < KN ? LN::row(sk, 32 * i, 16 * j)
-                          : j < KS ? LR::row(sk + OR, 32 * i, 16 * (j - KN)) : LV::row(sk + OV, 32 * i, 16 * (j - KS));
+            return j < 2 * M1 ? row_at(j / M1, j % M1) : col_at((j - 2 * M1) / M2, (j - 2 * M1) % M2);
           },
           [&](int j, frag a) {
-            if (j < KS) s = M32<T>::mma(a, qf[j], s);
-            else g = M32<T>::mma(a, gf[j - KS], g);
-          });
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(s[r] * c2 - l2) * (g[r] - dl);
-      if (t0 + 32 > kl || (d.causal && t0 + 31 > w0 + off)) {
-        const int seen = min(kl, d.causal ? row + off + 1 : kl) - t0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (reg_row(r) >= seen) s[r] = 0.f;
-      }
-      const frag ds[2] = {pack_frag<T>(s, 0), pack_frag<T>(s, 1)};
-      in_groups<2 * NT, 4, frag>(
-          [&](int j) {
-            const int t = j / NT, n = j % NT;
-            return n < NN ? LN::col(sk, 32 * i + 16 * t, 32 * n) : LR::col(sk + OR, 32 * i + 16 * t, 32 * (n - NN));
+            if (j < 2 * M1) score(j / M1, j % M1, a);
+            else grad((j - 2 * M1) / M2, (j - 2 * M1) % M2, a);
           },
-          [&](int j, frag a) { acc[j % NT] = M32<T>::mma(a, ds[j / NT], acc[j % NT]); });
+          [&](int j) {
+            if (j >= M1 && j < 2 * M1 && (j - M1) % (M1 / 4) == 1 && (j - M1) / (M1 / 4) < 4) prob(0, (j - M1) / (M1 / 4));
+            if (M2 >= 8 && j >= 2 * M1 && j < 2 * M1 + M2 && (j - 2 * M1) % (M2 / 4) == 1 && (j - 2 * M1) / (M2 / 4) < 4)
+              prob(1, (j - 2 * M1) / (M2 / 4));
+            if (M2 < 8 && j >= 2 * M1 && j < 2 * M1 + 4) prob(1, j - 2 * M1);
+          });
+    } else {
+      in_groups<M1, 4, frag>([&](int j) { return row_at(0, j); }, [&](int j, frag a) { score(0, j, a); });
+#pragma unroll
+      for (int k = 0; k < 4; ++k) prob(0, k);
+      in_groups<M2, 4, frag>([&](int j) { return col_at(0, j); }, [&](int j, frag a) { grad(0, j, a); });
     }
+  };
+  // tiles that every row of this wave sees whole, those on the diagonal or the last key, those that none sees
+  const int whole = w0 >= ql ? 0 : min(end, d.causal ? min(kl, w0 + off + 1) : kl) - TK + 1;
+  const int any = w0 >= ql ? 0 : min(end, d.causal ? w0 + 32 + off : kl);
+  for (; k0 < whole; k0 += TK, buf ^= 1) {
+    stage();
+    step(IntC<0>());
   }
+  for (; k0 < any; k0 += TK, buf ^= 1) {
+    stage();
+    step(IntC<1>());
+  }
+  for (; k0 < end; k0 += TK, buf ^= 1) stage();
   if (row >= d.T) return;
   T* out = dq + (((int64_t)b * d.T + row) * d.H + h) * (d.dn + d.dr);
 #pragma unroll
@@ -440,7 +480,7 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
     if constexpr (NS == 2) {
       constexpr int G = M1 % 4 || M2 % 4 ? 5 : 4;  // whole groups a phase: a phase's work starts after the one before
       static_assert(M1 % G == 0 && M2 % G == 0, "whole groups");
-      in_groups<2 * M1 + 2 * M2, G, 6, frag>(
+      in_groups<2 * M1 + 2 * M2, G, kAhead, 6, frag>(
           [&](int j) {
             return j < 2 * M1 ? row_at(j / M1, j % M1) : col_at((j - 2 * M1) / M2, (j - 2 * M1) % M2);
           },
