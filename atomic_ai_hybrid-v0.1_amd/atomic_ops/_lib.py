@@ -26,7 +26,7 @@ ERRORS = {
 }
 ATOMIC_F32, ATOMIC_BF16 = 0, 1
 GDN2_SAVE, GDN2_REUSE, GDN2_SANITIZE_H0 = 1, 2, 4
-ATOMIC_ERR_REUSE = -7
+ATOMIC_ERR_SHAPE, ATOMIC_ERR_REUSE = -1, -7
 
 
 class Gdn2Args(ctypes.Structure):
@@ -269,7 +269,8 @@ _SIGS = {
     "atomic_mamba2_proj_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(Mamba2ProjArgs), ctypes.c_int]),
     "atomic_mamba2_proj_fwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 16 + [_P, ctypes.c_size_t, _P]),
     "atomic_mamba2_proj_bwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 24 + [_P, ctypes.c_size_t, _P]),
-    "atomic_latent_fwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 7 + [_P]),
+    "atomic_latent_fwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentArgs)]),
+    "atomic_latent_fwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 7 + [_P, ctypes.c_size_t, _P]),
     "atomic_latent_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentArgs)]),
     "atomic_latent_bwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 11 + [_P, ctypes.c_size_t, _P]),
     "atomic_latent_append": (ctypes.c_int, [ctypes.POINTER(LatentAppendArgs)] + [_P] * 10 + [_P]),

@@ -100,7 +100,7 @@ def make_args(q, kv, k_pe, scale, causal, dout=None):
     return args, (q, kv, k_pe, dout)
 
 
-def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, timer=None):
+def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, workspace=None, timer=None):
     """``(o, lse)``: o [B, T, H, dv] in q's dtype and lse [B, H, T] float32.
 
     Query i of batch row b sees the keys j < kv_lens[b]; with ``causal`` those
@@ -114,10 +114,16 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, timer
     if timer is not None:
         args.profile = timer.arm()
     B, T, H = q.shape[:3]
+    nbytes = lib.atomic_latent_fwd_workspace_size(ctypes.byref(args))
+    if nbytes == 0:
+        raise _lib.AtomicError("atomic_latent_fwd: ATOMIC_ERR_SHAPE: unsupported or inconsistent dimensions",
+                               _lib.ATOMIC_ERR_SHAPE)
+    if workspace is None or workspace.numel() < nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     o = torch.empty(B, T, H, args.dv, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
     rc = lib.atomic_latent_fwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
-                               _ptr(o), _ptr(lse), _stream(q.device))
+                               _ptr(o), _ptr(lse), _ptr(workspace), workspace.numel(), _stream(q.device))
     _lib.check(rc, "atomic_latent_fwd")
     return o, lse
 

@@ -127,8 +127,8 @@ struct LTile {
 // operand read from LDS `LA` groups ahead (left alone, the compiler reads each
 // fragment right before its MFMA and waits for it there).  work(i) is other work
 // done at slot i; VN > 0 spreads a group's vector instructions over its MFMAs, VN
-// after each, where they run while the matrix pipe is busy.
-template <int N, int G, int LA, int VN, typename F, typename L, typename U, typename K>
+// after each, where they run while the matrix pipe is busy.  A use may be MF MFMAs.
+template <int N, int G, int LA, int VN, typename F, int MF = 1, typename L, typename U, typename K>
 __device__ __forceinline__ void in_groups(L&& load, U&& use, K&& work) {
   F f[LA + 1][G];
   static_for<(LA * G < N ? LA * G : N)>([&](auto j) { f[j.value / G][j.value % G] = load(j.value); });
@@ -148,7 +148,7 @@ __device__ __forceinline__ void in_groups(L&& load, U&& use, K&& work) {
     });
     if constexpr (VN > 0) {
       __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
-      static_for<G>([&](auto) {
+      static_for<G * MF>([&](auto) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
         __builtin_amdgcn_sched_group_barrier(0x002, VN, 0);  // vector
       });

@@ -61,47 +61,65 @@ __device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) /
 __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3); }
 
 // ------------------------------------------------------------------ forward
-// 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens (32
-// in fp32).  Two tiles in LDS: while one is computed with, the next is loaded
-// straight to LDS; one barrier a tile.  Two workgroups a CU (80 KB of LDS and 256
-// registers a lane each), so that one's MFMAs run beside the other's softmax.
-template <typename T, int DN, int DR, int DV>
-__global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
-                                                     const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
-                                                     const int32_t* __restrict__ kv_lens, T* __restrict__ o,
-                                                     float* __restrict__ lse) {
+// 32 query rows of a head a wave, NW waves a workgroup, against tiles of 64 tokens
+// (32 in fp32) that go straight to LDS, one tile ahead; one barrier a tile.  Two
+// waves a SIMD with 256 registers each, so that one's MFMAs run beside the other's
+// softmax.  Eight waves share a tile where there are row blocks enough: with four
+// (and two workgroups a CU) the tiles come out of L2 twice as often.
+//
+// With `parts` > 1 the keys of a row block are divided over that many workgroups
+// (few row blocks against many keys); each leaves its accumulators, reference and
+// sum, which latent_fwd_join joins.
+template <typename T, int DN, int DR, int DV, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void latent_fwd(LatDims d, int parts, const T* __restrict__ q,
+                                                         const T* __restrict__ kv, const T* __restrict__ kpe,
+                                                         const int32_t* __restrict__ q_lens,
+                                                         const int32_t* __restrict__ kv_lens, T* __restrict__ o,
+                                                         float* __restrict__ lse, float* __restrict__ pacc,
+                                                         float* __restrict__ pstat) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, NT = DV / 32, TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
+  constexpr int RB = 32 * NW, NB = 2;  // rows a workgroup, tiles in LDS
   typedef LTile<T, DN> LN;
   typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LV;
   typedef typename M32<T>::frag frag;
   constexpr int OR = TK * LN::ROWB, OV = OR + TK * LR::ROWB, STAGE = OV + TK * LV::ROWB;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[NB * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
-  blk = d.blocks - 1 - blk;  // with causal the long rows first
+  const int part = blk % parts;
+  blk = (d.blocks - 1 - blk) / parts;  // with causal the long rows first (`parts` divides `blocks`)
   const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
-  const int w0 = 128 * blk + 32 * wave_id();  // this wave's first row
+  const int w0 = RB * blk + 32 * wave_id();  // this wave's first row
   const int row = w0 + (lane_id() & 31);
-  const int last = min(128 * blk + 127, ql - 1);  // the workgroup's last row
-  int end = kl;                                   // keys that any row sees
+  const int last = min(RB * blk + RB - 1, ql - 1);  // the workgroup's last row
+  int begin = 0, end = kl;                          // keys that any row sees
   if (d.causal) end = min(end, last + off + 1);
-  if (last < 128 * blk) end = 0;
+  if (last < RB * blk) end = 0;
+  if (parts > 1) {
+    const int tiles = (max(end, 0) + TK - 1) / TK;
+    begin = (int)((int64_t)tiles * part / parts) * TK;
+    end = min(end, (int)((int64_t)tiles * (part + 1) / parts) * TK);
+  }
   const T* qr = q + b * d.qs[0] + (int64_t)max(min(row, ql - 1), 0) * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
-  RowDma<T, DN, TK, 4> dn;
-  RowDma<T, DR, TK, 4> dr;
-  RowDma<T, DV, TK, 4> dv;
+  RowDma<T, DN, TK, NW> dn;
+  RowDma<T, DR, TK, NW> dr;
+  RowDma<T, DV, TK, NW> dv;
   dn.init(kb, d.ks[1], d.dn);
   dr.init(kpe + b * d.ps[0], d.ps[1], d.dr);
   dv.init(kb + d.dn, d.ks[1], d.dv);
   frag qf[KS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
+  // (a scale of zero as the smallest number: a masked score stays infinite; a negative one changes q's sign)
+  const float c2 = d.scale == 0.f ? FLT_MIN : fabsf(d.scale) * kLog2e;
+  if (d.scale < 0.f) {
+#pragma unroll
+    for (int t = 0; t < KS; ++t) qf[t] = -qf[t];
+  }
   f32x16 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
-  // (a scale of zero as the smallest number: a masked score stays infinite)
-  const float c2 = d.scale == 0.f ? FLT_MIN : d.scale * kLog2e;
   float m = -INFINITY, sum = 0.f;  // reference (of c2 times the scores, see kLag) and this lane's part of the sum
   const uint32_t l0 = lds_addr(lds);
   auto load = [&](int k0, int buf) {
@@ -111,12 +129,15 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
     dv.load(k0, kl - 1, at + OV);
   };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the query: no later wait for it drains the tiles
-  if (end > 0) load(0, 0);
+  constexpr int PER = RowDma<T, DN, TK, NW>::N + RowDma<T, DR, TK, NW>::N + RowDma<T, DV, TK, NW>::N;
+  if (begin < end) load(begin, 0);
+  if (NB == 3 && begin + TK < end) load(begin + TK, 1);
   int buf = 0;
-  for (int k0 = 0; k0 < end; k0 += TK, buf ^= 1) {
-    vm_wait<0>();
-    bare_barrier();  // the tile is there, and nobody reads the other one any more
-    if (k0 + TK < end) load(k0 + TK, buf ^ 1);
+  for (int k0 = begin; k0 < end; k0 += TK, buf = buf + 1 == NB ? 0 : buf + 1) {
+    if (NB == 3 && k0 + TK < end) vm_wait<PER>();
+    else vm_wait<0>();
+    bare_barrier();  // the tile is there, and nobody reads the one before it any more
+    if (k0 + (NB - 1) * TK < end) load(k0 + (NB - 1) * TK, buf == 0 ? NB - 1 : buf - 1);
     if (w0 >= ql || (d.causal && k0 > w0 + 31 + off)) continue;  // nothing visible to this wave
     const char* sk = lds + buf * STAGE;
     f32x16 s[NS];
@@ -134,13 +155,14 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (32 * i + reg_row(r) >= seen) s[i][r] = c2 < 0.f ? INFINITY : -INFINITY;
+          if (32 * i + reg_row(r) >= seen) s[i][r] = -INFINITY;
     }
-    float top = s[0][0] * c2;
+    float top = s[0][0];
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r] * c2);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+    top *= c2;
     if (__any(top > m + kLag)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m, top), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
@@ -151,13 +173,13 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= fade;
     }
-    const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
+    const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
     frag p[2 * NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[i][r] = fast_exp2(s[i][r] * c2 - ref);
+        s[i][r] = fast_exp2(__builtin_fmaf(s[i][r], c2, ref));
         sum += s[i][r];
       }
       p[2 * i] = pack_frag<T>(s[i], 0);
@@ -168,7 +190,26 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
   }
   if (row >= d.T) return;
   sum += __shfl_xor(sum, 32);
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  const int64_t at = ((int64_t)b * d.H + h) * d.T + row;
+  if (parts > 1) {
+    const int64_t pr = (int64_t)part * d.B * d.H * d.T + at;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int c = 32 * n + reg_row(r);
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = acc[n][r + j];
+        if (c < d.dv) store4(pacc + pr * d.dv + c, v);
+      }
+    if (lane_id() < 32) {
+      pstat[2 * pr] = row < ql ? m : -INFINITY;
+      pstat[2 * pr + 1] = row < ql ? sum : 0.f;
+    }
+    return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* orow = o + (((int64_t)b * d.T + row) * d.H + h) * d.dv;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -180,8 +221,31 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, const T* __restr
       for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] * inv : 0.f;
       if (c < d.dv) store4(orow + c, v);
     }
-  if (lane_id() < 32)
-    lse[((int64_t)b * d.H + h) * d.T + row] = row < ql && sum != 0.f ? m * kLn2 + fast_log2(sum) * kLn2 : -INFINITY;
+  if (lane_id() < 32) lse[at] = row < ql && sum != 0.f ? m * kLn2 + fast_log2(sum) * kLn2 : -INFINITY;
+}
+
+// o and lse of rows whose keys were divided: four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void latent_fwd_join(LatDims d, int parts, const float* __restrict__ pacc,
+                                                       const float* __restrict__ pstat, T* __restrict__ o,
+                                                       float* __restrict__ lse) {
+  const int per = d.dv / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, at = i / per, rows = (int64_t)d.B * d.H * d.T;
+  if (at >= rows) return;
+  const int c = (int)(i % per) * 4;
+  float m = -INFINITY, sum = 0.f;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, pstat[2 * (p * rows + at)]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x4 x = zero4();
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float w = fast_exp2(pstat[2 * (p * rows + at)] - ref);
+    sum += w * pstat[2 * (p * rows + at) + 1];
+    x += w * *reinterpret_cast<const f32x4*>(pacc + (p * rows + at) * d.dv + c);
+  }
+  const int t = (int)(at % d.T), h = (int)(at / d.T % d.H), b = (int)(at / d.T / d.H);
+  store4(o + (((int64_t)b * d.T + t) * d.H + h) * d.dv + c, x * (sum == 0.f ? 0.f : 1.f / sum));
+  if (c == 0) lse[at] = sum == 0.f ? -INFINITY : m * kLn2 + fast_log2(sum) * kLn2;
 }
 
 // ----------------------------------------------------------------- backward
@@ -592,6 +656,21 @@ static int lat_dispatch(const atomic_latent_args* a, F&& f) {
   return small ? f(float(), Widths<64, 32, 64>()) : f(float(), Widths<128, 64, 128>());
 }
 
+// The forward's waves a workgroup and parts of the keys.
+struct FwdPlan { int waves, parts; };
+static FwdPlan fwd_plan(const atomic_latent_args* a) {
+  FwdPlan p{4, 1};
+  const int64_t bh = (int64_t)a->batch * a->heads;
+  if (a->dtype == ATOMIC_BF16 && bh * ((a->tq + 255) / 256) >= 256) p.waves = 8;
+  const int64_t wgs = bh * ((a->tq + 32 * p.waves - 1) / (32 * p.waves)), tiles = (a->tk + 63) / 64;
+  while (p.parts < 16 && p.parts * wgs <= 256 && 8 * p.parts <= tiles) p.parts *= 2;
+  return p;
+}
+static size_t fwd_stat_bytes(const atomic_latent_args* a, const FwdPlan& p) {
+  return ((size_t)p.parts * a->batch * a->heads * a->tq * 2 * sizeof(float) + 255) / 256 * 256;
+}
+constexpr size_t kNoWorkspace = 16;  // what a size function returns where none is needed (0 is a refusal)
+
 static size_t lat_stat_bytes(const atomic_latent_args* a) {
   return (size_t)a->batch * a->heads * stat_rows(a->tq) * 2 * sizeof(float);
 }
@@ -600,21 +679,52 @@ static size_t lat_stat_bytes(const atomic_latent_args* a) {
 
 using namespace ah;
 
+extern "C" size_t atomic_latent_fwd_workspace_size(const atomic_latent_args* a) {
+  if (lat_check(a) != ATOMIC_OK) return 0;
+  const FwdPlan p = fwd_plan(a);
+  return p.parts > 1 ? fwd_stat_bytes(a, p) + (size_t)p.parts * a->batch * a->heads * a->tq * a->dv * sizeof(float)
+                     : kNoWorkspace;
+}
+
 extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
-                                 const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* stream) {
+                                 const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
   if (int rc = lat_check(a)) return rc;
   if (!q || !kv || !k_pe || !o || !lse) return ATOMIC_ERR_NULL;
   if (!aligned16({q, kv, k_pe, o})) return ATOMIC_ERR_SHAPE;
-  LatDims d = lat_dims(a);
-  d.blocks = (d.T + 127) / 128;
+  const FwdPlan p = fwd_plan(a);
+  if (p.parts > 1) {
+    if (!workspace || workspace_bytes < atomic_latent_fwd_workspace_size(a) || !aligned16({workspace}))
+      return ATOMIC_ERR_WORKSPACE;
+    ws_tag_clobber(workspace, atomic_latent_fwd_workspace_size(a));
+  }
+  float* pstat = (float*)workspace;
+  float* pacc = (float*)((char*)workspace + fwd_stat_bytes(a, p));
   const hipStream_t st = (hipStream_t)stream;
   Launch L{a->profile, st};
   return lat_dispatch(a, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    return L("latent_fwd", [&] {
-      hipLaunchKernelGGL((latent_fwd<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256), 0,
-                         st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, (T*)o, lse);
+    LatDims d = lat_dims(a);
+    d.blocks = (d.T + 32 * p.waves - 1) / (32 * p.waves) * p.parts;
+    int rc = L("latent_fwd", [&] {
+      auto go = [&](auto g) {
+        hipLaunchKernelGGL((latent_fwd<T, W::DN, W::DR, W::DV, decltype(g)::value>),
+                           dim3((unsigned)(d.B * d.H * d.blocks)), dim3((unsigned)(64 * p.waves)), 0, st, d, p.parts, (const T*)q,
+                           (const T*)kv, (const T*)k_pe, q_lens, kv_lens, (T*)o, lse, pacc, pstat);
+      };
+      if constexpr (sizeof(T) == 2) {
+        if (p.waves == 8) go(IntC<8>());
+        else go(IntC<4>());
+      } else {
+        go(IntC<4>());
+      }
+    });
+    if (rc || p.parts == 1) return rc;
+    const int64_t n = (int64_t)d.B * d.H * d.T * (d.dv / 4);
+    return L("latent_fwd_join", [&] {
+      hipLaunchKernelGGL((latent_fwd_join<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, d, p.parts, pacc,
+                         pstat, (T*)o, lse);
     });
   });
 }

@@ -805,11 +805,16 @@ typedef struct atomic_latent_args {
   atomic_profile* profile;  /* optional per-kernel event timing, or NULL */
 } atomic_latent_args;
 
+/* Bytes of workspace the forward needs; 0 for unsupported args. */
+size_t atomic_latent_fwd_workspace_size(const atomic_latent_args* a);
+
 /* Forward: o [B, tq, H, dv] dtype and lse [B, H, tq] fp32 (the natural log of
  * the sum of the scores' exponentials), both dense.  q_lens and kv_lens are
- * int32 [B] device arrays, or NULL. */
+ * int32 [B] device arrays, or NULL.  The workspace may be NULL where the size
+ * above is at most 16. */
 int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
-                      const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* stream);
+                      const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace the backward needs; 0 for unsupported args. */
 size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a);
