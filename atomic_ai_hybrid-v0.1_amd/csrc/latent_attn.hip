@@ -298,7 +298,7 @@ template <typename T, int DN, int DR, int DV>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
     LatDims d, const T* __restrict__ q, const T* __restrict__ kv, const T* __restrict__ kpe,
     const int32_t* __restrict__ q_lens, const int32_t* __restrict__ kv_lens, const float* __restrict__ stat,
-    const T* __restrict__ dout, T* __restrict__ dq) {
+    const T* __restrict__ dout, T* __restrict__ dq, int parts, float* __restrict__ pq) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, VS = DV / 16, NN = DN / 32, NT = (DN + DR) / 32;
   constexpr int TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
   typedef LTile<T, DN> LN;
@@ -309,14 +309,20 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
-  blk = d.blocks - 1 - blk;
+  const int part = blk % parts;
+  blk = (d.blocks - 1 - blk) / parts;
   const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
   const int w0 = 128 * blk + 32 * wave_id();
   const int row = w0 + (lane_id() & 31);
   const int last = min(128 * blk + 127, ql - 1);
-  int end = kl;
+  int begin = 0, end = kl;
   if (d.causal) end = min(end, last + off + 1);
   if (last < 128 * blk) end = 0;
+  if (parts > 1) {
+    const int tiles = (max(end, 0) + TK - 1) / TK;
+    begin = (int)((int64_t)tiles * part / parts) * TK;
+    end = min(end, (int)((int64_t)tiles * (part + 1) / parts) * TK);
+  }
   const int rowc = max(min(row, ql - 1), 0);
   const T* qr = q + b * d.qs[0] + (int64_t)rowc * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
@@ -343,8 +349,8 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
     dv.load(k0, kl - 1, at + OV);
   };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  if (end > 0) load(0, 0);
-  int k0 = 0, buf = 0;
+  if (begin < end) load(begin, 0);
+  int k0 = begin, buf = 0;
   auto stage = [&] {  // this tile is there, the next one on its way
     vm_wait<0>();
     bare_barrier();
@@ -423,6 +429,7 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   for (; k0 < end; k0 += TK, buf ^= 1) stage();
   if (row >= d.T) return;
   T* out = dq + (((int64_t)b * d.T + row) * d.H + h) * (d.dn + d.dr);
+  float* po = pq + ((((int64_t)part * d.B + b) * d.T + row) * d.H + h) * (d.dn + d.dr);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -431,10 +438,10 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
       f32x4 v;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] * d.scale : 0.f;
-      if (32 * n < DN) {
-        if (c < d.dn) store4(out + c, v);
-      } else if (c - DN < d.dr) {
-        store4(out + d.dn + c - DN, v);
+      const int at = 32 * n < DN ? c : d.dn + c - DN;
+      if (32 * n < DN ? c < d.dn : c - DN < d.dr) {
+        if (parts > 1) store4(po + at, v);
+        else store4(out + at, v);
       }
     }
 }
@@ -448,7 +455,8 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
                                                          const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
                                                          const int32_t* __restrict__ kv_lens,
                                                          const float* __restrict__ stat, const T* __restrict__ dout,
-                                                         T* __restrict__ dkv, float* __restrict__ dkp) {
+                                                         T* __restrict__ dkv, float* __restrict__ dkp, int parts,
+                                                         float* __restrict__ pkv) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, VS = DV / 16, NN = DN / 32, NK = (DN + DR) / 32, NV = DV / 32;
   constexpr int TQ = sizeof(T) == 2 ? 64 : 32, NS = TQ / 32;
   typedef LTile<T, DN> LN;
@@ -459,6 +467,8 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
   int b, h, blk;
   lat_map(d, b, h, blk);
+  const int part = blk % parts;
+  blk /= parts;
   const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
   const int w0 = 128 * blk + 32 * wave_id();  // this wave's first token
   const int tok = w0 + (lane_id() & 31);
@@ -467,6 +477,12 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   if (d.causal) first = max(0, 128 * blk - off);
   if (128 * blk >= kl) first = ql;
   first &= ~(TQ - 1);
+  int stop = ql;
+  if (parts > 1) {
+    const int tiles = max(0, (ql - first + TQ - 1) / TQ), from = first;
+    first = from + (int)((int64_t)tiles * part / parts) * TQ;
+    stop = min(ql, from + (int)((int64_t)tiles * (part + 1) / parts) * TQ);
+  }
   const T* qb = q + b * d.qs[0] + h * d.qs[2];
   const T* gb = dout + b * d.gs[0] + h * d.gs[2];
   const T* kr = kv + b * d.ks[0] + (int64_t)tokc * d.ks[1] + h * d.ks[2];
@@ -496,12 +512,12 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   for (int n = 0; n < NV; ++n) av[n] = zero16();
   const float c2 = d.scale * kLog2e;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  if (first < ql) load(first, 0);
+  if (first < stop) load(first, 0);
   int q0 = first, buf = 0;
   auto stage = [&] {  // this tile is there, the next one on its way
     vm_wait<0>();
     bare_barrier();
-    if (q0 + TQ < ql) load(q0 + TQ, buf ^ 1);
+    if (q0 + TQ < stop) load(q0 + TQ, buf ^ 1);
   };
   // One tile.  Its two halves follow each other by a phase: the scores of the
   // second half run beside the first half's exponentials, the gradients of the
@@ -574,52 +590,63 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   };
   // tiles that this wave's tokens are not visible to, those on the diagonal, the rest
   // (a wave without tokens only keeps the others company)
-  for (; q0 < ql && (w0 >= kl || (d.causal && w0 > q0 + TQ - 1 + off)); q0 += TQ, buf ^= 1) stage();
-  for (; q0 < ql && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
+  for (; q0 < stop && (w0 >= kl || (d.causal && w0 > q0 + TQ - 1 + off)); q0 += TQ, buf ^= 1) stage();
+  for (; q0 < stop && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<1>());
   }
-  for (; q0 < ql; q0 += TQ, buf ^= 1) {
+  for (; q0 < stop; q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<0>());
   }
   if (tok >= d.S) return;
-  T* out = dkv + (((int64_t)b * d.S + tok) * d.H + h) * (d.dn + d.dv);
-  float* op = dkp + (((int64_t)b * d.H + h) * d.S + tok) * d.dr;
+  const int64_t wide = d.dn + d.dv, at = (((int64_t)b * d.S + tok) * d.H + h) * wide;
+  T* out = dkv + at;
+  float* po = pkv + (int64_t)part * d.B * d.S * d.H * wide + at;
+  float* op = dkp + ((((int64_t)part * d.B + b) * d.H + h) * d.S + tok) * d.dr;
 #pragma unroll
-  for (int n = 0; n < NK; ++n)
+  for (int n = 0; n < NK + NV; ++n)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int c = 32 * n + reg_row(r);
+      const int c = 32 * (n < NK ? n : n - NK) + reg_row(r);
       f32x4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = tok < kl ? ak[n][r + j] * d.scale : 0.f;
-      if (32 * n < DN) {
-        if (c < d.dn) store4(out + c, v);
-      } else if (c - DN < d.dr) {
-        store4(op + c - DN, v);
+      for (int j = 0; j < 4; ++j)
+        v[j] = tok >= kl ? 0.f : n < NK ? ak[n < NK ? n : 0][r + j] * d.scale : av[n < NK ? 0 : n - NK][r + j];
+      if (n >= NN && n < NK) {
+        if (c - DN < d.dr) store4(op + c - DN, v);
+      } else if (c < (n < NK ? d.dn : d.dv)) {
+        const int x = n < NK ? c : d.dn + c;
+        if (parts > 1) store4(po + x, v);
+        else store4(out + x, v);
       }
-    }
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int c = 32 * n + reg_row(r);
-      f32x4 v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = tok < kl ? av[n][r + j] : 0.f;
-      if (c < d.dv) store4(out + d.dn + c, v);
     }
 }
 
-// dk_pe = the heads' parts summed in their order: four elements a thread.
+// The parts of a gradient summed in their order: four elements a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void latent_bwd_dkpe(LatDims d, const float* __restrict__ dkp, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void latent_bwd_join(int64_t n, int parts, const float* __restrict__ p,
+                                                       T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 s = zero4();
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) s += *reinterpret_cast<const f32x4*>(p + k * n + i);
+  store4(out + i, s);
+}
+
+// dk_pe = the heads' shares (of every part of the queries) summed in their order: four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void latent_bwd_dkpe(LatDims d, int parts, const float* __restrict__ dkp,
+                                                       T* __restrict__ out) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, per = (int64_t)d.S * d.dr;
   if (i >= d.B * per) return;
-  const float* p = dkp + i / per * d.H * per + i % per;
   f32x4 s = zero4();
-  for (int h = 0; h < d.H; ++h) s += *reinterpret_cast<const f32x4*>(p + h * per);
+  for (int k = 0; k < parts; ++k) {
+    const float* p = dkp + ((int64_t)k * d.B + i / per) * d.H * per + i % per;
+#pragma unroll 4
+    for (int h = 0; h < d.H; ++h) s += *reinterpret_cast<const f32x4*>(p + h * per);
+  }
   store4(out + i, s);
 }
 
@@ -679,8 +706,27 @@ static size_t fwd_stat_bytes(const atomic_latent_args* a, const FwdPlan& p) {
 }
 constexpr size_t kNoWorkspace = 16;  // what a size function returns where none is needed (0 is a refusal)
 
-static size_t lat_stat_bytes(const atomic_latent_args* a) {
-  return (size_t)a->batch * a->heads * stat_rows(a->tq) * 2 * sizeof(float);
+// The backward's parts of the keys (dq) and of the queries (dk, dv), and its workspace.
+struct BwdPlan {
+  int qparts, kparts;
+  size_t stat, dkp, pq, pkv;  // bytes
+};
+static int parts_for(int64_t wgs, int64_t tiles) {
+  int p = 1;
+  while (p < 16 && 2 * p * wgs <= 256 && 4 * p <= tiles) p *= 2;
+  return p;
+}
+static BwdPlan bwd_plan(const atomic_latent_args* a) {
+  const int64_t bh = (int64_t)a->batch * a->heads, tile = a->dtype == ATOMIC_BF16 ? 64 : 32;
+  BwdPlan p;
+  p.qparts = parts_for(bh * ((a->tq + 127) / 128), (a->tk + tile - 1) / tile);
+  p.kparts = parts_for(bh * ((a->tk + 127) / 128), (a->tq + tile - 1) / tile);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  p.stat = up((size_t)bh * stat_rows(a->tq) * 2 * sizeof(float));
+  p.dkp = up((size_t)p.kparts * bh * a->tk * a->dr * sizeof(float));
+  p.pq = p.qparts > 1 ? up((size_t)p.qparts * bh * a->tq * (a->dn + a->dr) * sizeof(float)) : 0;
+  p.pkv = p.kparts > 1 ? up((size_t)p.kparts * bh * a->tk * (a->dn + a->dv) * sizeof(float)) : 0;
+  return p;
 }
 
 }  // namespace ah
@@ -739,7 +785,8 @@ extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, con
 
 extern "C" size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a) {
   if (lat_check(a) != ATOMIC_OK) return 0;
-  return lat_stat_bytes(a) + (size_t)a->batch * a->heads * a->tk * a->dr * sizeof(float);
+  const BwdPlan p = bwd_plan(a);
+  return p.stat + p.dkp + p.pq + p.pkv;
 }
 
 extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
@@ -752,8 +799,11 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
   if (!workspace || workspace_bytes < atomic_latent_bwd_workspace_size(a) || !aligned16({workspace}))
     return ATOMIC_ERR_WORKSPACE;
   ws_tag_clobber(workspace, atomic_latent_bwd_workspace_size(a));
+  const BwdPlan p = bwd_plan(a);
   float* stat = (float*)workspace;
-  float* dkp = (float*)((char*)workspace + lat_stat_bytes(a));
+  float* dkp = (float*)((char*)stat + p.stat);
+  float* pq = (float*)((char*)dkp + p.dkp);
+  float* pkv = (float*)((char*)pq + p.pq);
   const hipStream_t st = (hipStream_t)stream;
   Launch L{a->profile, st};
   return lat_dispatch(a, [&](auto t, auto w) {
@@ -766,23 +816,33 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
                          (const T*)dout, lse, q_lens, stat);
     });
     if (rc) return rc;
-    d.blocks = (d.S + 127) / 128;
+    auto join = [&](const char* name, int64_t n, int parts, const float* from, void* to) {
+      return parts == 1 ? (int)ATOMIC_OK : L(name, [&] {
+        hipLaunchKernelGGL((latent_bwd_join<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, n, parts,
+                           from, (T*)to);
+      });
+    };
+    d.blocks = (d.S + 127) / 128 * p.kparts;
     rc = L("latent_bwd_dkv", [&] {
       hipLaunchKernelGGL((latent_bwd_dkv<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
                          0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
-                         (const T*)dout, (T*)dkv, dkp);
+                         (const T*)dout, (T*)dkv, dkp, p.kparts, pkv);
     });
     if (rc) return rc;
-    d.blocks = (d.T + 127) / 128;
+    rc = join("latent_bwd_dkv_join", (int64_t)d.B * d.S * d.H * (d.dn + d.dv), p.kparts, pkv, dkv);
+    if (rc) return rc;
+    d.blocks = (d.T + 127) / 128 * p.qparts;
     rc = L("latent_bwd_dq", [&] {
       hipLaunchKernelGGL((latent_bwd_dq<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
                          0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
-                         (const T*)dout, (T*)dq);
+                         (const T*)dout, (T*)dq, p.qparts, pq);
     });
+    if (rc) return rc;
+    rc = join("latent_bwd_dq_join", (int64_t)d.B * d.T * d.H * (d.dn + d.dr), p.qparts, pq, dq);
     if (rc) return rc;
     return L("latent_bwd_dkpe", [&] {
       hipLaunchKernelGGL((latent_bwd_dkpe<T>), dim3((unsigned)(((int64_t)d.B * d.S * d.dr / 4 + 255) / 256)),
-                         dim3(256), 0, st, d, dkp, (T*)dk_pe);
+                         dim3(256), 0, st, d, p.kparts, dkp, (T*)dk_pe);
     });
   });
 }
