@@ -28,8 +28,11 @@ from . import _lib
 _DT = {torch.float32: _lib.ATOMIC_F32, torch.bfloat16: _lib.ATOMIC_BF16}
 
 
+_PIECE = {torch.float32: 3, torch.bfloat16: 7}   # elements of a 16-byte piece, less one
+
+
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
 def _stream(device):
@@ -41,11 +44,14 @@ def _strided(t, n):
     strides (0 for a dimension of one).  The last dimension has to be dense and
     the strides and the address whole 16-byte pieces; anything else is copied.
     Every other order of the first dimensions is read in place."""
-    piece = 16 // t.element_size()
+    mask = _PIECE[t.dtype]
     for _ in range(2):
-        shape, st = t.shape, t.stride()
-        s = [st[i] if shape[i] > 1 else 0 for i in range(n)]
-        if (shape[-1] == 1 or st[-1] == 1) and not any(x % piece for x in s) and t.data_ptr() % 16 == 0:
+        s, odd = t.stride(), t.data_ptr() & 15
+        if s[-1] == 1 and not odd and not any(x & mask for x in s[:n]):
+            return t, s[:n]
+        shape = t.shape
+        s = tuple(s[i] if shape[i] > 1 else 0 for i in range(n))
+        if (shape[-1] == 1 or t.stride(-1) == 1) and not odd and not any(x & mask for x in s):
             return t, s
         t = t.clone() if t.is_contiguous() else t.contiguous()
     raise ValueError("latent attention: rows have to be whole 16-byte pieces (dimensions that are multiples of 8)")
@@ -53,22 +59,23 @@ def _strided(t, n):
 
 def _operands(what, *named):
     """Checks that the operands are on one HIP device and of one supported dtype."""
-    first = named[0][1]
+    name0, first = named[0]
     if not first.is_cuda:
         raise ValueError(f"{what}: inputs must be HIP device tensors")
-    if first.dtype not in _DT:
-        raise TypeError(f"{what}: {named[0][0]} must be bfloat16 or float32")
+    dtype, device = first.dtype, first.get_device()
+    if dtype not in _DT:
+        raise TypeError(f"{what}: {name0} must be bfloat16 or float32")
     for name, t in named[1:]:
-        if t.device != first.device:
-            raise ValueError(f"{what}: {name} must be on {named[0][0]}'s device")
-        if t.dtype != first.dtype:
-            raise TypeError(f"{what}: {name} must have {named[0][0]}'s dtype")
+        if t.get_device() != device:
+            raise ValueError(f"{what}: {name} must be on {name0}'s device")
+        if t.dtype != dtype:
+            raise TypeError(f"{what}: {name} must have {name0}'s dtype")
 
 
 def _index(what, name, t, shape, dtype, device):
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device:
+    if t.dtype != dtype or t.shape != shape or t.get_device() != device:
         raise ValueError(f"{what}: {name} must be {str(dtype)[6:]} {list(shape)} on the inputs' device")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # ------------------------------------------------------------ expanded form
@@ -80,9 +87,11 @@ def _check(q, kv, k_pe, q_lens, kv_lens):
     S, dr = k_pe.shape[1:]
     if kv.shape[:3] != (B, S, H) or k_pe.shape[0] != B or not 0 < dr < d or kv.shape[3] <= d - dr:
         raise ValueError("q must be [B, T, H, dn + dr], kv [B, S, H, dn + dv] and k_pe [B, S, dr]")
-    lens = [None if t is None else _index("latent attention", n, t, (B,), torch.int32, q.device)
-            for n, t in (("q_lens", q_lens), ("kv_lens", kv_lens))]
-    return lens
+    if q_lens is not None:
+        q_lens = _index("latent attention", "q_lens", q_lens, (B,), torch.int32, q.get_device())
+    if kv_lens is not None:
+        kv_lens = _index("latent attention", "kv_lens", kv_lens, (B,), torch.int32, q.get_device())
+    return q_lens, kv_lens
 
 
 def make_args(q, kv, k_pe, scale, causal, dout=None):
@@ -96,7 +105,7 @@ def make_args(q, kv, k_pe, scale, causal, dout=None):
     if dout is not None:
         dout, gs = _strided(dout, 3)
     args = _lib.LatentArgs(B, T, S, H, d - dr, dr, kv.shape[3] - (d - dr), _DT[q.dtype], 1 if causal else 0, scale,
-                           tuple(qs), tuple(ks), tuple(ps), tuple(gs))
+                           qs, ks, ps, gs)
     return args, (q, kv, k_pe, dout)
 
 
@@ -138,7 +147,7 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     _operands("latent attention", ("q", q), ("o", o), ("dout", dout))
     if o.shape != (B, T, H, dv) or dout.shape != o.shape:
         raise ValueError("o and dout must be [B, T, H, dv]")
-    if lse.shape != (B, H, T) or lse.dtype != torch.float32 or lse.device != q.device:
+    if lse.shape != (B, H, T) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise ValueError("lse must be float32 [B, H, T] on q's device")
     lib = _lib.load()
     args, (q, kv, k_pe, dout) = make_args(q, kv, k_pe, scale, causal, dout)
@@ -184,9 +193,9 @@ def attention(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None):
 # ------------------------------------------------------------ paged cache
 def _tables(what, cos, sin, dr, device):
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != dr // 2 or \
-            cos.shape[0] < 1 or sin.shape != cos.shape or cos.device != device or sin.device != device:
+            cos.shape[0] < 1 or sin.shape != cos.shape or cos.get_device() != device or sin.get_device() != device:
         raise ValueError(f"{what}: cos and sin must be float32 [positions, dr / 2] on the inputs' device")
-    return cos.contiguous(), sin.contiguous()
+    return cos if cos.is_contiguous() else cos.contiguous(), sin if sin.is_contiguous() else sin.contiguous()
 
 
 def _cache(what, cache, width):
@@ -210,6 +219,7 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
     if k_pe.dim() != 2:
         raise ValueError("latent append: k_pe must be [N, dr]")
     N, dr = k_pe.shape
+    dev = k_pe.get_device()
     pages, page, dc, cs = 1, 1, 8, (0,)
     if cache is not None:
         if c_kv is None or slots is None or c_kv.dim() != 2 or c_kv.shape[0] != N:
@@ -217,10 +227,10 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
         dc = c_kv.shape[1]
         _cache("latent append", cache, dc + dr)
         pages, page = cache.shape[:2]
-        slots = _index("latent append", "slots", slots, (N,), torch.int64, k_pe.device)
+        slots = _index("latent append", "slots", slots, (N,), torch.int64, dev)
         c_kv, cs = _strided(c_kv, 1)
-    positions = _index("latent append", "positions", positions, (N,), torch.int32, k_pe.device)
-    cos, sin = _tables("latent append", cos, sin, dr, k_pe.device)
+    positions = _index("latent append", "positions", positions, (N,), torch.int32, dev)
+    cos, sin = _tables("latent append", cos, sin, dr, dev)
     k_pe, ks = _strided(k_pe, 1)
     H, dn, qs, q_out = 1, 8, (0, 0), None
     if q is not None:
@@ -231,7 +241,7 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = torch.empty(N, dr, dtype=k_pe.dtype, device=k_pe.device)
     args = _lib.LatentAppendArgs(N, H, dn, dr, dc, _DT[k_pe.dtype], page, pages, cos.shape[0], 1 if interleaved else 0,
-                                 cs[0], ks[0], tuple(qs))
+                                 cs[0], ks[0], qs)
     if timer is not None:
         args.profile = timer.arm()
     rc = _lib.load().atomic_latent_append(ctypes.byref(args), _ptr(c_kv), _ptr(k_pe), _ptr(slots), _ptr(positions),
@@ -255,6 +265,7 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
     if q.dim() != 4 or w_kv.dim() != 3 or w_kv.shape[0] != q.shape[2]:
         raise ValueError("latent decode: q must be [B, n, H, dn + dr] and w_kv [H, dn + dv, dc]")
     B, n, H, d = q.shape
+    dev = q.get_device()
     dc = w_kv.shape[2]
     if cache.dim() != 3 or not 0 < cache.shape[2] - dc < d or w_kv.shape[1] <= d - (cache.shape[2] - dc):
         raise ValueError("latent decode: cache must be [pages, page, dc + dr], w_kv [H, dn + dv, dc]")
@@ -262,18 +273,18 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
     _cache("latent decode", cache, dc + dr)
     if page_table.dim() != 2:
         raise ValueError("latent decode: page_table must be int32 [B, pages]")
-    page_table = _index("latent decode", "page_table", page_table, (B, page_table.shape[1]), torch.int32, q.device)
-    kv_lens = _index("latent decode", "kv_lens", kv_lens, (B,), torch.int32, q.device)
+    page_table = _index("latent decode", "page_table", page_table, (B, page_table.shape[1]), torch.int32, dev)
+    kv_lens = _index("latent decode", "kv_lens", kv_lens, (B,), torch.int32, dev)
     if (cos is None) != (sin is None):
         raise ValueError("latent decode: cos and sin come together")
     if cos is not None:
-        cos, sin = _tables("latent decode", cos, sin, dr, q.device)
+        cos, sin = _tables("latent decode", cos, sin, dr, dev)
     q, qs = _strided(q, 3)
     w_kv, _ = _strided(w_kv.contiguous(), 2)
     lib = _lib.load()
     args = _lib.LatentDecodeArgs(B, n, H, d - dr, dr, w_kv.shape[1] - (d - dr), dc, _DT[q.dtype], cache.shape[1],
                                  cache.shape[0], page_table.shape[1], 0 if cos is None else cos.shape[0],
-                                 1 if interleaved else 0, scale, tuple(qs))
+                                 1 if interleaved else 0, scale, qs)
     if timer is not None:
         args.profile = timer.arm()
     nbytes = lib.atomic_latent_decode_workspace_size(ctypes.byref(args))
