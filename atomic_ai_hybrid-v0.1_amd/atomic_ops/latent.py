@@ -28,6 +28,7 @@ from . import _lib
 _DT = {torch.float32: _lib.ATOMIC_F32, torch.bfloat16: _lib.ATOMIC_BF16}
 
 
+_MOST_ROW_BYTES = 1 << 25
 _PIECE = {torch.float32: 3, torch.bfloat16: 7}   # elements of a 16-byte piece, less one
 
 
@@ -94,16 +95,22 @@ def _check(q, kv, k_pe, q_lens, kv_lens):
     return q_lens, kv_lens
 
 
+def _rows(t, n):
+    """``_strided`` for [B, rows, ...]; rows more than 32 MB apart are copied too."""
+    t, s = _strided(t, n)
+    return (t, s) if s[1] * t.element_size() <= _MOST_ROW_BYTES else _strided(t.contiguous(), n)
+
+
 def make_args(q, kv, k_pe, scale, causal, dout=None):
     """``(args, operands)``: the args struct and the operands as the library reads them."""
     B, T, H, d = q.shape
     S, dr = k_pe.shape[1:]
-    q, qs = _strided(q, 3)
-    kv, ks = _strided(kv, 3)
-    k_pe, ps = _strided(k_pe, 2)
+    q, qs = _rows(q, 3)
+    kv, ks = _rows(kv, 3)
+    k_pe, ps = _rows(k_pe, 2)
     gs = (0, 0, 0)
     if dout is not None:
-        dout, gs = _strided(dout, 3)
+        dout, gs = _rows(dout, 3)
     args = _lib.LatentArgs(B, T, S, H, d - dr, dr, kv.shape[3] - (d - dr), _DT[q.dtype], 1 if causal else 0, scale,
                            qs, ks, ps, gs)
     return args, (q, kv, k_pe, dout)

@@ -280,6 +280,22 @@ __device__ __forceinline__ void dma16_raw_s(uint64_t base, uint32_t off, uint32_
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst)
                : "memory", "m0");
 }
+// The same through a buffer descriptor (buffer_of) at the lane's byte offset plus
+// a uniform one; what lies past the descriptor's bytes is written as zeros.
+typedef uint32_t buffer_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ buffer_t buffer_of(uint64_t base, uint32_t bytes) {
+  buffer_t d;
+  d[0] = __builtin_amdgcn_readfirstlane((uint32_t)base);
+  d[1] = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu);  // raw: no stride, no swizzle
+  d[2] = __builtin_amdgcn_readfirstlane(bytes);
+  d[3] = 0x00020000;  // 32-bit data
+  return d;
+}
+__device__ __forceinline__ void dma16_buf(buffer_t d, uint32_t lane_off, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_off), "s"(d),
+               "s"(off), "s"(dst)
+               : "memory", "m0");
+}
 // One dword a lane to 256 consecutive bytes.
 __device__ __forceinline__ void dma4_raw(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");

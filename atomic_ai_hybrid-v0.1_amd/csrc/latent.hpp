@@ -163,40 +163,95 @@ __device__ __forceinline__ void in_groups(L&& load, U&& use) {
 
 // Rows of a matrix (W elements, `width` of them real) straight to an LTile of ROWS
 // rows, NW waves taking 1 KB each in turn: wave w's i-th load covers the rows
-// RPI (w + NW i) .. + RPI - 1.  Rows past `last` repeat it (what lies there is never
-// read and the products are masked); the padding of the width reads the row's first
+// RPI (w + NW i) .. + RPI - 1.  Rows past `last` are zeros (their products are masked,
+// and what lies there is never read); the padding of the width reads the row's first
 // piece (the other operand is zero there, or the product's column is not stored).
+//
+// A load is one instruction and no vector arithmetic, to be spread over the MFMAs
+// of a tile: a CU takes 64 bytes a clock on this path, so a tile's 40 KB sent for at
+// once hold every wave up for 600 to 1000 clocks.
+constexpr int64_t kMostRowBytes = 1 << 25;  // a tile's byte offsets have to fit 31 bits
 template <typename T, int W, int ROWS, int NW>
 struct RowDma {
   typedef LTile<T, W> L;
   static constexpr int RPI = 64 / L::NC, N = ROWS / RPI / NW, STEP = NW * RPI;
   static constexpr int NZ = STEP >= 16 ? 1 : 16 / STEP;  // the swizzle repeats every 16 rows
   static_assert(RPI * L::NC == 64 && N * STEP == ROWS && (STEP >= 16 || 16 % STEP == 0), "whole loads");
-  const char* base;  // uniform: row 0
-  int64_t ld;        // bytes a row
-  int r0, cb[NZ];    // this lane's row in the first load, byte in the row
+  uint64_t base;      // the first row aimed at
+  int left;           // rows from it to the last
+  uint32_t ld, wide;  // bytes between rows, bytes of a row
+  uint32_t at[NZ];    // this lane's byte in the first load
+  buffer_t d;
   __device__ __forceinline__ void init(const T* p, int64_t stride, int width) {
-    base = (const char*)p;
-    ld = stride * (int64_t)sizeof(T);
-    r0 = RPI * wave_id() + lane_id() / L::NC;
+    base = (uint64_t)p;
+    ld = (uint32_t)(stride * (int64_t)sizeof(T));
+    wide = width * (uint32_t)sizeof(T);
+    const int r0 = RPI * wave_id() + lane_id() / L::NC;
 #pragma unroll
     for (int z = 0; z < NZ; ++z) {
       const int c = (lane_id() % L::NC) ^ L::swz(r0 + z * STEP);
-      cb[z] = c * L::VEC < width ? 16 * c : 0;
+      at[z] = r0 * ld + (c * L::VEC < width ? 16 * c : 0);
     }
   }
-  // `dst`: the tile's LDS address
-  __device__ __forceinline__ void load(int k0, int last, uint32_t dst) const {
-    dst += 1024 * wave_id();
-    if (k0 + ROWS - 1 <= last) {
-      const char* p = base + k0 * ld + (int64_t)r0 * ld;
+  // the rows k0 .. last are next, a tile at a time; zeros past them
+  __device__ __forceinline__ void start(int k0, int last) {
+    ld = __builtin_amdgcn_readfirstlane(ld);
+    base += (uint64_t)k0 * ld;
+    base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base);
+    left = __builtin_amdgcn_readfirstlane(last - k0 + 1);
+  }
+  __device__ __forceinline__ void aim() {
+    d = buffer_of(base, left > 0 ? (uint32_t)(min(left, ROWS) - 1) * ld + wide : 0);
+    base += ROWS * (uint64_t)ld;
+    left -= ROWS;
+  }
+  // the same for one tile by itself, without `start`
+  __device__ __forceinline__ void aim_at(int k0, int last) {
+    d = buffer_of(base + (uint64_t)k0 * ld, k0 <= last ? (uint32_t)min(last - k0, ROWS - 1) * ld + wide : 0);
+  }
+  // this wave's i-th load; `dst`: the tile's LDS address
+  __device__ __forceinline__ void load(int i, uint32_t dst) const {
+    dma16_buf(d, at[i % NZ], (uint32_t)(i * STEP) * ld, dst + 1024 * (wave_id() + NW * i));
+  }
+};
+// Three of them one after the other: the tiles of a stage.
+template <typename A, typename B, typename C>
+struct StageDma {
+  A a;
+  B b;
+  C c;
+  uint32_t ob, oc;  // where the second and the third tile lie behind the first
+  static constexpr int N = A::N + B::N + C::N;
+  __device__ __forceinline__ void start(int k0, int last) {
+    a.start(k0, last);
+    b.start(k0, last);
+    c.start(k0, last);
+  }
+  __device__ __forceinline__ void aim() {
+    a.aim();
+    b.aim();
+    c.aim();
+  }
+  __device__ __forceinline__ void aim_at(int k0, int last) {
+    a.aim_at(k0, last);
+    b.aim_at(k0, last);
+    c.aim_at(k0, last);
+  }
+  __device__ __forceinline__ void load(int i, uint32_t dst) const {
+    if (i < A::N) a.load(i, dst);
+    else if (i < A::N + B::N) b.load(i - A::N, dst + ob);
+    else c.load(i - A::N - B::N, dst + oc);
+  }
+  // the loads that belong to slot j of `slots`
+  __device__ __forceinline__ void at_slot(int j, int slots, uint32_t dst) const {
 #pragma unroll
-      for (int i = 0; i < N; ++i) dma16_raw(p + ((int64_t)(i * STEP) * ld + cb[i % NZ]), dst + 1024 * NW * i);
-    } else {
+    for (int i = 0; i < N; ++i)
+      if (i * slots / N == j) load(i, dst);
+  }
+  __device__ __forceinline__ void all(uint32_t dst) const {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        dma16_raw(base + ((int64_t)min(k0 + r0 + i * STEP, last) * ld + cb[i % NZ]), dst + 1024 * NW * i);
-    }
+    for (int i = 0; i < N; ++i) load(i, dst);
   }
 };
 

@@ -82,7 +82,8 @@ __global__ __launch_bounds__(64 * NW, 2) void latent_fwd(LatDims d, int parts, c
                                                          float* __restrict__ lse, float* __restrict__ pacc,
                                                          float* __restrict__ pstat) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, NT = DV / 32, TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
-  constexpr int RB = 32 * NW, NB = 2;  // rows a workgroup, tiles in LDS
+  constexpr int FG = 1, FL = 3;  // fragments are read three MFMAs ahead
+  constexpr int RB = 32 * NW, NB = NW == 8 ? 3 : 2;  // rows a workgroup, tiles in LDS
   typedef LTile<T, DN> LN;
   typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LV;
@@ -107,12 +108,12 @@ __global__ __launch_bounds__(64 * NW, 2) void latent_fwd(LatDims d, int parts, c
   }
   const T* qr = q + b * d.qs[0] + (int64_t)max(min(row, ql - 1), 0) * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
-  RowDma<T, DN, TK, NW> dn;
-  RowDma<T, DR, TK, NW> dr;
-  RowDma<T, DV, TK, NW> dv;
-  dn.init(kb, d.ks[1], d.dn);
-  dr.init(kpe + b * d.ps[0], d.ps[1], d.dr);
-  dv.init(kb + d.dn, d.ks[1], d.dv);
+  StageDma<RowDma<T, DN, TK, NW>, RowDma<T, DR, TK, NW>, RowDma<T, DV, TK, NW>> dma;
+  dma.a.init(kb, d.ks[1], d.dn);
+  dma.b.init(kpe + b * d.ps[0], d.ps[1], d.dr);
+  dma.c.init(kb + d.dn, d.ks[1], d.dv);
+  dma.ob = OR;
+  dma.oc = OV;
   frag qf[KS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   // (a scale of zero as the smallest number: a masked score stays infinite; a negative one changes q's sign)
@@ -126,40 +127,35 @@ __global__ __launch_bounds__(64 * NW, 2) void latent_fwd(LatDims d, int parts, c
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
   float m = -INFINITY, sum = 0.f;  // reference (of c2 times the scores, see kLag) and this lane's part of the sum
   const uint32_t l0 = lds_addr(lds);
-  auto load = [&](int k0, int buf) {
-    const uint32_t at = l0 + buf * STAGE;
-    dn.load(k0, kl - 1, at);
-    dr.load(k0, kl - 1, at + OR);
-    dv.load(k0, kl - 1, at + OV);
-  };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the query: no later wait for it drains the tiles
-  constexpr int PER = RowDma<T, DN, TK, NW>::N + RowDma<T, DR, TK, NW>::N + RowDma<T, DV, TK, NW>::N;
-  if (begin < end) load(begin, 0);
-  if (NB == 3 && begin + TK < end) load(begin + TK, 1);
-  int buf = 0;
-  for (int k0 = begin; k0 < end; k0 += TK, buf = buf + 1 == NB ? 0 : buf + 1) {
-    if (NB == 3 && k0 + TK < end) vm_wait<PER>();
-    else vm_wait<0>();
-    bare_barrier();  // the tile is there, and nobody reads the one before it any more
-    if (k0 + (NB - 1) * TK < end) load(k0 + (NB - 1) * TK, buf == 0 ? NB - 1 : buf - 1);
-    if (w0 >= ql || (d.causal && k0 > w0 + 31 + off)) continue;  // nothing visible to this wave
-    const char* sk = lds + buf * STAGE;
-    f32x16 s[NS];
+  constexpr int PER = decltype(dma)::N;
+  f32x16 s[NS];
+  // Scores of a tile, masked, and a new reference where one is far above its row's.
+  // `to`: where the tile that `dma` aims at goes, sent for along the way (with eight
+  // waves beside the values, with four beside the scores).  Past the last key there
+  // are tiles of zeros, so that every tile sends for one and waits alike.
+  auto scores = [&](const char* sk, int k0, uint32_t to) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) s[i] = zero16();
-    in_groups<KS * NS, 4, frag>(
+    in_groups<KS * NS, FG, FL, 0, frag>(
         [&](int j) {
           const int t = j / NS, i = j % NS;
           return t < KN ? LN::row(sk, 32 * i, 16 * t) : LR::row(sk + OR, 32 * i, 16 * (t - KN));
         },
-        [&](int j, frag a) { s[j % NS] = M32<T>::mma(a, qf[j / NS], s[j % NS]); });
+        [&](int j, frag a) { s[j % NS] = M32<T>::mma(a, qf[j / NS], s[j % NS]); },
+        [&](int j) {
+          if (NW == 4) dma.at_slot(j, KS * NS, to);
+        });
     if (k0 + TK > kl || (d.causal && k0 + TK - 1 > w0 + off)) {
-      const int seen = min(kl, d.causal ? row + off + 1 : kl) - k0;
+      const int seen = min(kl, d.causal ? row + off + 1 : kl) - k0 - reg_row(0);
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * i + reg_row(r) >= seen) s[i][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+          int lim = seen;  // (each compare by itself: chained, their conditions fill the scalar registers)
+          asm volatile("" : "+v"(lim));
+          s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? s[i][r] : -INFINITY;
+        }
     }
     float top = s[0][0];
 #pragma unroll
@@ -177,21 +173,86 @@ __global__ __launch_bounds__(64 * NW, 2) void latent_fwd(LatDims d, int parts, c
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[n][r] *= fade;
     }
+  };
+  // The tile's probabilities and their products with the values; the second half's
+  // exponentials run beside the first half's products.
+  auto values = [&](const char* sk, uint32_t to) {
     const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
     frag p[2 * NS];
+    auto quad = [&](int i, int k) {  // four tokens
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[i][r] = fast_exp2(__builtin_fmaf(s[i][r], c2, ref));
-        sum += s[i][r];
+      for (int j = 0; j < 4; ++j) {
+        const float x = fast_exp2(__builtin_fmaf(s[i][4 * k + j], c2, ref));
+        sum += x;
+        p[2 * i + k / 2][4 * (k & 1) + j] = (T)x;
       }
-      p[2 * i] = pack_frag<T>(s[i], 0);
-      p[2 * i + 1] = pack_frag<T>(s[i], 1);
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) quad(0, k);
+    __builtin_amdgcn_sched_barrier(0);
+    in_groups<2 * NS * NT, FG, FL, NS == 2 ? 14 : 0, frag>(
+        [&](int j) { return LV::col(sk + OV, 16 * (j / NT), 32 * (j % NT)); },
+        [&](int j, frag a) { acc[j % NT] = M32<T>::mma(a, p[j / NT], acc[j % NT]); },
+        [&](int j) {
+          if (NW == 8) dma.at_slot(j, 2 * NS * NT, to);
+          if (NS == 2 && j < 4) quad(1, j);
+        });
+    static_assert(NS == 1 || 2 * NT >= 4, "the second half's probabilities are there in time");
+  };
+  auto sees = [&](int k0) { return w0 < ql && !(d.causal && k0 > w0 + 31 + off); };  // anything of the tile at k0
+  dma.start(begin, min(kl, end) - 1);
+  if constexpr (NW == 8) {
+    // Waves 4-7 run half a tile behind waves 0-3, which share their SIMDs: one wave's
+    // scores beside the other's softmax and values.  (The scores' wave goes first
+    // where both could: a matrix instruction leaves seven of eight issue slots.)
+    // Barrier 2 t lets the first wave of a SIMD into tile t, barrier 2 t + 1 the
+    // second.  Tile t is read until barrier 2 t + 3; with three places in LDS tile
+    // t + 2 is sent for after barrier 2 t + 1 (the second waves' share after 2 t + 2)
+    // and has to be there at barrier 2 t + 4.
+    const bool second = wave_id() >= 4;
+    dma.aim();
+    dma.all(l0);
+    dma.aim();
+    dma.all(l0 + STAGE);
+    vm_wait<PER>();
+    bare_barrier();
+    if (second) bare_barrier();
+    int at = 0, far = 2;  // the tile's place, and its successor's successor's
+    for (int k0 = begin; k0 < end; k0 += TK) {
+      const char* sk = lds + at * STAGE;
+      const uint32_t to = l0 + far * STAGE;
+      __builtin_amdgcn_s_setprio(3);
+      if (sees(k0)) scores(sk, k0, to);
+      __builtin_amdgcn_s_setprio(0);
+      if (second) vm_wait<0>();  // (its share of tile t + 1)
+      bare_barrier();
+      dma.aim();
+      if (sees(k0)) values(sk, to);
+      else dma.all(to);
+      if (!second) vm_wait<PER>();
+      far = at;
+      at = at == 2 ? 0 : at + 1;
+      bare_barrier();
     }
-    in_groups<2 * NS * NT, 4, frag>([&](int j) { return LV::col(sk + OV, 16 * (j / NT), 32 * (j % NT)); },
-                                    [&](int j, frag a) { acc[j % NT] = M32<T>::mma(a, p[j / NT], acc[j % NT]); });
+    if (!second) bare_barrier();
+  } else {
+    dma.aim();
+    dma.all(l0);
+    int buf = 0;
+    for (int k0 = begin; k0 < end; k0 += TK, buf ^= 1) {
+      vm_wait<0>();
+      bare_barrier();  // the tile is there, and nobody reads the other one any more
+      const uint32_t to = l0 + (buf ^ 1) * STAGE;
+      dma.aim();
+      if (sees(k0)) {
+        scores(lds + buf * STAGE, k0, to);
+        values(lds + buf * STAGE, 0);
+      } else {
+        dma.all(to);
+      }
+    }
   }
+  vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
   if (row >= d.T) return;
   sum += __shfl_xor(sum, 32);
   const int64_t at = ((int64_t)b * d.H + h) * d.T + row;
@@ -326,12 +387,12 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   const int rowc = max(min(row, ql - 1), 0);
   const T* qr = q + b * d.qs[0] + (int64_t)rowc * d.qs[1] + h * d.qs[2];
   const T* kb = kv + b * d.ks[0] + h * d.ks[2];
-  RowDma<T, DN, TK, 4> dn;
-  RowDma<T, DR, TK, 4> dr;
-  RowDma<T, DV, TK, 4> dv;
-  dn.init(kb, d.ks[1], d.dn);
-  dr.init(kpe + b * d.ps[0], d.ps[1], d.dr);
-  dv.init(kb + d.dn, d.ks[1], d.dv);
+  StageDma<RowDma<T, DN, TK, 4>, RowDma<T, DR, TK, 4>, RowDma<T, DV, TK, 4>> dma;
+  dma.a.init(kb, d.ks[1], d.dn);
+  dma.b.init(kpe + b * d.ps[0], d.ps[1], d.dr);
+  dma.c.init(kb + d.dn, d.ks[1], d.dv);
+  dma.ob = OR;
+  dma.oc = OV;
   frag qf[KS], gf[VS];
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   row_frags<T, DV, 0>(gf, dout + b * d.gs[0] + (int64_t)rowc * d.gs[1] + h * d.gs[2], d.dv, (const T*)nullptr, 0);
@@ -342,19 +403,17 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
   const float c2 = d.scale * kLog2e;
   const uint32_t l0 = lds_addr(lds);
-  auto load = [&](int k0, int buf) {
-    const uint32_t at = l0 + buf * STAGE;
-    dn.load(k0, kl - 1, at);
-    dr.load(k0, kl - 1, at + OR);
-    dv.load(k0, kl - 1, at + OV);
-  };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  if (begin < end) load(begin, 0);
+  const int past = begin < end ? end - 1 : -1;  // the last key wanted
+  dma.aim_at(begin, past);
+  dma.all(l0);
   int k0 = begin, buf = 0;
-  auto stage = [&] {  // this tile is there, the next one on its way
+  uint32_t to;         // where the next tile goes
+  auto stage = [&] {  // this tile is there; the next one (past the last, zeros) is sent for along the way
     vm_wait<0>();
     bare_barrier();
-    if (k0 + TK < end) load(k0 + TK, buf ^ 1);
+    to = l0 + (buf ^ 1) * STAGE;
+    dma.aim_at(k0 + TK, past);
   };
   // one tile, its halves a phase apart as in latent_bwd_dkv
   auto step = [&](auto masked) {
@@ -403,12 +462,14 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
             else grad((j - 2 * M1) / M2, (j - 2 * M1) % M2, a);
           },
           [&](int j) {
+            dma.at_slot(j, 2 * M1 + 2 * M2, to);
             if (j >= M1 && j < 2 * M1 && (j - M1) % (M1 / 4) == 1 && (j - M1) / (M1 / 4) < 4) prob(0, (j - M1) / (M1 / 4));
             if (M2 >= 8 && j >= 2 * M1 && j < 2 * M1 + M2 && (j - 2 * M1) % (M2 / 4) == 1 && (j - 2 * M1) / (M2 / 4) < 4)
               prob(1, (j - 2 * M1) / (M2 / 4));
             if (M2 < 8 && j >= 2 * M1 && j < 2 * M1 + 4) prob(1, j - 2 * M1);
           });
     } else {
+      dma.all(to);
       in_groups<M1, 4, frag>([&](int j) { return row_at(0, j); }, [&](int j, frag a) { score(0, j, a); });
 #pragma unroll
       for (int k = 0; k < 4; ++k) prob(0, k);
@@ -426,7 +487,11 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
     stage();
     step(IntC<1>());
   }
-  for (; k0 < end; k0 += TK, buf ^= 1) stage();
+  for (; k0 < end; k0 += TK, buf ^= 1) {
+    stage();
+    dma.all(to);
+  }
+  vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
   if (row >= d.T) return;
   T* out = dq + (((int64_t)b * d.T + row) * d.H + h) * (d.dn + d.dr);
   float* po = pq + ((((int64_t)part * d.B + b) * d.T + row) * d.H + h) * (d.dn + d.dr);
@@ -486,21 +551,18 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   const T* qb = q + b * d.qs[0] + h * d.qs[2];
   const T* gb = dout + b * d.gs[0] + h * d.gs[2];
   const T* kr = kv + b * d.ks[0] + (int64_t)tokc * d.ks[1] + h * d.ks[2];
-  RowDma<T, DN, TQ, 4> dn;
-  RowDma<T, DR, TQ, 4> dr;
-  RowDma<T, DV, TQ, 4> dg;
-  dn.init(qb, d.qs[1], d.dn);
-  dr.init(qb + d.dn, d.qs[1], d.dr);
-  dg.init(gb, d.gs[1], d.dv);
+  StageDma<RowDma<T, DN, TQ, 4>, RowDma<T, DR, TQ, 4>, RowDma<T, DV, TQ, 4>> dma;
+  dma.a.init(qb, d.qs[1], d.dn);
+  dma.b.init(qb + d.dn, d.qs[1], d.dr);
+  dma.c.init(gb, d.gs[1], d.dv);
+  dma.ob = OR;
+  dma.oc = OG;
   // wave 0 brings delta, wave 1 lse (64 rows; an fp32 tile uses half of them)
   const float* sb = stat + ((wave_id() & 1 ? (int64_t)d.B * d.H : 0) + (int64_t)b * d.H + h) * stat_rows(d.T);
   const uint32_t l0 = lds_addr(lds);
-  auto load = [&](int r0, int buf) {
-    const uint32_t at = l0 + buf * STAGE;
-    dn.load(r0, ql - 1, at);
-    dr.load(r0, ql - 1, at + OR);
-    dg.load(r0, ql - 1, at + OG);
-    if (wave_id() < 2) dma4_raw(sb + (r0 & ~63) + lane_id(), at + OS + 256 * wave_id());
+  auto aim = [&](int r0, uint32_t to) {
+    dma.aim_at(r0, ql - 1);
+    if (r0 < ql && wave_id() < 2) dma4_raw(sb + (r0 & ~63) + lane_id(), to + OS + 256 * wave_id());
   };
   frag kf[KS], vf[VS];
   row_frags<T, DN, DR>(kf, kr, d.dn, kpe + b * d.ps[0] + (int64_t)tokc * d.ps[1], d.dr);
@@ -512,12 +574,15 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   for (int n = 0; n < NV; ++n) av[n] = zero16();
   const float c2 = d.scale * kLog2e;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  if (first < stop) load(first, 0);
+  aim(first, l0);
+  dma.all(l0);
   int q0 = first, buf = 0;
-  auto stage = [&] {  // this tile is there, the next one on its way
+  uint32_t to;         // where the next tile goes
+  auto stage = [&] {  // this tile is there; the next one (past the last, zeros) is sent for along the way
     vm_wait<0>();
     bare_barrier();
-    if (q0 + TQ < stop) load(q0 + TQ, buf ^ 1);
+    to = l0 + (buf ^ 1) * STAGE;
+    aim(q0 + TQ, to);
   };
   // One tile.  Its two halves follow each other by a phase: the scores of the
   // second half run beside the first half's exponentials, the gradients of the
@@ -577,11 +642,13 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
             else grad((j - 2 * M1) / M2, (j - 2 * M1) % M2, a);
           },
           [&](int j) {
+            dma.at_slot(j, 2 * M1 + 2 * M2, to);
             if (j >= M1 && j < 2 * M1 && (j - M1) % (M1 / 4) == 1 && (j - M1) / (M1 / 4) < 4) prob(0, (j - M1) / (M1 / 4));
             if (j >= 2 * M1 && j < 2 * M1 + M2 && (j - 2 * M1) % (M2 / 4) == 1 && (j - 2 * M1) / (M2 / 4) < 4)
               prob(1, (j - 2 * M1) / (M2 / 4));
           });
     } else {
+      dma.all(to);
       in_groups<M1, 4, frag>([&](int j) { return row_at(0, j); }, [&](int j, frag a) { score(0, j, a); });
 #pragma unroll
       for (int k = 0; k < 4; ++k) prob(0, k);
@@ -590,7 +657,10 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   };
   // tiles that this wave's tokens are not visible to, those on the diagonal, the rest
   // (a wave without tokens only keeps the others company)
-  for (; q0 < stop && (w0 >= kl || (d.causal && w0 > q0 + TQ - 1 + off)); q0 += TQ, buf ^= 1) stage();
+  for (; q0 < stop && (w0 >= kl || (d.causal && w0 > q0 + TQ - 1 + off)); q0 += TQ, buf ^= 1) {
+    stage();
+    dma.all(to);
+  }
   for (; q0 < stop && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<1>());
@@ -599,6 +669,7 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
     stage();
     step(IntC<0>());
   }
+  vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
   if (tok >= d.S) return;
   const int64_t wide = d.dn + d.dv, at = (((int64_t)b * d.S + tok) * d.H + h) * wide;
   T* out = dkv + at;
@@ -663,6 +734,9 @@ static int lat_check(const atomic_latent_args* a) {
   if (bh > INT32_MAX || bh * ((most + 127) / 128) > INT32_MAX || bh * (stat_rows((int)most) / 16) > INT32_MAX ||
       (int64_t)a->batch * ((a->tk + 15) / 16) * a->dr > INT32_MAX)
     return ATOMIC_ERR_SHAPE;
+  const int64_t es = a->dtype == ATOMIC_BF16 ? 2 : 4;
+  for (int64_t s : {a->q_stride[1], a->kv_stride[1], a->kpe_stride[1], a->do_stride[1]})
+    if (s > kMostRowBytes / es) return ATOMIC_ERR_SHAPE;
   if (!whole_pieces({a->q_stride[0], a->q_stride[1], a->q_stride[2], a->kv_stride[0], a->kv_stride[1],
                      a->kv_stride[2], a->kpe_stride[0], a->kpe_stride[1], a->do_stride[0], a->do_stride[1],
                      a->do_stride[2]}, a->dtype))

@@ -797,7 +797,7 @@ typedef struct atomic_latent_args {
   float scale;        /* of the scores                                      */
   /* strides of q [B, tq, H, dn + dr], kv [B, tk, H, dn + dv] (k_nope | v) and
      do [B, tq, H, dv]: batch row, token, head; of k_pe [B, tk, dr]: batch row,
-     token.  The last dimension is dense. */
+     token.  The last dimension is dense; a token stride is 32 MB at most. */
   int64_t q_stride[3];
   int64_t kv_stride[3];
   int64_t kpe_stride[2];

@@ -183,6 +183,21 @@ def test_rows_further_apart_than_32_bits():
         assert torch.equal(a, b)
 
 
+def test_tokens_further_apart_than_a_tile_reaches():
+    """Tokens 33 MB apart (the tokens of a transposed tensor) are copied, in the library's own call refused."""
+    banner("latent expanded token strides past the library's")
+    B, T, H, dn, dr, dv = 1, 3, 2, 64, 32, 64
+    q, kv, k_pe, _ = (t.cuda() for t in _inputs(B, T, T, H, dn, dr, dv, BF16, seed=16))
+    ld = (1 << 24) + 8 * H * (dn + dv)
+    far = torch.empty(2 * ld + H * (dn + dv), dtype=BF16, device="cuda").as_strided(kv.shape, (8, ld, dn + dv, 1))
+    far.copy_(kv)
+    for a, b in zip(L.forward(q, far, k_pe, 0.1), L.forward(q, kv, k_pe, 0.1)):
+        assert torch.equal(a, b)
+    args, _ = L.make_args(q, kv, k_pe, 0.1, True)
+    args.kv_stride[1] = ld
+    assert _lib.load().atomic_latent_fwd_workspace_size(args) == 0
+
+
 def _tables(rows, dr):
     a = torch.arange(rows, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(0, dr, 2, dtype=torch.float64) / dr)
     return a.cos().float(), a.sin().float()
