@@ -181,12 +181,14 @@ struct RowDma {
   int left;           // rows from it to the last
   uint32_t ld, wide;  // bytes between rows, bytes of a row
   uint32_t at[NZ];    // this lane's byte in the first load
+  int w;              // this wave among the NW
   buffer_t d;
   __device__ __forceinline__ void init(const T* p, int64_t stride, int width) {
+    w = NW == 1 ? 0 : wave_id();
     base = (uint64_t)p;
     ld = (uint32_t)(stride * (int64_t)sizeof(T));
     wide = width * (uint32_t)sizeof(T);
-    const int r0 = RPI * wave_id() + lane_id() / L::NC;
+    const int r0 = RPI * w + lane_id() / L::NC;
 #pragma unroll
     for (int z = 0; z < NZ; ++z) {
       const int c = (lane_id() % L::NC) ^ L::swz(r0 + z * STEP);
@@ -212,7 +214,7 @@ struct RowDma {
   }
   // this wave's i-th load; `dst`: the tile's LDS address
   __device__ __forceinline__ void load(int i, uint32_t dst) const {
-    dma16_buf(d, at[i % NZ], (uint32_t)(i * STEP) * ld, dst + 1024 * (wave_id() + NW * i));
+    dma16_buf(d, at[i % NZ], (uint32_t)(i * STEP) * ld, dst + 1024 * (w + NW * i));
   }
 };
 // Three of them one after the other: the tiles of a stage.

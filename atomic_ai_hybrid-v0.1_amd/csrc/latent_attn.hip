@@ -515,13 +515,20 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
 // gradient accumulators in registers: one wave a SIMD), against tiles of query
 // rows staged as the forward's tokens are, with delta and lse beside them.  The
 // rotated key's gradient leaves as this head's part, fp32 [B, H, S, dr].
-template <typename T, int DN, int DR, int DV>
+//
+// With DS the score gradients go to memory too, for latent_bwd_dq_ds: [B, H, tiles of
+// 64 rows, S, 64] bf16, a token's rows in the order of this kernel's registers
+// (ds_piece), 16 bytes a lane as they are, so that a wave writes 4 KB in a row.  (In
+// rows of T the 32 tokens of a wave lay a power of two apart: 1710 us instead of
+// 1484 at B2 T8192 H16.)  They are the last memory operations of a tile, so the wait for
+// the next tile's loads leaves them in flight.
+template <typename T, int DN, int DR, int DV, bool DS>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
                                                          const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
                                                          const int32_t* __restrict__ kv_lens,
                                                          const float* __restrict__ stat, const T* __restrict__ dout,
                                                          T* __restrict__ dkv, float* __restrict__ dkp, int parts,
-                                                         float* __restrict__ pkv) {
+                                                         float* __restrict__ pkv, T* __restrict__ dst) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, VS = DV / 16, NN = DN / 32, NK = (DN + DR) / 32, NV = DV / 32;
   constexpr int TQ = sizeof(T) == 2 ? 64 : 32, NS = TQ / 32;
   typedef LTile<T, DN> LN;
@@ -577,9 +584,14 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   aim(first, l0);
   dma.all(l0);
   int q0 = first, buf = 0;
-  uint32_t to;         // where the next tile goes
+  uint32_t to;            // where the next tile goes
+  bool stored = false;    // the tile before ended with its 2 NS stores
+  T* dsp = nullptr;       // this lane's piece of the score gradients at q0 = 0
+  if constexpr (DS)
+    dsp = dst + (((int64_t)b * d.H + h) * (stat_rows(d.T) / 64) * d.S + min(tok, d.S - 1)) * 64 + 8 * (lane_id() >> 5);
   auto stage = [&] {  // this tile is there; the next one (past the last, zeros) is sent for along the way
-    vm_wait<0>();
+    if (DS && stored) vm_wait<2 * NS>();
+    else vm_wait<0>();
     bare_barrier();
     to = l0 + (buf ^ 1) * STAGE;
     aim(q0 + TQ, to);
@@ -630,6 +642,13 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
         ds[i][k / 2][4 * (k & 1) + j] = (T)y;
       }
     };
+    auto put = [&](int i) {
+      if (tok < d.S) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          *reinterpret_cast<frag*>(dsp + (int64_t)q0 * d.S + 32 * i + 16 * t) = ds[i][t];
+      }
+    };
     if constexpr (NS == 2) {
       constexpr int G = M1 % 4 || M2 % 4 ? 5 : 4;  // whole groups a phase: a phase's work starts after the one before
       static_assert(M1 % G == 0 && M2 % G == 0, "whole groups");
@@ -642,10 +661,11 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
             else grad((j - 2 * M1) / M2, (j - 2 * M1) % M2, a);
           },
           [&](int j) {
-            dma.at_slot(j, 2 * M1 + 2 * M2, to);
+            dma.at_slot(j, DS ? 2 * M1 : 2 * M1 + 2 * M2, to);
             if (j >= M1 && j < 2 * M1 && (j - M1) % (M1 / 4) == 1 && (j - M1) / (M1 / 4) < 4) prob(0, (j - M1) / (M1 / 4));
             if (j >= 2 * M1 && j < 2 * M1 + M2 && (j - 2 * M1) % (M2 / 4) == 1 && (j - 2 * M1) / (M2 / 4) < 4)
               prob(1, (j - 2 * M1) / (M2 / 4));
+            if (DS && j >= 2 * M1 && (j - 2 * M1) % M2 == 0) put((j - 2 * M1) / M2);
           });
     } else {
       dma.all(to);
@@ -664,10 +684,12 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   for (; q0 < stop && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<1>());
+    stored = true;
   }
   for (; q0 < stop; q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<0>());
+    stored = true;
   }
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
   if (tok >= d.S) return;
@@ -692,6 +714,134 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
         else store4(out + x, v);
       }
     }
+}
+
+// Where rows c .. c + 3 (c a multiple of 4) lie in a token's row of the score
+// gradients: the piece and the byte in it.  Sixteen rows are two pieces, one of each
+// half of the wave: its registers' rows 4 h .. + 3 and 8 + 4 h .. + 3.
+__device__ __forceinline__ int ds_piece(int c) { return 2 * (c >> 4) + ((c >> 2) & 1); }
+__device__ __forceinline__ int ds_byte(int c) { return 8 * ((c >> 3) & 1); }
+
+// dq from the score gradients that latent_bwd_dkv left: 256 query rows of a head a
+// workgroup, 64 a wave, against tiles of 32 tokens, three of them on their way.
+// dq^T += k^T ds^T; a fragment of k serves two MFMAs.  Bound by reading the score
+// gradients (2 bytes a pair).
+template <int DN, int DR>
+__global__ __launch_bounds__(256, 1) void latent_bwd_dq_ds(LatDims d, const bf16* __restrict__ kv,
+                                                           const bf16* __restrict__ kpe,
+                                                           const int32_t* __restrict__ q_lens,
+                                                           const int32_t* __restrict__ kv_lens,
+                                                           const bf16* __restrict__ ds, bf16* __restrict__ dq,
+                                                           int parts, float* __restrict__ pq) {
+  constexpr int NN = DN / 32, NT = (DN + DR) / 32, TK = 32, NB = 4, RG = 2, RW = 32 * RG, RB = 4 * RW;
+  typedef LTile<bf16, DN> LN;
+  typedef LTile<bf16, DR> LR;
+  typedef LTile<bf16, RW> LS;
+  typedef bf16x8 frag;
+  constexpr int OR = TK * LN::ROWB, OS = OR + TK * LR::ROWB, STAGE = OS + 4 * TK * LS::ROWB;
+  __shared__ __attribute__((aligned(1024))) char lds[NB * STAGE];
+  int b, h, blk;
+  lat_map(d, b, h, blk);
+  const int part = blk % parts;
+  blk = (d.blocks - 1 - blk) / parts;
+  const int ql = clamp_len(q_lens, b, d.T), kl = clamp_len(kv_lens, b, d.S), off = kl - ql;
+  const int w0 = RB * blk + RW * wave_id();
+  const int last = min(RB * blk + RB - 1, ql - 1);
+  int begin = 0, end = kl;
+  // (the score gradients are there for whole tiles of 64 rows)
+  if (d.causal) end = min(end, (last | 63) + off + 1);
+  if (last < RB * blk) end = 0;
+  if (parts > 1) {
+    const int tiles = (max(end, 0) + TK - 1) / TK;
+    begin = (int)((int64_t)tiles * part / parts) * TK;
+    end = min(end, (int)((int64_t)tiles * (part + 1) / parts) * TK);
+  }
+  const bf16* kb = kv + b * d.ks[0] + h * d.ks[2];
+  StageDma<RowDma<bf16, DN, TK, 4>, RowDma<bf16, DR, TK, 4>, RowDma<bf16, RW, TK, 1>> dma;
+  dma.a.init(kb, d.ks[1], d.dn);
+  dma.b.init(kpe + b * d.ps[0], d.ps[1], d.dr);
+  // (every wave brings its own rows' score gradients)
+  dma.c.init(ds + (((int64_t)b * d.H + h) * (stat_rows(d.T) / 64) + min(w0, ql - 1) / 64) * d.S * 64, 64, RW);
+  dma.ob = OR;
+  dma.oc = OS + wave_id() * TK * LS::ROWB;
+  f32x16 acc[RG][NT];
+#pragma unroll
+  for (int g = 0; g < RG; ++g)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[g][n] = zero16();
+  const uint32_t l0 = lds_addr(lds);
+  constexpr int PER = decltype(dma)::N;
+  dma.start(begin, end - 1);
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) {
+    dma.aim();
+    dma.all(l0 + i * STAGE);
+  }
+  // keys that this wave's rows have gradients for (in whole groups of 32)
+  const int any = w0 >= ql ? 0 : min(end, d.causal ? w0 + RW + off : kl);
+  const int l = lane_id(), t4 = l & 15, rr = 4 * (l >> 5) + (t4 >> 2);
+  int buf = 0;
+  for (int k0 = begin; k0 < end; k0 += TK, buf = (buf + 1) % NB) {
+    vm_wait<(NB - 2) * PER>();
+    bare_barrier();  // the tile is there, and nobody reads the one before it any more
+    const uint32_t to = l0 + (buf + NB - 1) % NB * STAGE;
+    dma.aim();
+    const char* sk = lds + buf * STAGE;
+    auto ds_at = [&](int g, int r0) {  // the rows of group g, 16 tokens from r0
+      const int c = 32 * g + 16 * ((l >> 4) & 1) + 4 * (t4 & 3);
+      typedef __attribute__((address_space(3))) bf16x4* lds_p;
+      const char* s = sk + OS + wave_id() * TK * LS::ROWB + ds_byte(c);
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + LS::off(r0 + rr, ds_piece(c))));
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + LS::off(r0 + 8 + rr, ds_piece(c))));
+      return (frag)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+#pragma unroll
+    for (int g = 0; g < RG; ++g)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) in_accum(acc[g][n]);
+    if (k0 < any) {
+      frag f[2][RG];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int g = 0; g < RG; ++g) f[t][g] = ds_at(g, 16 * t);
+      in_groups<2 * NT, 1, 4, 0, frag>(
+          [&](int j) {
+            const int r = 16 * (j / NT), n = j % NT;
+            return n < NN ? LN::col(sk, r, 32 * n) : LR::col(sk + OR, r, 32 * (n - NN));
+          },
+          [&](int j, frag a) {
+#pragma unroll
+            for (int g = 0; g < RG; ++g) acc[g][j % NT] = M32<bf16>::mma(a, f[j / NT][g], acc[g][j % NT]);
+          },
+          [&](int j) { dma.at_slot(j, 2 * NT, to); });
+    } else {
+      dma.all(to);
+    }
+  }
+  vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const int row = w0 + 32 * g + (l & 31);
+    if (row >= d.T) continue;
+    const int64_t wide = d.dn + d.dr, at = (((int64_t)b * d.T + row) * d.H + h) * wide;
+    bf16* out = dq + at;
+    float* po = pq + (int64_t)part * d.B * d.T * d.H * wide + at;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int c = 32 * n + reg_row(r);
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[g][n][r + j] * d.scale : 0.f;
+        const int x = n < NN ? c : d.dn + c - DN;
+        if (n < NN ? c < d.dn : c - DN < d.dr) {
+          if (parts > 1) store4(po + x, v);
+          else store4(out + x, v);
+        }
+      }
+  }
 }
 
 // The parts of a gradient summed in their order: four elements a thread.
@@ -782,20 +932,26 @@ constexpr size_t kNoWorkspace = 16;  // what a size function returns where none 
 
 // The backward's parts of the keys (dq) and of the queries (dk, dv), and its workspace.
 struct BwdPlan {
-  int qparts, kparts;
-  size_t stat, dkp, pq, pkv;  // bytes
+  int qrows, qparts, kparts;         // rows a workgroup of the dq kernel
+  size_t stat, dkp, pq, pkv, ds;     // bytes; ds: the score gradients, 0 where dq computes them again
 };
 static int parts_for(int64_t wgs, int64_t tiles) {
   int p = 1;
   while (p < 16 && 2 * p * wgs <= 256 && 4 * p <= tiles) p *= 2;
   return p;
 }
+// Score gradients up to this size are kept between the two kernels (bf16).
+constexpr int64_t kMostDs = (int64_t)4 << 30;
 static BwdPlan bwd_plan(const atomic_latent_args* a) {
   const int64_t bh = (int64_t)a->batch * a->heads, tile = a->dtype == ATOMIC_BF16 ? 64 : 32;
-  BwdPlan p;
-  p.qparts = parts_for(bh * ((a->tq + 127) / 128), (a->tk + tile - 1) / tile);
-  p.kparts = parts_for(bh * ((a->tk + 127) / 128), (a->tq + tile - 1) / tile);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  BwdPlan p;
+  const int64_t per = 2 * bh * a->tk;  // bytes a query row; (the product of both stays in 62 bits)
+  const bool keep = a->dtype == ATOMIC_BF16 && stat_rows(a->tq) <= kMostDs / per;
+  p.ds = keep ? up((size_t)(per * stat_rows(a->tq))) : 0;
+  p.qrows = keep ? 256 : 128;
+  p.qparts = parts_for(bh * ((a->tq + p.qrows - 1) / p.qrows), (a->tk + tile - 1) / tile);
+  p.kparts = parts_for(bh * ((a->tk + 127) / 128), (a->tq + tile - 1) / tile);
   p.stat = up((size_t)bh * stat_rows(a->tq) * 2 * sizeof(float));
   p.dkp = up((size_t)p.kparts * bh * a->tk * a->dr * sizeof(float));
   p.pq = p.qparts > 1 ? up((size_t)p.qparts * bh * a->tq * (a->dn + a->dr) * sizeof(float)) : 0;
@@ -860,7 +1016,7 @@ extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, con
 extern "C" size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a) {
   if (lat_check(a) != ATOMIC_OK) return 0;
   const BwdPlan p = bwd_plan(a);
-  return p.stat + p.dkp + p.pq + p.pkv;
+  return p.stat + p.dkp + p.pq + p.pkv + p.ds;
 }
 
 extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
@@ -878,6 +1034,7 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
   float* dkp = (float*)((char*)stat + p.stat);
   float* pq = (float*)((char*)dkp + p.dkp);
   float* pkv = (float*)((char*)pq + p.pq);
+  void* ds = (char*)pkv + p.pkv;
   const hipStream_t st = (hipStream_t)stream;
   Launch L{a->profile, st};
   return lat_dispatch(a, [&](auto t, auto w) {
@@ -898,18 +1055,34 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
     };
     d.blocks = (d.S + 127) / 128 * p.kparts;
     rc = L("latent_bwd_dkv", [&] {
-      hipLaunchKernelGGL((latent_bwd_dkv<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
-                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
-                         (const T*)dout, (T*)dkv, dkp, p.kparts, pkv);
+      auto go = [&](auto keep) {
+        hipLaunchKernelGGL((latent_bwd_dkv<T, W::DN, W::DR, W::DV, decltype(keep)::value != 0>),
+                           dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256), 0, st, d, (const T*)q, (const T*)kv,
+                           (const T*)k_pe, q_lens, kv_lens, stat, (const T*)dout, (T*)dkv, dkp, p.kparts, pkv,
+                           (T*)ds);
+      };
+      if constexpr (sizeof(T) == 2) {
+        if (p.ds) go(IntC<1>());
+        else go(IntC<0>());
+      } else {
+        go(IntC<0>());
+      }
     });
     if (rc) return rc;
     rc = join("latent_bwd_dkv_join", (int64_t)d.B * d.S * d.H * (d.dn + d.dv), p.kparts, pkv, dkv);
     if (rc) return rc;
-    d.blocks = (d.T + 127) / 128 * p.qparts;
+    d.blocks = (d.T + p.qrows - 1) / p.qrows * p.qparts;
     rc = L("latent_bwd_dq", [&] {
-      hipLaunchKernelGGL((latent_bwd_dq<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256),
-                         0, st, d, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat,
-                         (const T*)dout, (T*)dq, p.qparts, pq);
+      const dim3 grid((unsigned)(d.B * d.H * d.blocks));
+      if constexpr (sizeof(T) == 2) {
+        if (p.ds) {
+          hipLaunchKernelGGL((latent_bwd_dq_ds<W::DN, W::DR>), grid, dim3(256), 0, st, d, (const T*)kv,
+                             (const T*)k_pe, q_lens, kv_lens, (const T*)ds, (T*)dq, p.qparts, pq);
+          return;
+        }
+      }
+      hipLaunchKernelGGL((latent_bwd_dq<T, W::DN, W::DR, W::DV>), grid, dim3(256), 0, st, d, (const T*)q,
+                         (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat, (const T*)dout, (T*)dq, p.qparts, pq);
     });
     if (rc) return rc;
     rc = join("latent_bwd_dq_join", (int64_t)d.B * d.T * d.H * (d.dn + d.dr), p.qparts, pq, dq);
