@@ -844,31 +844,38 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq_ds(LatDims d, const bf16
   }
 }
 
-// The parts of a gradient summed in their order: four elements a thread.
+// What is left to sum, in one launch, four elements a thread and each sum in a fixed
+// order: the parts of dk / dv (n1 elements) and of dq (n2; 0 where there is one part),
+// and dk_pe from the shares of the heads and of the parts of the queries.
+struct FinishJobs {
+  int64_t n1, n2;
+  unsigned b1, b2;  // workgroups of the first two
+  int kparts, qparts;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void latent_bwd_join(int64_t n, int parts, const float* __restrict__ p,
-                                                       T* __restrict__ out) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4 s = zero4();
+__global__ __launch_bounds__(256) void latent_bwd_finish(LatDims d, FinishJobs f, const float* __restrict__ pkv,
+                                                         const float* __restrict__ pq, const float* __restrict__ dkp,
+                                                         T* __restrict__ dkv, T* __restrict__ dq,
+                                                         T* __restrict__ dkpe) {
+  auto join = [&](unsigned blk, int64_t n, int parts, const float* p, T* out) {
+    const int64_t i = ((int64_t)blk * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    f32x4 s = zero4();
 #pragma unroll 4
-  for (int k = 0; k < parts; ++k) s += *reinterpret_cast<const f32x4*>(p + k * n + i);
-  store4(out + i, s);
-}
-
-// dk_pe = the heads' shares (of every part of the queries) summed in their order: four elements a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void latent_bwd_dkpe(LatDims d, int parts, const float* __restrict__ dkp,
-                                                       T* __restrict__ out) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, per = (int64_t)d.S * d.dr;
+    for (int k = 0; k < parts; ++k) s += *reinterpret_cast<const f32x4*>(p + k * n + i);
+    store4(out + i, s);
+  };
+  if (blockIdx.x < f.b1) return join(blockIdx.x, f.n1, f.kparts, pkv, dkv);
+  if (blockIdx.x < f.b1 + f.b2) return join(blockIdx.x - f.b1, f.n2, f.qparts, pq, dq);
+  const int64_t i = ((int64_t)(blockIdx.x - f.b1 - f.b2) * 256 + threadIdx.x) * 4, per = (int64_t)d.S * d.dr;
   if (i >= d.B * per) return;
   f32x4 s = zero4();
-  for (int k = 0; k < parts; ++k) {
+  for (int k = 0; k < f.kparts; ++k) {
     const float* p = dkp + ((int64_t)k * d.B + i / per) * d.H * per + i % per;
 #pragma unroll 4
     for (int h = 0; h < d.H; ++h) s += *reinterpret_cast<const f32x4*>(p + h * per);
   }
-  store4(out + i, s);
+  store4(dkpe + i, s);
 }
 
 // ------------------------------------------------------------------ host
@@ -1047,12 +1054,6 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
                          (const T*)dout, lse, q_lens, stat);
     });
     if (rc) return rc;
-    auto join = [&](const char* name, int64_t n, int parts, const float* from, void* to) {
-      return parts == 1 ? (int)ATOMIC_OK : L(name, [&] {
-        hipLaunchKernelGGL((latent_bwd_join<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, n, parts,
-                           from, (T*)to);
-      });
-    };
     d.blocks = (d.S + 127) / 128 * p.kparts;
     rc = L("latent_bwd_dkv", [&] {
       auto go = [&](auto keep) {
@@ -1069,8 +1070,6 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
       }
     });
     if (rc) return rc;
-    rc = join("latent_bwd_dkv_join", (int64_t)d.B * d.S * d.H * (d.dn + d.dv), p.kparts, pkv, dkv);
-    if (rc) return rc;
     d.blocks = (d.T + p.qrows - 1) / p.qrows * p.qparts;
     rc = L("latent_bwd_dq", [&] {
       const dim3 grid((unsigned)(d.B * d.H * d.blocks));
@@ -1085,11 +1084,14 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
                          (const T*)kv, (const T*)k_pe, q_lens, kv_lens, stat, (const T*)dout, (T*)dq, p.qparts, pq);
     });
     if (rc) return rc;
-    rc = join("latent_bwd_dq_join", (int64_t)d.B * d.T * d.H * (d.dn + d.dr), p.qparts, pq, dq);
-    if (rc) return rc;
-    return L("latent_bwd_dkpe", [&] {
-      hipLaunchKernelGGL((latent_bwd_dkpe<T>), dim3((unsigned)(((int64_t)d.B * d.S * d.dr / 4 + 255) / 256)),
-                         dim3(256), 0, st, d, p.kparts, dkp, (T*)dk_pe);
+    FinishJobs f{p.kparts > 1 ? (int64_t)d.B * d.S * d.H * (d.dn + d.dv) : 0,
+                 p.qparts > 1 ? (int64_t)d.B * d.T * d.H * (d.dn + d.dr) : 0, 0, 0, p.kparts, p.qparts};
+    f.b1 = (unsigned)((f.n1 / 4 + 255) / 256);
+    f.b2 = (unsigned)((f.n2 / 4 + 255) / 256);
+    const unsigned b3 = (unsigned)(((int64_t)d.B * d.S * d.dr / 4 + 255) / 256);
+    return L("latent_bwd_finish", [&] {
+      hipLaunchKernelGGL((latent_bwd_finish<T>), dim3(f.b1 + f.b2 + b3), dim3(256), 0, st, d, f, pkv, pq, dkp,
+                         (T*)dkv, (T*)dq, (T*)dk_pe);
     });
   });
 }
