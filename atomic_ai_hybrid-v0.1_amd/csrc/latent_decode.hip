@@ -485,14 +485,19 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
 }
 
 // o: 16 query tokens of a head times 64 rows of its value projection a
-// workgroup, 16 a wave.
-template <typename T>
+// workgroup, 16 a wave.  With JOIN it joins the splits itself (up to kUpSplits of
+// them): where that is a few dozen loads a thread, a launch less is worth more than
+// the same parts read once instead of dv / 64 times.
+constexpr int kUpSplits = 64;
+template <typename T, bool JOIN>
 __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict__ w_kv, const float* __restrict__ olat,
-                                                 T* __restrict__ o) {
+                                                 const float* __restrict__ part, const float* __restrict__ stat,
+                                                 const int32_t* __restrict__ kv_lens, T* __restrict__ o) {
   constexpr int V = 16 / (int)sizeof(T), LD = 512 + V, PARTS = sizeof(T) == 2 ? 2 : 1, KS = 16;
   __shared__ __attribute__((aligned(16))) T so[PARTS][16 * LD];
+  __shared__ float sw[JOIN ? 16 : 1][kUpSplits];
   const int h = blockIdx.x, v0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, KP = (d.dc + 31) / 32 * 32;
-  const int vr = v0 + 16 * wave_id();
+  const int vr = v0 + 16 * wave_id(), rows = d.n * d.H;
   const T* w = w_kv + ((int64_t)h * (d.dn + d.dv) + d.dn + min(vr + (lane_id() & 15), d.dv - 1)) * d.dc;
   typename M16<T>::frag wf[KS];  // all of this wave's weights in flight before the rows are waited for
 #pragma unroll
@@ -500,11 +505,47 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
     const int k = 32 * t + 8 * (lane_id() >> 4);
     wf[t] = ld_frag(k < d.dc ? w + k : (const T*)lat_zeros);
   }
+  if constexpr (JOIN) {  // the splits' weights: sixteen threads a row
+    const int r = min(r0 + (int)(threadIdx.x >> 4), R - 1), b = r / d.n, g = threadIdx.x & 15;
+    const int ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
+    const float* st = stat + 2 * ((int64_t)b * d.splits * rows + r % d.n * d.H + h);
+    float m = -INFINITY, sum = 0.f, ms[kUpSplits / 16], ls[kUpSplits / 16];
+#pragma unroll
+    for (int i = 0; i < kUpSplits / 16; ++i) {
+      const int s = g + 16 * i;
+      ms[i] = s < ns ? st[2 * (int64_t)s * rows] : -INFINITY;
+      ls[i] = s < ns ? st[2 * (int64_t)s * rows + 1] : 0.f;
+      m = fmaxf(m, ms[i]);
+    }
+#pragma unroll
+    for (int x = 8; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < kUpSplits / 16; ++i) {
+      ms[i] = fast_exp2(ms[i] - ref);
+      sum += ms[i] * ls[i];
+    }
+#pragma unroll
+    for (int x = 8; x; x >>= 1) sum += __shfl_xor(sum, x);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < kUpSplits / 16; ++i) sw[threadIdx.x >> 4][g + 16 * i] = ms[i] * inv;
+    __syncthreads();
+  }
 #pragma unroll 4
   for (int e = threadIdx.x; e < 16 * (KP / 4); e += 256) {
     const int r = e / (KP / 4), c = e % (KP / 4) * 4;
     f32x4 x = zero4();
-    if (c < d.dc && r0 + r < R) x = *reinterpret_cast<const f32x4*>(olat + ((int64_t)(r0 + r) * d.H + h) * d.dc + c);
+    if (c < d.dc && r0 + r < R) {
+      if constexpr (JOIN) {
+        const int b = (r0 + r) / d.n, ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
+        const float* p = part + ((int64_t)b * d.splits * rows + (r0 + r) % d.n * d.H + h) * d.dc + c;
+#pragma unroll 8
+        for (int s = 0; s < ns; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
+      } else {
+        x = *reinterpret_cast<const f32x4*>(olat + ((int64_t)(r0 + r) * d.H + h) * d.dc + c);
+      }
+    }
     store4(&so[0][r * LD + c], x);
     if constexpr (PARTS == 2) {
 #pragma unroll
@@ -581,6 +622,11 @@ static DecDims dec_dims(const atomic_latent_decode_args* a) {
   d.chunk = (int)((chunk + tile - 1) / tile * tile);
   d.splits = (int)((most + d.chunk - 1) / d.chunk);
   return d;
+}
+// Whether latent_up joins the splits: at most 64 loads a thread, in steps of eight.
+static bool dec_up_joins(const DecDims& d) {
+  const int64_t rows = (int64_t)d.B * d.n < 16 ? (int64_t)d.B * d.n : 16;
+  return d.splits > 1 && d.splits <= kUpSplits && d.splits * ((rows * d.dc / 4 + 255) / 256) <= 64;
 }
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 static size_t dec_qa_bytes(const DecDims& d, int dtype) {
@@ -676,7 +722,8 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
         launch_split<T, 512>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat, olat);
     });
     if (rc) return rc;
-    if (d.splits > 1) {
+    const bool joins = dec_up_joins(d);
+    if (d.splits > 1 && !joins) {
       int ways = 1;  // about four splits a thread
       while (ways < 16 && 4 * ways < d.splits) ways *= 2;
       const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
@@ -687,8 +734,13 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
       if (rc) return rc;
     }
     return L("latent_up", [&] {
-      hipLaunchKernelGGL((latent_up<T>), dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
-                         (const T*)w_kv, olat, (T*)o);
+      auto go = [&](auto j) {
+        hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0>),
+                           dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
+                           (const T*)w_kv, olat, part, stat, kv_lens, (T*)o);
+      };
+      if (joins) go(IntC<1>());
+      else go(IntC<0>());
     });
   };
   return a->dtype == ATOMIC_BF16 ? go(bf16()) : go(float());
