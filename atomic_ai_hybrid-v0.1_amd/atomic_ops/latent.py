@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -79,6 +80,15 @@ def _index(what, name, t, shape, dtype, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _workspace(ws, nbytes, device):
+    """The caller's workspace where it is large enough, else a new one."""
+    if ws is None or ws.numel() < nbytes:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise ValueError("latent attention: workspace must be dense uint8 on the inputs' device")
+    return ws
+
+
 # ------------------------------------------------------------ expanded form
 def _check(q, kv, k_pe, q_lens, kv_lens):
     _operands("latent attention", ("q", q), ("kv", kv), ("k_pe", k_pe))
@@ -123,7 +133,10 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, works
     with j <= i + kv_lens[b] - q_lens[b] (queries stand at the end of the keys).
     ``q_lens`` / ``kv_lens`` are int32 [B] on the device (the whole T / S without
     them).  A query that sees no key, and one past its length, has o = 0 and
-    lse = -inf.  Inputs of any batch, token and head strides are read in place."""
+    lse = -inf.  What lies past the lengths does not matter; within them an
+    infinity or NaN in a token's values may reach queries that do not see it (a
+    weight of zero times it).  Inputs of any batch, token and head strides are
+    read in place."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
     lib = _lib.load()
     args, (q, kv, k_pe, _) = make_args(q, kv, k_pe, scale, causal)
@@ -134,8 +147,7 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, works
     if nbytes == 0:
         raise _lib.AtomicError("atomic_latent_fwd: ATOMIC_ERR_SHAPE: unsupported or inconsistent dimensions",
                                _lib.ATOMIC_ERR_SHAPE)
-    if workspace is None or workspace.numel() < nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    workspace = _workspace(workspace, nbytes, q.device)
     o = torch.empty(B, T, H, args.dv, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
     rc = lib.atomic_latent_fwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
@@ -163,8 +175,7 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     nbytes = lib.atomic_latent_bwd_workspace_size(ctypes.byref(args))
     if nbytes == 0:
         raise _lib.AtomicError("atomic_latent_bwd_workspace_size: unsupported shape")
-    if workspace is None or workspace.numel() < nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    workspace = _workspace(workspace, nbytes, q.device)
     o, lse = o.contiguous(), lse.contiguous()
     dq, dkv, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, kv, k_pe))
     rc = lib.atomic_latent_bwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
@@ -180,15 +191,16 @@ class LatentAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, kv, k_pe, scale, causal, q_lens, kv_lens):
         o, lse = forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)
-        ctx.save_for_backward(q, kv, k_pe, o, lse)
-        ctx.scale, ctx.causal, ctx.lens = scale, causal, (q_lens, kv_lens)
+        ctx.save_for_backward(q, kv, k_pe, o, lse, q_lens, kv_lens)
+        ctx.scale, ctx.causal = scale, causal
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
-        q, kv, k_pe, o, lse = ctx.saved_tensors
-        dq, dkv, dk = backward(q, kv, k_pe, o, lse, dout.to(q.dtype), ctx.scale, causal=ctx.causal,
-                               q_lens=ctx.lens[0], kv_lens=ctx.lens[1])
+        q, kv, k_pe, o, lse, q_lens, kv_lens = ctx.saved_tensors
+        dq, dkv, dk = backward(q, kv, k_pe, o, lse, dout.to(q.dtype), ctx.scale, causal=ctx.causal, q_lens=q_lens,
+                               kv_lens=kv_lens)
         return dq, dkv, dk, None, None, None, None
 
 
@@ -215,7 +227,7 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
 
     Row ``slots[t]`` (page slots[t] // page, row slots[t] % page; int64 [N])
     becomes [c_kv[t] | rotate(k_pe[t])]; a negative slot, or one past the cache,
-    leaves it as it is.  ``positions`` int32 [N] choose the rows of the float32
+    leaves it as it is; one that occurs twice holds either token's row.  ``positions`` int32 [N] choose the rows of the float32
     tables ``cos`` / ``sin`` [positions, dr / 2]; the rotation turns the pairs
     (i, i + dr / 2), or (2 i, 2 i + 1) with ``interleaved``.  Returns
     ``(k, q)``: the rotated keys [N, dr] and, where ``q`` [N, H, dn + dr] is
@@ -297,8 +309,7 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
     nbytes = lib.atomic_latent_decode_workspace_size(ctypes.byref(args))
     if nbytes == 0:
         raise _lib.AtomicError("atomic_latent_decode_workspace_size: unsupported shape")
-    if workspace is None or workspace.numel() < nbytes:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    workspace = _workspace(workspace, nbytes, q.device)
     o = torch.empty(B, n, H, args.dv, dtype=q.dtype, device=q.device)
     rc = lib.atomic_latent_decode(ctypes.byref(args), _ptr(q), _ptr(w_kv), _ptr(cache), _ptr(page_table),
                                   _ptr(kv_lens), _ptr(cos), _ptr(sin), _ptr(o), _ptr(workspace), workspace.numel(),

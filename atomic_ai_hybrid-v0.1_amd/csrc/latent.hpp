@@ -86,41 +86,65 @@ struct LTile {
   }
   // (the piece's upper bits apart: they become the read's immediate offset)
   static __device__ __forceinline__ int off(int r, int c) {
-    constexpr int M = NC == 8 ? 7 : 15;
     return r * ROWB + (((c & M) ^ swz(r)) << 4) + ((c & ~M) << 4);
   }
-  // row operand: lane (l % 32) holds row r0 + l % 32, elements k0 + 8 (l / 32) .. + 7
-  static __device__ __forceinline__ typename M32<T>::frag row(const char* s, int r0, int k0) {
-    const int l = lane_id(), r = r0 + (l & 31), k = k0 + 8 * (l >> 5);
+  // Row operand: lane (l % 32) holds row r0 + l % 32, elements k0 + 8 (l / 32) .. + 7.
+  // `base`: the tile's LDS address plus row_base.  r0 is a multiple of 32 and k0 of 16,
+  // so what differs between two reads is a constant: one exclusive-or and the immediate
+  // offset.  (Addresses of their own would be kept in registers over the loop; the
+  // forward spilled 20 of them, and every reload waited for the tile in flight.)
+  static __device__ __forceinline__ uint32_t row_base() {
+    const int l = lane_id();
+    return off(l & 31, 8 / VEC * (l >> 5));
+  }
+  static __device__ __forceinline__ typename M32<T>::frag row(uint32_t base, int r0, int k0) {
+    typedef const __attribute__((address_space(3))) char* lds_p;
+    const lds_p p = (lds_p)(base ^ piece(k0 / VEC)) + r0 * ROWB + above(k0 / VEC);
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const bf16x8*>(s + off(r, k / 8));
+      return *(const __attribute__((address_space(3))) bf16x8*)p;
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(s + off(r, k / 4));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(s + off(r, k / 4 + 1));
+      const lds_p p1 = (lds_p)(base ^ piece(k0 / VEC + 1)) + r0 * ROWB + above(k0 / VEC);
+      const f32x4 a = *(const __attribute__((address_space(3))) f32x4*)p;
+      const f32x4 b = *(const __attribute__((address_space(3))) f32x4*)p1;
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  // column operand: lane (l % 32) holds column c0 + l % 32 of the 16 rows from r0, in the order that
-  // a result's registers have: rows r0 + 4 (l / 32) + j and r0 + 8 + 4 (l / 32) + j
-  static __device__ __forceinline__ typename M32<T>::frag col(const char* s, int r0, int c0) {
-    const int l = lane_id(), h = l >> 5;
+  // Column operand: lane (l % 32) holds column c0 + l % 32 of the 16 rows from r0, in the order that
+  // a result's registers have: rows r0 + 4 (l / 32) + j and r0 + 8 + 4 (l / 32) + j.
+  // r0 is a multiple of 16 and c0 of 32; the swizzle of 8 a + 4 h + b is that of the three apart.
+  static __device__ __forceinline__ uint32_t col_base() {
+    const int l = lane_id(), h = l >> 5, t = l & 15;
     if constexpr (sizeof(T) == 2) {
-      const int t = l & 15, r = r0 + 4 * h + (t >> 2), c = c0 + 16 * ((l >> 4) & 1) + 4 * (t & 3);
-      typedef __attribute__((address_space(3))) bf16x4* lds_p;
-      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + off(r, c / 8) + 2 * (c & 7)));
-      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + off(r + 8, c / 8) + 2 * (c & 7)));
+      const int c = 16 * ((l >> 4) & 1) + 4 * (t & 3);
+      return off(4 * h + (t >> 2), c / 8) + 2 * (c & 7);
+    } else {
+      return off(4 * h, (l & 31) / 4) + 4 * (l & 3);
+    }
+  }
+  static __device__ __forceinline__ typename M32<T>::frag col(uint32_t base, int r0, int c0) {
+    typedef const __attribute__((address_space(3))) char* lds_p;
+    const int c = c0 / VEC;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) bf16x4* v4_p;
+      const lds_p p = (lds_p)(base ^ piece(c)) + r0 * ROWB + above(c);
+      const lds_p p8 = (lds_p)(base ^ piece(c) ^ (swz(8) << 4)) + (r0 + 8) * ROWB + above(c);
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((v4_p)p);
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((v4_p)p8);
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const int c = c0 + (l & 31);
       f32x8 z;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int r = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
-        z[j] = *reinterpret_cast<const float*>(s + off(r, c / 4) + 4 * (c & 3));
+        const int r = 8 * (j >> 2) + (j & 3);
+        const lds_p p = (lds_p)(base ^ piece(c) ^ (swz(r) << 4)) + (r0 + r) * ROWB + above(c);
+        z[j] = *(const __attribute__((address_space(3))) float*)p;
       }
       return z;
     }
   }
+  static constexpr int M = NC == 8 ? 7 : 15;
+  static __device__ __forceinline__ uint32_t piece(int c) { return (c & M) << 4; }
+  static __device__ __forceinline__ int above(int c) { return (c & ~M) << 4; }
 };
 
 // use(i, load(i)) for i in [0, N), each use one MFMA, in groups of G, with its

@@ -7,9 +7,10 @@
 //   o[h] = w_kv[h, dn:] o_lat[h]                             (up)
 //
 // All heads of a sequence read the same cache row, once, as key and as value.
-// q_lat and the probabilities are rounded to the operand type, as the MFMA
-// takes them; o_lat stays fp32 to the end (in bf16 it enters the last product as
-// the sum of two bf16 numbers).
+// q_lat is rounded to the operand type, as the MFMA takes it; the probabilities
+// and o_lat, fp32, enter their products as the sum of two bf16 numbers (the cache's
+// bytes leave the matrix instructions idle, and a probability of eight bits costs o
+// as much as o's own rounding: 0.0025 of a row's norm instead of 0.0018).
 #include "latent.hpp"
 
 namespace ah {
@@ -224,7 +225,7 @@ __device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 
 // computes with the 16 rows w % MT and the tokens of MT waves.  The waves of a
 // row group join at the end.
 //
-// Bound by the cache's bytes: 16 heads need 30 operations a byte.  So the tiles go
+// Bound by the cache's bytes: 16 heads need 46 operations a byte.  So the tiles go
 // straight to LDS, two of them (147 KB with 512 bf16 latents), and a wave that has
 // its rows to itself (MT = 1) never meets a barrier: it loads what it reads.  The
 // split's page numbers lie in LDS, so no wait for an index drains the tiles in flight.
@@ -234,6 +235,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
                                                         const int32_t* __restrict__ kv_lens, float* __restrict__ part,
                                                         float* __restrict__ stat, float* __restrict__ olat) {
   constexpr int DR = 64, W = DC + DR, KS = W / 32, NT = DC / 16, TK = 16 * NW, TW = NW / MT, V = 16 / (int)sizeof(T);
+  constexpr int NP = sizeof(T) == 2 ? 2 : 1;    // operands of a probability
   constexpr int PC = DC / V, PR = DR / V;       // pieces of a row's latent and rotated key
   constexpr int IC = PC * 16 / 64, IR = PR * 16 / 64;  // loads of one wave for its 16 tokens
   typedef DTile<T, DC> LC;
@@ -351,30 +353,42 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
       for (int n = 0; n < NT; ++n) acc[n] *= fade;
     }
     const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
-    half p[MT];
+    half p[NP][MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = fast_exp2(s[i][r] - ref);
+        float e = fast_exp2(s[i][r] - ref);
         sum += e;
-        p[i][r] = (T)e;
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          p[k][i][r] = (T)e;
+          e -= (float)p[k][i][r];
+        }
       }
     const char* kc = sk + (buf * NW + MT * tw) * (SC + SR);
     if constexpr (MT == 1) {
       in_groups<NT, 16 / (int)sizeof(T), half>([&](int n) { return LC::col16(kc, 0, 16 * n); },
-                                               [&](int n, half a) { acc[n] = M16<T>::mma4(a, p[0], acc[n]); });
+                                               [&](int n, half a) {
+#pragma unroll
+                                                 for (int k = 0; k < NP; ++k) acc[n] = M16<T>::mma4(a, p[k][0], acc[n]);
+                                               });
     } else {  // 32 tokens an instruction
 #pragma unroll
       for (int i = 0; i < MT; i += 2) {
-        const frag pp = __builtin_shufflevector(p[i], p[i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        frag pp[NP];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) pp[k] = __builtin_shufflevector(p[k][i], p[k][i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
         const char* ka = kc + i * (SC + SR);
         in_groups<NT, 8 / (int)sizeof(T), frag>(
             [&](int n) {
               return __builtin_shufflevector(LC::col16(ka, 0, 16 * n), LC::col16(ka + SC + SR, 0, 16 * n), 0, 1, 2, 3,
                                              4, 5, 6, 7);
             },
-            [&](int n, frag a) { acc[n] = M16<T>::mma(a, pp, acc[n]); });
+            [&](int n, frag a) {
+#pragma unroll
+              for (int k = 0; k < NP; ++k) acc[n] = M16<T>::mma(a, pp[k], acc[n]);
+            });
       }
     }
     // every read of this buffer has returned before it is loaded again

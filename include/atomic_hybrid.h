@@ -783,7 +783,8 @@ int atomic_mamba2_proj_bwd(const atomic_mamba2_proj_args* a, const void* x_bc, c
  * j <= i + kl - ql.  Lengths outside [0, tq] / [0, tk] are taken to the nearer
  * end.  A query that sees no key has o = 0, lse = -inf and zero gradients, and
  * so have the rows past the lengths; what the inputs hold past the lengths
- * does not matter. */
+ * does not matter.  Within them, an infinity or NaN in a token's values may reach
+ * queries that do not see it (a weight of zero times it). */
 typedef struct atomic_latent_args {
   int32_t batch;      /* B                                                  */
   int32_t tq;         /* query rows of the padded batch, >= 1               */

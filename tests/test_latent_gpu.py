@@ -64,6 +64,8 @@ SHAPES = [
     (4, 65, 300, 1, 96, 32, 64, True, [65, 64, 1, 33], [300, 0, 128, 20]),
     (2, 40, 129, 5, 8, 8, 8, False, [40, 3], [128, 129]),
     (1, 300, 500, 6, 128, 32, 96, True, [256], [384]),
+    (1, 70, 2100, 1, 128, 64, 128, True, None, [2049]),      # the keys divided over eight workgroups
+    (1, 2100, 70, 1, 64, 32, 64, False, [2049], None),       # and the queries
 ]
 
 
@@ -90,6 +92,76 @@ def test_expanded_matches_the_formulas(B, T, S, H, dn, dr, dv, causal, ql, kl, d
         assert a.dtype == dtype
         _within(a, b, 1.5 * s, U[dtype], n)
     assert (grads[0].cpu()[empty.transpose(1, 2)] == 0).all()
+
+
+def _against_the_oracle(shape, dtype, seed, scale=None):
+    B, T, S, H, dn, dr, dv, causal, ql, kl = shape
+    q, kv, k_pe, do = _inputs(B, T, S, H, dn, dr, dv, dtype, seed=seed)
+    _spoil((q, do, kv, k_pe), (ql, ql, kl, kl))
+    scale = (dn + dr) ** -0.5 if scale is None else scale
+    d = [t.cuda() for t in (q, kv, k_pe)]
+    kw = dict(causal=causal, q_lens=_i32(ql), kv_lens=_i32(kl))
+    o, lse = L.forward(*d, scale, **kw)
+    grads = L.backward(*d, o, lse, do.cuda(), scale, **kw)
+    torch.cuda.synchronize()
+    o_ref, lse_ref, mag = ol.expanded(q, kv, k_pe, scale, causal, ql, kl)
+    _within(o, o_ref, mag, U[dtype], "o")
+    seen = lse_ref != -INF
+    assert torch.equal(lse.cpu() == -INF, ~seen)
+    assert ((lse.double().cpu() - lse_ref).abs()[seen] <= 2e-5 * (1 + lse_ref.abs()[seen])).all()
+    want, size = ol.expanded_grads(q, kv, k_pe, do, scale, causal, ql, kl)
+    for n, a, b, z in zip(("dq", "dkv", "dk_pe"), grads, want, size):
+        _within(a, b, 1.5 * z, U[dtype], n)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_row_blocks(causal):
+    """More row blocks than the card holds at once."""
+    banner(f"latent expanded, many row blocks causal={causal}")
+    _against_the_oracle((8, 300, 333, 17, 128, 64, 128, causal, [300, 0, 37, 256, 257, 64, 1, 129],
+                         [333, 12, 0, 256, 300, 65, 64, 100]), BF16, seed=21)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_negative_and_zero_scale(scale, dtype):
+    """With a scale of zero every visible key weighs the same, and q, k have no gradient."""
+    banner(f"latent expanded scale {scale} {dtype}")
+    _against_the_oracle((2, 90, 150, 2, 64, 32, 64, True, [90, 20], [150, 10]), dtype, seed=22, scale=scale)
+
+
+def test_more_score_gradients_than_are_kept():
+    """Two bytes a pair of the padded lengths pass 4 GB: dq computes its scores again."""
+    banner("latent backward past the kept score gradients")
+    T, ql, kl = 46400, 200, 230
+    q, kv, k_pe, do = _inputs(1, ql, kl, 1, 128, 64, 128, BF16, seed=23)
+    pad = lambda t, n: torch.cat((t, t.new_full((1, T - n, *t.shape[2:]), NAN)), 1).cuda()
+    d = [pad(q, ql), pad(kv, kl), pad(k_pe, kl)]
+    for causal in (True, False):
+        kw = dict(causal=causal, q_lens=_i32([ql]), kv_lens=_i32([kl]))
+        o, lse = L.forward(*d, 0.07, **kw)
+        grads = L.backward(*d, o, lse, pad(do, ql), 0.07, **kw)
+        torch.cuda.synchronize()
+        want, size = ol.expanded_grads(q, kv, k_pe, do, 0.07, causal)
+        for n, x, a, b, z in zip(("dq", "dkv", "dk_pe"), (ql, kl, kl), grads, want, size):
+            _within(a[:, :x], b, 1.5 * z, U[BF16], n)
+            assert (a[:, x:] == 0).all()
+
+
+def test_lengths_belong_to_the_graph():
+    """Lengths changed after the forward are an error in the backward, as any saved tensor's change is;
+    a second derivative is refused."""
+    banner("latent expanded saved lengths")
+    q, kv, k_pe, _ = (t.cuda() for t in _inputs(1, 8, 8, 1, 64, 32, 64, BF16, seed=24))
+    ln = _i32([8])
+    o = L.attention(q.requires_grad_(True), kv, k_pe, 0.1, kv_lens=ln)
+    ln.fill_(3)
+    with pytest.raises(RuntimeError, match="modified"):
+        o.float().sum().backward()
+    o = L.attention(q, kv, k_pe, 0.1)
+    g, = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
 
 
 def test_gradient_follows_differences():
@@ -294,6 +366,18 @@ def test_decode_matches_the_expanded_formula(H, n, lens, dn, dr, dv, dc, page, d
         _rows_within(o, want, 2.0 ** -8 if dtype == BF16 else U[F32])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decode_of_many_sequences(dtype):
+    """Splits of many tiles, one of the sequences far longer than the others."""
+    banner(f"latent decode many sequences {dtype}")
+    lens = [9000] + [137 * i % 2000 for i in range(63)]
+    q, w, cache, table, ln = _paged(64, 4, 1, lens, 64, 32, 64, 64, 48, dtype, seed=25)
+    for scale in (0.1, -0.1, 0.0):
+        o = L.decode(*(t.cuda() for t in (q, w, cache, table, ln)), scale)
+        torch.cuda.synchronize()
+        _rows_within(o, ol.decode(q, w, cache, table, lens, scale), 2.0 ** -8 if dtype == BF16 else U[F32])
+
+
 def test_decode_reads_strided_queries_and_lengths_past_the_table():
     banner("latent decode strides")
     q, w, cache, table, ln = (t.cuda() for t in _paged(2, 4, 2, [128, 96], 64, 32, 64, 128, 32, BF16, seed=1))
@@ -379,6 +463,19 @@ def test_refusals():
     o, lse = L.forward(q, kv, k_pe, 1.0)
     with pytest.raises(ValueError, match="dout"):
         L.backward(q, kv, k_pe, o, lse, o[:, :3], 1.0)
+    for ws in (torch.zeros(1 << 20, dtype=torch.uint8), z(1 << 20), z(1 << 20, dt=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            L.forward(q, kv, k_pe, 1.0, workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            L.backward(q, kv, k_pe, o, lse, o, 1.0, workspace=ws)
+    args, _ = L.make_args(q, kv, k_pe, 1.0, True, o)
+    lib, p = _lib.load(), lambda t: t.data_ptr()
+    small = z(64, dt=torch.uint8)
+    for call in (lambda ws, n: lib.atomic_latent_bwd(args, p(q), p(kv), p(k_pe), None, None, p(o), p(lse), p(o), p(q),
+                                                     p(kv), p(k_pe), ws, n, None),):
+        for ws, n in ((None, 1 << 20), (p(small), 64)):
+            with pytest.raises(_lib.AtomicError, match="WORKSPACE"):
+                _lib.check(call(ws, n), "atomic_latent_bwd")
     w, cache, table, ln = z(2, 128, 64), z(3, 16, 96), z(1, 2, dt=torch.int32), z(1, dt=torch.int32)
     qd = z(1, 1, 2, 96)
     assert (L.decode(qd, w, cache, table, ln, 1.0) == 0).all()
