@@ -270,9 +270,9 @@ _SIGS = {
     "atomic_mamba2_proj_fwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 16 + [_P, ctypes.c_size_t, _P]),
     "atomic_mamba2_proj_bwd": (ctypes.c_int, [ctypes.POINTER(Mamba2ProjArgs)] + [_P] * 24 + [_P, ctypes.c_size_t, _P]),
     "atomic_latent_fwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentArgs)]),
-    "atomic_latent_fwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 7 + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_fwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 8 + [_P, ctypes.c_size_t, _P]),
     "atomic_latent_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentArgs)]),
-    "atomic_latent_bwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 11 + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_bwd": (ctypes.c_int, [ctypes.POINTER(LatentArgs)] + [_P] * 12 + [_P, ctypes.c_size_t, _P]),
     "atomic_latent_append": (ctypes.c_int, [ctypes.POINTER(LatentAppendArgs)] + [_P] * 10 + [_P]),
     "atomic_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentDecodeArgs)]),
     "atomic_latent_decode": (ctypes.c_int, [ctypes.POINTER(LatentDecodeArgs)] + [_P] * 8 + [_P, ctypes.c_size_t, _P]),

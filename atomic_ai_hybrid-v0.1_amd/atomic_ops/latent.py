@@ -126,8 +126,10 @@ def make_args(q, kv, k_pe, scale, causal, dout=None):
     return args, (q, kv, k_pe, dout)
 
 
-def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, workspace=None, timer=None):
+def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, save=False, workspace=None, timer=None):
     """``(o, lse)``: o [B, T, H, dv] in q's dtype and lse [B, H, T] float32.
+    With ``save`` ``(o, lse, rest)``: rest, for ``backward``, is what o's rounding
+    to bfloat16 left out (None in float32).
 
     Query i of batch row b sees the keys j < kv_lens[b]; with ``causal`` those
     with j <= i + kv_lens[b] - q_lens[b] (queries stand at the end of the keys).
@@ -150,22 +152,31 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, works
     workspace = _workspace(workspace, nbytes, q.device)
     o = torch.empty(B, T, H, args.dv, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
+    rest = torch.empty_like(o) if save and q.dtype == torch.bfloat16 else None
     rc = lib.atomic_latent_fwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
-                               _ptr(o), _ptr(lse), _ptr(workspace), workspace.numel(), _stream(q.device))
+                               _ptr(o), _ptr(lse), _ptr(rest), _ptr(workspace), workspace.numel(), _stream(q.device))
     _lib.check(rc, "atomic_latent_fwd")
-    return o, lse
+    return (o, lse, rest) if save else (o, lse)
 
 
-def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_lens=None, workspace=None, timer=None):
+def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_lens=None, rest=None, workspace=None,
+             timer=None):
     """``(dq, dkv, dk_pe)`` in the inputs' shapes and dtype from the forward's
-    ``o`` and ``lse``; k_pe's gradient is summed over the heads.  The same
-    inputs give the same bits."""
+    ``o``, ``lse`` and ``rest``; k_pe's gradient is summed over the heads.  A
+    score's gradient is a difference of do . v and do . o: without ``rest``, o's
+    rounding is most of what is left where a query sees few keys.  The same inputs
+    give the same bits."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
     B, T, H, d = q.shape
     dv = kv.shape[3] - (d - k_pe.shape[2])
     _operands("latent attention", ("q", q), ("o", o), ("dout", dout))
     if o.shape != (B, T, H, dv) or dout.shape != o.shape:
         raise ValueError("o and dout must be [B, T, H, dv]")
+    if rest is not None:
+        _operands("latent attention", ("q", q), ("rest", rest))
+        if rest.shape != o.shape:
+            raise ValueError("rest must be [B, T, H, dv]")
+        rest = rest.contiguous()
     if lse.shape != (B, H, T) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise ValueError("lse must be float32 [B, H, T] on q's device")
     lib = _lib.load()
@@ -179,8 +190,8 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     o, lse = o.contiguous(), lse.contiguous()
     dq, dkv, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, kv, k_pe))
     rc = lib.atomic_latent_bwd(ctypes.byref(args), _ptr(q), _ptr(kv), _ptr(k_pe), _ptr(q_lens), _ptr(kv_lens),
-                               _ptr(o), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dkv), _ptr(dk), _ptr(workspace),
-                               workspace.numel(), _stream(q.device))
+                               _ptr(o), _ptr(lse), _ptr(rest), _ptr(dout), _ptr(dq), _ptr(dkv), _ptr(dk),
+                               _ptr(workspace), workspace.numel(), _stream(q.device))
     _lib.check(rc, "atomic_latent_bwd")
     return dq, dkv, dk
 
@@ -190,22 +201,24 @@ class LatentAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, k_pe, scale, causal, q_lens, kv_lens):
-        o, lse = forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)
-        ctx.save_for_backward(q, kv, k_pe, o, lse, q_lens, kv_lens)
+        o, lse, rest = forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens, save=True)
+        ctx.save_for_backward(q, kv, k_pe, o, lse, rest, q_lens, kv_lens)
         ctx.scale, ctx.causal = scale, causal
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, kv, k_pe, o, lse, q_lens, kv_lens = ctx.saved_tensors
+        q, kv, k_pe, o, lse, rest, q_lens, kv_lens = ctx.saved_tensors
         dq, dkv, dk = backward(q, kv, k_pe, o, lse, dout.to(q.dtype), ctx.scale, causal=ctx.causal, q_lens=q_lens,
-                               kv_lens=kv_lens)
+                               kv_lens=kv_lens, rest=rest)
         return dq, dkv, dk, None, None, None, None
 
 
 def attention(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None):
     """o [B, T, H, dv] of ``forward``, differentiable in q, kv and k_pe."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad or k_pe.requires_grad)):
+        return forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)[0]
     return LatentAttention.apply(q, kv, k_pe, scale, causal, q_lens, kv_lens)
 
 

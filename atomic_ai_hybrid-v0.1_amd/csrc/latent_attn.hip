@@ -70,6 +70,13 @@ __device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) /
 // SIMD has 256 registers in each).
 template <typename F> __device__ __forceinline__ void in_accum(F& x) { asm volatile("" : "+a"(x)); }
 
+// What rounding to T leaves out.
+template <typename T> __device__ __forceinline__ f32x4 rounding(f32x4 x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] -= (float)(T)x[j];
+  return x;
+}
+
 // Token of register r of a score tile (from its first token).
 __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3); }
 
@@ -93,10 +100,10 @@ template <typename T, int DN, int DR, int DV>
 __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, int parts, const T* __restrict__ q, const T* __restrict__ kv,
                                                     const T* __restrict__ kpe, const int32_t* __restrict__ q_lens,
                                                     const int32_t* __restrict__ kv_lens, T* __restrict__ o,
-                                                    float* __restrict__ lse, float* __restrict__ pacc,
-                                                    float* __restrict__ pstat) {
+                                                    float* __restrict__ lse, T* __restrict__ rest,
+                                                    float* __restrict__ pacc, float* __restrict__ pstat) {
   constexpr int KN = DN / 16, KS = (DN + DR) / 16, NT = DV / 32, TK = sizeof(T) == 2 ? 64 : 32, NS = TK / 32;
-  constexpr int FG = 1, FL = 3;  // fragments are read three MFMAs ahead
+  constexpr int FG = sizeof(T) == 2 ? 2 : 1, FL = 2;  // fragments are read four MFMAs ahead (fp32: sixteen)
   typedef LTile<T, DN> LN;
   typedef LTile<T, DR> LR;
   typedef LTile<T, DV> LV;
@@ -264,7 +271,10 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, int parts, const
       f32x4 v;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] * inv : 0.f;
-      if (c < d.dv) store4(orow + c, v);
+      if (c < d.dv) {
+        store4(orow + c, v);
+        if (rest) store4(rest + (orow - o) + c, rounding<T>(v));
+      }
     }
   if (lane_id() < 32) lse[at] = row < ql && sum != 0.f ? m * kLn2 + fast_log2(sum) * kLn2 : -INFINITY;
 }
@@ -273,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, int parts, const
 template <typename T>
 __global__ __launch_bounds__(256) void latent_fwd_join(LatDims d, int parts, const float* __restrict__ pacc,
                                                        const float* __restrict__ pstat, T* __restrict__ o,
-                                                       float* __restrict__ lse) {
+                                                       float* __restrict__ lse, T* __restrict__ rest) {
   const int per = d.dv / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, at = i / per, rows = (int64_t)d.B * d.H * d.T;
   if (at >= rows) return;
@@ -289,7 +299,10 @@ __global__ __launch_bounds__(256) void latent_fwd_join(LatDims d, int parts, con
     x += w * *reinterpret_cast<const f32x4*>(pacc + (p * rows + at) * d.dv + c);
   }
   const int t = (int)(at % d.T), h = (int)(at / d.T % d.H), b = (int)(at / d.T / d.H);
-  store4(o + (((int64_t)b * d.T + t) * d.H + h) * d.dv + c, x * (sum == 0.f ? 0.f : 1.f / sum));
+  const int64_t to = (((int64_t)b * d.T + t) * d.H + h) * d.dv + c;
+  x *= sum == 0.f ? 0.f : 1.f / sum;
+  store4(o + to, x);
+  if (rest) store4(rest + to, rounding<T>(x));
   if (c == 0) lse[at] = sum == 0.f ? -INFINITY : m * kLn2 + fast_log2(sum) * kLn2;
 }
 
@@ -298,9 +311,12 @@ __global__ __launch_bounds__(256) void latent_fwd_join(LatDims d, int parts, con
 // can hold an lse of infinity (every p of theirs is zero).
 __host__ __device__ inline int64_t stat_rows(int T) { return (int64_t)(T + 63) / 64 * 64; }
 
-// stat: delta and lse in powers of two, each [B, H, stat_rows]: sixteen lanes a row.
+// stat: delta (from o and, in bf16, what its rounding left out: 13 us of B2 T8192 H16's
+// 2.8 ms, for a row that sees few keys most of its scores' gradients) and lse in powers
+// of two, each [B, H, stat_rows]: sixteen lanes a row.
 template <typename T>
-__global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restrict__ o, const T* __restrict__ dout,
+__global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restrict__ o, const T* __restrict__ rest,
+                                                    const T* __restrict__ dout,
                                                     const float* __restrict__ lse, const int32_t* __restrict__ q_lens,
                                                     float* __restrict__ stat) {
   const int64_t TP = stat_rows(d.T), j = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, t, h)
@@ -320,6 +336,11 @@ __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restri
   for (int c = 8 * (threadIdx.x & 15); c < d.dv; c += 128) {
     float x[8], y[8];
     load8(o + i * d.dv + c, x);
+    if (rest) {
+      load8(rest + i * d.dv + c, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] += y[j];
+    }
     load8(g + c, y);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s += x[j] * y[j];
@@ -969,11 +990,11 @@ extern "C" size_t atomic_latent_fwd_workspace_size(const atomic_latent_args* a) 
 }
 
 extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
-                                 const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* workspace,
-                                 size_t workspace_bytes, void* stream) {
+                                 const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* o_rest,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = lat_check(a)) return rc;
   if (!q || !kv || !k_pe || !o || !lse) return ATOMIC_ERR_NULL;
-  if (!aligned16({q, kv, k_pe, o})) return ATOMIC_ERR_SHAPE;
+  if (!aligned16({q, kv, k_pe, o, o_rest})) return ATOMIC_ERR_SHAPE;
   const int parts = fwd_parts(a);
   if (parts > 1) {
     if (!workspace || workspace_bytes < atomic_latent_fwd_workspace_size(a) || !aligned16({workspace}))
@@ -987,17 +1008,18 @@ extern "C" int atomic_latent_fwd(const atomic_latent_args* a, const void* q, con
   return lat_dispatch(a, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
+    T* rest = sizeof(T) == 2 ? (T*)o_rest : nullptr;
     LatDims d = lat_dims(a);
     d.blocks = (d.T + 127) / 128 * parts;
     int rc = L("latent_fwd", [&] {
       hipLaunchKernelGGL((latent_fwd<T, W::DN, W::DR, W::DV>), dim3((unsigned)(d.B * d.H * d.blocks)), dim3(256), 0, st,
-                         d, parts, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, (T*)o, lse, pacc, pstat);
+                         d, parts, (const T*)q, (const T*)kv, (const T*)k_pe, q_lens, kv_lens, (T*)o, lse, rest, pacc, pstat);
     });
     if (rc || parts == 1) return rc;
     const int64_t n = (int64_t)d.B * d.H * d.T * (d.dv / 4);
     return L("latent_fwd_join", [&] {
       hipLaunchKernelGGL((latent_fwd_join<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, d, parts, pacc,
-                         pstat, (T*)o, lse);
+                         pstat, (T*)o, lse, rest);
     });
   });
 }
@@ -1010,11 +1032,11 @@ extern "C" size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a) 
 
 extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
                                  const int32_t* q_lens, const int32_t* kv_lens, const void* o, const float* lse,
-                                 const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
+                                 const void* o_rest, const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
                                  size_t workspace_bytes, void* stream) {
   if (int rc = lat_check(a)) return rc;
   if (!q || !kv || !k_pe || !o || !lse || !dout || !dq || !dkv || !dk_pe) return ATOMIC_ERR_NULL;
-  if (!aligned16({q, kv, k_pe, o, dout, dq, dkv, dk_pe})) return ATOMIC_ERR_SHAPE;
+  if (!aligned16({q, kv, k_pe, o, o_rest, dout, dq, dkv, dk_pe})) return ATOMIC_ERR_SHAPE;
   if (!workspace || workspace_bytes < atomic_latent_bwd_workspace_size(a) || !aligned16({workspace}))
     return ATOMIC_ERR_WORKSPACE;
   ws_tag_clobber(workspace, atomic_latent_bwd_workspace_size(a));
@@ -1033,7 +1055,7 @@ extern "C" int atomic_latent_bwd(const atomic_latent_args* a, const void* q, con
     const int64_t rows = (int64_t)d.B * stat_rows(d.T) * d.H;
     int rc = L("latent_delta", [&] {
       hipLaunchKernelGGL((latent_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, d, (const T*)o,
-                         (const T*)dout, lse, q_lens, stat);
+                         sizeof(T) == 2 ? (const T*)o_rest : nullptr, (const T*)dout, lse, q_lens, stat);
     });
     if (rc) return rc;
     d.blocks = (d.S + 127) / 128 * p.kparts;

@@ -190,28 +190,39 @@ template <> struct M16<float> {
 template <typename T, int W>
 struct DTile : LTile<T, W, 16> {
   typedef LTile<T, W, 16> L;
-  static __device__ __forceinline__ typename M16<T>::frag row16(const char* s, int r0, int k0) {
-    const int l = lane_id(), r = r0 + (l & 15), k = k0 + 8 * (l >> 4);
+  // (from base addresses as in LTile: row16_base and col16_base plus the tile's LDS address)
+  static __device__ __forceinline__ uint32_t row16_base() {
+    return L::off(lane_id() & 15, 8 / L::VEC * (lane_id() >> 4));
+  }
+  static __device__ __forceinline__ typename M16<T>::frag row16(uint32_t base, int k0) {
+    typedef const __attribute__((address_space(3))) char* lds_p;
+    const int c = k0 / L::VEC;
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const bf16x8*>(s + L::off(r, k / 8));
+      return *(const __attribute__((address_space(3))) bf16x8*)((lds_p)(base ^ L::piece(c)) + L::above(c));
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(s + L::off(r, k / 4));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(s + L::off(r, k / 4 + 1));
+      const f32x4 a = *(const __attribute__((address_space(3))) f32x4*)((lds_p)(base ^ L::piece(c)) + L::above(c));
+      const f32x4 b = *(const __attribute__((address_space(3))) f32x4*)((lds_p)(base ^ L::piece(c + 1)) + L::above(c));
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  static __device__ __forceinline__ typename M16<T>::half col16(const char* s, int r0, int c0) {
+  static __device__ __forceinline__ uint32_t col16_base() {
     const int l = lane_id(), t = l & 15, g = l >> 4;
+    if constexpr (sizeof(T) == 2) return L::off(4 * g + (t >> 2), (t & 3) >> 1) + 8 * (t & 1);
+    else return L::off(4 * g, t >> 2) + 4 * (t & 3);
+  }
+  static __device__ __forceinline__ typename M16<T>::half col16(uint32_t base, int c0) {
+    typedef const __attribute__((address_space(3))) char* lds_p;
+    const int c = c0 / L::VEC;
     if constexpr (sizeof(T) == 2) {
-      const int r = r0 + 4 * g + (t >> 2), c = c0 + 4 * (t & 3);
-      typedef __attribute__((address_space(3))) bf16x4* lds_p;
-      return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_p)(s + L::off(r, c / 8) + 2 * (c & 7)));
+      typedef __attribute__((address_space(3))) bf16x4* v4_p;
+      return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((v4_p)((lds_p)(base ^ L::piece(c)) + L::above(c)));
     } else {
-      const int c = c0 + t;
       f32x4 z;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        z[j] = *reinterpret_cast<const float*>(s + L::off(r0 + 4 * g + j, c / 4) + 4 * (c & 3));
+      for (int j = 0; j < 4; ++j) {
+        const lds_p p = (lds_p)(base ^ L::piece(c) ^ (L::swz(j) << 4)) + j * L::ROWB + L::above(c);
+        z[j] = *(const __attribute__((address_space(3))) float*)p;
+      }
       return z;
     }
   }
@@ -321,10 +332,12 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
     f32x4 s[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const char* kc = sk + (buf * NW + MT * tw + i) * (SC + SR);
+      const uint32_t kc = lds0 + (buf * NW + MT * tw + i) * (SC + SR);
+      uint32_t rc = kc + LC::row16_base(), rr = kc + SC + LR::row16_base();
+      asm volatile("" : "+v"(rc), "+v"(rr));
       f32x4 x[2] = {zero4(), zero4()};  // two chains: each waits for its own result only
-      in_groups<KS, 24 / (int)sizeof(T) / 2, frag>(
-          [&](int t) { return 32 * t < DC ? LC::row16(kc, 0, 32 * t) : LR::row16(kc + SC, 0, 32 * t - DC); },
+      in_groups<KS, sizeof(T) == 2 ? 6 : 2, frag>(
+          [&](int t) { return 32 * t < DC ? LC::row16(rc, 32 * t) : LR::row16(rr, 32 * t - DC); },
           [&](int t, frag a) { x[t & 1] = M16<T>::mma(a, qf[t], x[t & 1]); });
       s[i] = x[0] + x[1];
     }
@@ -366,9 +379,10 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
           e -= (float)p[k][i][r];
         }
       }
-    const char* kc = sk + (buf * NW + MT * tw) * (SC + SR);
+    uint32_t cc = lds0 + buf * NW * (SC + SR) + MT * tw * (SC + SR) + LC::col16_base();
+    asm volatile("" : "+v"(cc));
     if constexpr (MT == 1) {
-      in_groups<NT, 16 / (int)sizeof(T), half>([&](int n) { return LC::col16(kc, 0, 16 * n); },
+      in_groups<NT, sizeof(T) == 2 ? 8 : 2, half>([&](int n) { return LC::col16(cc, 16 * n); },
                                                [&](int n, half a) {
 #pragma unroll
                                                  for (int k = 0; k < NP; ++k) acc[n] = M16<T>::mma4(a, p[k][0], acc[n]);
@@ -379,10 +393,10 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
         frag pp[NP];
 #pragma unroll
         for (int k = 0; k < NP; ++k) pp[k] = __builtin_shufflevector(p[k][i], p[k][i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-        const char* ka = kc + i * (SC + SR);
-        in_groups<NT, 8 / (int)sizeof(T), frag>(
+        const uint32_t ca = cc + i * (SC + SR);
+        in_groups<NT, sizeof(T) == 2 ? 4 : 1, frag>(
             [&](int n) {
-              return __builtin_shufflevector(LC::col16(ka, 0, 16 * n), LC::col16(ka + SC + SR, 0, 16 * n), 0, 1, 2, 3,
+              return __builtin_shufflevector(LC::col16(ca, 16 * n), LC::col16(ca + SC + SR, 16 * n), 0, 1, 2, 3,
                                              4, 5, 6, 7);
             },
             [&](int n, frag a) {

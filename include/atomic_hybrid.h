@@ -810,22 +810,25 @@ typedef struct atomic_latent_args {
 size_t atomic_latent_fwd_workspace_size(const atomic_latent_args* a);
 
 /* Forward: o [B, tq, H, dv] dtype and lse [B, H, tq] fp32 (the natural log of
- * the sum of the scores' exponentials), both dense.  q_lens and kv_lens are
+ * the sum of the scores' exponentials), both dense.  o_rest: NULL, or in bf16 what
+ * o's rounding left out, rounded itself, laid out as o (fp32: not written).  q_lens and kv_lens are
  * int32 [B] device arrays, or NULL.  The workspace may be NULL where the size
  * above is at most 16. */
 int atomic_latent_fwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
-                      const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* workspace,
-                      size_t workspace_bytes, void* stream);
+                      const int32_t* q_lens, const int32_t* kv_lens, void* o, float* lse, void* o_rest,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace the backward needs; 0 for unsupported args. */
 size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a);
 
-/* Backward from the forward's o and lse and the upstream gradient do: dq
+/* Backward from the forward's o, o_rest (or NULL) and lse and the upstream gradient
+ * do.  A score's gradient is a difference of do . v_j and do . o: without o_rest, o's
+ * rounding is most of what is left where a query sees few keys.  dq
  * [B, tq, H, dn + dr], dkv [B, tk, H, dn + dv], dk_pe [B, tk, dr] (summed over
  * the heads), dense, dtype.  The same inputs give the same bits. */
 int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
                       const int32_t* q_lens, const int32_t* kv_lens, const void* o, const float* lse,
-                      const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
+                      const void* o_rest, const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,
                       size_t workspace_bytes, void* stream);
 
 /* The paged cache: [pages, page, dc + dr] dtype, dense; a token's row holds its

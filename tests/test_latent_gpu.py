@@ -112,6 +112,11 @@ def _against_the_oracle(shape, dtype, seed, scale=None):
     want, size = ol.expanded_grads(q, kv, k_pe, do, scale, causal, ql, kl)
     for n, a, b, z in zip(("dq", "dkv", "dk_pe"), grads, want, size):
         _within(a, b, 1.5 * z, U[dtype], n)
+    _, _, rest = L.forward(*d, scale, save=True, **kw)
+    if dtype == BF16:
+        _within(o.double() + rest.double(), o_ref, mag, 2.0 ** -8, "o and what its rounding left out")
+    for n, a, b, z in zip(("dq", "dkv", "dk_pe"), L.backward(*d, o, lse, do.cuda(), scale, rest=rest, **kw), want, size):
+        _within(a, b, 1.5 * z, U[dtype], n)
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -146,6 +151,24 @@ def test_more_score_gradients_than_are_kept():
         for n, x, a, b, z in zip(("dq", "dkv", "dk_pe"), (ql, kl, kl), grads, want, size):
             _within(a[:, :x], b, 1.5 * z, U[BF16], n)
             assert (a[:, x:] == 0).all()
+
+
+def test_scores_of_one_key_have_no_gradient():
+    """A query that sees one key: do . v less do . o is zero.  With what o's
+    rounding left out, itself rounded, o is known to 2^-16; the two sums of 128
+    products differ by 128 * 2^-24 of their sizes, the difference is rounded (in a
+    ratio) and so is its product: within 2^-15 of the terms' sizes."""
+    banner("latent expanded one key")
+    for T, S, causal, ql, kl in ((3, 1, False, None, None), (64, 64, True, [1], [1])):
+        q, kv, k_pe, do = _inputs(1, T, S, 2, 128, 64, 128, BF16, seed=26)
+        x = [t.cuda().requires_grad_(True) for t in (q, kv, k_pe)]
+        o = L.attention(*x, 0.07, causal=causal, q_lens=_i32(ql), kv_lens=_i32(kl))
+        grads = torch.autograd.grad(o, x, do.cuda())
+        want, size = ol.expanded_grads(q, kv, k_pe, do, 0.07, causal, ql, kl)
+        for i in (0, 2):
+            assert (grads[i].double().cpu() - want[i]).abs().sub(2.0 ** -15 * size[i]).max() <= 0
+        assert torch.equal(L.forward(*(t.detach() for t in x), 0.07, causal=causal, q_lens=_i32(ql),
+                                     kv_lens=_i32(kl))[0], o.detach())
 
 
 def test_lengths_belong_to_the_graph():
@@ -222,8 +245,8 @@ def test_autograd_broadcast_gradient_and_repeats():
         assert torch.equal(a, b)
     ones = torch.ones_like(runs[0][0])
     with torch.no_grad():
-        o, lse = L.forward(*x, 0.07)
-        for a, b in zip(L.backward(*x, o, lse, ones, 0.07), runs[0][1:]):
+        o, lse, rest = L.forward(*x, 0.07, save=True)
+        for a, b in zip(L.backward(*x, o, lse, ones, 0.07, rest=rest), runs[0][1:]):
             assert torch.equal(a, b)
 
 
@@ -471,7 +494,7 @@ def test_refusals():
     args, _ = L.make_args(q, kv, k_pe, 1.0, True, o)
     lib, p = _lib.load(), lambda t: t.data_ptr()
     small = z(64, dt=torch.uint8)
-    for call in (lambda ws, n: lib.atomic_latent_bwd(args, p(q), p(kv), p(k_pe), None, None, p(o), p(lse), p(o), p(q),
+    for call in (lambda ws, n: lib.atomic_latent_bwd(args, p(q), p(kv), p(k_pe), None, None, p(o), p(lse), None, p(o), p(q),
                                                      p(kv), p(k_pe), ws, n, None),):
         for ws, n in ((None, 1 << 20), (p(small), 64)):
             with pytest.raises(_lib.AtomicError, match="WORKSPACE"):

@@ -115,13 +115,13 @@ def test_the_library_refuses_what_it_cannot_run():
                 dict(batch=1 << 20, heads=1 << 20), dict(q_stride=(1440, 288, 92)), dict(kv_stride=(-8, 384, 128))):
         assert size(_args(**bad)) == 0, bad
     null = ctypes.c_void_p(0)
-    assert lib.atomic_latent_fwd(ctypes.byref(_args()), *[null] * 8, 0, null) == -5
-    assert lib.atomic_latent_fwd(None, *[null] * 8, 0, null) == -5
+    assert lib.atomic_latent_fwd(ctypes.byref(_args()), *[null] * 9, 0, null) == -5
+    assert lib.atomic_latent_fwd(None, *[null] * 9, 0, null) == -5
     one = ctypes.c_void_p(16)
     # operands off 16 bytes and a missing workspace are refused before anything is launched
-    assert lib.atomic_latent_fwd(ctypes.byref(_args()), ctypes.c_void_p(8), one, one, null, null, one, one, null, 0,
+    assert lib.atomic_latent_fwd(ctypes.byref(_args()), ctypes.c_void_p(8), one, one, null, null, one, one, null, null, 0,
                                  null) == -1
-    assert lib.atomic_latent_bwd(ctypes.byref(_args()), one, one, one, null, null, *[one] * 6, null, 0, null) == -3
+    assert lib.atomic_latent_bwd(ctypes.byref(_args()), one, one, one, null, null, one, one, null, *[one] * 4, null, 0, null) == -3
     d = lambda **k: _lib.LatentDecodeArgs(*{**dict(batch=2, tokens=1, heads=4, dn=64, dr=32, dv=64, dc=128, dtype=1,
                                                    page=16, pages=9, table_pages=4, rope_rows=99, interleaved=0,
                                                    scale=0.1), **k}.values(), (384, 384, 96))
