@@ -11,6 +11,9 @@ the same sums with U32 = 2e-5, a score of 192 products being off by up to
 scores of unit spread each contributes 0.58 * 2^-8 to a row's 2-norm, together
 2^-8: a row may be off by four times that, all rows by twice.
 """
+import importlib.util
+import os
+
 import pytest
 import torch
 
@@ -464,6 +467,16 @@ def test_other_streams_and_graph_replays():
         torch.cuda.synchronize()
         replayed = out.clone()
         assert torch.equal(replayed, step())
+
+
+def test_the_example_layer_agrees_with_itself():
+    """examples/latent_layer.py: training steps, a prompt and single tokens of one layer."""
+    banner("latent example layer")
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "latent_layer.py")
+    spec = importlib.util.spec_from_file_location("latent_layer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    example.main(B=2, T=80, prompt=65, page=16, steps=2)
 
 
 def test_refusals():
