@@ -56,13 +56,6 @@ template <typename T> __device__ __forceinline__ typename M32<T>::frag zero_frag
   for (int j = 0; j < 8; ++j) z[j] = (T)0.f;
   return z;
 }
-// registers 8 s .. 8 s + 7 of a result as the next product's operand
-template <typename T> __device__ __forceinline__ typename M32<T>::frag pack_frag(const f32x16& x, int s) {
-  typename M32<T>::frag z;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = (T)x[8 * s + j];
-  return z;
-}
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll

@@ -84,14 +84,14 @@ __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_
 // 128 query rows of a head a workgroup, 32 a wave, against tiles of 64 tokens (32 in
 // fp32) that go straight to LDS, one tile ahead; one barrier a tile.  Two workgroups a
 // CU, so two waves a SIMD with 256 registers each: one's MFMAs run beside the other's
-// softmax.  (Eight waves on one tile, the two of a SIMD half a tile apart, take half the
-// tiles out of L2 and still lose, by the longer workgroups' tails: 264 us against 252 at
-// B8 T4096 H6, 650 against 630 at B2 T8192 H16; 318 against 337 at B1 T8192 H16.)
+// softmax.  (Eight waves on one tile, the two of a SIMD half a tile apart, took half the
+// tiles out of L2 and still lost, by the longer workgroups' tails: 264 us against 242 at
+// B8 T4096 H6, 650 against 605 at B2 T8192 H16, 318 against 316 at B1 T8192 H16.)
 //
 // Bound by the matrix instructions, for which the card lowers its clock: without a pause
 // it takes 20.8 ns an instruction and SIMD (1.63 PF/s).  B2 T8192 H16, 128/64/128,
-// causal: 630 us, 1.09 PF/s, where the library's product of two 8192 x 8192 matrices
-// reaches 1.20.
+// causal: 605 to 640 us, 1.07 to 1.14 PF/s, where the library's product of two
+// 8192 x 8192 matrices reaches 1.21.
 //
 // With `parts` > 1 the keys of a row block are divided over that many workgroups
 // (few row blocks against many keys); each leaves its accumulators, reference and
@@ -356,8 +356,8 @@ __global__ __launch_bounds__(256) void latent_delta(LatDims d, const T* __restri
 
 // dq where the score gradients are not kept (fp32, and bf16 above kMostDs): 128 query
 // rows of a head a workgroup, 32 a wave, against tiles of tokens staged as in the
-// forward; scores and their gradients once more.  B2 T8192 H16 bf16: 1093 us, where
-// latent_bwd_dq_ds takes 530 and costs latent_bwd_dkv 240.
+// forward; scores and their gradients once more.  B2 T8192 H16 bf16: 1068 us, where
+// latent_bwd_dq_ds takes 531 and its score gradients cost latent_bwd_dkv 195.
 template <typename T, int DN, int DR, int DV>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
     LatDims d, const T* __restrict__ q, const T* __restrict__ kv, const T* __restrict__ kpe,
@@ -523,13 +523,13 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
 // rotated key's gradient leaves as this head's part, fp32 [B, H, S, dr].
 //
 // Four of the backward's five products (scores, dp, dv, dk) run here, bound by the
-// matrix instructions: B2 T8192 H16 causal 1480 to 1530 us, 0.9 PF/s.
+// matrix instructions: B2 T8192 H16 causal 1500 us, 0.92 PF/s.
 //
 // With DS the score gradients go to memory too, for latent_bwd_dq_ds: [B, H, tiles of
 // 64 rows, S, 64] bf16, a token's rows in the order of this kernel's registers
 // (ds_piece), 16 bytes a lane as they are, so that a wave writes 4 KB in a row.  (In
 // rows of T the 32 tokens of a wave lay a power of two apart: 1710 us instead of
-// 1484 at B2 T8192 H16.)  They are the last memory operations of a tile, so the wait for
+// 1484 at B2 T8192 H16, when that was changed.)  They are the last memory operations of a tile, so the wait for
 // the next tile's loads leaves them in flight.
 template <typename T, int DN, int DR, int DV, bool DS>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __restrict__ q, const T* __restrict__ kv,
@@ -937,7 +937,9 @@ static int lat_dispatch(const atomic_latent_args* a, F&& f) {
   return small ? f(float(), Widths<64, 32, 64>()) : f(float(), Widths<128, 64, 128>());
 }
 
-// The forward's parts of the keys: while they leave some of the card free, and of eight tiles or more.
+// The forward's parts of the keys: doubled while they fill no more than half of the 512
+// places, and of eight tiles or more (B2 T517 over S4500, H6: 111 us in one part, 46 in
+// eight and their join, when that was made).
 static int fwd_parts(const atomic_latent_args* a) {
   const int64_t wgs = (int64_t)a->batch * a->heads * ((a->tq + 127) / 128), tiles = (a->tk + 63) / 64;
   int p = 1;
@@ -954,12 +956,16 @@ struct BwdPlan {
   int qrows, qparts, kparts;         // rows a workgroup of the dq kernel
   size_t stat, dkp, pq, pkv, ds;     // bytes; ds: the score gradients, 0 where dq computes them again
 };
+// The backward's: as long as they fit the 256 CUs (one workgroup each) and have four
+// tiles or more (fp32 B2 T512 H4, training: 286 us of kernels in one part, 108 in several).
 static int parts_for(int64_t wgs, int64_t tiles) {
   int p = 1;
   while (p < 16 && 2 * p * wgs <= 256 && 4 * p <= tiles) p *= 2;
   return p;
 }
-// Score gradients up to this size are kept between the two kernels (bf16).
+// Score gradients up to this size are kept between the two kernels (bf16): both of them
+// together take 2040 us against 2380 at B2 T8192 H16 and 880 against 1030 at B8 T4096 H6.
+// What the size costs is memory only; 4 GB is 1.4 % of the card's.
 constexpr int64_t kMostDs = (int64_t)4 << 30;
 static BwdPlan bwd_plan(const atomic_latent_args* a) {
   const int64_t bh = (int64_t)a->batch * a->heads, tile = a->dtype == ATOMIC_BF16 ? 64 : 32;
