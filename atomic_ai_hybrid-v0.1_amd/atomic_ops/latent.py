@@ -16,6 +16,7 @@ cache [pages, page, dc + dr] whose rows are [latent | rotated key]:
   ``append``   writes tokens into the cache and rotates keys and queries
   ``decode``   reads it
 The two forms of the same weights and tokens give the same outputs up to rounding.
+No queries, keys or tokens (a dimension of zero) give empty or zero outputs.
 """
 from __future__ import annotations
 
@@ -141,6 +142,10 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, save=
     read in place."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
     lib = _lib.load()
+    if not (q.numel() and kv.numel()):      # no queries, or none that sees a key
+        o = q.new_zeros(*q.shape[:3], kv.shape[3] - (q.shape[3] - k_pe.shape[2]))
+        lse = q.new_full((q.shape[0], q.shape[2], q.shape[1]), float("-inf"), dtype=torch.float32)
+        return (o, lse, torch.zeros_like(o) if q.dtype == torch.bfloat16 else None) if save else (o, lse)
     args, (q, kv, k_pe, _) = make_args(q, kv, k_pe, scale, causal)
     if timer is not None:
         args.profile = timer.arm()
@@ -180,6 +185,8 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     if lse.shape != (B, H, T) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise ValueError("lse must be float32 [B, H, T] on q's device")
     lib = _lib.load()
+    if not (q.numel() and kv.numel()):
+        return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) for t in (q, kv, k_pe))
     args, (q, kv, k_pe, dout) = make_args(q, kv, k_pe, scale, causal, dout)
     if timer is not None:
         args.profile = timer.arm()
@@ -272,6 +279,8 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
         H, dn = q.shape[1], q.shape[2] - dr
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = torch.empty(N, dr, dtype=k_pe.dtype, device=k_pe.device)
+    if N == 0:
+        return k_out, q_out
     args = _lib.LatentAppendArgs(N, H, dn, dr, dc, _DT[k_pe.dtype], page, pages, cos.shape[0], 1 if interleaved else 0,
                                  cs[0], ks[0], qs)
     if timer is not None:
@@ -311,6 +320,8 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
         raise ValueError("latent decode: cos and sin come together")
     if cos is not None:
         cos, sin = _tables("latent decode", cos, sin, dr, dev)
+    if not (q.numel() and page_table.numel()):      # no queries, or none with a token to see
+        return q.new_zeros(B, n, H, w_kv.shape[1] - (d - dr))
     q, qs = _strided(q, 3)
     w_kv, _ = _strided(w_kv.contiguous(), 2)
     lib = _lib.load()

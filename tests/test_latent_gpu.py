@@ -479,6 +479,26 @@ def test_the_example_layer_agrees_with_itself():
     example.main(B=2, T=80, prompt=65, page=16, steps=2)
 
 
+def test_nothing_to_do():
+    """Dimensions of zero: no queries, no keys, no tokens to append, no pages."""
+    banner("latent empty dimensions")
+    z = lambda *s, dt=BF16: torch.ones(*s, dtype=dt, device="cuda")
+    for B, T, S in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        x = [t.requires_grad_(True) for t in (z(B, T, 2, 96), z(B, S, 2, 128), z(B, S, 32))]
+        o = L.attention(*x, 0.1)
+        assert o.shape == (B, T, 2, 64) and (o == 0).all()
+        assert (L.forward(*(t.detach() for t in x), 0.1)[1] == -INF).all()
+        for t, g in zip(x, torch.autograd.grad(o.float().sum(), x)):
+            assert g.shape == t.shape and (g == 0).all()
+    cache, w, cs = z(3, 16, 96), z(2, 128, 64), z(9, 16, dt=F32)
+    before = cache.clone()
+    k, q = L.append(cache, z(0, 64), z(0, 32), z(0, dt=torch.int64), z(0, dt=torch.int32), cs, cs, q=z(0, 2, 96))
+    assert k.shape == (0, 32) and q.shape == (0, 2, 96) and torch.equal(cache, before)
+    assert L.decode(z(0, 1, 2, 96), w, cache, z(0, 2, dt=torch.int32), z(0, dt=torch.int32), 0.1).shape == (0, 1, 2, 64)
+    none = L.decode(z(2, 1, 2, 96), w, cache, z(2, 0, dt=torch.int32), z(2, dt=torch.int32), 0.1)
+    assert none.shape == (2, 1, 2, 64) and (none == 0).all()
+
+
 def test_refusals():
     banner("latent refusals")
     z = lambda *s, dt=BF16: torch.zeros(*s, dtype=dt, device="cuda")
