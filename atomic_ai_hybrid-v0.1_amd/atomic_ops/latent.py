@@ -169,8 +169,9 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     """``(dq, dkv, dk_pe)`` in the inputs' shapes and dtype from the forward's
     ``o``, ``lse`` and ``rest``; k_pe's gradient is summed over the heads.  A
     score's gradient is a difference of do . v and do . o: without ``rest``, o's
-    rounding is most of what is left where a query sees few keys.  The same inputs
-    give the same bits."""
+    rounding is most of what is left where a query sees few keys; one that sees a
+    single key gives its score a gradient of exactly zero.  The same inputs give the
+    same bits."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
     B, T, H, d = q.shape
     dv = kv.shape[3] - (d - k_pe.shape[2])

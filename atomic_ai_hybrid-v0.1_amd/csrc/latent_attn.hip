@@ -13,6 +13,11 @@
 // MFMA takes them; everything else (scores, the running maximum and sum, lse, delta,
 // every accumulator) is fp32.
 //
+// A query that sees one key (always the first) has p = 1 whatever its score, so ds = 0.
+// Formed as do . v - do . o it would be what the two sums' roundings leave (the one in
+// the order of the matrix instructions, the other in latent_delta's), 1e-7 of the terms
+// where the gradient is zero: its ds is therefore formed with a weight of zero.
+//
 // Masked places are replaced, not weighted, so a masked score may be anything; a
 // masked value enters a product with a weight of zero, as in any tiled or plain form,
 // so an infinity or NaN in a later token of a causal sequence can reach the queries
@@ -400,7 +405,9 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
   row_frags<T, DN, DR>(qf, qr, d.dn, qr + d.dn, d.dr);
   row_frags<T, DV, 0>(gf, dout + b * d.gs[0] + (int64_t)rowc * d.gs[1] + h * d.gs[2], d.dv, (const T*)nullptr, 0);
   const int64_t at = ((int64_t)b * d.H + h) * stat_rows(d.T) + rowc;
-  const float dl = stat[at], l2 = stat[(int64_t)d.B * d.H * stat_rows(d.T) + at];
+  // (a row of one key: an lse of infinity makes its p zero)
+  const bool one = (d.causal ? min(kl, row + off + 1) : kl) == 1;
+  const float dl = stat[at], l2 = one ? INFINITY : stat[(int64_t)d.B * d.H * stat_rows(d.T) + at];
   f32x16 acc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n] = zero16();
@@ -607,8 +614,9 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
   };
   // One tile.  Its two halves follow each other by a phase: the scores of the
   // second half run beside the first half's exponentials, the gradients of the
-  // first beside the second's.  Only the diagonal needs a mask: rows past the last
-  // query have an lse of infinity, tokens past the last key are not stored.
+  // first beside the second's.  Only the diagonal needs a mask (and a sequence of one
+  // key its ds of zero): rows past the last query have an lse of infinity, tokens past
+  // the last key are not stored.
   auto step = [&](auto masked) {
     const uint32_t at = l0 + buf * STAGE;
     uint32_t rn = at + LN::row_base(), rr = at + OR + LR::row_base(), rg = at + OG + LG::row_base();
@@ -646,9 +654,10 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
         const int r = 4 * k + j;
         float x = fast_exp2(s[i][r] * c2 - l4[j]), y = x * (g[i][r] - d4[j]);
         if constexpr (decltype(masked)::value) {
-          const bool ok = tok <= q0 + 32 * i + reg_row(r) + off;
-          x = ok ? x : 0.f;
-          y = ok ? y : 0.f;
+          const int end = d.causal ? q0 + 32 * i + reg_row(r) + off : kl - 1;  // the last token that the row sees
+          y = end == 0 ? 0.f * (g[i][r] - d4[j]) : y;                          // (a NaN stays one)
+          x = tok <= end ? x : 0.f;
+          y = tok <= end ? y : 0.f;
         }
         p[i][k / 2][4 * (k & 1) + j] = (T)x;
         ds[i][k / 2][4 * (k & 1) + j] = (T)y;
@@ -693,7 +702,7 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dkv(LatDims d, const T* __r
     stage();
     dma.all(to);
   }
-  for (; q0 < stop && d.causal && w0 + 31 > q0 + off; q0 += TQ, buf ^= 1) {
+  for (; q0 < stop && (kl == 1 || (d.causal && w0 + 31 > q0 + off)); q0 += TQ, buf ^= 1) {
     stage();
     step(IntC<1>());
     stored = true;

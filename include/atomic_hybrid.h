@@ -823,9 +823,10 @@ size_t atomic_latent_bwd_workspace_size(const atomic_latent_args* a);
 
 /* Backward from the forward's o, o_rest (or NULL) and lse and the upstream gradient
  * do.  A score's gradient is a difference of do . v_j and do . o: without o_rest, o's
- * rounding is most of what is left where a query sees few keys.  dq
- * [B, tq, H, dn + dr], dkv [B, tk, H, dn + dv], dk_pe [B, tk, dr] (summed over
- * the heads), dense, dtype.  The same inputs give the same bits. */
+ * rounding is most of what is left where a query sees few keys; one that sees a
+ * single key gives its score a gradient of exactly zero.  dq [B, tq, H, dn + dr],
+ * dkv [B, tk, H, dn + dv], dk_pe [B, tk, dr] (summed over the heads), dense, dtype.
+ * The same inputs give the same bits. */
 int atomic_latent_bwd(const atomic_latent_args* a, const void* q, const void* kv, const void* k_pe,
                       const int32_t* q_lens, const int32_t* kv_lens, const void* o, const float* lse,
                       const void* o_rest, const void* dout, void* dq, void* dkv, void* dk_pe, void* workspace,

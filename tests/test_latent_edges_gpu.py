@@ -1,0 +1,74 @@
+"""Latent attention on the GPU at its edges."""
+import pytest
+import torch
+
+from _util import banner
+from atomic_ops import latent as L
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+NAN, INF = float("nan"), float("inf")
+
+
+def _inputs(B, T, S, H, dn, dr, dv, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype)
+    return r(B, T, H, dn + dr), r(B, S, H, dn + dv), r(B, S, dr), r(B, T, H, dv)
+
+
+def _i32(v):
+    return None if v is None else torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,T,S,H,widths,causal,ql,kl,alone", [
+    # alone: batch row -> the query rows that see one key
+    (8, 1, 1, 3, (128, 64, 128), True, None, None, lambda b: range(1)),
+    (2, 3, 1, 2, (64, 32, 64), False, None, None, lambda b: range(3)),
+    (1, 300, 1, 2, (128, 64, 128), False, None, None, lambda b: range(300)),
+    (1, 300, 1, 1, (56, 24, 72), True, None, None, lambda b: [299]),
+    (3, 64, 64, 2, (128, 64, 128), True, [1, 40, 64], [1, 1, 1], lambda b: [(0, 39, 63)[b]]),
+    (3, 64, 64, 2, (128, 64, 128), False, [1, 40, 64], [1, 1, 1], lambda b: range((1, 40, 64)[b])),
+    (2, 300, 300, 2, (128, 64, 128), True, None, None, lambda b: [0]),
+    (1, 200, 70, 2, (96, 32, 64), True, None, None, lambda b: [130]),
+    (1, 700, 40, 1, (64, 32, 64), True, [690], [33], lambda b: [657]),   # the queries divided over workgroups
+])
+def test_a_query_of_one_key_gives_its_score_no_gradient(B, T, S, H, widths, causal, ql, kl, alone, dtype):
+    """p is 1 whatever the score, so ds is zero: dq of such a query is zero, not a
+    rounding, and so are the keys' gradients where no other query sees anything."""
+    banner(f"latent one key B{B} T{T} S{S} H{H} {widths} causal={causal} {ql} {kl} {dtype}")
+    dn, dr, dv = widths
+    q, kv, k_pe, do = (t.cuda() for t in _inputs(B, T, S, H, dn, dr, dv, dtype, seed=T + S))
+    kw = dict(causal=causal, q_lens=_i32(ql), kv_lens=_i32(kl))
+    o, lse, rest = L.forward(q, kv, k_pe, 0.2, save=True, **kw)
+    for r in (rest, None):
+        dq, dkv, dk_pe = L.backward(q, kv, k_pe, o, lse, do, 0.2, rest=r, **kw)
+        for b in range(B):
+            assert (dq[b, list(alone(b))] == 0).all()
+            n = T if ql is None else ql[b]
+            first = max(0, n - (S if kl is None else kl[b])) if causal else 0   # the first query that sees anything
+            if len(list(alone(b))) == n - first:
+                assert (dq[b] == 0).all() and (dkv[b, ..., :dn] == 0).all() and (dk_pe[b] == 0).all()
+            assert (dkv[b, 0, :, dn:] != 0).any()     # the value's gradient is there all the same
+    # a NaN of the output's gradient is not hidden by the zero
+    do[0, alone(0)[0]] = NAN
+    dq = L.backward(q, kv, k_pe, o, lse, do, 0.2, rest=rest, **kw)[0]
+    assert torch.isnan(dq[0, alone(0)[0]]).all()
+
+
+def test_a_query_of_one_key_where_scores_are_computed_again():
+    """As above past the score gradients that are kept (bfloat16, 4 GB)."""
+    banner("latent one key, scores again")
+    T = 46400
+    d = [torch.zeros(1, T, *s, dtype=BF16, device="cuda") for s in ((1, 192), (1, 256), (64,))]
+    do = torch.zeros(1, T, 1, 128, dtype=BF16, device="cuda")
+    small = _inputs(1, 90, 70, 1, 128, 64, 128, BF16, seed=1)
+    for t, x in zip((*d, do), small):
+        t[:, :x.shape[1]] = x.cuda()
+    for ql, kl, causal, alone in ((90, 70, True, [20]), (90, 1, False, range(90)), (1, 1, True, [0])):
+        kw = dict(causal=causal, q_lens=_i32([ql]), kv_lens=_i32([kl]))
+        o, lse, rest = L.forward(*d, 0.2, save=True, **kw)
+        dq, dkv, dk_pe = L.backward(*d, o, lse, do, 0.2, rest=rest, **kw)
+        assert (dq[0, list(alone)] == 0).all()
+        assert kl > 1 or ((dkv[..., :128] == 0).all() and (dk_pe == 0).all() and (dkv[..., 128:] != 0).any())
