@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256, 2) void latent_fwd(LatDims d, int parts, const
         const int c = 32 * n + reg_row(r);
         f32x4 v;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = acc[n][r + j];
+        for (int j = 0; j < 4; ++j) v[j] = row < ql ? acc[n][r + j] : 0.f;  // (a weight of zero would keep a NaN)
         if (c < d.dv) store4(pacc + pr * d.dv + c, v);
       }
     if (lane_id() < 32) {

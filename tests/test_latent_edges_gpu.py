@@ -72,3 +72,21 @@ def test_a_query_of_one_key_where_scores_are_computed_again():
         dq, dkv, dk_pe = L.backward(*d, o, lse, do, 0.2, rest=rest, **kw)
         assert (dq[0, list(alone)] == 0).all()
         assert kl > 1 or ((dkv[..., :128] == 0).all() and (dk_pe == 0).all() and (dkv[..., 128:] != 0).any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,S", [(70, 200), (70, 2100)])      # the keys in one part, and in several
+def test_rows_past_the_length_are_zero_beside_a_last_query_that_is_not_finite(T, S, dtype):
+    banner(f"latent padding beside NaN T{T} S{S} {dtype}")
+    n = 40
+    for bad in ("q", "v"):
+        q, kv, k_pe, _ = (t.cuda() for t in _inputs(2, T, S, 2, 64, 32, 64, dtype, seed=S))
+        if bad == "q":
+            q[0, n - 1] = NAN
+        else:
+            kv[0, S - 1, :, 64:] = INF     # the last key, which the last query alone sees
+        o, lse, rest = L.forward(q, kv, k_pe, 0.1, q_lens=_i32([n, T]), save=True)
+        assert not torch.isfinite(o[0, n - 1]).any()
+        assert (o[0, n:] == 0).all() and (lse[0, :, n:] == -INF).all()
+        assert rest is None or (rest[0, n:] == 0).all()
+        assert torch.isfinite(o[1]).all() and torch.isfinite(o[0, :n - 1]).all() or bad == "v"
