@@ -44,7 +44,7 @@ def _stream(device):
 
 def _strided(t, n):
     """``(tensor, strides)``: t as the library reads it, with its first n
-    strides (0 for a dimension of one).  The last dimension has to be dense and
+    strides (that of a dimension of one is never stepped along).  The last dimension has to be dense and
     the strides and the address whole 16-byte pieces; anything else is copied.
     Every other order of the first dimensions is read in place."""
     mask = _PIECE[t.dtype]
@@ -109,7 +109,11 @@ def _check(q, kv, k_pe, q_lens, kv_lens):
 def _rows(t, n):
     """``_strided`` for [B, rows, ...]; rows more than 32 MB apart are copied too."""
     t, s = _strided(t, n)
-    return (t, s) if s[1] * t.element_size() <= _MOST_ROW_BYTES else _strided(t.contiguous(), n)
+    if s[1] * t.element_size() <= _MOST_ROW_BYTES:
+        return t, s
+    if t.shape[1] == 1:
+        return t, (s[0], 0, *s[2:])
+    return _strided(t.contiguous(), n)
 
 
 def make_args(q, kv, k_pe, scale, causal, dout=None):

@@ -90,3 +90,20 @@ def test_rows_past_the_length_are_zero_beside_a_last_query_that_is_not_finite(T,
         assert (o[0, n:] == 0).all() and (lse[0, :, n:] == -INF).all()
         assert rest is None or (rest[0, n:] == 0).all()
         assert torch.isfinite(o[1]).all() and torch.isfinite(o[0, :n - 1]).all() or bad == "v"
+
+
+def test_one_token_of_a_tensor_laid_out_token_first():
+    """Tokens 50 MB apart of which one is taken: the dense tensors' bits."""
+    banner("latent one token of far apart ones")
+    B, H, dn, dr, dv = 1024, 128, 128, 64, 128
+    wide = torch.empty(3, B, H, dn + dr, dtype=BF16, device="cuda")
+    q, kv, k_pe, do = (t.cuda() for t in _inputs(B, 1, 2, 1, dn, dr, dv, BF16, seed=3))
+    q, kv, do = (t.expand(-1, -1, H, -1) for t in (q, kv, do))
+    wide[1] = q[:, 0]
+    one = wide.transpose(0, 1)[:, 1:2]
+    assert one.stride(1) * 2 > 1 << 25
+    o, lse = L.forward(one, kv, k_pe, 0.1)
+    o2, lse2 = L.forward(q, kv, k_pe, 0.1)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    for a, b in zip(L.backward(one, kv, k_pe, o, lse, do, 0.1), L.backward(q, kv, k_pe, o, lse, do, 0.1)):
+        assert torch.equal(a, b)
