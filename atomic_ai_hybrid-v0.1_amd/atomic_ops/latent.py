@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -58,6 +59,11 @@ def _strided(t, n):
             return t, s
         t = t.clone() if t.is_contiguous() else t.contiguous()
     raise ValueError("latent attention: rows have to be whole 16-byte pieces (dimensions that are multiples of 8)")
+
+
+def _tangents(*ts):
+    """Whether any of the tensors carries a forward-mode tangent."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _operands(what, *named):
@@ -228,8 +234,10 @@ class LatentAttention(torch.autograd.Function):
 
 
 def attention(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None):
-    """o [B, T, H, dv] of ``forward``, differentiable in q, kv and k_pe."""
-    if not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad or k_pe.requires_grad)):
+    """o [B, T, H, dv] of ``forward``, differentiable in q, kv and k_pe (reverse
+    mode; forward-mode tangents are refused)."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad or k_pe.requires_grad)) and \
+            not _tangents(q, kv, k_pe):
         return forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)[0]
     return LatentAttention.apply(q, kv, k_pe, scale, causal, q_lens, kv_lens)
 

@@ -1,6 +1,7 @@
 """Latent attention on the GPU at its edges."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from _util import banner
 from atomic_ops import latent as L
@@ -107,3 +108,18 @@ def test_one_token_of_a_tensor_laid_out_token_first():
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
     for a, b in zip(L.backward(one, kv, k_pe, o, lse, do, 0.1), L.backward(q, kv, k_pe, o, lse, do, 0.1)):
         assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused():
+    """No tangent is computed, so none may get lost: dual tensors are an error, with and without a graph."""
+    banner("latent forward mode")
+    q, kv, k_pe, _ = (t.cuda() for t in _inputs(1, 8, 8, 1, 64, 32, 64, BF16, seed=24))
+    for i in range(3):
+        for graph in (False, True):
+            x = [t.clone().requires_grad_(graph) for t in (q, kv, k_pe)]
+            with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+                x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+                L.attention(*x, 0.1)
+    with forward_ad.dual_level():      # an open level by itself changes nothing
+        o = L.attention(q, kv, k_pe, 0.1)
+    assert torch.equal(o, L.attention(q, kv, k_pe, 0.1))
