@@ -61,9 +61,19 @@ def _strided(t, n):
     raise ValueError("latent attention: rows have to be whole 16-byte pieces (dimensions that are multiples of 8)")
 
 
+def _in_graph(*ts):
+    """Whether a call with these tensors belongs to a graph."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _tangents(*ts):
-    """Whether any of the tensors carries a forward-mode tangent."""
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+    """Whether any of the tensors carries a forward-mode tangent.  (The level by
+    itself first, as unpack_dual does: 1.5 us less of a call of 18.)"""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _operands(what, *named):
@@ -236,8 +246,7 @@ class LatentAttention(torch.autograd.Function):
 def attention(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None):
     """o [B, T, H, dv] of ``forward``, differentiable in q, kv and k_pe (reverse
     mode; forward-mode tangents are refused)."""
-    if not (torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad or k_pe.requires_grad)) and \
-            not _tangents(q, kv, k_pe):
+    if not (_in_graph(q, kv, k_pe) or _tangents(q, kv, k_pe)):
         return forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)[0]
     return LatentAttention.apply(q, kv, k_pe, scale, causal, q_lens, kv_lens)
 
@@ -265,7 +274,43 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
     (i, i + dr / 2), or (2 i, 2 i + 1) with ``interleaved``.  Returns
     ``(k, q)``: the rotated keys [N, dr] and, where ``q`` [N, H, dn + dr] is
     given, q with its last dr elements rotated (else None).  ``cache`` None
-    (with c_kv and slots None) only rotates."""
+    (with c_kv and slots None) only rotates.
+
+    The returned k and q are differentiable in k_pe and q (reverse mode).  What
+    enters the cache leaves the graph there: c_kv has no gradient from this call,
+    and a cache or tables that require one are refused."""
+    given = (cache, c_kv, k_pe, q, cos, sin)
+    if _in_graph(*given) or _tangents(*given):
+        return LatentAppend.apply(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer)
+    return _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer)
+
+
+class LatentAppend(torch.autograd.Function):
+    """``append`` with the gradients of k_pe and q: a rotation is orthogonal, so
+    they are the outputs' gradients turned back, by the angle's negative."""
+
+    @staticmethod
+    def forward(ctx, cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer):
+        if any(t is not None and t.requires_grad for t in (cache, cos, sin)):
+            raise ValueError("latent append: cache, cos and sin have no gradient")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, cos, sin)
+        ctx.interleaved = interleaved
+        ctx.k = k_pe.shape, k_pe.dtype, k_pe.device
+        return _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dk, dq):
+        positions, cos, sin = ctx.saved_tensors
+        shape, dtype, device = ctx.k
+        k = torch.zeros(shape, dtype=dtype, device=device) if dk is None else dk.to(dtype)
+        k, q = _append(None, None, k, None, positions, cos, -sin, None if dq is None else dq.to(dtype),
+                       ctx.interleaved, None)
+        return None, None, None if dk is None else k, None, None, None, None, q, None, None
+
+
+def _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer):
     named = [("k_pe", k_pe)] + [(n, t) for n, t in (("c_kv", c_kv), ("cache", cache), ("q", q)) if t is not None]
     _operands("latent append", *named)
     if k_pe.dim() != 2:

@@ -5,6 +5,7 @@ from torch.autograd import forward_ad
 
 from _util import banner
 from atomic_ops import latent as L
+from oracle import latent as ol
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +124,84 @@ def test_forward_mode_is_refused():
     with forward_ad.dual_level():      # an open level by itself changes nothing
         o = L.attention(q, kv, k_pe, 0.1)
     assert torch.equal(o, L.attention(q, kv, k_pe, 0.1))
+
+
+def _tables(rows, dr):
+    a = torch.arange(rows, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(0, dr, 2, dtype=torch.float64) / dr)
+    return a.cos().float(), a.sin().float()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,H,dn,dr,inter", [(1, 1, 128, 64, False), (37, 3, 56, 24, True), (300, 2, 64, 32, False)])
+def test_append_keeps_the_graph(N, H, dn, dr, inter, dtype):
+    """k and q of ``append`` against the rotation's own gradient in 64 bits.  Its
+    terms are two fp32 products and a sum, rounded once more in bf16 (at most
+    three and a half 2^-24 of two terms of up to 6 each, and 2^-8 of itself).
+    The unrotated part is passed on as it is; what the cache takes has no gradient."""
+    banner(f"latent append graph N{N} H{H} {dn}/{dr} interleaved={inter} {dtype}")
+    g = torch.Generator().manual_seed(N)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype)
+    k, q, gk, gq, c, cache = r(N, dr), r(N, H, dn + dr), r(N, dr), r(N, H, dn + dr), r(N, 64), r(N, 1, 64 + dr)
+    pos = torch.randint(0, 60, (N,), generator=g, dtype=torch.int32)      # some past the tables
+    cos, sin = _tables(50, dr)
+    kx, qx, cx = (t.cuda().requires_grad_(True) for t in (k, q, c))
+    dev, slots = cache.cuda(), torch.arange(N, device="cuda")
+    ko, qo = L.append(dev, cx, kx, slots, pos.cuda(), cos.cuda(), sin.cuda(), q=qx, interleaved=inter)
+    assert ko.requires_grad and qo.requires_grad and not dev.requires_grad
+    with torch.no_grad():      # the same bits as without a graph
+        k2, q2 = L.append(dev.clone(), cx, kx, slots, pos.cuda(), cos.cuda(), sin.cuda(), q=qx, interleaved=inter)
+    assert torch.equal(ko, k2) and torch.equal(qo, q2) and not k2.requires_grad
+    assert torch.equal(dev[:, 0], torch.cat((cx, ko), 1).detach())
+    dk, dq, dc = torch.autograd.grad((ko, qo), (kx, qx, cx), (gk.cuda(), gq.cuda()), allow_unused=True)
+    assert dc is None
+    at = pos.clamp(max=49)
+    want = []
+    for x, up in ((k, gk), (q[..., dn:], gq[..., dn:])):
+        x = x.double().requires_grad_(True)
+        y = ol.rotate(x, at, cos, sin, inter)
+        want.append(torch.autograd.grad(y, x, up.double())[0])
+    tol = lambda x: (2.0 ** -8 if dtype == BF16 else 0.0) * x.abs() + 3.5 * 2.0 ** -24 * 12
+    for a, b in ((dk, want[0]), (dq[..., dn:], want[1])):
+        assert a.dtype == dtype and ((a.double().cpu() - b).abs() <= tol(b)).all()
+    assert torch.equal(dq[..., :dn].cpu(), gq[..., :dn])
+    # one of the two outputs by itself, keys without queries, a gradient that is one number broadcast
+    ko, qo = L.append(None, None, kx, None, pos.cuda(), cos.cuda(), sin.cuda(), q=qx, interleaved=inter)
+    assert torch.equal(torch.autograd.grad(qo, qx, gq.cuda(), retain_graph=True)[0], dq)
+    assert torch.equal(torch.autograd.grad(ko, kx, gk.cuda())[0], dk)
+    ko, none = L.append(None, None, kx, None, pos.cuda(), cos.cuda(), sin.cuda(), interleaved=inter)
+    ones, = torch.autograd.grad(ko.sum(), kx)
+    ko, none = L.append(None, None, kx, None, pos.cuda(), cos.cuda(), sin.cuda(), interleaved=inter)
+    assert none is None and torch.equal(ones, torch.autograd.grad(ko, kx, torch.ones_like(ko))[0])
+
+
+def test_gradient_of_append_follows_differences():
+    """float32, linear in the inputs: the slope along a direction is the difference
+    itself, up to the roundings (2^-24 of each of 2e3 terms' sizes, over a step of 1)."""
+    banner("latent append differences")
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()
+    q, u, up, k = r(9, 2, 96), r(9, 2, 96), r(9, 2, 96), r(9, 32)
+    cos, sin = (t.cuda() for t in _tables(50, 32))
+    pos = torch.arange(9, dtype=torch.int32, device="cuda") * 5
+    f = lambda x: L.append(None, None, k, None, pos, cos, sin, q=x)[1]
+    x = q.clone().requires_grad_(True)
+    d, = torch.autograd.grad(f(x), x, up)
+    slope = ((f(q + u).double() - f(q).double()) * up.double()).sum()
+    assert abs(slope - (d.double() * u.double()).sum()) < 1e-3
+
+
+def test_append_refuses_what_has_no_gradient():
+    banner("latent append refusals in a graph")
+    z = lambda *s: torch.zeros(*s, device="cuda")
+    pos, slots = torch.zeros(5, dtype=torch.int32, device="cuda"), torch.arange(5, device="cuda")
+    for i in range(3):
+        cache, cos, sin = (z(*s).requires_grad_(i == j) for j, s in enumerate(((5, 1, 96), (9, 16), (9, 16))))
+        with pytest.raises(ValueError, match="no gradient"):
+            L.append(cache, z(5, 64), z(5, 32), slots, pos, cos, sin)
+    k = z(5, 32)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        L.append(None, None, forward_ad.make_dual(k, torch.ones_like(k)), None, pos, z(9, 16), z(9, 16))
+    ko, _ = L.append(None, None, k.requires_grad_(True), None, pos, z(9, 16), z(9, 16))
+    d, = torch.autograd.grad(ko.square().sum(), k, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
