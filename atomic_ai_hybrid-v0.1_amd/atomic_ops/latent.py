@@ -10,7 +10,7 @@ holds it.  Operands are bfloat16 or float32 (one dtype).
 Expanded form (prompts and training): ``kv`` [B, S, H, dn + dv] is the
 up-projection's output and ``k_pe`` [B, S, dr] the rotated key.
   ``attention``           differentiable in q, kv and k_pe
-  ``forward``/``backward``  the two directions by themselves
+  ``forward``/``backward``  the two directions by themselves, outside any graph
 Absorbed form (single tokens, or a few a sequence), over the latents of a paged
 cache [pages, page, dc + dr] whose rows are [latent | rotated key]:
   ``append``   writes tokens into the cache and rotates keys and queries
@@ -359,7 +359,29 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
     b stands at position kv_lens[b] - n + t and sees the tokens up to and with
     its own; one before the sequence's start (as in an empty sequence) has
     o = 0.  With ``cos`` / ``sin`` the last dr elements of q are rotated by that
-    position on the way, without them they are taken as rotated already."""
+    position on the way, without them they are taken as rotated already.
+
+    There is no gradient: in a graph (grad enabled and an input that requires it) a
+    backward that comes back to o is an error, and forward-mode tangents are refused."""
+    given = (q, w_kv, cache, cos, sin)
+    if _in_graph(*given) or _tangents(*given):
+        return LatentDecode.apply(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer)
+    return _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer)
+
+
+class LatentDecode(torch.autograd.Function):
+    """``decode`` in a graph, so that one which leads through it does not end there unnoticed."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _decode(*args)
+
+    @staticmethod
+    def backward(ctx, do):
+        raise RuntimeError("latent decode has no gradient (latent.attention has one)")
+
+
+def _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer):
     _operands("latent decode", ("q", q), ("w_kv", w_kv), ("cache", cache))
     if q.dim() != 4 or w_kv.dim() != 3 or w_kv.shape[0] != q.shape[2]:
         raise ValueError("latent decode: q must be [B, n, H, dn + dr] and w_kv [H, dn + dv, dc]")

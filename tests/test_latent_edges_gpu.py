@@ -205,3 +205,27 @@ def test_append_refuses_what_has_no_gradient():
     d, = torch.autograd.grad(ko.square().sum(), k, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         d.sum().backward()
+
+
+def test_decode_in_a_graph():
+    """The same bits, and an error instead of a gradient that is not there."""
+    banner("latent decode graph")
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+    table, ln = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4), _i32([60, 17])
+    for i in range(3):
+        x = [r(2, 1, 4, 96), r(4, 128, 128), r(8, 16, 160)]
+        with torch.no_grad():
+            want = L.decode(*x, table, ln, 0.1)
+        x[i].requires_grad_(True)
+        with torch.no_grad():
+            o = L.decode(*x, table, ln, 0.1)
+        assert torch.equal(o, want) and not o.requires_grad
+        o = L.decode(*x, table, ln, 0.1)
+        assert torch.equal(o, want)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            o.float().sum().backward()
+        x = [t.detach() for t in x]
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            L.decode(*x, table, ln, 0.1)
