@@ -269,9 +269,11 @@ def append(cache, c_kv, k_pe, slots, positions, cos, sin, *, q=None, interleaved
 
     Row ``slots[t]`` (page slots[t] // page, row slots[t] % page; int64 [N])
     becomes [c_kv[t] | rotate(k_pe[t])]; a negative slot, or one past the cache,
-    leaves it as it is; one that occurs twice holds either token's row.  ``positions`` int32 [N] choose the rows of the float32
-    tables ``cos`` / ``sin`` [positions, dr / 2]; the rotation turns the pairs
-    (i, i + dr / 2), or (2 i, 2 i + 1) with ``interleaved``.  Returns
+    leaves it as it is.  Slots have to differ: the row of one that occurs twice is a
+    mixture of the tokens' (a row is written by many threads, the tokens' in no order).
+    ``positions`` int32 [N] choose the rows of the float32 tables ``cos`` / ``sin``
+    [positions, dr / 2]; the rotation turns the pairs (i, i + dr / 2), or
+    (2 i, 2 i + 1) with ``interleaved``.  Returns
     ``(k, q)``: the rotated keys [N, dr] and, where ``q`` [N, H, dn + dr] is
     given, q with its last dr elements rotated (else None).  ``cache`` None
     (with c_kv and slots None) only rotates.

@@ -857,8 +857,9 @@ typedef struct atomic_latent_append_args {
 
 /* Appends N tokens: row slots[t] of the cache (page slots[t] / page, row
  * slots[t] % page) becomes [c_kv[t] | rotate(k_pe[t], positions[t])]; a slot
- * outside the cache (-1 by custom) leaves it as it is.  Slots that occur twice
- * in a call hold either token's row.  k_out [N, dr] receives the rotated keys
+ * outside the cache (-1 by custom) leaves it as it is.  Slots have to differ: the
+ * row of one that occurs twice in a call is a mixture of the tokens' (each element
+ * is one of theirs, undetermined which).  k_out [N, dr] receives the rotated keys
  * and, where q [N, H, dn + dr] is given, q_out (dense) q with its last dr
  * elements rotated.  cache or k_out may be NULL (not written).  Positions
  * outside the tables are taken to the nearer end. */

@@ -229,3 +229,27 @@ def test_decode_in_a_graph():
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
             x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
             L.decode(*x, table, ln, 0.1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_slots_that_occur_twice_mix_their_own_tokens_only(dtype):
+    """A slot given to several tokens: every element of its row is one of theirs, all
+    other rows are as they would be."""
+    banner(f"latent append repeated slots {dtype}")
+    g = torch.Generator().manual_seed(11)
+    N, dc, dr = 400, 512, 64
+    down, cache = (torch.randn(*s, generator=g).to(dtype) for s in ((N, dc + dr), (30, 16, dc + dr)))
+    slots = torch.randperm(480, generator=g)[:N]
+    slots[100:300] = slots[50]
+    slots[399] = slots[0]
+    cos, sin = (t.cuda() for t in _tables(50, dr))
+    dev, pos = cache.cuda(), torch.arange(N, dtype=torch.int32, device="cuda") % 50
+    k, _ = L.append(dev, down.cuda()[:, :dc], down.cuda()[:, dc:], slots.cuda(), pos, cos, sin)
+    rows, got = torch.cat((down[:, :dc], k.cpu()), 1), dev.cpu().view(480, -1)
+    want = cache.view(480, -1).clone()
+    want[slots] = rows
+    for s in slots.unique().tolist():
+        mine = (slots == s).nonzero().flatten()
+        assert (got[s] == rows[mine]).any(0).all()
+        want[s] = got[s]
+    assert torch.equal(got, want)
