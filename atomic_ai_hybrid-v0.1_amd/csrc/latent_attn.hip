@@ -11,7 +11,12 @@
 // too, unless the backward's first large kernel leaves them for its second (bf16, up
 // to 4 GB).  p and ds are rounded to the operand type for the second product, as its
 // MFMA takes them; everything else (scores, the running maximum and sum, lse, delta,
-// every accumulator) is fp32.
+// every accumulator) is fp32.  In bf16 that rounding is as large as the result's own:
+// of the norm, o is off by 0.0021 to 0.0023 and a gradient by 0.0023 to 0.0024 (0.0027
+// where a query sees five keys or fewer) where their own roundings are 0.0017.  p and ds
+// as two bf16 numbers each would leave only the results' roundings and make 8 MFMAs more
+// of a 32 x 32 tile's 20 in the forward, 20 more of 40 in latent_bwd_dkv, and the score
+// gradients in memory twice as large.
 //
 // A query that sees one key (always the first) has p = 1 whatever its score, so ds = 0.
 // Formed as do . v - do . o it would be what the two sums' roundings leave (the one in
@@ -90,13 +95,13 @@ __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_
 // fp32) that go straight to LDS, one tile ahead; one barrier a tile.  Two workgroups a
 // CU, so two waves a SIMD with 256 registers each: one's MFMAs run beside the other's
 // softmax.  (Eight waves on one tile, the two of a SIMD half a tile apart, took half the
-// tiles out of L2 and still lost, by the longer workgroups' tails: 264 us against 242 at
-// B8 T4096 H6, 650 against 605 at B2 T8192 H16, 318 against 316 at B1 T8192 H16.)
+// tiles out of L2 and still lost, by the longer workgroups' tails: 9 % at B8 T4096 H6,
+// 7 % at B2 T8192 H16, 1 % at B1 T8192 H16, both timed in turn when that was changed.)
 //
-// Bound by the matrix instructions, for which the card lowers its clock: without a pause
-// it takes 20.8 ns an instruction and SIMD (1.63 PF/s).  B2 T8192 H16, 128/64/128,
-// causal: 605 to 640 us, 1.07 to 1.14 PF/s, where the library's product of two
-// 8192 x 8192 matrices reaches 1.21.
+// Bound by the matrix instructions and the clock that the card holds under them: at
+// B2 T8192 H16, 128/64/128, causal the matrix pipes are busy for 59 % of the kernel's
+// cycles at 1.4 to 1.7 GHz, 655 to 690 us, 1.0 to 1.05 PF/s, where the library's product
+// of two 8192 x 8192 matrices reaches 1.21.
 //
 // With `parts` > 1 the keys of a row block are divided over that many workgroups
 // (few row blocks against many keys); each leaves its accumulators, reference and
@@ -530,7 +535,8 @@ __global__ __launch_bounds__(256, 1) void latent_bwd_dq(
 // rotated key's gradient leaves as this head's part, fp32 [B, H, S, dr].
 //
 // Four of the backward's five products (scores, dp, dv, dk) run here, bound by the
-// matrix instructions: B2 T8192 H16 causal 1500 us, 0.92 PF/s.
+// matrix instructions and what stands between them (one wave a SIMD): B2 T8192 H16
+// causal 1610 to 1670 us, 0.82 to 0.85 PF/s, the matrix pipes busy for 45 % of the cycles.
 //
 // With DS the score gradients go to memory too, for latent_bwd_dq_ds: [B, H, tiles of
 // 64 rows, S, 64] bf16, a token's rows in the order of this kernel's registers
@@ -746,8 +752,8 @@ __device__ __forceinline__ int ds_byte(int c) { return 8 * ((c >> 3) & 1); }
 // dq from the score gradients that latent_bwd_dkv left: 256 query rows of a head a
 // workgroup, 64 a wave, against tiles of 32 tokens, three of them on their way.
 // dq^T += k^T ds^T; a fragment of k serves two MFMAs.  Bound by reading the score
-// gradients (2 bytes a pair): B2 T8192 H16 causal 530 us for 2.1 GB, 4.1 TB/s where a
-// copy reaches 5.0.
+// gradients (2 bytes a pair): B2 T8192 H16 causal 540 to 550 us for 2.1 GB, 3.9 TB/s where
+// a copy reaches 5.0.
 template <int DN, int DR>
 __global__ __launch_bounds__(256, 1) void latent_bwd_dq_ds(LatDims d, const bf16* __restrict__ kv,
                                                            const bf16* __restrict__ kpe,

@@ -239,12 +239,16 @@ __device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 
 // computes with the 16 rows w % MT and the tokens of MT waves.  The waves of a
 // row group join at the end.
 //
-// Bound by the cache's bytes: 16 heads need 46 operations a byte.  So the tiles go
-// straight to LDS, two of them (147 KB with 512 bf16 latents), and a wave that has
-// its rows to itself (MT = 1) never meets a barrier: it loads what it reads.  The
-// split's page numbers lie in LDS, so no wait for an index drains the tiles in flight.
-// 64 sequences of up to 8192 tokens, 16 heads: 92 to 95 us for 440 MB, 4.7 TB/s; 4 of
-// 32768: 33 us, 4.6 TB/s; both where a copy reaches 5.0.
+// Bound by the cache's bytes: 16 heads need 44 operations a byte (30, and 14 for the
+// probabilities' second number).  So the tiles go straight to LDS, two of them (with 512
+// bf16 latents 74 KB at two waves, so two workgroups a CU, and 147 KB at four), and a
+// wave that has its rows to itself (MT = 1) never meets a barrier: it loads what it
+// reads.  The split's page numbers lie in LDS, so no wait for an index drains the tiles
+// in flight.  64 sequences of up to 8192 tokens, 16 heads: 95 to 97 us for 440 MB,
+// 4.6 TB/s; 4 of 32768: 33 us, 4.6 TB/s; both where a copy reaches 5.0.
+//
+// (float32 with 512 latents: the query's fragments take 144 registers and the
+// accumulators 128; 3 registers lie in scratch memory with MT = 1, 54 with MT = 2.)
 template <typename T, int DC, int MT, int NW>
 __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
                                                         const T* __restrict__ cache, const int32_t* __restrict__ table,
@@ -645,7 +649,9 @@ static DecDims dec_dims(const atomic_latent_decode_args* a) {
   const int mt = dec_row_tiles(a), rt = 16 * mt, tile = mt == 4 ? 64 : 32;
   d.groups = (d.n * d.H + rt - 1) / rt;
   // As many workgroups as the card holds at once if every sequence were as long as
-  // its table: two a CU with two waves each in bf16, else one (the tiles' LDS).
+  // its table (the host does not know the lengths, so a table wider than the sequences
+  // costs parallelism: 64 of 1024 tokens, 16 heads, whole calls: 42 us with a table as
+  // wide, 89 with one of 8192 tokens, 293 with one of 131072): two a CU with two waves each in bf16, else one (the tiles' LDS).
   // Split and join together, us: 64 sequences of up to 8192 tokens, 16 heads: 116 in
   // splits of 512, 103 of 1024; 4 of 32768: 42 of 256 or 512, 56 of 128; 8 of 4096
   // with 64 rows: 33 of 128, 36 of 256, 46 of 64; one of 777: 18 of 32, 22 of 128.

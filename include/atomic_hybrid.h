@@ -872,7 +872,12 @@ int atomic_latent_append(const atomic_latent_append_args* a, const void* c_kv, c
  * tokens up to and with that one; a position below zero sees nothing (o = 0).
  * Token j of sequence b lies in page page_table[b][j / page], row j % page;
  * entries past the last needed one are not used, page numbers outside the
- * cache and lengths outside [0, table_pages * page] are taken to the nearer end. */
+ * cache and lengths outside [0, table_pages * page] are taken to the nearer end.
+ * An infinity or NaN in a token's row may reach the query tokens of the same call
+ * that stand before it (a weight of zero times it).
+ *
+ * How the tokens are divided over the card, and the workspace, follow the table's
+ * width: a table much wider than the longest sequence gives the same outputs later. */
 typedef struct atomic_latent_decode_args {
   int32_t batch;       /* B                                                 */
   int32_t tokens;      /* n                                                 */
