@@ -120,6 +120,20 @@ class LatentDecodeArgs(ctypes.Structure):
                 ("scale", ctypes.c_float), ("q_stride", ctypes.c_int64 * 3), ("profile", ctypes.c_void_p)]
 
 
+class LatentSharedArgs(ctypes.Structure):
+    _fields_ = [("dec", LatentDecodeArgs), ("prefixes", ctypes.c_int32), ("prefix_pages", ctypes.c_int32),
+                ("scored", ctypes.c_int32), ("weights_stride", ctypes.c_int64)]
+
+
+class LatentEvictArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("dtype", ctypes.c_int32), ("row", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("pages", ctypes.c_int32), ("table_pages", ctypes.c_int32),
+                ("width", ctypes.c_int32), ("keep", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("recent", ctypes.c_int32), ("weights_stride", ctypes.c_int64), ("order_stride", ctypes.c_int64),
+                ("weights_out_stride", ctypes.c_int64), ("order_out_stride", ctypes.c_int64),
+                ("profile", ctypes.c_void_p)]
+
+
 PROFILE_MAX = 16
 
 
@@ -276,6 +290,11 @@ _SIGS = {
     "atomic_latent_append": (ctypes.c_int, [ctypes.POINTER(LatentAppendArgs)] + [_P] * 10 + [_P]),
     "atomic_latent_decode_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentDecodeArgs)]),
     "atomic_latent_decode": (ctypes.c_int, [ctypes.POINTER(LatentDecodeArgs)] + [_P] * 8 + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_decode_shared_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentSharedArgs)]),
+    "atomic_latent_decode_shared": (ctypes.c_int, [ctypes.POINTER(LatentSharedArgs)] + [_P] * 11
+                                    + [_P, ctypes.c_size_t, _P]),
+    "atomic_latent_evict_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LatentEvictArgs)]),
+    "atomic_latent_evict": (ctypes.c_int, [ctypes.POINTER(LatentEvictArgs)] + [_P] * 9 + [_P, ctypes.c_size_t, _P]),
 }
 
 _lib = None

@@ -13,8 +13,10 @@ up-projection's output and ``k_pe`` [B, S, dr] the rotated key.
   ``forward``/``backward``  the two directions by themselves, outside any graph
 Absorbed form (single tokens, or a few a sequence), over the latents of a paged
 cache [pages, page, dc + dr] whose rows are [latent | rotated key]:
-  ``append``   writes tokens into the cache and rotates keys and queries
-  ``decode``   reads it
+  ``append``         writes tokens into the cache and rotates keys and queries
+  ``decode``         reads it; on request gathers each token's attention weight
+  ``decode_shared``  the same for sequences that share a prefix, read once for all
+  ``evict``          leaves the tokens with the largest weights in the cache
 The two forms of the same weights and tokens give the same outputs up to rounding.
 No queries, keys or tokens (a dimension of zero) give empty or zero outputs.
 """
@@ -352,8 +354,8 @@ def _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer
     return k_out, q_out
 
 
-def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, interleaved=False, workspace=None,
-           timer=None):
+def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, interleaved=False, weights=None,
+           workspace=None, timer=None):
     """o [B, n, H, dv]: n query tokens a sequence over its cached latents.
 
     ``q`` [B, n, H, dn + dr]; ``page_table`` int32 [B, pages of the longest];
@@ -361,8 +363,17 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
     b stands at position kv_lens[b] - n + t and sees the tokens up to and with
     its own; one before the sequence's start (as in an empty sequence) has
     o = 0.  With ``cos`` / ``sin`` the last dr elements of q are rotated by that
-    position on the way, without them they are taken as rotated already.  An infinity
-    or NaN in a cached row may reach the query tokens of the call that stand before it.
+    position on the way, without them they are taken as rotated already (by
+    ``append``, as after an eviction, when the rows say nothing of the positions).
+    An infinity or NaN in a cached row may reach the query tokens of the call that
+    stand before it.
+
+    ``weights`` float32 [B, tokens of the table or more] gathers what ``evict`` goes by:
+    to weights[b, j] is added, in place, the sum over heads and query tokens of the
+    softmax weight of token j; those of the n newest tokens are set to it, they begin
+    here.  What lies past the length stays as it is.  The query then enters the scores
+    as two bfloat16 numbers, so that the weights are float32's (and o a little nearer
+    to the exact one than without them).
 
     The tokens are divided over the card by the table's width, not by the lengths (which
     the host does not know): hand over a table no wider than the longest sequence needs
@@ -371,10 +382,26 @@ def decode(q, w_kv, cache, page_table, kv_lens, scale, *, cos=None, sin=None, in
 
     There is no gradient: in a graph (grad enabled and an input that requires it) a
     backward that comes back to o is an error, and forward-mode tangents are refused."""
-    given = (q, w_kv, cache, cos, sin)
-    if _in_graph(*given) or _tangents(*given):
-        return LatentDecode.apply(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer)
-    return _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer)
+    given = (q, w_kv, cache, cos, sin, weights)
+    args = (q, w_kv, cache, None, None, page_table, kv_lens, scale, cos, sin, interleaved, weights, workspace, timer)
+    return (LatentDecode.apply if _in_graph(*given) or _tangents(*given) else _decode)(*args)
+
+
+def decode_shared(q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, *, cos=None, sin=None,
+                  interleaved=False, weights=None, workspace=None, timer=None):
+    """``decode`` for sequences that share prefixes, each read once for all that follow it.
+
+    ``prefix_table`` int32 [G, pages of the longest] and ``prefix_lens`` int32 [G]
+    are the prefixes' tokens in the same cache; the batch is G equal runs, sequence b
+    follows prefix b // (B / G).  ``page_table`` and ``kv_lens`` are each sequence's own
+    tokens, those after the prefix (a length of zero: the prefix only).  Query t
+    stands at position prefix_lens[g] + kv_lens[b] - n + t and sees the tokens up to and
+    with its own: what ``decode`` gives for the two tables as one, up to rounding.
+    ``weights`` are those of the own tokens; a prefix's are not gathered."""
+    given = (q, w_kv, cache, cos, sin, weights)
+    args = (q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, cos, sin, interleaved, weights,
+            workspace, timer)
+    return (LatentDecode.apply if _in_graph(*given) or _tangents(*given) else _decode)(*args)
 
 
 class LatentDecode(torch.autograd.Function):
@@ -389,7 +416,19 @@ class LatentDecode(torch.autograd.Function):
         raise RuntimeError("latent decode has no gradient (latent.attention has one)")
 
 
-def _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, workspace, timer):
+def _per_token(what, name, t, B, least, dtype, device):
+    """Checks a [B, tokens] state whose rows the library reads or writes in place; its row stride."""
+    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or t.shape[1] < least or t.get_device() != device or \
+            t.requires_grad:
+        raise ValueError(f"{what}: {name} must be {str(dtype)[6:]} [{B}, {least} or more] on the inputs' device, "
+                         "without a gradient")
+    if t.shape[1] > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what}: {name} must have dense rows that do not overlap")
+    return t.stride(0) if B > 1 else t.shape[1]
+
+
+def _decode(q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, cos, sin, interleaved, weights,
+            workspace, timer):
     _operands("latent decode", ("q", q), ("w_kv", w_kv), ("cache", cache))
     if q.dim() != 4 or w_kv.dim() != 3 or w_kv.shape[0] != q.shape[2]:
         raise ValueError("latent decode: q must be [B, n, H, dn + dr] and w_kv [H, dn + dv, dc]")
@@ -404,11 +443,24 @@ def _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, w
         raise ValueError("latent decode: page_table must be int32 [B, pages]")
     page_table = _index("latent decode", "page_table", page_table, (B, page_table.shape[1]), torch.int32, dev)
     kv_lens = _index("latent decode", "kv_lens", kv_lens, (B,), torch.int32, dev)
+    G = front = 0
+    if prefix_table is not None:
+        if prefix_table.dim() != 2 or prefix_lens.dim() != 1:
+            raise ValueError("latent decode: prefix_table must be int32 [G, pages] and prefix_lens int32 [G]")
+        G, front = prefix_table.shape
+        if G == 0 and B or G and B % G:
+            raise ValueError(f"latent decode: {G} prefixes do not divide a batch of {B}")
+        prefix_table = _index("latent decode", "prefix_table", prefix_table, (G, front), torch.int32, dev)
+        prefix_lens = _index("latent decode", "prefix_lens", prefix_lens, (G,), torch.int32, dev)
     if (cos is None) != (sin is None):
         raise ValueError("latent decode: cos and sin come together")
     if cos is not None:
         cos, sin = _tables("latent decode", cos, sin, dr, dev)
-    if not (q.numel() and page_table.numel()):      # no queries, or none with a token to see
+    stride = 0
+    if weights is not None:
+        stride = _per_token("latent decode", "weights", weights, B, page_table.shape[1] * cache.shape[1], torch.float32,
+                            dev)
+    if not (q.numel() and (page_table.numel() or front)):      # no queries, or none with a token to see
         return q.new_zeros(B, n, H, w_kv.shape[1] - (d - dr))
     q, qs = _strided(q, 3)
     w_kv, _ = _strided(w_kv.contiguous(), 2)
@@ -418,13 +470,93 @@ def _decode(q, w_kv, cache, page_table, kv_lens, scale, cos, sin, interleaved, w
                                  1 if interleaved else 0, scale, qs)
     if timer is not None:
         args.profile = timer.arm()
-    nbytes = lib.atomic_latent_decode_workspace_size(ctypes.byref(args))
+    plain = not G and weights is None
+    if not plain:
+        args = _lib.LatentSharedArgs(args, G, front, weights is not None, stride)
+    size = lib.atomic_latent_decode_workspace_size if plain else lib.atomic_latent_decode_shared_workspace_size
+    nbytes = size(ctypes.byref(args))
     if nbytes == 0:
         raise _lib.AtomicError("atomic_latent_decode_workspace_size: unsupported shape")
     workspace = _workspace(workspace, nbytes, q.device)
-    o = torch.empty(B, n, H, args.dv, dtype=q.dtype, device=q.device)
-    rc = lib.atomic_latent_decode(ctypes.byref(args), _ptr(q), _ptr(w_kv), _ptr(cache), _ptr(page_table),
-                                  _ptr(kv_lens), _ptr(cos), _ptr(sin), _ptr(o), _ptr(workspace), workspace.numel(),
-                                  _stream(q.device))
-    _lib.check(rc, "atomic_latent_decode")
+    o = torch.empty(B, n, H, w_kv.shape[1] - (d - dr), dtype=q.dtype, device=q.device)
+    if plain:
+        rc = lib.atomic_latent_decode(ctypes.byref(args), _ptr(q), _ptr(w_kv), _ptr(cache), _ptr(page_table),
+                                      _ptr(kv_lens), _ptr(cos), _ptr(sin), _ptr(o), _ptr(workspace),
+                                      workspace.numel(), _stream(q.device))
+        _lib.check(rc, "atomic_latent_decode")
+    else:
+        rc = lib.atomic_latent_decode_shared(ctypes.byref(args), _ptr(q), _ptr(w_kv), _ptr(cache), _ptr(prefix_table),
+                                             _ptr(prefix_lens), _ptr(page_table), _ptr(kv_lens), _ptr(cos), _ptr(sin),
+                                             _ptr(weights), _ptr(o), _ptr(workspace), workspace.numel(),
+                                             _stream(q.device))
+        _lib.check(rc, "atomic_latent_decode_shared")
     return o
+
+
+def evict(cache, page_table, kv_lens, weights, order, keep, *, sinks=0, recent=1, in_place=False, workspace=None,
+          timer=None):
+    """``(kv_lens, weights, order, source)`` after an eviction: of each sequence with
+    more than ``keep`` tokens, keep stay in the cache.
+
+    ``weights`` float32 [B, W] are the tokens' gathered attention weights (``decode``)
+    and ``order`` int32 [B, W] their places among all tokens of their sequence, W being
+    the table's tokens or more.  order holds -1 in rows that no eviction has seen: such
+    tokens are taken as the newest, in the order of their rows, so a program begins
+    with -1 everywhere and hands on what this call returns.  The first ``sinks`` tokens
+    (order < sinks) and the ``recent`` newest stay whatever their weights, of the others
+    those with the largest (equal ones: the lowest rows first; a NaN counts as the
+    least).  Kept tokens in rows past keep move into the rows below that became free, in
+    the order of the rows on both sides; nothing else in ``cache`` is written.
+
+    The new kv_lens are at most keep; the new weights and order hold 0 and -1 past
+    them.  ``source`` int32 [B, keep] is the row that each row's token was in (-1 past
+    the length).  With ``in_place`` kv_lens, weights and order are written over and
+    returned.  Without it the inputs stay, and the same call does the same once more.
+    A sequence's pages must be its own: of a prefix that others share, only what
+    follows it can be evicted (``decode_shared``)."""
+    what = "latent evict"
+    if not cache.is_cuda:
+        raise ValueError(f"{what}: inputs must be HIP device tensors")
+    if cache.dtype not in _DT:
+        raise TypeError(f"{what}: cache must be bfloat16 or float32")
+    if cache.dim() != 3 or cache.requires_grad:
+        raise ValueError(f"{what}: cache must be a dense [pages, page, dc + dr], without a gradient")
+    _cache(what, cache, cache.shape[2])
+    dev = cache.get_device()
+    if page_table.dim() != 2:
+        raise ValueError(f"{what}: page_table must be int32 [B, pages]")
+    B, per = page_table.shape
+    page_table = _index(what, "page_table", page_table, (B, per), torch.int32, dev)
+    lens = _index(what, "kv_lens", kv_lens, (B,), torch.int32, dev)
+    if in_place and lens is not kv_lens:
+        raise ValueError(f"{what}: kv_lens must be dense to be written in place")
+    if not 0 <= sinks <= keep or not 0 <= recent <= keep - sinks or keep < 1:
+        raise ValueError(f"{what}: sinks and recent must be 0 or more and together at most keep")
+    pages, page, row = cache.shape
+    ws = _per_token(what, "weights", weights, B, per * page, torch.float32, dev)
+    os = _per_token(what, "order", order, B, per * page, torch.int32, dev)
+    if order.shape != weights.shape:
+        raise ValueError(f"{what}: weights and order must have one shape")
+    W = weights.shape[1]
+    source = torch.empty(B, keep, dtype=torch.int32, device=cache.device)
+    if in_place:
+        out, wos, oos = (kv_lens, weights, order), ws, os
+    else:
+        out, wos, oos = (torch.empty_like(lens), weights.new_empty(B, W), order.new_empty(B, W)), W, W
+    if not (B and per and pages and page):      # no token anywhere
+        out[0].zero_(), out[1].zero_(), out[2].fill_(-1), source.fill_(-1)
+        return (*out, source)
+    lib = _lib.load()
+    args = _lib.LatentEvictArgs(B, _DT[cache.dtype], row, page, pages, per, W, keep, sinks, recent, ws, os, wos, oos)
+    if timer is not None:
+        args.profile = timer.arm()
+    nbytes = lib.atomic_latent_evict_workspace_size(ctypes.byref(args))
+    if nbytes == 0:
+        raise _lib.AtomicError("atomic_latent_evict: ATOMIC_ERR_SHAPE: unsupported or inconsistent dimensions",
+                               _lib.ATOMIC_ERR_SHAPE)
+    workspace = _workspace(workspace, nbytes, cache.device)
+    rc = lib.atomic_latent_evict(ctypes.byref(args), _ptr(cache), _ptr(page_table), _ptr(lens), _ptr(weights),
+                                 _ptr(order), *(_ptr(t) for t in out), _ptr(source), _ptr(workspace),
+                                 workspace.numel(), _stream(cache.device))
+    _lib.check(rc, "atomic_latent_evict")
+    return (*out, source)

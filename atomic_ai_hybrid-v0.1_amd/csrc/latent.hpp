@@ -63,6 +63,13 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// What rounding to T leaves out.
+template <typename T> __device__ __forceinline__ f32x4 rounding(f32x4 x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] -= (float)(T)x[j];
+  return x;
+}
+
 // A tile of rows of W elements in LDS as 16-byte pieces, piece c of row r at
 // place c ^ swz(r).  With FR rows a fragment (32 or 16), the row reads (16 bytes a
 // lane) and the transposed reads (8 bytes a lane) both run without bank conflicts

@@ -80,13 +80,6 @@ __device__ __forceinline__ void row_frags(typename M32<T>::frag (&f)[(W0 + W1) /
 // SIMD has 256 registers in each).
 template <typename F> __device__ __forceinline__ void in_accum(F& x) { asm volatile("" : "+a"(x)); }
 
-// What rounding to T leaves out.
-template <typename T> __device__ __forceinline__ f32x4 rounding(f32x4 x) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] -= (float)(T)x[j];
-  return x;
-}
-
 // Token of register r of a score tile (from its first token).
 __device__ __forceinline__ int reg_row(int r) { return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3); }
 

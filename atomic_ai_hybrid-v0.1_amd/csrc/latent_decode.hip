@@ -7,6 +7,11 @@
 //   o[h] = w_kv[h, dn:] o_lat[h]                             (up)
 //
 // All heads of a sequence read the same cache row, once, as key and as value.
+// Sequences that share a prefix read it together: its rows are then those of all of them
+// (latent_split over the prefix first, then over each sequence's own tokens; the parts of
+// both are joined alike).  Where the tokens' weights are gathered, latent_weigh forms them
+// from the scores, once the rows' sums are known.
+//
 // q_lat is rounded to the operand type, as the MFMA takes it; the probabilities
 // and o_lat, fp32, enter their products as the sum of two bf16 numbers (the cache's
 // bytes leave the matrix instructions idle; with probabilities of eight bits o was off
@@ -24,10 +29,11 @@ struct AppDims {
 };
 
 // Four pairs of one row: elements 8 u .. 8 u + 7 (interleaved) or 4 u .. + 3 of both halves.
+// y1 receives the same, or with LO what y0's rounding left out.
 template <typename T> struct Vec4;
 template <> struct Vec4<bf16> { typedef bf16x4 t; };
 template <> struct Vec4<float> { typedef f32x4 t; };
-template <typename T>
+template <typename T, bool LO = false>
 __device__ __forceinline__ void rotate4(const T* x, const float* cr, const float* sr, int u, int dr, bool inter,
                                         T* y0, T* y1) {
   typedef typename Vec4<T>::t v4;
@@ -57,8 +63,8 @@ __device__ __forceinline__ void rotate4(const T* x, const float* cr, const float
     store4(y0 + b, o1);
   }
   if (y1) {
-    store4(y1 + a, o0);
-    store4(y1 + b, o1);
+    store4(y1 + a, LO ? rounding<T>(o0) : o0);
+    store4(y1 + b, LO ? rounding<T>(o1) : o1);
   }
 }
 
@@ -107,16 +113,36 @@ struct DecDims {
   int chunk, splits, groups;  // tokens a split (whole tiles), splits of the longest sequence, row groups
   float scale;
   int64_t qs[3];
+  int share;         // latent_split: sequences whose rows read the same tokens (those of a prefix, or one)
+  int slot0, slots;  // its first slot among a row's parts, and all of them
+  // prefixes: sequences of each (0: there are none), tokens a split, slots, tokens their table holds, lengths
+  int pre_share, pre_chunk, pre_splits, pre_most;
+  const int32_t* pre_lens;
 };
 constexpr int kDecChunk = 1024, kDecPages = kDecChunk + 1;  // tokens of a split, pages that they can lie in
 __device__ __forceinline__ int dec_len(const DecDims& d, const int32_t* kv_lens, int b) {
   return (int)min((int64_t)max(kv_lens[b], 0), (int64_t)d.table * d.page);
 }
+// Length of the prefix that sequence b's own tokens follow.
+__device__ __forceinline__ int pre_len(const DecDims& d, int b) {
+  return d.pre_share ? min(max(d.pre_lens[b / d.pre_share], 0), d.pre_most) : 0;
+}
+// The parts of sequence b's rows: those of the prefix's splits, then those of its own.
+struct Parts {
+  int front, all, skip;  // splits of the prefix, of both, slots to leave out between them
+  __device__ __forceinline__ Parts(const DecDims& d, const int32_t* kv_lens, int b) {
+    front = d.pre_share ? (pre_len(d, b) + d.pre_chunk - 1) / d.pre_chunk : 0;
+    all = front + (d.splits ? (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk : 0);
+    skip = d.pre_splits - front;
+  }
+  __device__ __forceinline__ int slot(int s) const { return s < front ? s : s + skip; }
+};
 
 // q_lat [B n, H, dc | rotated q_pe]: a head, 16 query tokens and 64 latent
 // columns a workgroup, 16 columns a wave; one more column block rotates.  Latency: 4 to
-// 6 us with 4 to 64 sequences of 16 heads (4 MB of weights).
-template <typename T>
+// 6 us with 4 to 64 sequences of 16 heads (4 MB of weights).  With LO each row is
+// followed by what its rounding left out (bf16; zeros in fp32 have no place).
+template <typename T, bool LO>
 __global__ __launch_bounds__(256) void latent_absorb(DecDims d, const T* __restrict__ q, const T* __restrict__ w_kv,
                                                      const int32_t* __restrict__ kv_lens,
                                                      const float* __restrict__ cos, const float* __restrict__ sin,
@@ -125,19 +151,26 @@ __global__ __launch_bounds__(256) void latent_absorb(DecDims d, const T* __restr
   __shared__ __attribute__((aligned(16))) T sw[128 * LW];
   __shared__ __attribute__((aligned(16))) T sq[16 * LQ];
   const int h = blockIdx.x, c0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, wide = d.dc + d.dr;
+  constexpr int NR = LO ? 2 : 1;
   if (c0 >= d.dc) {
     for (int e = threadIdx.x; e < 16 * (d.dr / 8); e += 256) {
       const int r = r0 + e / (d.dr / 8), u = e % (d.dr / 8);
       if (r >= R) break;
       const T* x = q + r / d.n * d.qs[0] + r % d.n * d.qs[1] + h * d.qs[2] + d.dn;
-      T* y = qa + ((int64_t)r * d.H + h) * wide + d.dc;
+      T* y = qa + ((int64_t)r * d.H + h) * NR * wide + d.dc;
       if (cos) {
-        const int64_t p = min(max(dec_len(d, kv_lens, r / d.n) - d.n + r % d.n, 0), d.rope - 1);
-        rotate4(x, cos + p * (d.dr / 2), sin + p * (d.dr / 2), u, d.dr, d.inter, y, (T*)nullptr);
+        const int64_t at = (int64_t)pre_len(d, r / d.n) + dec_len(d, kv_lens, r / d.n) - d.n + r % d.n;
+        const int64_t p = min(max(at, (int64_t)0), (int64_t)d.rope - 1);
+        rotate4<T, LO>(x, cos + p * (d.dr / 2), sin + p * (d.dr / 2), u, d.dr, d.inter, y, LO ? y + wide : (T*)nullptr);
       } else {
         float t[8];
         load8(x + 8 * u, t);
         store8(y + 8 * u, t);
+        if constexpr (LO) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t[j] = 0.f;
+          store8(y + wide + 8 * u, t);
+        }
       }
     }
     return;
@@ -159,7 +192,11 @@ __global__ __launch_bounds__(256) void latent_absorb(DecDims d, const T* __restr
   __syncthreads();
   const f32x4 z = tile_mma<T, true, false>(zero4(), sw, LW, sq, LQ, 16 * wave_id(), 0, KP);
   const int r = r0 + tile_col(), c = c0 + 16 * wave_id() + tile_row(0);
-  if (r < R && c < d.dc) store4(qa + ((int64_t)r * d.H + h) * wide + c, z);
+  if (r < R && c < d.dc) {
+    T* y = qa + ((int64_t)r * d.H + h) * NR * wide + c;
+    store4(y, z);
+    if constexpr (LO) store4(y + wide, rounding<T>(z));
+  }
 }
 
 // 16 x 16 fragments of eight k values a lane (row operand) and of the four
@@ -249,13 +286,21 @@ __device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 
 //
 // (float32 with 512 latents: the query's fragments take 144 registers and the
 // accumulators 128; 3 registers lie in scratch memory with MT = 1, 54 with MT = 2.)
-template <typename T, int DC, int MT, int NW>
+//
+// The rows of a launch are those of `share` sequences after one another: one, or all that
+// follow the same prefix (`own`, then, are the lengths of what follows it).  With SCORED the
+// query enters as two bf16 numbers, and where `score` is given the scores in powers of
+// two are left there for latent_weigh, a wave's 16 x 16 of them as they lie in its registers.
+template <typename T, int DC, int MT, int NW, bool SCORED>
 __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
                                                         const T* __restrict__ cache, const int32_t* __restrict__ table,
-                                                        const int32_t* __restrict__ kv_lens, float* __restrict__ part,
-                                                        float* __restrict__ stat, float* __restrict__ olat) {
+                                                        const int32_t* __restrict__ kv_lens,
+                                                        const int32_t* __restrict__ own, int own_most,
+                                                        float* __restrict__ part, float* __restrict__ stat,
+                                                        float* __restrict__ olat, float* __restrict__ score) {
   constexpr int DR = 64, W = DC + DR, KS = W / 32, NT = DC / 16, TK = 16 * NW, TW = NW / MT, V = 16 / (int)sizeof(T);
   constexpr int NP = sizeof(T) == 2 ? 2 : 1;    // operands of a probability
+  constexpr int NQ = SCORED && sizeof(T) == 2 ? 2 : 1;  // and of a query
   constexpr int PC = DC / V, PR = DR / V;       // pieces of a row's latent and rotated key
   constexpr int IC = PC * 16 / 64, IR = PR * 16 / 64;  // loads of one wave for its 16 tokens
   typedef DTile<T, DC> LC;
@@ -267,23 +312,28 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
   __shared__ int32_t spt[kDecPages];
   __shared__ float sm[NW][16], ss[NW][16];
   const int sp = blockIdx.x, b = blockIdx.z, wv = wave_id(), lane = lane_id(), rw = wv % MT, tw = wv / MT;
-  const int len = dec_len(d, kv_lens, b), rows = d.n * d.H, wide = d.dc + d.dr;
+  const int len = dec_len(d, kv_lens, b), each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
-  if (first >= len && (sp > 0 || d.splits > 1)) return;  // (one split only: it writes the empty sequence's zeros)
+  if (first >= len && (sp > 0 || d.slots > 1)) return;  // (one split only: it writes the empty sequence's zeros)
   const int page0 = first / d.page;
   for (int i = threadIdx.x; first < end && i <= (end - 1) / d.page - page0; i += 64 * NW)
     spt[i] = min(max(table[(int64_t)b * d.table + page0 + i], 0), d.pages - 1);
   const int row = 16 * (blockIdx.y * MT + rw) + (lane & 15);
-  const int seen = len - d.n + min(row, rows - 1) / d.H + 1;  // tokens that this lane's row sees
-  const int least = len - d.n + 1;                            // and that every row sees
-  const T* qr = qa + ((int64_t)b * rows + min(row, rows - 1)) * wide;
-  frag qf[KS];
+  const int seq = b * d.share + min(row, rows - 1) / each;  // this lane's row: its sequence, and its place there
+  const int place = min(row, rows - 1) % each;
+  int seen = len - d.n + place / d.H + 1;  // tokens that it sees
+  if (own) seen += min(max(own[seq], 0), own_most);
+  const int least = len - d.n + 1;  // and that every row sees
+  const T* qr = qa + ((int64_t)seq * each + place) * NQ * wide;
+  frag qf[NQ][KS];
 #pragma unroll
-  for (int t = 0; t < KS; ++t) {
-    const int k = 32 * t + 8 * (lane >> 4);
-    if (32 * t < DC) qf[t] = ld_frag(k < d.dc ? qr + k : (const T*)lat_zeros);
-    else qf[t] = ld_frag(k - DC < d.dr ? qr + d.dc + k - DC : (const T*)lat_zeros);
-  }
+  for (int u = 0; u < NQ; ++u)
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      const int k = 32 * t + 8 * (lane >> 4);
+      if (32 * t < DC) qf[u][t] = ld_frag(k < d.dc ? qr + u * wide + k : (const T*)lat_zeros);
+      else qf[u][t] = ld_frag(k - DC < d.dr ? qr + u * wide + d.dc + k - DC : (const T*)lat_zeros);
+    }
   __syncthreads();  // the page numbers are there
   const uint32_t lds0 = lds_addr(sk);
   constexpr int RL = PC >= 64 ? PC / 64 : 1;  // loads a row
@@ -347,7 +397,10 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
       f32x4 x[2] = {zero4(), zero4()};  // two chains: each waits for its own result only
       in_groups<KS, sizeof(T) == 2 ? 6 : 2, frag>(
           [&](int t) { return 32 * t < DC ? LC::row16(rc, 32 * t) : LR::row16(rr, 32 * t - DC); },
-          [&](int t, frag a) { x[t & 1] = M16<T>::mma(a, qf[t], x[t & 1]); });
+          [&](int t, frag a) {
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) x[(t ^ u) & 1] = M16<T>::mma(a, qf[u][t], x[(t ^ u) & 1]);
+          });
       s[i] = x[0] + x[1];
     }
 #pragma unroll
@@ -359,6 +412,17 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (16 * i + tile_row(r) >= lim) s[i][r] = -INFINITY;
+    }
+    if constexpr (SCORED) {
+      if (score) {  // (tiles past the end have no place)
+        const int tiles = (d.table * d.page + 15) / 16;
+        const int64_t at = (int64_t)b * (gridDim.y * MT) + blockIdx.y * MT + rw;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int tile = k0 / 16 + MT * tw + i;
+          if (16 * tile < end) store4(score + ((at * tiles + tile) * 64 + lane) * 4, s[i]);
+        }
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -456,19 +520,19 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
     }
   }
   if (tw != 0 || row >= rows) return;
-  float* dst = part + (((int64_t)b * d.splits + sp) * rows + row) * d.dc;
+  const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
+  float* dst = part + at * d.dc;
   float by = 1.f;
-  if (d.splits == 1) {  // nothing to join
+  if (d.slots == 1) {  // nothing to join
     by = sum == 0.f ? 0.f : 1.f / sum;
-    dst = olat + ((int64_t)b * rows + row) * d.dc;
+    dst = olat + ((int64_t)seq * each + place) * d.dc;
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int c = 16 * n + tile_row(0);
     if (c < d.dc) store4(dst + c, acc[n] * by);
   }
-  if (lane < 16 && d.splits > 1) {
-    const int64_t at = ((int64_t)b * d.splits + sp) * rows + row;
+  if (lane < 16 && (SCORED || d.slots > 1)) {
     stat[2 * at] = m;
     stat[2 * at + 1] = sum;
   }
@@ -492,13 +556,13 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
   f32x4 x = zero4();
   if (ok) {
     const int b = (int)(row / rows);
-    const int ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
-    const int64_t at = (int64_t)b * d.splits * rows + row % rows;
-    for (int s = g; s < ns; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)s * rows)]);
+    const Parts ps(d, kv_lens, b);
+    const int64_t at = (int64_t)b * d.slots * rows + row % rows;
+    for (int s = g; s < ps.all; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)ps.slot(s) * rows)]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
-    for (int s = g; s < ns; s += ways) {
-      const int64_t a = at + (int64_t)s * rows;
+    for (int s = g; s < ps.all; s += ways) {
+      const int64_t a = at + (int64_t)ps.slot(s) * rows;
       const float w = fast_exp2(stat[2 * a] - ref);
       sum += w * stat[2 * a + 1];
       x += w * *reinterpret_cast<const f32x4*>(part + a * d.dc + c);
@@ -544,14 +608,14 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
   }
   if constexpr (JOIN) {  // the splits' weights: sixteen threads a row
     const int r = min(r0 + (int)(threadIdx.x >> 4), R - 1), b = r / d.n, g = threadIdx.x & 15;
-    const int ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
-    const float* st = stat + 2 * ((int64_t)b * d.splits * rows + r % d.n * d.H + h);
+    const Parts ps(d, kv_lens, b);
+    const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r % d.n * d.H + h);
     float m = -INFINITY, sum = 0.f, ms[kUpSplits / 16], ls[kUpSplits / 16];
 #pragma unroll
     for (int i = 0; i < kUpSplits / 16; ++i) {
       const int s = g + 16 * i;
-      ms[i] = s < ns ? st[2 * (int64_t)s * rows] : -INFINITY;
-      ls[i] = s < ns ? st[2 * (int64_t)s * rows + 1] : 0.f;
+      ms[i] = s < ps.all ? st[2 * (int64_t)ps.slot(s) * rows] : -INFINITY;
+      ls[i] = s < ps.all ? st[2 * (int64_t)ps.slot(s) * rows + 1] : 0.f;
       m = fmaxf(m, ms[i]);
     }
 #pragma unroll
@@ -575,10 +639,12 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
     f32x4 x = zero4();
     if (c < d.dc && r0 + r < R) {
       if constexpr (JOIN) {
-        const int b = (r0 + r) / d.n, ns = (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk;
-        const float* p = part + ((int64_t)b * d.splits * rows + (r0 + r) % d.n * d.H + h) * d.dc + c;
+        const int b = (r0 + r) / d.n;
+        const Parts ps(d, kv_lens, b);
+        const float* p = part + ((int64_t)b * d.slots * rows + (r0 + r) % d.n * d.H + h) * d.dc + c;
 #pragma unroll 8
-        for (int s = 0; s < ns; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
+        for (int s = 0; s < ps.all; ++s)
+          x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)ps.slot(s) * rows * d.dc);
       } else {
         x = *reinterpret_cast<const f32x4*>(olat + ((int64_t)(r0 + r) * d.H + h) * d.dc + c);
       }
@@ -605,6 +671,62 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
   if (r < R && v < d.dv) store4(o + ((int64_t)r * d.H + h) * d.dv + v, acc);
 }
 
+// weights[b, j] += sum over the query rows of p_j = 2^(s_j - lse), from the scores that
+// latent_split left; the n newest tokens' begin here.  Each token's sum is made by one
+// wave in a fixed order: over the row tiles, then across the 16 rows of a tile.  A
+// workgroup forms the rows' lse from the parts' statistics (the rows that a tile is padded
+// with, and those that see nothing, get infinity) and goes over kWeighTiles tiles.
+constexpr int kWeighTiles = 16;
+__global__ __launch_bounds__(256) void latent_weigh(DecDims d, int row_tiles, const float* __restrict__ score,
+                                                    const float* __restrict__ stat,
+                                                    const int32_t* __restrict__ kv_lens, int64_t stride,
+                                                    float* __restrict__ weights) {
+  __shared__ float lse[4096 + 64];
+  const int b = blockIdx.y, rows = d.n * d.H, len = dec_len(d, kv_lens, b), lane = lane_id();
+  if (16 * kWeighTiles * (int)blockIdx.x >= len) return;
+  const Parts ps(d, kv_lens, b);
+  for (int r = threadIdx.x; r < 16 * row_tiles; r += 256) {
+    float m = -INFINITY, sum = 0.f;
+    if (r < rows) {
+      const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r);
+      for (int s = 0; s < ps.all; ++s) {
+        const int64_t a = 2 * (int64_t)ps.slot(s) * rows;
+        const float ms = st[a], mn = fmaxf(m, ms);
+        if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + st[a + 1] * fast_exp2(ms - mn);
+        m = mn;
+      }
+    }
+    // (a NaN among a row's scores stays one)
+    lse[r] = sum == 0.f ? INFINITY : m + fast_log2(sum);
+  }
+  __syncthreads();
+  const int tiles = (d.table * d.page + 15) / 16;
+#pragma unroll
+  for (int i = 0; i < kWeighTiles / 4; ++i) {
+    const int tile = kWeighTiles * blockIdx.x + 4 * i + wave_id();
+    if (16 * tile >= len) break;
+    f32x4 x = zero4();
+#pragma unroll 4
+    for (int g = 0; g < row_tiles; ++g) {
+      const f32x4 s = *reinterpret_cast<const f32x4*>(
+          score + ((((int64_t)b * row_tiles + g) * tiles + tile) * 64 + lane) * 4);
+      const float z = lse[16 * g + (lane & 15)];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] += fast_exp2(s[r] - z);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int k = 1; k < 16; k *= 2) x[r] += __shfl_xor(x[r], k);
+    if ((lane & 15) < 4) {
+      const int j = 16 * tile + tile_row(lane & 3);
+      const float add = (lane & 2) ? ((lane & 1) ? x[3] : x[2]) : ((lane & 1) ? x[1] : x[0]);
+      float* w = weights + b * stride + j;
+      if (j < len) *w = (j < len - d.n ? *w : 0.f) + add;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host
 static int app_check(const atomic_latent_append_args* a) {
   if (!a) return ATOMIC_ERR_NULL;
@@ -622,12 +744,13 @@ static int app_check(const atomic_latent_append_args* a) {
   return ATOMIC_OK;
 }
 
-static int dec_check(const atomic_latent_decode_args* a) {
+// `least`: pages that a table has to have
+static int dec_check(const atomic_latent_decode_args* a, int least = 1) {
   if (!a) return ATOMIC_ERR_NULL;
   if (int rc = latent_widths_check(a->dn, a->dr, a->dtype)) return rc;
   if (a->dv < 8 || a->dv > 128 || a->dv % 8 || a->dc < 8 || a->dc > 512 || a->dc % 8 || a->batch < 1 ||
       a->tokens < 1 || a->heads < 1 || (int64_t)a->tokens * a->heads > 4096 || a->page < 1 || a->pages < 1 ||
-      a->table_pages < 1 || (a->interleaved != 0 && a->interleaved != 1))
+      a->table_pages < least || (a->interleaved != 0 && a->interleaved != 1))
     return ATOMIC_ERR_SHAPE;
   // grid dimensions and token numbers
   if (a->batch > 65535 || (int64_t)a->batch * a->tokens > 65535 * 16 ||
@@ -637,17 +760,34 @@ static int dec_check(const atomic_latent_decode_args* a) {
   return ATOMIC_OK;
 }
 
-// Rows a workgroup of latent_split takes, in tiles of 16.
-static int dec_row_tiles(const atomic_latent_decode_args* a) {
-  const int rows = a->tokens * a->heads;
-  return rows <= 16 ? 1 : rows <= 32 || a->dtype != ATOMIC_BF16 ? 2 : 4;
+static int shared_check(const atomic_latent_shared_args* a) {
+  if (!a) return ATOMIC_ERR_NULL;
+  if (int rc = dec_check(&a->dec, 0)) return rc;
+  const atomic_latent_decode_args* c = &a->dec;
+  if (a->prefixes < 0 || a->prefix_pages < 0 || (a->scored != 0 && a->scored != 1) ||
+      (int64_t)a->prefix_pages * c->page > (1 << 30) ||
+      (c->table_pages < 1 && (a->prefixes == 0 || a->prefix_pages < 1)))  // no token at all
+    return ATOMIC_ERR_SHAPE;
+  // the rows that read a prefix are one grid dimension
+  if (a->prefixes && (c->batch % a->prefixes ||
+                      (int64_t)(c->batch / a->prefixes) * c->tokens * c->heads > (1 << 20)))
+    return ATOMIC_ERR_SHAPE;
+  if (a->scored && a->weights_stride < (int64_t)c->table_pages * c->page) return ATOMIC_ERR_SHAPE;
+  return ATOMIC_OK;
 }
 
-static DecDims dec_dims(const atomic_latent_decode_args* a) {
-  DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, a->table_pages,
-            a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]}};
-  const int mt = dec_row_tiles(a), rt = 16 * mt, tile = mt == 4 ? 64 : 32;
-  d.groups = (d.n * d.H + rt - 1) / rt;
+// Rows a workgroup of latent_split takes, in tiles of 16.
+static int dec_row_tiles(int64_t rows, int dtype) {
+  return rows <= 16 ? 1 : rows <= 32 || dtype != ATOMIC_BF16 ? 2 : 4;
+}
+
+static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table) {
+  DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, table,
+            a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]},
+            share, 0, 0, 0, 1, 0, 0, nullptr};
+  const int64_t rows = (int64_t)share * d.n * d.H;
+  const int mt = dec_row_tiles(rows, a->dtype), rt = 16 * mt, tile = mt == 4 ? 64 : 32;
+  d.groups = (int)((rows + rt - 1) / rt);
   // As many workgroups as the card holds at once if every sequence were as long as
   // its table (the host does not know the lengths, so a table wider than the sequences
   // costs parallelism: 64 of 1024 tokens, 16 heads, whole calls: 42 us with a table as
@@ -656,27 +796,55 @@ static DecDims dec_dims(const atomic_latent_decode_args* a) {
   // splits of 512, 103 of 1024; 4 of 32768: 42 of 256 or 512, 56 of 128; 8 of 4096
   // with 64 rows: 33 of 128, 36 of 256, 46 of 64; one of 777: 18 of 32, 22 of 128.
   const int64_t slots = mt == 4 || a->dtype != ATOMIC_BF16 ? 256 : 512;
-  const int64_t most = (int64_t)d.table * d.page, want = (most * d.B * d.groups + slots - 1) / slots;
+  const int64_t most = (int64_t)d.table * d.page, want = (most * units * d.groups + slots - 1) / slots;
   const int64_t chunk = want < tile ? tile : want > kDecChunk ? kDecChunk : want;
   d.chunk = (int)((chunk + tile - 1) / tile * tile);
   d.splits = (int)((most + d.chunk - 1) / d.chunk);
+  d.slots = d.splits;
   return d;
 }
+
+// A call's launches over the sequences' own tokens and over the prefixes (with `front.splits` 0 there is none).
+struct DecPlan {
+  DecDims own, front;
+};
+static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages) {
+  DecPlan p{dec_dims(a, a->batch, 1, a->table_pages), {}};
+  if (!prefixes) return p;
+  p.front = dec_dims(a, prefixes, a->batch / prefixes, prefix_pages);
+  p.own.slot0 = p.front.splits;
+  p.own.slots = p.front.slots = p.own.splits + p.front.splits;
+  p.own.pre_share = p.front.share;
+  p.own.pre_chunk = p.front.chunk;
+  p.own.pre_splits = p.front.splits;
+  p.own.pre_most = prefix_pages * a->page;
+  return p;
+}
+
 // Whether latent_up joins the splits: at most 48 loads a thread, in steps of eight
 // (25 loads: 14.6 us against 7.4 + 7.2 of two launches, 64: 25.7 against 9 + 10).
 static bool dec_up_joins(const DecDims& d) {
   const int64_t rows = (int64_t)d.B * d.n < 16 ? (int64_t)d.B * d.n : 16;
-  return d.splits > 1 && d.splits <= kUpSplits && d.splits * ((rows * d.dc / 4 + 255) / 256) <= 48;
+  return d.slots > 1 && d.slots <= kUpSplits && d.slots * ((rows * d.dc / 4 + 255) / 256) <= 48;
 }
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-static size_t dec_qa_bytes(const DecDims& d, int dtype) {
-  return up256((size_t)d.B * d.n * d.H * (d.dc + d.dr) * (dtype == ATOMIC_BF16 ? 2 : 4));
+// What a call leaves in its workspace, part after part.
+struct DecSpace {
+  size_t qa, olat, stat, part, score, all;
+};
+static DecSpace dec_space(const DecDims& d, int dtype, bool scored) {
+  const size_t rows = (size_t)d.B * d.n * d.H, es = dtype == ATOMIC_BF16 ? 2 : 4;
+  const size_t parts = d.slots > 1 ? rows * d.slots : 0;  // one split needs no parts
+  const size_t tiles = (size_t)d.groups * dec_row_tiles((int64_t)d.n * d.H, dtype) * (((size_t)d.table * d.page + 15) / 16);
+  DecSpace s;
+  s.qa = 0;
+  s.olat = s.qa + up256(rows * (d.dc + d.dr) * es * (scored && es == 2 ? 2 : 1));
+  s.stat = s.olat + up256(rows * d.dc * sizeof(float));
+  s.part = s.stat + up256((scored ? rows * d.slots : parts) * 2 * sizeof(float));
+  s.score = s.part + up256(parts * d.dc * sizeof(float));
+  s.all = s.score + (scored ? (size_t)d.B * tiles * 256 * sizeof(float) : 0);
+  return s;
 }
-static size_t dec_olat_bytes(const DecDims& d) { return up256((size_t)d.B * d.n * d.H * d.dc * sizeof(float)); }
-// one split needs no parts
-static size_t dec_part_rows(const DecDims& d) { return d.splits > 1 ? (size_t)d.B * d.splits * d.n * d.H : 0; }
-static size_t dec_stat_bytes(const DecDims& d) { return up256(dec_part_rows(d) * 2 * sizeof(float)); }
-static size_t dec_part_bytes(const DecDims& d) { return dec_part_rows(d) * d.dc * sizeof(float); }
 
 }  // namespace ah
 
@@ -709,24 +877,99 @@ extern "C" int atomic_latent_append(const atomic_latent_append_args* a, const vo
   });
 }
 
-extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
-  if (dec_check(a) != ATOMIC_OK) return 0;
-  const DecDims d = dec_dims(a);
-  return dec_qa_bytes(d, a->dtype) + dec_olat_bytes(d) + dec_stat_bytes(d) + dec_part_bytes(d);
-}
-
-template <typename T, int DC>
-static void launch_split(const DecDims& d, int mt, hipStream_t st, const T* qa, const void* cache, const int32_t* table,
-                         const int32_t* kv_lens, float* part, float* stat, float* olat) {
-  const dim3 grid((unsigned)d.splits, (unsigned)d.groups, (unsigned)d.B);
+template <typename T, int DC, bool SCORED>
+static void launch_split(const DecDims& d, int units, int dtype, hipStream_t st, const T* qa, const void* cache,
+                         const int32_t* table, const int32_t* lens, const int32_t* own, int own_most, float* part,
+                         float* stat, float* olat, float* score) {
+  const dim3 grid((unsigned)d.splits, (unsigned)d.groups, (unsigned)units);
   auto go = [&](auto m) {
     constexpr int NW = decltype(m)::value == 4 ? 4 : 2;
-    hipLaunchKernelGGL((latent_split<T, DC, decltype(m)::value, NW>), grid, dim3(64 * NW), 0, st, d, qa,
-                       (const T*)cache, table, kv_lens, part, stat, olat);
+    hipLaunchKernelGGL((latent_split<T, DC, decltype(m)::value, NW, SCORED>), grid, dim3(64 * NW), 0, st, d, qa,
+                       (const T*)cache, table, lens, own, own_most, part, stat, olat, score);
   };
+  const int mt = dec_row_tiles((int64_t)d.share * d.n * d.H, dtype);
   if (mt == 1) go(IntC<1>());
   else if (mt == 2) go(IntC<2>());
   else if constexpr (sizeof(T) == 2) go(IntC<4>());
+}
+
+struct DecPtrs {
+  const void *q, *w_kv, *cache;
+  const int32_t *prefix_table, *prefix_lens, *table, *lens;
+  const float *cos, *sin;
+  float* weights;
+  int64_t weights_stride;
+  void *o, *ws;
+};
+
+template <typename T, bool SCORED>
+static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, const DecPtrs& p,
+                   hipStream_t st) {
+  DecPlan plan = dec_plan(a, prefixes, prefix_pages);
+  plan.own.pre_lens = p.prefix_lens;
+  const DecDims& d = plan.own;
+  const DecSpace at = dec_space(d, a->dtype, SCORED);
+  Launch L{a->profile, st};
+  char* ws = (char*)p.ws;
+  T* qa = (T*)(ws + at.qa);
+  float *olat = (float*)(ws + at.olat), *stat = (float*)(ws + at.stat), *part = (float*)(ws + at.part);
+  float* score = SCORED ? (float*)(ws + at.score) : nullptr;
+  const unsigned rt = (unsigned)((d.B * d.n + 15) / 16);
+  int rc = L("latent_absorb", [&] {
+    hipLaunchKernelGGL((latent_absorb<T, SCORED && sizeof(T) == 2>),
+                       dim3((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt), dim3(256), 0, st, d, (const T*)p.q,
+                       (const T*)p.w_kv, p.lens, p.cos, p.sin, qa);
+  });
+  if (rc) return rc;
+  auto split = [&](const DecDims& x, int units, const int32_t* table, const int32_t* lens, const int32_t* own,
+                   int own_most, float* sc) {
+    if (d.dc <= 256)
+      launch_split<T, 256, SCORED>(x, units, a->dtype, st, qa, p.cache, table, lens, own, own_most, part, stat, olat, sc);
+    else
+      launch_split<T, 512, SCORED>(x, units, a->dtype, st, qa, p.cache, table, lens, own, own_most, part, stat, olat, sc);
+  };
+  if (plan.front.splits) {
+    rc = L("latent_split (prefix)", [&] {
+      split(plan.front, prefixes, p.prefix_table, p.prefix_lens, p.lens, d.table * d.page, nullptr);
+    });
+    if (rc) return rc;
+  }
+  if (d.splits) {
+    rc = L("latent_split", [&] { split(d, d.B, p.table, p.lens, nullptr, 0, score); });
+    if (rc) return rc;
+  }
+  const bool joins = dec_up_joins(d);
+  if (d.slots > 1 && !joins) {
+    int ways = 1;  // about four splits a thread
+    while (ways < 16 && 4 * ways < d.slots) ways *= 2;
+    const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
+    rc = L("latent_join", [&] {
+      hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, part,
+                         stat, p.lens, olat);
+    });
+    if (rc) return rc;
+  }
+  rc = L("latent_up", [&] {
+    auto go = [&](auto j) {
+      hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0>),
+                         dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
+                         (const T*)p.w_kv, olat, part, stat, p.lens, (T*)p.o);
+    };
+    if (joins) go(IntC<1>());
+    else go(IntC<0>());
+  });
+  if (rc || !SCORED || !d.splits) return rc;
+  return L("latent_weigh", [&] {
+    const int64_t tokens = (int64_t)d.table * d.page;
+    hipLaunchKernelGGL(latent_weigh, dim3((unsigned)((tokens + 16 * kWeighTiles - 1) / (16 * kWeighTiles)), (unsigned)d.B),
+                       dim3(256), 0, st, d, d.groups * dec_row_tiles((int64_t)d.n * d.H, a->dtype), score, stat, p.lens,
+                       p.weights_stride, p.weights);
+  });
+}
+
+extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
+  if (dec_check(a) != ATOMIC_OK) return 0;
+  return dec_space(dec_plan(a, 0, 0).own, a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -740,48 +983,36 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
   if (!workspace || workspace_bytes < atomic_latent_decode_workspace_size(a) || !aligned16({workspace}))
     return ATOMIC_ERR_WORKSPACE;
   ws_tag_clobber(workspace, atomic_latent_decode_workspace_size(a));
-  const DecDims d = dec_dims(a);
-  const hipStream_t st = (hipStream_t)stream;
-  Launch L{a->profile, st};
-  auto go = [&](auto t) {
+  const DecPtrs p{q, w_kv, cache, nullptr, nullptr, page_table, kv_lens, cos, sin, nullptr, 0, o, workspace};
+  return a->dtype == ATOMIC_BF16 ? dec_run<bf16, false>(a, 0, 0, p, (hipStream_t)stream)
+                                 : dec_run<float, false>(a, 0, 0, p, (hipStream_t)stream);
+}
+
+extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
+  if (shared_check(a) != ATOMIC_OK) return 0;
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages).own, a->dec.dtype, a->scored != 0).all;
+}
+
+extern "C" int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,
+                                           const void* cache, const int32_t* prefix_table, const int32_t* prefix_lens,
+                                           const int32_t* page_table, const int32_t* kv_lens, const float* cos,
+                                           const float* sin, float* weights, void* o, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  if (int rc = shared_check(a)) return rc;
+  if (!q || !w_kv || !cache || !kv_lens || !o || !cos != !sin || (a->dec.table_pages && !page_table) ||
+      (a->prefixes && (!prefix_lens || (a->prefix_pages && !prefix_table))) || (a->scored && !weights))
+    return ATOMIC_ERR_NULL;
+  if (cos && a->dec.rope_rows < 1) return ATOMIC_ERR_SHAPE;
+  if (!aligned16({q, w_kv, cache, cos, sin, o})) return ATOMIC_ERR_SHAPE;
+  const size_t bytes = atomic_latent_decode_shared_workspace_size(a);
+  if (!workspace || workspace_bytes < bytes || !aligned16({workspace})) return ATOMIC_ERR_WORKSPACE;
+  ws_tag_clobber(workspace, bytes);
+  const DecPtrs p{q,   w_kv, cache, prefix_table, prefix_lens,       page_table, kv_lens,
+                  cos, sin,  weights, a->weights_stride, o, workspace};
+  const auto run = [&](auto t) {
     typedef decltype(t) T;
-    T* qa = (T*)workspace;
-    float* olat = (float*)((char*)workspace + dec_qa_bytes(d, a->dtype));
-    float* stat = (float*)((char*)olat + dec_olat_bytes(d));
-    float* part = (float*)((char*)stat + dec_stat_bytes(d));
-    const unsigned rt = (unsigned)((d.B * d.n + 15) / 16);
-    int rc = L("latent_absorb", [&] {
-      hipLaunchKernelGGL((latent_absorb<T>), dim3((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt), dim3(256), 0,
-                         st, d, (const T*)q, (const T*)w_kv, kv_lens, cos, sin, qa);
-    });
-    if (rc) return rc;
-    rc = L("latent_split", [&] {
-      if (d.dc <= 256)
-        launch_split<T, 256>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat, olat);
-      else
-        launch_split<T, 512>(d, dec_row_tiles(a), st, qa, cache, page_table, kv_lens, part, stat, olat);
-    });
-    if (rc) return rc;
-    const bool joins = dec_up_joins(d);
-    if (d.splits > 1 && !joins) {
-      int ways = 1;  // about four splits a thread
-      while (ways < 16 && 4 * ways < d.splits) ways *= 2;
-      const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
-      rc = L("latent_join", [&] {
-        hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, part,
-                           stat, kv_lens, olat);
-      });
-      if (rc) return rc;
-    }
-    return L("latent_up", [&] {
-      auto go = [&](auto j) {
-        hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0>),
-                           dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
-                           (const T*)w_kv, olat, part, stat, kv_lens, (T*)o);
-      };
-      if (joins) go(IntC<1>());
-      else go(IntC<0>());
-    });
+    return a->scored ? dec_run<T, true>(&a->dec, a->prefixes, a->prefix_pages, p, (hipStream_t)stream)
+                     : dec_run<T, false>(&a->dec, a->prefixes, a->prefix_pages, p, (hipStream_t)stream);
   };
-  return a->dtype == ATOMIC_BF16 ? go(bf16()) : go(float());
+  return a->dec.dtype == ATOMIC_BF16 ? run(bf16()) : run(float());
 }

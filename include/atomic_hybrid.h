@@ -909,6 +909,79 @@ int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, cons
                          const float* cos, const float* sin, void* o, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* The same for sequences that share prefixes, read once for all of them, and with the
+ * attention weight that each cached token gathers.
+ *
+ * The batch is `prefixes` equal runs of sequences: sequence b follows prefix
+ * g = b / (batch / prefixes), and its tokens are the prefix_lens[g] tokens of
+ * prefix_table[g], then its own kv_lens[b] of page_table[b].  Query t stands at
+ * position prefix_lens[g] + kv_lens[b] - n + t among them and sees those up to and
+ * with its own, as atomic_latent_decode does over the two tables as one.
+ *
+ * With scored = 1, weights[b * weights_stride + j] receives, for each own token
+ * j < kv_lens[b], the sum of its softmax weights over the heads and query tokens:
+ * added to what stands there, except for the n newest tokens (j >= kv_lens[b] - n),
+ * whose sums begin with this call.  What lies past the length stays as it is.  Each sum
+ * is made in a fixed order.  The workspace then holds the scores: 4 bytes a query row
+ * (of whole tiles of 16 to 64 rows a sequence) and token of the table. */
+typedef struct atomic_latent_shared_args {
+  atomic_latent_decode_args dec; /* as above; table_pages may be 0 with prefixes      */
+  int32_t prefixes;              /* 0 (none), or a divisor of dec.batch; at most 2^20
+                                    query rows (tokens and heads) follow one          */
+  int32_t prefix_pages;          /* entries of a prefix_table row, 0 or more          */
+  int32_t scored;                /* 0 or 1                                            */
+  int64_t weights_stride;        /* of weights: sequence; at least table_pages * page */
+} atomic_latent_shared_args;
+
+/* Bytes of workspace; 0 for unsupported args. */
+size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a);
+
+/* prefix_table int32 [prefixes, prefix_pages], prefix_lens int32 [prefixes] (both NULL
+ * without prefixes); weights float32, NULL unless scored. */
+int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,
+                                const void* cache, const int32_t* prefix_table, const int32_t* prefix_lens,
+                                const int32_t* page_table, const int32_t* kv_lens, const float* cos,
+                                const float* sin, float* weights, void* o, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Eviction: of each sequence longer than `keep` tokens, keep are left.
+ *
+ * order[b, j] says how old the token in row j of sequence b is: its place among all the
+ * sequence's tokens.  A row that no eviction has seen holds -1; such rows are taken as the
+ * newest, in the order of their rows.  The first `sinks` tokens (order < sinks) and the
+ * `recent` newest stay; of the others those with the largest weights, among equal ones
+ * the lowest rows (a NaN counts as less than every number).  Kept tokens from rows >= keep
+ * move into the rows below keep that became free, the k-th into the k-th, with their cache
+ * rows, weights and order; nothing else moves.
+ *
+ * kv_lens_out [batch] (at most keep), weights_out and order_out [batch, width] receive
+ * the new state (0 and -1 past the lengths) and may be kv_lens, weights and order
+ * themselves; source [batch, keep] the row that each row's token was in (-1 past the
+ * length).  Called again with the same kv_lens, weights and order, when only the cache
+ * has changed, it does the same again.  Sequences must not share pages. */
+typedef struct atomic_latent_evict_args {
+  int32_t batch;          /* B                                                        */
+  int32_t dtype;          /* of the cache: ATOMIC_F32 / ATOMIC_BF16                   */
+  int32_t row;            /* elements of a cache row: a multiple of 8, 16 .. 576      */
+  int32_t page;           /* tokens a page                                            */
+  int32_t pages;          /* pages of the cache                                       */
+  int32_t table_pages;    /* entries of a page_table row                              */
+  int32_t width;          /* of weights and order: at least table_pages * page        */
+  int32_t keep;           /* 1 or more                                                */
+  int32_t sinks, recent;  /* 0 or more, together at most keep                         */
+  int64_t weights_stride, order_stride;         /* sequence; at least width           */
+  int64_t weights_out_stride, order_out_stride;
+  atomic_profile* profile;
+} atomic_latent_evict_args;
+
+/* Bytes of workspace; 0 for unsupported args. */
+size_t atomic_latent_evict_workspace_size(const atomic_latent_evict_args* a);
+
+int atomic_latent_evict(const atomic_latent_evict_args* a, void* cache, const int32_t* page_table,
+                        const int32_t* kv_lens, const float* weights, const int32_t* order,
+                        int32_t* kv_lens_out, float* weights_out, int32_t* order_out, int32_t* source,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

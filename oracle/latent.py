@@ -134,3 +134,75 @@ def decode(q, w_kv, cache, table, kv_lens, scale, cos=None, sin=None, interleave
                 s = (up[:, :dn] @ q[b, t, h, :dn].to(F) + rows[:pos + 1, dc:] @ qp) * scale
                 o[b, t, h] = torch.softmax(s, 0) @ up[:, dn:]
     return o
+
+
+def _tokens(cache, table, ln):
+    page = cache.shape[1]
+    rows = [cache[int(table[j // page]), j % page] for j in range(ln)]
+    return torch.stack(rows).to(F) if rows else torch.zeros(0, cache.shape[2], dtype=F)
+
+
+def decode_shared(q, w_kv, cache, prefix_table, prefix_lens, table, kv_lens, scale, cos=None, sin=None,
+                  interleaved=False):
+    """(o [B, n, H, dv], weights [B, tokens of the table]): the sequences' own tokens
+    stand behind their prefix's; ``weights`` sum each own token's probabilities over the
+    heads and query tokens.  ``prefix_table`` None: no prefixes."""
+    B, n, H, d = q.shape
+    dc = w_kv.shape[2]
+    dn = d - (cache.shape[2] - dc)
+    page = cache.shape[1]
+    w = w_kv.to(F)
+    o = torch.zeros(B, n, H, w.shape[1] - dn, dtype=F)
+    weights = torch.zeros(B, table.shape[1] * page, dtype=F)
+    for b in range(B):
+        ln = min(max(int(kv_lens[b]), 0), table.shape[1] * page)
+        rows = _tokens(cache, table[b], ln)
+        P = 0
+        if prefix_table is not None:
+            g = b // (B // prefix_table.shape[0])
+            P = min(max(int(prefix_lens[g]), 0), prefix_table.shape[1] * page)
+            rows = torch.cat((_tokens(cache, prefix_table[g], P), rows))
+        up = torch.einsum("hrc,jc->hjr", w, rows[:, :dc])                       # each head's keys and values
+        for t in range(n):
+            pos = P + ln - n + t
+            if pos < 0:
+                continue
+            qp = q[b, t, :, dn:].to(F)
+            if cos is not None:
+                qp = rotate(qp, torch.full((H,), pos), cos, sin, interleaved)
+            seen = slice(0, pos + 1)
+            s = (torch.einsum("hjr,hr->hj", up[:, seen, :dn], q[b, t, :, :dn].to(F)) + qp @ rows[seen, dc:].t()) * scale
+            p = torch.softmax(s, 1)
+            o[b, t] = torch.einsum("hj,hjv->hv", p, up[:, seen, dn:])
+            own = p[:, P:].sum(0)
+            weights[b, :own.numel()] += own
+    return o, weights
+
+
+def gathered(before, add, kv_lens, n):
+    """The weights [B, W] after a step of n query tokens whose sums are ``add`` [B, ...]."""
+    after = before.to(F).clone()
+    for b, ln in enumerate(kv_lens):
+        for j in range(min(max(int(ln), 0), add.shape[1])):
+            after[b, j] = (after[b, j] if j < int(ln) - n else 0) + add[b, j]
+    return after
+
+
+def evict(kv_lens, weights, order, keep, sinks, recent):
+    """(kv_lens, weights, order, source) as lists of the sequences' rows; a list's
+    length is the new length."""
+    out = []
+    for b, ln in enumerate(kv_lens):
+        w, age = [float(x) for x in weights[b, :ln]], [int(x) for x in order[b, :ln]]
+        fresh = [j for j in range(ln) if age[j] < 0]
+        top = max(age, default=-1)
+        for j in fresh:
+            age[j] = max(top, -1) + 1 + j - fresh[0]
+        new = max(age, default=-1)
+        safe = lambda j: age[j] < sinks or age[j] > new - recent  # noqa: E731
+        rank = lambda j: (not safe(j), math.isnan(w[j]), -w[j] if not math.isnan(w[j]) else 0, j)  # noqa: E731
+        stay = set(sorted(range(ln), key=rank)[:keep])
+        came = iter(sorted(j for j in stay if j >= keep))
+        source = [j if j in stay else next(came) for j in range(min(ln, keep))]
+        out.append((len(source), [w[j] for j in source], [age[j] for j in source], source))
+    return tuple(list(x) for x in zip(*out))
