@@ -20,7 +20,7 @@ BUILD_DIR = os.path.join(HERE, "_build")
 
 # translation units (each includes the kernel sources it launches)
 UNITS = ["gdn2_host.hip", "mamba2_host.hip", "norm_gate.hip", "prologue.hip", "stage256.hip",
-         "stage256_bwd.hip", "latent_attn.hip", "latent_decode.hip", "latent_evict.hip"]
+         "stage256_bwd.hip", "latent_attn.hip", "latent_decode.hip", "latent_prefix.hip", "latent_evict.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

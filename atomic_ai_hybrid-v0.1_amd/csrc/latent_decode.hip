@@ -17,7 +17,7 @@
 // bytes leave the matrix instructions idle; with probabilities of eight bits o was off
 // by 0.0025 of its norm at 64 sequences of up to 8192 tokens, now by 0.0023, of which
 // its own rounding is 0.0017 and q_lat's most of the rest).
-#include "latent.hpp"
+#include "latent_decode.hpp"
 
 namespace ah {
 
@@ -108,36 +108,6 @@ __global__ __launch_bounds__(256) void latent_append(AppDims d, const T* __restr
 }
 
 // ------------------------------------------------------------------- decode
-struct DecDims {
-  int B, n, H, dn, dr, dv, dc, page, pages, table, rope, inter;
-  int chunk, splits, groups;  // tokens a split (whole tiles), splits of the longest sequence, row groups
-  float scale;
-  int64_t qs[3];
-  int share;         // latent_split: sequences whose rows read the same tokens (those of a prefix, or one)
-  int slot0, slots;  // its first slot among a row's parts, and all of them
-  // prefixes: sequences of each (0: there are none), tokens a split, slots, tokens their table holds, lengths
-  int pre_share, pre_chunk, pre_splits, pre_most;
-  const int32_t* pre_lens;
-};
-constexpr int kDecChunk = 1024, kDecPages = kDecChunk + 1;  // tokens of a split, pages that they can lie in
-__device__ __forceinline__ int dec_len(const DecDims& d, const int32_t* kv_lens, int b) {
-  return (int)min((int64_t)max(kv_lens[b], 0), (int64_t)d.table * d.page);
-}
-// Length of the prefix that sequence b's own tokens follow.
-__device__ __forceinline__ int pre_len(const DecDims& d, int b) {
-  return d.pre_share ? min(max(d.pre_lens[b / d.pre_share], 0), d.pre_most) : 0;
-}
-// The parts of sequence b's rows: those of the prefix's splits, then those of its own.
-struct Parts {
-  int front, all, skip;  // splits of the prefix, of both, slots to leave out between them
-  __device__ __forceinline__ Parts(const DecDims& d, const int32_t* kv_lens, int b) {
-    front = d.pre_share ? (pre_len(d, b) + d.pre_chunk - 1) / d.pre_chunk : 0;
-    all = front + (d.splits ? (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk : 0);
-    skip = d.pre_splits - front;
-  }
-  __device__ __forceinline__ int slot(int s) const { return s < front ? s : s + skip; }
-};
-
 // q_lat [B n, H, dc | rotated q_pe]: a head, 16 query tokens and 64 latent
 // columns a workgroup, 16 columns a wave; one more column block rotates.  Latency: 4 to
 // 6 us with 4 to 64 sequences of 16 heads (4 MB of weights).  With LO each row is
@@ -267,9 +237,6 @@ struct DTile : LTile<T, W, 16> {
     }
   }
 };
-
-// Eight zeros: the source of the padding of a latent narrower than its tile.
-__device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 
 // One split of one sequence against 16 MT of its query rows (row t H + h).  NW
 // waves go over tiles of 16 NW tokens: wave w loads 16 tokens of each tile and
@@ -807,11 +774,16 @@ static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share
 // A call's launches over the sequences' own tokens and over the prefixes (with `front.splits` 0 there is none).
 struct DecPlan {
   DecDims own, front;
+  bool many;  // the prefixes' rows are many: latent_prefix takes them
 };
-static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages) {
-  DecPlan p{dec_dims(a, a->batch, 1, a->table_pages), {}};
+static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, bool scored) {
+  DecPlan p{dec_dims(a, a->batch, 1, a->table_pages), {}, false};
   if (!prefixes) return p;
   p.front = dec_dims(a, prefixes, a->batch / prefixes, prefix_pages);
+  DecDims many = p.front;
+  p.many = !scored && a->dtype == ATOMIC_BF16 && a->dc > 256 && prefix_plan(many, prefixes) &&
+           many.splits + p.own.splits > 1;
+  if (p.many) p.front = many;
   p.own.slot0 = p.front.splits;
   p.own.slots = p.front.slots = p.own.splits + p.front.splits;
   p.own.pre_share = p.front.share;
@@ -905,7 +877,7 @@ struct DecPtrs {
 template <typename T, bool SCORED>
 static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, const DecPtrs& p,
                    hipStream_t st) {
-  DecPlan plan = dec_plan(a, prefixes, prefix_pages);
+  DecPlan plan = dec_plan(a, prefixes, prefix_pages, SCORED);
   plan.own.pre_lens = p.prefix_lens;
   const DecDims& d = plan.own;
   const DecSpace at = dec_space(d, a->dtype, SCORED);
@@ -929,8 +901,14 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
       launch_split<T, 512, SCORED>(x, units, a->dtype, st, qa, p.cache, table, lens, own, own_most, part, stat, olat, sc);
   };
   if (plan.front.splits) {
-    rc = L("latent_split (prefix)", [&] {
-      split(plan.front, prefixes, p.prefix_table, p.prefix_lens, p.lens, d.table * d.page, nullptr);
+    rc = L(plan.many ? "latent_prefix" : "latent_split (prefix)", [&] {
+      const int own_most = d.table * d.page;
+      if constexpr (sizeof(T) == 2 && !SCORED) {
+        if (plan.many)
+          return launch_prefix(plan.front, prefixes, st, qa, p.cache, p.prefix_table, p.prefix_lens, p.lens, own_most,
+                               part, stat);
+      }
+      split(plan.front, prefixes, p.prefix_table, p.prefix_lens, p.lens, own_most, nullptr);
     });
     if (rc) return rc;
   }
@@ -969,7 +947,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
 
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(a, 0, 0).own, a->dtype, false).all;
+  return dec_space(dec_plan(a, 0, 0, false).own, a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -990,7 +968,7 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
 
 extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
   if (shared_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages).own, a->dec.dtype, a->scored != 0).all;
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0).own, a->dec.dtype, a->scored != 0).all;
 }
 
 extern "C" int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,

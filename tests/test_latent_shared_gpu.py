@@ -95,8 +95,19 @@ CASES = [
 ]
 
 
+# rows enough that a prefix's tokens are bound by matrix instructions (wide latents in bf16)
+MANY = [
+    ([256], [0] * 33, 1, 1, 128, 64, 128, 512, 64),                          # 33 rows of one head
+    ([300], [0, 40, 2] * 5, 3, 6, 128, 64, 128, 512, 16),                    # queries that stand in the prefix
+    ([1, 700, 0, 257], [5, 0, 33, 64] * 3, 1, 20, 56, 24, 72, 448, 24),      # prefixes of one token, none, many
+    ([2049], [17 * i % 50 for i in range(9)], 2, 15, 64, 32, 64, 264, 1),    # 270 rows; a token past a split
+    ([33, 500], [20] * 8, 4, 40, 128, 32, 96, 320, 128),
+    ([256], [3, 0], 19, 16, 64, 32, 64, 512, 256),                           # more queries than own tokens
+]
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page", CASES)
+@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page", CASES + MANY)
 def test_shared_matches_the_formula(pre, own, n, H, dn, dr, dv, dc, page, dtype):
     banner(f"latent shared {pre} {own} n{n} H{H} {dn}/{dr}/{dv}/{dc} page {page} {dtype}")
     q, w, cache, pt, pl, table, ln = _case(pre, own, n, H, dn, dr, dv, dc, page, dtype, seed=H + n + pre[0])
@@ -154,11 +165,21 @@ def test_decode_gathers_the_weights(lens, n, H, dn, dr, dv, dc, page, dtype):
     _weights_within(a, torch.zeros_like(before), add, lens, n, UW[dtype])
 
 
-@pytest.mark.parametrize("scale", [-0.1, 0.0])
-def test_negative_and_zero_scale(scale):
-    banner(f"latent shared scale {scale}")
+@pytest.mark.parametrize("dc,H", [(128, 4), (512, 18)])
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+def test_other_scales(scale, dc, H):
+    """Negative, zero, and large enough that single tokens carry a row and its reference moves often
+    (a score of spread s is off by s times what one of unit spread is)."""
+    banner(f"latent shared scale {scale} {dc} {H}")
     pre, own = [300, 77], [40, 1, 0, 90]
-    q, w, cache, pt, pl, table, ln = _case(pre, own, 2, 4, 64, 32, 64, 128, 32, BF16, seed=31)
+    q, w, cache, pt, pl, table, ln = _case(pre, own, 2, H, 64, 32, 64, dc, 32, BF16, seed=31)
+    if scale == 3.0:
+        o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), scale)
+        want, _ = ol.decode_shared(q, w, cache, pt, pl, table, own, scale)
+        spread = scale * (64 + 32) ** 0.5      # dn + dr products of unit spread
+        assert torch.isfinite(o).all()
+        assert (o.double().cpu() - want).norm() <= 2 * U[BF16] * spread * want.norm()
+        return
     weights = torch.zeros(4, 96, device="cuda")
     o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), scale, weights=weights)
     want, add = ol.decode_shared(q, w, cache, pt, pl, table, own, scale)
@@ -166,11 +187,12 @@ def test_negative_and_zero_scale(scale):
     _weights_within(weights, torch.zeros(4, 96), add, own, 2, UW[BF16])
 
 
-def test_many_rows_behind_one_prefix():
-    """More query rows than the card's workgroups hold at once, and a prefix of many splits."""
-    banner("latent shared many rows")
+@pytest.mark.parametrize("dc", [256, 512])
+def test_many_rows_behind_one_prefix(dc):
+    """Twelve row blocks and a prefix of many splits."""
+    banner(f"latent shared many rows {dc}")
     pre, own = [2600], [3 + 5 * i % 40 for i in range(48)]
-    q, w, cache, pt, pl, table, ln = _case(pre, own, 1, 32, 64, 32, 64, 256, 64, BF16, seed=32)
+    q, w, cache, pt, pl, table, ln = _case(pre, own, 1, 32, 64, 32, 64, dc, 64, BF16, seed=32)
     o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), 0.1)
     want, _ = ol.decode_shared(q, w, cache, pt, pl, table, own, 0.1)
     _rows_within(o, want, U[BF16])
