@@ -259,12 +259,11 @@ struct DTile : LTile<T, W, 16> {
 // query enters as two bf16 numbers, and where `score` is given the scores in powers of
 // two are left there for latent_weigh, a wave's 16 x 16 of them as they lie in its registers.
 template <typename T, int DC, int MT, int NW, bool SCORED>
-__global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
-                                                        const T* __restrict__ cache, const int32_t* __restrict__ table,
-                                                        const int32_t* __restrict__ kv_lens,
-                                                        const int32_t* __restrict__ own, int own_most,
-                                                        float* __restrict__ part, float* __restrict__ stat,
-                                                        float* __restrict__ olat, float* __restrict__ score) {
+__device__ __forceinline__ void split_tokens(const DecDims& d, int b, const T* __restrict__ qa,
+                                             const T* __restrict__ cache, const int32_t* __restrict__ table,
+                                             const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ own,
+                                             int own_most, float* __restrict__ part, float* __restrict__ stat,
+                                             float* __restrict__ olat, float* __restrict__ score) {
   constexpr int DR = 64, W = DC + DR, KS = W / 32, NT = DC / 16, TK = 16 * NW, TW = NW / MT, V = 16 / (int)sizeof(T);
   constexpr int NP = sizeof(T) == 2 ? 2 : 1;    // operands of a probability
   constexpr int NQ = SCORED && sizeof(T) == 2 ? 2 : 1;  // and of a query
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
   __shared__ __attribute__((aligned(1024))) char sk[2 * NW * (SC + SR)];
   __shared__ int32_t spt[kDecPages];
   __shared__ float sm[NW][16], ss[NW][16];
-  const int sp = blockIdx.x, b = blockIdx.z, wv = wave_id(), lane = lane_id(), rw = wv % MT, tw = wv / MT;
+  const int sp = blockIdx.x, wv = wave_id(), lane = lane_id(), rw = wv % MT, tw = wv / MT;
   const int len = dec_len(d, kv_lens, b), each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
   if (first >= len && (sp > 0 || d.slots > 1)) return;  // (one split only: it writes the empty sequence's zeros)
@@ -383,7 +382,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
     if constexpr (SCORED) {
       if (score) {  // (tiles past the end have no place)
         const int tiles = (d.table * d.page + 15) / 16;
-        const int64_t at = (int64_t)b * (gridDim.y * MT) + blockIdx.y * MT + rw;
+        const int64_t at = (int64_t)b * (d.groups * MT) + blockIdx.y * MT + rw;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           const int tile = k0 / 16 + MT * tw + i;
@@ -505,6 +504,34 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
   }
 }
 
+template <typename T, int DC, int MT, int NW, bool SCORED>
+__global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
+                                                        const T* __restrict__ cache, const int32_t* __restrict__ table,
+                                                        const int32_t* __restrict__ kv_lens,
+                                                        const int32_t* __restrict__ own, int own_most,
+                                                        float* __restrict__ part, float* __restrict__ stat,
+                                                        float* __restrict__ olat, float* __restrict__ score) {
+  split_tokens<T, DC, MT, NW, SCORED>(d, blockIdx.z, qa, cache, table, kv_lens, own, own_most, part, stat, olat, score);
+}
+// Prefixes and own tokens in one launch, where both are small (a launch less): grid z
+// below `units` are prefixes.
+template <typename T, int DC, int MT, int NW, bool SCORED>
+__global__ __launch_bounds__(64 * NW) void latent_split_both(DecDims f, DecDims d, int units, const T* __restrict__ qa,
+                                                             const T* __restrict__ cache,
+                                                             const int32_t* __restrict__ prefix_table,
+                                                             const int32_t* __restrict__ prefix_lens,
+                                                             const int32_t* __restrict__ table,
+                                                             const int32_t* __restrict__ kv_lens,
+                                                             float* __restrict__ part, float* __restrict__ stat,
+                                                             float* __restrict__ olat, float* __restrict__ score) {
+  const bool front = (int)blockIdx.z < units;
+  const int own_most = d.table * d.page;
+  if (front) d = f;
+  if ((int)blockIdx.x >= d.splits || (int)blockIdx.y >= d.groups) return;
+  split_tokens<T, DC, MT, NW, SCORED>(d, front ? blockIdx.z : blockIdx.z - units, qa, cache,
+                                      front ? prefix_table : table, front ? prefix_lens : kv_lens,
+                                      front ? kv_lens : nullptr, own_most, part, stat, olat, front ? nullptr : score);
+}
 // o_lat [B n H, dc]: the splits of a row joined.  16 `ways` threads take 64
 // columns of a row, thread group g the splits g, g + ways, ...; the groups join
 // through LDS.  (With few rows and many splits the parts are spread over the card
@@ -552,18 +579,95 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
   store4(olat + row * d.dc + c, x * (sum == 0.f ? 0.f : 1.f / sum));
 }
 
+// weights[b, j] += sum over the query rows of p_j = 2^(s_j - lse), from the scores that
+// latent_split left; the n newest tokens' begin here.  Each token's sum is made by one
+// wave in a fixed order: over the row tiles, then across the 16 rows of a tile.  A
+// workgroup forms the rows' lse from the parts' statistics, sixteen lanes a row (the rows that
+// a tile is padded with, and those that see nothing, get infinity), and goes over
+// kWeighTiles tiles.  Reads 4 bytes a row and token, where latent_split read 1152 a token.
+constexpr int kWeighTiles = 16, kMostRows = 4096;
+struct Weigh {
+  int row_tiles, first;  // row tiles of a sequence; latent_up's grid x where its workgroups begin
+  const float* score;
+  float* weights;
+  int64_t stride;
+};
+__device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, const float* __restrict__ stat,
+                                             const int32_t* __restrict__ kv_lens, float* lse) {
+  const int per = (int)(((int64_t)d.table * d.page + 16 * kWeighTiles - 1) / (16 * kWeighTiles));
+  const int64_t id = ((int64_t)(blockIdx.x - x.first) * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z;
+  const int b = (int)(id / per), chunk = (int)(id % per), rows = d.n * d.H, lane = lane_id();
+  if (b >= d.B) return;
+  const int len = dec_len(d, kv_lens, b);
+  if (16 * kWeighTiles * chunk >= len) return;
+  const Parts ps(d, kv_lens, b);
+  for (int r = threadIdx.x >> 4; r < 16 * x.row_tiles; r += 16) {
+    float m = -INFINITY, sum = 0.f;
+    if (r < rows) {
+      const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r);
+      for (int s = lane & 15; s < ps.all; s += 16) {
+        const float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
+        const float mn = fmaxf(m, a.x);
+        if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + a.y * fast_exp2(a.x - mn);
+        m = mn;
+      }
+    }
+#pragma unroll
+    for (int k = 1; k < 16; k *= 2) {
+      const float mo = __shfl_xor(m, k), so = __shfl_xor(sum, k), mn = fmaxf(m, mo);
+      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + so * fast_exp2(mo - mn);
+      m = mn;
+    }
+    // (a NaN among a row's scores stays one)
+    if ((lane & 15) == 0) lse[r] = sum == 0.f ? INFINITY : m + fast_log2(sum);
+  }
+  __syncthreads();
+  const int tiles = (d.table * d.page + 15) / 16;
+  f32x4 w[kWeighTiles / 4];
+#pragma unroll
+  for (int i = 0; i < kWeighTiles / 4; ++i) w[i] = zero4();
+  const int t0 = kWeighTiles * chunk + wave_id();
+#pragma unroll 2
+  for (int g = 0; g < x.row_tiles; ++g) {
+    const float z = lse[16 * g + (lane & 15)];
+    const float* sc = x.score + ((((int64_t)b * x.row_tiles + g) * tiles) * 64 + lane) * 4;
+    f32x4 s[kWeighTiles / 4];
+#pragma unroll
+    for (int i = 0; i < kWeighTiles / 4; ++i)  // (tiles past the last repeat it)
+      s[i] = *reinterpret_cast<const f32x4*>(sc + (int64_t)min(t0 + 4 * i, (len - 1) / 16) * 256);
+#pragma unroll
+    for (int i = 0; i < kWeighTiles / 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w[i][r] += fast_exp2(s[i][r] - z);
+  }
+#pragma unroll
+  for (int i = 0; i < kWeighTiles / 4; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int k = 1; k < 16; k *= 2) w[i][r] += __shfl_xor(w[i][r], k);
+    const int j = 16 * (t0 + 4 * i) + tile_row(lane & 3);
+    const float add = (lane & 2) ? ((lane & 1) ? w[i][3] : w[i][2]) : ((lane & 1) ? w[i][1] : w[i][0]);
+    float* to = x.weights + b * x.stride + j;
+    if ((lane & 15) < 4 && j < len) *to = (j < len - d.n ? *to : 0.f) + add;
+  }
+}
+
 // o: 16 query tokens of a head times 64 rows of its value projection a
 // workgroup, 16 a wave.  With JOIN it joins the splits itself (up to kUpSplits of
 // them): where that is a few dozen loads a thread, a launch less is worth more than
 // the same parts read once instead of dv / 64 times.  Latency: 5 to 8 us without the join.
+// With SCORED the workgroups from grid x `x.first` on gather the tokens' weights instead.
 constexpr int kUpSplits = 64;
-template <typename T, bool JOIN>
+template <typename T, bool JOIN, bool SCORED>
 __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict__ w_kv, const float* __restrict__ olat,
                                                  const float* __restrict__ part, const float* __restrict__ stat,
-                                                 const int32_t* __restrict__ kv_lens, T* __restrict__ o) {
+                                                 const int32_t* __restrict__ kv_lens, T* __restrict__ o, Weigh x) {
   constexpr int V = 16 / (int)sizeof(T), LD = 512 + V, PARTS = sizeof(T) == 2 ? 2 : 1, KS = 16;
   __shared__ __attribute__((aligned(16))) T so[PARTS][16 * LD];
   __shared__ float sw[JOIN ? 16 : 1][kUpSplits];
+  static_assert(sizeof(so) >= (kMostRows + 64) * sizeof(float), "a float for each row of a sequence's row tiles");
+  if (SCORED && (int)blockIdx.x >= x.first) return latent_weigh(d, x, stat, kv_lens, reinterpret_cast<float*>(so));
   const int h = blockIdx.x, v0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, KP = (d.dc + 31) / 32 * 32;
   const int vr = v0 + 16 * wave_id(), rows = d.n * d.H;
   const T* w = w_kv + ((int64_t)h * (d.dn + d.dv) + d.dn + min(vr + (lane_id() & 15), d.dv - 1)) * d.dc;
@@ -638,62 +742,6 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
   if (r < R && v < d.dv) store4(o + ((int64_t)r * d.H + h) * d.dv + v, acc);
 }
 
-// weights[b, j] += sum over the query rows of p_j = 2^(s_j - lse), from the scores that
-// latent_split left; the n newest tokens' begin here.  Each token's sum is made by one
-// wave in a fixed order: over the row tiles, then across the 16 rows of a tile.  A
-// workgroup forms the rows' lse from the parts' statistics (the rows that a tile is padded
-// with, and those that see nothing, get infinity) and goes over kWeighTiles tiles.
-constexpr int kWeighTiles = 16;
-__global__ __launch_bounds__(256) void latent_weigh(DecDims d, int row_tiles, const float* __restrict__ score,
-                                                    const float* __restrict__ stat,
-                                                    const int32_t* __restrict__ kv_lens, int64_t stride,
-                                                    float* __restrict__ weights) {
-  __shared__ float lse[4096 + 64];
-  const int b = blockIdx.y, rows = d.n * d.H, len = dec_len(d, kv_lens, b), lane = lane_id();
-  if (16 * kWeighTiles * (int)blockIdx.x >= len) return;
-  const Parts ps(d, kv_lens, b);
-  for (int r = threadIdx.x; r < 16 * row_tiles; r += 256) {
-    float m = -INFINITY, sum = 0.f;
-    if (r < rows) {
-      const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r);
-      for (int s = 0; s < ps.all; ++s) {
-        const int64_t a = 2 * (int64_t)ps.slot(s) * rows;
-        const float ms = st[a], mn = fmaxf(m, ms);
-        if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + st[a + 1] * fast_exp2(ms - mn);
-        m = mn;
-      }
-    }
-    // (a NaN among a row's scores stays one)
-    lse[r] = sum == 0.f ? INFINITY : m + fast_log2(sum);
-  }
-  __syncthreads();
-  const int tiles = (d.table * d.page + 15) / 16;
-#pragma unroll
-  for (int i = 0; i < kWeighTiles / 4; ++i) {
-    const int tile = kWeighTiles * blockIdx.x + 4 * i + wave_id();
-    if (16 * tile >= len) break;
-    f32x4 x = zero4();
-#pragma unroll 4
-    for (int g = 0; g < row_tiles; ++g) {
-      const f32x4 s = *reinterpret_cast<const f32x4*>(
-          score + ((((int64_t)b * row_tiles + g) * tiles + tile) * 64 + lane) * 4);
-      const float z = lse[16 * g + (lane & 15)];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] += fast_exp2(s[r] - z);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int k = 1; k < 16; k *= 2) x[r] += __shfl_xor(x[r], k);
-    if ((lane & 15) < 4) {
-      const int j = 16 * tile + tile_row(lane & 3);
-      const float add = (lane & 2) ? ((lane & 1) ? x[3] : x[2]) : ((lane & 1) ? x[1] : x[0]);
-      float* w = weights + b * stride + j;
-      if (j < len) *w = (j < len - d.n ? *w : 0.f) + add;
-    }
-  }
-}
-
 // ------------------------------------------------------------------ host
 static int app_check(const atomic_latent_append_args* a) {
   if (!a) return ATOMIC_ERR_NULL;
@@ -748,12 +796,12 @@ static int dec_row_tiles(int64_t rows, int dtype) {
   return rows <= 16 ? 1 : rows <= 32 || dtype != ATOMIC_BF16 ? 2 : 4;
 }
 
-static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table) {
+static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table, int mt) {
   DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, table,
             a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]},
             share, 0, 0, 0, 1, 0, 0, nullptr};
   const int64_t rows = (int64_t)share * d.n * d.H;
-  const int mt = dec_row_tiles(rows, a->dtype), rt = 16 * mt, tile = mt == 4 ? 64 : 32;
+  const int rt = 16 * mt, tile = mt == 4 ? 64 : 32;
   d.groups = (int)((rows + rt - 1) / rt);
   // As many workgroups as the card holds at once if every sequence were as long as
   // its table (the host does not know the lengths, so a table wider than the sequences
@@ -774,16 +822,30 @@ static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share
 // A call's launches over the sequences' own tokens and over the prefixes (with `front.splits` 0 there is none).
 struct DecPlan {
   DecDims own, front;
-  bool many;  // the prefixes' rows are many: latent_prefix takes them
+  int own_tiles, front_tiles;  // row tiles of a workgroup
+  bool many;                   // the prefixes' rows are many: latent_prefix takes them
+  bool both;                   // one launch for both
 };
 static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, bool scored) {
-  DecPlan p{dec_dims(a, a->batch, 1, a->table_pages), {}, false};
+  DecPlan p{};
+  p.own_tiles = dec_row_tiles((int64_t)a->tokens * a->heads, a->dtype);
+  p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
   if (!prefixes) return p;
-  p.front = dec_dims(a, prefixes, a->batch / prefixes, prefix_pages);
+  const int share = a->batch / prefixes;
+  p.front_tiles = dec_row_tiles((int64_t)share * a->tokens * a->heads, a->dtype);
+  p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles);
   DecDims many = p.front;
   p.many = !scored && a->dtype == ATOMIC_BF16 && a->dc > 256 && prefix_plan(many, prefixes) &&
            many.splits + p.own.splits > 1;
   if (p.many) p.front = many;
+  // One launch costs less than what the own tokens lose by the prefix's row tiles while they
+  // are few.
+  p.both = !p.many && p.front_tiles <= 2 && p.front.splits && p.own.splits && a->batch + prefixes <= 65535 &&
+           (int64_t)a->batch * a->table_pages * a->page <= 32768;
+  if (p.both && p.own_tiles != p.front_tiles) {
+    p.own_tiles = p.front_tiles;
+    p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
+  }
   p.own.slot0 = p.front.splits;
   p.own.slots = p.front.slots = p.own.splits + p.front.splits;
   p.own.pre_share = p.front.share;
@@ -804,10 +866,11 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 struct DecSpace {
   size_t qa, olat, stat, part, score, all;
 };
-static DecSpace dec_space(const DecDims& d, int dtype, bool scored) {
+static DecSpace dec_space(const DecPlan& p, int dtype, bool scored) {
+  const DecDims& d = p.own;
   const size_t rows = (size_t)d.B * d.n * d.H, es = dtype == ATOMIC_BF16 ? 2 : 4;
   const size_t parts = d.slots > 1 ? rows * d.slots : 0;  // one split needs no parts
-  const size_t tiles = (size_t)d.groups * dec_row_tiles((int64_t)d.n * d.H, dtype) * (((size_t)d.table * d.page + 15) / 16);
+  const size_t tiles = (size_t)d.groups * p.own_tiles * (((size_t)d.table * d.page + 15) / 16);
   DecSpace s;
   s.qa = 0;
   s.olat = s.qa + up256(rows * (d.dc + d.dr) * es * (scored && es == 2 ? 2 : 1));
@@ -849,22 +912,6 @@ extern "C" int atomic_latent_append(const atomic_latent_append_args* a, const vo
   });
 }
 
-template <typename T, int DC, bool SCORED>
-static void launch_split(const DecDims& d, int units, int dtype, hipStream_t st, const T* qa, const void* cache,
-                         const int32_t* table, const int32_t* lens, const int32_t* own, int own_most, float* part,
-                         float* stat, float* olat, float* score) {
-  const dim3 grid((unsigned)d.splits, (unsigned)d.groups, (unsigned)units);
-  auto go = [&](auto m) {
-    constexpr int NW = decltype(m)::value == 4 ? 4 : 2;
-    hipLaunchKernelGGL((latent_split<T, DC, decltype(m)::value, NW, SCORED>), grid, dim3(64 * NW), 0, st, d, qa,
-                       (const T*)cache, table, lens, own, own_most, part, stat, olat, score);
-  };
-  const int mt = dec_row_tiles((int64_t)d.share * d.n * d.H, dtype);
-  if (mt == 1) go(IntC<1>());
-  else if (mt == 2) go(IntC<2>());
-  else if constexpr (sizeof(T) == 2) go(IntC<4>());
-}
-
 struct DecPtrs {
   const void *q, *w_kv, *cache;
   const int32_t *prefix_table, *prefix_lens, *table, *lens;
@@ -874,46 +921,85 @@ struct DecPtrs {
   void *o, *ws;
 };
 
+// Where a call's parts lie in its workspace.
+template <typename T> struct DecParts {
+  T* qa;
+  float *olat, *stat, *part, *score;
+};
+
+// latent_split over the prefixes (`front`) or the own tokens, or both where the plan says so.
+template <typename T, int DC, bool SCORED>
+static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStream_t st, const DecPtrs& p,
+                         const DecParts<T>& x) {
+  const DecDims &d = plan.own, &f = plan.front;
+  const int own_most = d.table * d.page;
+  auto go = [&](auto m) {
+    constexpr int MT = decltype(m)::value, NW = MT == 4 ? 4 : 2;
+    if constexpr (MT <= 2) {
+      if (plan.both) {
+        const dim3 grid((unsigned)(d.splits > f.splits ? d.splits : f.splits),
+                        (unsigned)(d.groups > f.groups ? d.groups : f.groups), (unsigned)(prefixes + d.B));
+        hipLaunchKernelGGL((latent_split_both<T, DC, MT, NW, SCORED>), grid, dim3(64 * NW), 0, st, f, d, prefixes, x.qa,
+                           (const T*)p.cache, p.prefix_table, p.prefix_lens, p.table, p.lens, x.part, x.stat, x.olat,
+                           x.score);
+        return;
+      }
+    }
+    if (front)
+      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED>),
+                         dim3((unsigned)f.splits, (unsigned)f.groups, (unsigned)prefixes), dim3(64 * NW), 0, st, f, x.qa,
+                         (const T*)p.cache, p.prefix_table, p.prefix_lens, p.lens, own_most, x.part, x.stat, x.olat,
+                         (float*)nullptr);
+    else
+      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED>),
+                         dim3((unsigned)d.splits, (unsigned)d.groups, (unsigned)d.B), dim3(64 * NW), 0, st, d, x.qa,
+                         (const T*)p.cache, p.table, p.lens, (const int32_t*)nullptr, 0, x.part, x.stat, x.olat, x.score);
+  };
+  const int mt = front ? plan.front_tiles : plan.own_tiles;
+  if (mt == 1) go(IntC<1>());
+  else if (mt == 2) go(IntC<2>());
+  else if constexpr (sizeof(T) == 2) go(IntC<4>());
+}
+
 template <typename T, bool SCORED>
 static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, const DecPtrs& p,
                    hipStream_t st) {
   DecPlan plan = dec_plan(a, prefixes, prefix_pages, SCORED);
   plan.own.pre_lens = p.prefix_lens;
   const DecDims& d = plan.own;
-  const DecSpace at = dec_space(d, a->dtype, SCORED);
+  const DecSpace at = dec_space(plan, a->dtype, SCORED);
   Launch L{a->profile, st};
   char* ws = (char*)p.ws;
-  T* qa = (T*)(ws + at.qa);
-  float *olat = (float*)(ws + at.olat), *stat = (float*)(ws + at.stat), *part = (float*)(ws + at.part);
-  float* score = SCORED ? (float*)(ws + at.score) : nullptr;
+  const DecParts<T> x{(T*)(ws + at.qa), (float*)(ws + at.olat), (float*)(ws + at.stat), (float*)(ws + at.part),
+                      SCORED ? (float*)(ws + at.score) : nullptr};
   const unsigned rt = (unsigned)((d.B * d.n + 15) / 16);
   int rc = L("latent_absorb", [&] {
     hipLaunchKernelGGL((latent_absorb<T, SCORED && sizeof(T) == 2>),
                        dim3((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt), dim3(256), 0, st, d, (const T*)p.q,
-                       (const T*)p.w_kv, p.lens, p.cos, p.sin, qa);
+                       (const T*)p.w_kv, p.lens, p.cos, p.sin, x.qa);
   });
   if (rc) return rc;
-  auto split = [&](const DecDims& x, int units, const int32_t* table, const int32_t* lens, const int32_t* own,
-                   int own_most, float* sc) {
-    if (d.dc <= 256)
-      launch_split<T, 256, SCORED>(x, units, a->dtype, st, qa, p.cache, table, lens, own, own_most, part, stat, olat, sc);
-    else
-      launch_split<T, 512, SCORED>(x, units, a->dtype, st, qa, p.cache, table, lens, own, own_most, part, stat, olat, sc);
+  auto split = [&](bool front) {
+    if (d.dc <= 256) launch_split<T, 256, SCORED>(plan, prefixes, front, st, p, x);
+    else launch_split<T, 512, SCORED>(plan, prefixes, front, st, p, x);
   };
-  if (plan.front.splits) {
+  if (plan.both) {
+    rc = L("latent_split_both", [&] { split(true); });
+    if (rc) return rc;
+  }
+  if (plan.front.splits && !plan.both) {
     rc = L(plan.many ? "latent_prefix" : "latent_split (prefix)", [&] {
-      const int own_most = d.table * d.page;
       if constexpr (sizeof(T) == 2 && !SCORED) {
         if (plan.many)
-          return launch_prefix(plan.front, prefixes, st, qa, p.cache, p.prefix_table, p.prefix_lens, p.lens, own_most,
-                               part, stat);
+          return launch_prefix(plan.front, prefixes, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
+                               d.table * d.page, x.part, x.stat);
       }
-      split(plan.front, prefixes, p.prefix_table, p.prefix_lens, p.lens, own_most, nullptr);
+      split(true);
     });
     if (rc) return rc;
   }
-  if (d.splits) {
-    rc = L("latent_split", [&] { split(d, d.B, p.table, p.lens, nullptr, 0, score); });
+  if (d.splits && !plan.both) {
+    rc = L("latent_split", [&] { split(false); });
     if (rc) return rc;
   }
   const bool joins = dec_up_joins(d);
@@ -922,32 +1008,31 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     while (ways < 16 && 4 * ways < d.slots) ways *= 2;
     const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
     rc = L("latent_join", [&] {
-      hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, part,
-                         stat, p.lens, olat);
+      hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, x.part,
+                         x.stat, p.lens, x.olat);
     });
     if (rc) return rc;
   }
-  rc = L("latent_up", [&] {
+  const Weigh wx{d.groups * plan.own_tiles, d.H, x.score, p.weights, p.weights_stride};
+  unsigned more = 0;  // the weights' workgroups
+  const unsigned gy = (unsigned)((d.dv + 63) / 64);
+  if (SCORED && d.splits) {
+    const int64_t per = ((int64_t)d.table * d.page + 16 * kWeighTiles - 1) / (16 * kWeighTiles);
+    more = (unsigned)((per * d.B + gy * rt - 1) / (gy * rt));
+  }
+  return L("latent_up", [&] {
     auto go = [&](auto j) {
-      hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0>),
-                         dim3((unsigned)d.H, (unsigned)((d.dv + 63) / 64), rt), dim3(256), 0, st, d,
-                         (const T*)p.w_kv, olat, part, stat, p.lens, (T*)p.o);
+      hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0, SCORED>), dim3((unsigned)d.H + more, gy, rt), dim3(256),
+                         0, st, d, (const T*)p.w_kv, x.olat, x.part, x.stat, p.lens, (T*)p.o, wx);
     };
     if (joins) go(IntC<1>());
     else go(IntC<0>());
-  });
-  if (rc || !SCORED || !d.splits) return rc;
-  return L("latent_weigh", [&] {
-    const int64_t tokens = (int64_t)d.table * d.page;
-    hipLaunchKernelGGL(latent_weigh, dim3((unsigned)((tokens + 16 * kWeighTiles - 1) / (16 * kWeighTiles)), (unsigned)d.B),
-                       dim3(256), 0, st, d, d.groups * dec_row_tiles((int64_t)d.n * d.H, a->dtype), score, stat, p.lens,
-                       p.weights_stride, p.weights);
   });
 }
 
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(a, 0, 0, false).own, a->dtype, false).all;
+  return dec_space(dec_plan(a, 0, 0, false), a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -968,7 +1053,7 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
 
 extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
   if (shared_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0).own, a->dec.dtype, a->scored != 0).all;
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0), a->dec.dtype, a->scored != 0).all;
 }
 
 extern "C" int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,

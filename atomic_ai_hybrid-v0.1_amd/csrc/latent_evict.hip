@@ -33,59 +33,78 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 constexpr int kDigit = 11, kBins = 1 << kDigit;  // 32 bits as 11, 11 and 10
 constexpr int kEvictKeys = 1 << 15;              // keys that LDS holds (128 KB)
+constexpr int kEvictList = 1 << 10;              // rows that move, as LDS holds them
 
-// Exclusive sum over the workgroup's waves; every thread of a wave gives the same x.
-// `tmp` is not read any more when the call returns.
-__device__ __forceinline__ int waves_below(int x, int* tmp, int& all) {
-  if (lane_id() == 0) tmp[wave_id()] = x;
+// Exclusive sums of x and y over the workgroup's waves; every thread of a wave gives the same.
+// `tmp` may be written again behind the caller's next barrier but one.
+__device__ __forceinline__ void waves_below(int& x, int& y, int2* tmp) {
+  if (lane_id() == 0) tmp[wave_id()] = make_int2(x, y);
   __syncthreads();
-  int below = 0, sum = 0;
+  x = y = 0;
 #pragma unroll
   for (int w = 0; w < kEvictWaves; ++w) {
-    if (w < wave_id()) below += tmp[w];
-    sum += tmp[w];
+    const int2 z = tmp[w];
+    x += w < wave_id() ? z.x : 0;
+    y += w < wave_id() ? z.y : 0;
   }
-  __syncthreads();
-  all = sum;
-  return below;
 }
 
 // One sequence.  Its rows are divided over the waves in runs, so that ranks in the order of the
-// rows are a wave's own count and the counts of the waves before it.  `keys` [width] a
-// sequence hold what LDS has no room for (LDS = false), `movers` [keep] the kept rows
-// past the budget.
+// rows are a wave's own count and the counts of the waves before it; a thread has eight rows in
+// flight at a time.  `key_space` [width] a sequence holds the keys that LDS has no room for
+// (LDS = false), `list_space` [keep] pairs of a hole and the kept row that goes there, past
+// the first kEvictList of them.
+//
+// Bound by latency and, in a long table, by what one CU can read.
 template <bool LDS>
 __global__ __launch_bounds__(kEvictThreads) void evict_select(EvictDims d, const int32_t* kv_lens, const float* weights,
                                                               const int32_t* order, int32_t* lens_out, float* w_out,
                                                               int32_t* o_out, int32_t* __restrict__ source,
                                                               uint32_t* __restrict__ key_space,
-                                                              int32_t* __restrict__ mover_space) {
+                                                              int2* __restrict__ list_space) {
   __shared__ uint32_t skeys[LDS ? kEvictKeys : 1];
   __shared__ int hist[kBins];
-  __shared__ int tmp[kEvictWaves], red[3], found[2];
+  __shared__ int2 list[kEvictList];
+  __shared__ int2 tmp[2][kEvictWaves];
+  __shared__ int red[3], found[3];
   const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
   const int len = (int)min((int64_t)max(kv_lens[b], 0), (int64_t)d.table * d.page), left = min(len, d.keep);
   const float* w = weights + b * d.ws;
   const int32_t* o = order + b * d.os;
   uint32_t* keys = LDS ? skeys : key_space + (int64_t)b * d.width;
-  int32_t* movers = mover_space + (int64_t)b * d.keep;
+  int2* more = list_space + (int64_t)b * d.keep;
   source += (int64_t)b * d.keep;
   w_out += b * d.wos;
   o_out += b * d.oos;
 
+  const int run = ((len + kEvictThreads - 1) / kEvictThreads) * 64;  // rows of a wave, whole lanes
+  const int j0 = min(len, wave_id() * run), j1 = min(len, j0 + run);
+  // f(i, j): eight times 64 rows of this wave, all lanes together; load(i, j) of them all before
+  auto rows = [&](auto load, auto f) {
+    for (int j = j0 + lane; j - lane < j1; j += 512) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) load(i, min(j + 64 * i, j1 - 1));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j - lane + 64 * i < j1) f(i, j + 64 * i, j + 64 * i < j1);
+    }
+  };
+
   // what no eviction has seen: from row `first` to row `last`; the largest order of the others
   if (tid < 3) red[tid] = tid ? -1 : INT32_MAX;
+  for (int i = tid; i < kBins; i += kEvictThreads) hist[i] = 0;
   __syncthreads();
-  int first = INT32_MAX, last = -1, top = -1;
-  for (int j = tid; j < len; j += kEvictThreads) {
-    const int x = o[j];
-    if (x < 0) {
-      first = min(first, j);
-      last = max(last, j);
-    } else {
-      top = max(top, x);
-    }
-  }
+  int first = INT32_MAX, last = -1, top = -1, ages[8];
+  rows([&](int i, int j) { ages[i] = o[j]; },
+       [&](int i, int j, bool here) {
+         const int x = ages[i];
+         if (here && x < 0) {
+           first = min(first, j);
+           last = max(last, j);
+         } else if (here) {
+           top = max(top, x);
+         }
+       });
 #pragma unroll
   for (int k = 32; k; k >>= 1) {
     first = min(first, __shfl_xor(first, k));
@@ -102,39 +121,51 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select(EvictDims d, const
   last = red[1];
   top = red[2];
   const int64_t newest = last < 0 ? top : (int64_t)top + 1 + last - first;
-  auto age = [&](int j) {  // the order of row j's token
-    const int x = o[j];
-    return x >= 0 ? (int64_t)x : (int64_t)top + 1 + j - first;
+  // the order of row j's token where x stands there
+  auto age = [&](int x, int j) { return x >= 0 ? (int64_t)x : (int64_t)top + 1 + j - first; };
+  auto put = [&](int to, float x, int64_t a, int from) {
+    source[to] = from;
+    w_out[to] = x;
+    o_out[to] = (int)min(a, (int64_t)INT32_MAX);
   };
-
-  if (len > d.keep) {
-    const int run = ((len + kEvictThreads - 1) / kEvictThreads) * 64;  // rows of a wave, whole lanes
-    const int j0 = min(len, wave_id() * run), j1 = min(len, j0 + run);
-    // f(row, here): all lanes of the wave together
-    auto rows = [&](auto f) {
-      for (int j = j0 + lane; j - lane < j1; j += 64) f(j, j < j1);
-    };
+  float ws[8];
+  if (len <= d.keep) {
+    rows(
+        [&](int i, int j) {
+          ages[i] = o[j];
+          ws[i] = w[j];
+        },
+        [&](int i, int j, bool here) {
+          if (here) put(j, ws[i], age(ages[i], j), j);
+        });
+  } else {
     // the keep-th largest key, digit by digit from the top: `low` its digits so far, `need`
-    // how many keys that begin with them are kept
-    uint32_t low = 0;
+    // how many of the `many` keys that begin with them are kept
+    uint32_t low = 0, ks[8];
     int need = d.keep, many = 0, shift = 32;
+    auto get = [&](int i, int j) { ks[i] = keys[j]; };
     for (int pass = 0; pass < 3; ++pass) {
       const int bits = pass < 2 ? kDigit : 32 - 2 * kDigit;
-      for (int i = tid; i < kBins; i += kEvictThreads) hist[i] = 0;
-      __syncthreads();
-      rows([&](int j, bool here) {
-        if (!here) return;
-        uint32_t k;
-        if (pass == 0) {
-          const int64_t a = age(j);
-          k = a < d.sinks || a > newest - d.recent ? kSafe : weight_key(w[j]);
-          keys[j] = k;
-        } else {
-          k = keys[j];
-          if ((k >> shift) != (low >> shift)) return;
-        }
-        atomicAdd(&hist[(k >> (shift - bits)) & ((1 << bits) - 1)], 1);
-      });
+      auto count = [&](uint32_t k) { atomicAdd(&hist[(k >> (shift - bits)) & ((1 << bits) - 1)], 1); };
+      if (pass == 0) {
+        rows(
+            [&](int i, int j) {
+              ages[i] = o[j];
+              ws[i] = w[j];
+            },
+            [&](int i, int j, bool here) {
+              const int64_t a = age(ages[i], j);
+              const uint32_t k = a < d.sinks || a > newest - d.recent ? kSafe : weight_key(ws[i]);
+              if (here) {
+                keys[j] = k;
+                count(k);
+              }
+            });
+      } else {
+        rows(get, [&](int i, int, bool here) {
+          if (here && (ks[i] >> shift) == (low >> shift)) count(ks[i]);
+        });
+      }
       __syncthreads();
       // keys in the bins above each bin: two bins a thread, from the top
       const int hi = kBins - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
@@ -144,31 +175,30 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select(EvictDims d, const
         const int y = __shfl_up(sum, k);
         if (lane >= k) sum += y;
       }
-      int all;
-      const int above = waves_below(__shfl(sum, 63), tmp, all) + sum - c0 - c1;
-      if (above < need && need <= above + c0) {
-        found[0] = hi;
-        found[1] = above;
-      } else if (above + c0 < need && need <= above + c0 + c1) {
-        found[0] = hi - 1;
-        found[1] = above + c0;
+      int above = __shfl(sum, 63), none = 0;
+      waves_below(above, none, tmp[0]);
+      above += sum - c0 - c1;
+      if (above < need && need <= above + c0 + c1) {
+        const bool lower = need > above + c0;
+        found[0] = lower ? hi - 1 : hi;
+        found[1] = lower ? above + c0 : above;
+        found[2] = lower ? c1 : c0;
       }
+      hist[hi] = hist[hi - 1] = 0;
       __syncthreads();
       shift -= bits;
       low |= (uint32_t)found[0] << shift;
       need -= found[1];
-      many = hist[found[0]];
-      __syncthreads();
+      many = found[2];
       if (many == need) break;  // all that begin with `low` are kept: the last digits do not matter
     }
     // `need` of the keys that begin with `low` are kept, the lowest rows first
-    int equal = 0, all;
+    int equal = 0, none = 0;
     if (many != need) {
-      rows([&](int j, bool here) { equal += __popcll(__ballot(here && keys[j] == low)); });
-      equal = waves_below(equal, tmp, all);
+      rows(get, [&](int i, int, bool here) { equal += __popcll(__ballot(here && ks[i] == low)); });
+      waves_below(equal, none, tmp[1]);
     }
-    auto kept = [&](int j, bool here, int& eq) {
-      const uint32_t k = here ? keys[j] : 0;
+    auto kept = [&](uint32_t k, bool here, int& eq) {
       if (many == need) return here && k >= low;
       const uint64_t same = __ballot(here && k == low);
       const bool stay = here && (k > low || (k == low && eq + lanes_below(same) < need));
@@ -176,38 +206,42 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select(EvictDims d, const
       return stay;
     };
     int eq = equal, holes = 0, moving = 0;
-    rows([&](int j, bool here) {
-      const bool stay = kept(j, here, eq);
+    rows(get, [&](int i, int j, bool here) {
+      const bool stay = kept(ks[i], here, eq);
       holes += __popcll(__ballot(here && !stay && j < d.keep));
       moving += __popcll(__ballot(stay && j >= d.keep));
     });
-    holes = waves_below(holes, tmp, all);
-    moving = waves_below(moving, tmp, all);
+    waves_below(holes, moving, tmp[0]);
     eq = equal;
-    rows([&](int j, bool here) {
-      const bool stay = kept(j, here, eq);
-      const uint64_t goes = __ballot(stay && j >= d.keep), free = __ballot(here && !stay && j < d.keep);
-      if (stay && j >= d.keep) movers[moving + lanes_below(goes)] = j;
-      if (here && j < d.keep) source[j] = stay ? j : ~(holes + lanes_below(free));  // a hole: its rank
-      moving += __popcll(goes);
-      holes += __popcll(free);
-    });
+    rows(
+        [&](int i, int j) {
+          get(i, j);
+          ages[i] = o[j];
+          ws[i] = w[j];
+        },
+        [&](int i, int j, bool here) {
+          const bool stay = kept(ks[i], here, eq), goes = stay && j >= d.keep, free = here && !stay && j < d.keep;
+          const uint64_t gm = __ballot(goes), fm = __ballot(free);
+          if (goes || free) {
+            const int r = goes ? moving + lanes_below(gm) : holes + lanes_below(fm);
+            int* at = (int*)(r < kEvictList ? list + r : more + r);
+            at[goes] = j;
+          } else if (stay) {
+            put(j, ws[i], age(ages[i], j), j);
+          }
+          moving += __popcll(gm);
+          holes += __popcll(fm);
+        });
+    // as many rows go as there are holes: the last wave's count
+    if (wave_id() == kEvictWaves - 1 && lane == 0) found[0] = holes;
     __threadfence_block();
     __syncthreads();
-  }
-  // the new state below the budget; then, when nothing past it is read any more, the rest
-  for (int j = tid; j < left; j += kEvictThreads) {
-    int from = j;
-    if (len > d.keep) {
-      from = source[j];
-      if (from < 0) from = movers[~from];
+    for (int r = tid; r < found[0]; r += kEvictThreads) {
+      const int2 x = r < kEvictList ? list[r] : more[r];
+      put(x.x, w[x.y], age(o[x.y], x.y), x.y);
     }
-    const float x = w[from];
-    const int a = (int)min(age(from), (int64_t)INT32_MAX);
-    source[j] = from;
-    w_out[j] = x;
-    o_out[j] = a;
   }
+  // past the length, when nothing there is read any more
   __syncthreads();
   for (int j = left + tid; j < d.width; j += kEvictThreads) {
     w_out[j] = 0.f;
@@ -269,7 +303,7 @@ using namespace ah;
 extern "C" size_t atomic_latent_evict_workspace_size(const atomic_latent_evict_args* a) {
   if (evict_check(a) != ATOMIC_OK) return 0;
   const size_t keys = evict_most(a) > kEvictKeys ? (size_t)a->batch * a->width : 0;
-  return (keys + (size_t)a->batch * a->keep) * 4;
+  return (keys + 2 * (size_t)a->batch * a->keep) * 4;
 }
 
 extern "C" int atomic_latent_evict(const atomic_latent_evict_args* a, void* cache, const int32_t* page_table,
@@ -288,15 +322,15 @@ extern "C" int atomic_latent_evict(const atomic_latent_evict_args* a, void* cach
                     a->weights_out_stride, a->order_out_stride};
   const hipStream_t st = (hipStream_t)stream;
   Launch L{a->profile, st};
-  int32_t* movers = (int32_t*)workspace;
-  uint32_t* keys = (uint32_t*)workspace + (size_t)a->batch * a->keep;
+  int2* list = (int2*)workspace;
+  uint32_t* keys = (uint32_t*)(list + (size_t)a->batch * a->keep);
   int rc = L("evict_select", [&] {
     if (evict_most(a) <= kEvictKeys)
       hipLaunchKernelGGL(evict_select<true>, dim3((unsigned)d.B), dim3(kEvictThreads), 0, st, d, kv_lens, weights,
-                         order, kv_lens_out, weights_out, order_out, source, keys, movers);
+                         order, kv_lens_out, weights_out, order_out, source, keys, list);
     else
       hipLaunchKernelGGL(evict_select<false>, dim3((unsigned)d.B), dim3(kEvictThreads), 0, st, d, kv_lens, weights,
-                         order, kv_lens_out, weights_out, order_out, source, keys, movers);
+                         order, kv_lens_out, weights_out, order_out, source, keys, list);
   });
   if (rc || evict_most(a) <= a->keep) return rc;
   return L("evict_move", [&] {

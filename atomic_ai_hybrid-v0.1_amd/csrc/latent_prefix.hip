@@ -3,6 +3,17 @@
 // instructions bound it (1900 operations a byte), not the cache's bytes.
 #include "latent_decode.hpp"
 
+#ifndef XG
+#define XG 2
+#define XL 2
+#endif
+#ifndef YG
+#define YG 2
+#define YL 2
+#endif
+#ifndef YV
+#define YV 4
+#endif
 namespace ah {
 
 // Keep a value in the accumulator half of the register file.
@@ -102,8 +113,19 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
     uint32_t ac = l0 + buf * STAGE + br, ar = l0 + buf * STAGE + SC + bp;
     asm volatile("" : "+v"(ac), "+v"(ar));
     s = zero16();
-    in_groups<KS, 2, 2, 0, frag>([&](int t) { return t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC)); },
-                                 [&](int t, frag a) { s = M32<bf16>::mma(a, qf[t], s); }, work);
+#ifdef CH2
+    f32x16 s1 = zero16();
+#endif
+    in_groups<KS, XG, XL, 0, frag>([&](int t) { return t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC)); },
+                                 [&](int t, frag a) {
+#ifdef CH2
+                                   if (t & 1) s1 = M32<bf16>::mma(a, qf[t], s1);
+                                   else
+#endif
+                                   s = M32<bf16>::mma(a, qf[t], s); }, work);
+#ifdef CH2
+    s += s1;
+#endif
     asm volatile("" : "+v"(s));
     if (first + k0 + TK > min(end, least)) {
       const int lim = min(end, seen) - first - k0 - 4 * (lane >> 5);
@@ -129,7 +151,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   auto values = [&](int buf, auto work) {
     uint32_t av = l0 + buf * STAGE + bc;
     asm volatile("" : "+v"(av));
-    in_groups<2 * NT, 2, 2, 4, frag>([&](int j) { return LC::col(av, 16 * (j / NT), 32 * (j % NT)); },
+    in_groups<2 * NT, YG, YL, YV, frag>([&](int j) { return LC::col(av, 16 * (j / NT), 32 * (j % NT)); },
                                      [&](int j, frag a) { acc[j % NT] = M32<bf16>::mma(a, p[j / NT], acc[j % NT]); },
                                      work);
 #pragma unroll
