@@ -76,12 +76,27 @@ def test_evict_keeps_what_the_oracle_keeps(lens, page, row, keep, sinks, recent,
     _check(_state(lens, page, row, dtype, seed=keep + row, settled=settled), keep, sinks, recent)
 
 
-def test_more_keys_than_lds_holds():
-    """Tables past 32768 tokens keep their keys in the workspace."""
+@pytest.mark.parametrize("most,keep", [(2048, 1900), (2049, 1900), (4096, 3000), (4097, 4000), (8192, 8063), (8192, 8064),
+                                       (8193, 5000), (8193, 8100), (10240, 2048), (10240, 6144), (12000, 11999), (9000, 1)])
+def test_around_the_limits_of_table_and_budget(most, keep):
+    """Tables that one workgroup takes and longer ones, few and many rows to move, budgets that end at a chunk's end."""
+    banner(f"latent evict table {most} keep {keep}")
+    _check(_state([most, most - 1, keep, keep + 1, most // 2], 1, 16, BF16, seed=most + keep, settled=min(keep, 700)), keep,
+           min(3, keep), min(keep - min(3, keep), 150))
+
+
+def test_long_tables():
+    """Many workgroups a sequence, ties across them, sequences that fit among those that do not."""
     banner("latent evict long tables")
     _check(_state([40000, 33000, 500], 128, 16, BF16, seed=3, settled=2000), 20000, 4, 700)
-    _check(_state([32768, 100], 128, 16, BF16, seed=4), 32000, 4, 700)
+    _check(_state([32768, 100, 0], 128, 16, BF16, seed=4), 32000, 4, 700)
     _check(_state([300, 100], 64, 16, BF16, seed=5, per=1000), 200, 4, 70)
+    _check(_state([300, 100], 64, 16, BF16, seed=5, per=1000), 70000, 4, 70)
+    cache, table, lens, w, order = _state([30000, 20001, 12345], 64, 16, BF16, seed=13, settled=300)
+    w[0] = 1.0
+    w[1] = (torch.arange(w.shape[1]) % 3).float()
+    for keep, recent in ((15000, 0), (20000, 100), (5000, 4000)):
+        _check((cache, table, lens, w, order), keep, 5, recent)
 
 
 def test_ties_and_what_is_no_number():
