@@ -487,7 +487,7 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, int b, const T* _
   }
   if (tw != 0 || row >= rows) return;
   const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
-  float* dst = part + at * d.dc;
+  float* dst = part + (((int64_t)seq * (d.slots - d.part0) + d.slot0 - d.part0 + sp) * each + place) * d.dc;
   float by = 1.f;
   if (d.slots == 1) {  // nothing to join
     by = sum == 0.f ? 0.f : 1.f / sum;
@@ -799,7 +799,7 @@ static int dec_row_tiles(int64_t rows, int dtype) {
 static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table, int mt) {
   DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, table,
             a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]},
-            share, 0, 0, 0, 1, 0, 0, nullptr};
+            share, 0, 0, 0, 0, 1, 0, 0, nullptr};
   const int64_t rows = (int64_t)share * d.n * d.H;
   const int rt = 16 * mt, tile = mt == 4 ? 64 : 32;
   d.groups = (int)((rows + rt - 1) / rt);
@@ -847,6 +847,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
     p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
   }
   p.own.slot0 = p.front.splits;
+  if (p.many) p.own.part0 = p.front.splits;
   p.own.slots = p.front.slots = p.own.splits + p.front.splits;
   p.own.pre_share = p.front.share;
   p.own.pre_chunk = p.front.chunk;
@@ -864,19 +865,20 @@ static bool dec_up_joins(const DecDims& d) {
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // What a call leaves in its workspace, part after part.
 struct DecSpace {
-  size_t qa, olat, stat, part, score, all;
+  size_t qa, olat, stat, part, front, score, all;
 };
-static DecSpace dec_space(const DecPlan& p, int dtype, bool scored) {
+static DecSpace dec_space(const DecPlan& p, int prefixes, int dtype, bool scored) {
   const DecDims& d = p.own;
   const size_t rows = (size_t)d.B * d.n * d.H, es = dtype == ATOMIC_BF16 ? 2 : 4;
-  const size_t parts = d.slots > 1 ? rows * d.slots : 0;  // one split needs no parts
+  const size_t parts = d.slots > 1 ? rows * (d.slots - d.part0) : 0;  // one split needs no parts
   const size_t tiles = (size_t)d.groups * p.own_tiles * (((size_t)d.table * d.page + 15) / 16);
   DecSpace s;
   s.qa = 0;
   s.olat = s.qa + up256(rows * (d.dc + d.dr) * es * (scored && es == 2 ? 2 : 1));
   s.stat = s.olat + up256(rows * d.dc * sizeof(float));
-  s.part = s.stat + up256((scored ? rows * d.slots : parts) * 2 * sizeof(float));
-  s.score = s.part + up256(parts * d.dc * sizeof(float));
+  s.part = s.stat + up256((scored || d.slots > 1 ? rows * d.slots : 0) * 2 * sizeof(float));
+  s.front = s.part + up256(parts * d.dc * sizeof(float));
+  s.score = s.front + (p.many ? up256(prefix_bytes(p.front, prefixes)) : 0);
   s.all = s.score + (scored ? (size_t)d.B * tiles * 256 * sizeof(float) : 0);
   return s;
 }
@@ -967,7 +969,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
   DecPlan plan = dec_plan(a, prefixes, prefix_pages, SCORED);
   plan.own.pre_lens = p.prefix_lens;
   const DecDims& d = plan.own;
-  const DecSpace at = dec_space(plan, a->dtype, SCORED);
+  const DecSpace at = dec_space(plan, prefixes, a->dtype, SCORED);
   Launch L{a->profile, st};
   char* ws = (char*)p.ws;
   const DecParts<T> x{(T*)(ws + at.qa), (float*)(ws + at.olat), (float*)(ws + at.stat), (float*)(ws + at.part),
@@ -992,7 +994,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
       if constexpr (sizeof(T) == 2 && !SCORED) {
         if (plan.many)
           return launch_prefix(plan.front, prefixes, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
-                               d.table * d.page, x.part, x.stat);
+                               d.table * d.page, ws + at.front, x.stat);
       }
       split(true);
     });
@@ -1002,8 +1004,13 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     rc = L("latent_split", [&] { split(false); });
     if (rc) return rc;
   }
-  const bool joins = dec_up_joins(d);
-  if (d.slots > 1 && !joins) {
+  const bool joins = !plan.many && dec_up_joins(d);
+  if (plan.many) {
+    rc = L("latent_prefix_join", [&] {
+      launch_prefix_join(plan.front, d, prefixes, st, ws + at.front, x.part, x.stat, p.lens, x.olat);
+    });
+    if (rc) return rc;
+  } else if (d.slots > 1 && !joins) {
     int ways = 1;  // about four splits a thread
     while (ways < 16 && 4 * ways < d.slots) ways *= 2;
     const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
@@ -1032,7 +1039,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
 
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(a, 0, 0, false), a->dtype, false).all;
+  return dec_space(dec_plan(a, 0, 0, false), 0, a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -1053,7 +1060,8 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
 
 extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
   if (shared_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0), a->dec.dtype, a->scored != 0).all;
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0), a->prefixes, a->dec.dtype, a->scored != 0)
+      .all;
 }
 
 extern "C" int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,

@@ -12,6 +12,7 @@ struct DecDims {
   int64_t qs[3];
   int share;         // latent_split: sequences whose rows read the same tokens (those of a prefix, or one)
   int slot0, slots;  // its first slot among a row's parts, and all of them
+  int part0;         // slots before the first whose part is fp32 (latent_prefix leaves its parts in its own way)
   // prefixes: sequences of each (0: there are none), tokens a split, slots, tokens their table holds, lengths
   int pre_share, pre_chunk, pre_splits, pre_most;
   const int32_t* pre_lens;
@@ -38,10 +39,15 @@ struct Parts {
 // Eight zeros: the source of the padding of a latent narrower than its tile.
 static __device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 
-// Whether latent_prefix takes the rows of these prefixes; divides their tokens for it, if so.
+// latent_prefix: the prefixes' tokens against the rows of all sequences that follow them (bf16).
+// Whether it takes the rows of `units` prefixes; divides their tokens for it, if so.
 bool prefix_plan(DecDims& d, int units);
-// The prefixes' tokens against the rows of all sequences that follow them, 128 a workgroup (bf16).
+// Bytes of the parts that it leaves for the join.
+size_t prefix_bytes(const DecDims& d, int units);
 void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
-                   const int32_t* lens, const int32_t* own, int own_most, float* part, float* stat);
+                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat);
+// Joins them with those of the own tokens (`d`).
+void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
+                        const float* part, const float* stat, const int32_t* kv_lens, float* olat);
 
 }  // namespace ah

@@ -3,17 +3,6 @@
 // instructions bound it (1900 operations a byte), not the cache's bytes.
 #include "latent_decode.hpp"
 
-#ifndef XG
-#define XG 2
-#define XL 2
-#endif
-#ifndef YG
-#define YG 2
-#define YL 2
-#endif
-#ifndef YV
-#define YV 4
-#endif
 namespace ah {
 
 // Keep a value in the accumulator half of the register file.
@@ -28,6 +17,12 @@ __device__ __forceinline__ void accum_mul(float& x, float f) {
                : "v"(f));
 }
 
+// Eight numbers of a part: of a lane's query and a block of 32 latent columns those that
+// registers 8 k .. 8 k + 7 of its accumulator hold, as fp16 times a power of two of the row
+// (rounded to 2^-11, a quarter of a bf16's step: 0.0003 of what is off by 0.0024 anyway;
+// in fp32 the parts of 1024 rows were 67 MB, 9 us to write and 25 to join).
+typedef _Float16 Part __attribute__((ext_vector_type(8)));
+
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
 template <int DC>
@@ -36,7 +31,8 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
                                                         const int32_t* __restrict__ table,
                                                         const int32_t* __restrict__ lens,
                                                         const int32_t* __restrict__ own, int own_most,
-                                                        float* __restrict__ part, float* __restrict__ stat) {
+                                                        Part* __restrict__ parts, float* __restrict__ scales,
+                                                        float* __restrict__ stat) {
   constexpr int DR = 64, KS = (DC + DR) / 16, KC = DC / 16, NT = DC / 32, TK = kPreTokens;
   typedef LTile<bf16, DC> LC;
   typedef LTile<bf16, DR> LR;
@@ -51,36 +47,58 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   xcd_group_map(blockIdx.x, d.splits * units, blocks, sp, blk);
   const int b = sp / d.splits, wv = wave_id(), lane = lane_id();
   sp %= d.splits;
-  const int len = dec_len(d, lens, b), each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
+  const int each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
+  const int row = kPreRows * blk + 32 * wv + (lane & 31), at = min(row, rows - 1);
+  const int seq = b * d.share + at / each, place = at % each;
+  // The queries of a wave go through the tile buffer of its number, row by row, while the
+  // tokens' places are looked up.  (Loaded as fragments, 32 rows an instruction, they took
+  // 9300 clocks.)
+  const uint32_t l0 = lds_addr(lds), wb = 2 * d.dc, rb = 2 * d.dr;
+  {
+    const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * wide);
+    const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, r) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane(lo, r);
+      const uint32_t off = 16 * lane ^ 16 * LC::swz(r);
+      dma16_raw((const void*)(off < wb ? base + off : (uint64_t)lat_zeros), to + r * LC::ROWB);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + lane / 8;
+      const uint64_t base = (uint64_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r);
+      const uint32_t off = 16 * (lane % 8) ^ 16 * LR::swz(r);
+      dma16_raw((const void*)(off < rb ? base + wb + off : (uint64_t)lat_zeros), to + SC + 8 * i * LR::ROWB);
+    }
+  }
+  const int len = dec_len(d, lens, b);
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
   if (first >= end) return;
   for (int i = threadIdx.x; i < end - first; i += 256) {
     const int j = first + i, pg = j / d.page;
     slot[i] = (uint32_t)min(max(table[(int64_t)b * d.table + pg], 0), d.pages - 1) * d.page + (j - pg * d.page);
   }
-  const int row = kPreRows * blk + 32 * wv + (lane & 31), at = min(row, rows - 1);
-  const int seq = b * d.share + at / each, place = at % each;
   const int seen = len + min(max(own[seq], 0), own_most) - d.n + place / d.H + 1;  // tokens that this lane's row sees
   const int least = len - d.n + 1;                                                 // and that every row sees
-  const bf16* qr = qa + ((int64_t)seq * each + place) * wide;
+  vm_wait<0>();
   frag qf[KS];
+  {
+    const uint32_t ac = l0 + wv * STAGE + LC::row_base(), ar = l0 + wv * STAGE + SC + LR::row_base();
 #pragma unroll
-  for (int t = 0; t < KS; ++t) {
-    const int k = 16 * t + 8 * (lane >> 5);
-    if (t < KC) qf[t] = ld_frag(k < d.dc ? qr + k : (const bf16*)lat_zeros);
-    else qf[t] = ld_frag(k - DC < d.dr ? qr + d.dc + k - DC : (const bf16*)lat_zeros);
+    for (int t = 0; t < KS; ++t) qf[t] = t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC));
   }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  __syncthreads();  // the rows' places are there
-  const uint32_t l0 = lds_addr(lds), wb = 2 * d.dc;
+  __syncthreads();  // the tokens' places are there, the buffers free
   // This wave's loads of the tile at k0 (from `first` on): eight latents, then their rotated keys.
-  uint32_t lo, hi;
-  auto aim = [&](int k0) {
-    const uint64_t a = (uint64_t)cache + (uint64_t)slot[min(k0 + PT * wv + (lane & 7), end - first - 1)] * (2 * wide);
+  // (Their places are read a tile ahead.)
+  uint32_t lo, hi, next;
+  auto look = [&](int k0) { next = slot[min(k0 + PT * wv + (lane & 7), end - first - 1)]; };
+  auto aim = [&] {
+    const uint64_t a = (uint64_t)cache + (uint64_t)next * (2 * wide);
     lo = (uint32_t)a;
     hi = (uint32_t)(a >> 32);
   };
-  auto load = [&](int i, uint32_t to) {
+  auto send = [&](int i, uint32_t to) __attribute__((always_inline)) {
     if (i < PT) {
       const int r = PT * wv + i;
       const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 |
@@ -92,7 +110,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
       const int r = PT * wv + lane / 8;
       const uint64_t base = (uint64_t)__shfl(hi, lane / 8) << 32 | (uint32_t)__shfl(lo, lane / 8);
       uint32_t off = 16 * (lane % 8) ^ 16 * LR::swz(r);
-      if (off >= 2 * (uint32_t)d.dr) off = 0;
+      if (off >= rb) off = 0;
       dma16_raw((const void*)(base + wb + off), to + SC + PT * wv * LR::ROWB);
     }
   };
@@ -108,25 +126,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   float m = -INFINITY, sum = 0.f;
   f32x16 s;
   const uint32_t br = LC::row_base(), bp = LR::row_base(), bc = LC::col_base();
-  // Scores of the tile at k0, masked.
-  auto scores = [&](int buf, int k0, auto work) {
-    uint32_t ac = l0 + buf * STAGE + br, ar = l0 + buf * STAGE + SC + bp;
-    asm volatile("" : "+v"(ac), "+v"(ar));
-    s = zero16();
-#ifdef CH2
-    f32x16 s1 = zero16();
-#endif
-    in_groups<KS, XG, XL, 0, frag>([&](int t) { return t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC)); },
-                                 [&](int t, frag a) {
-#ifdef CH2
-                                   if (t & 1) s1 = M32<bf16>::mma(a, qf[t], s1);
-                                   else
-#endif
-                                   s = M32<bf16>::mma(a, qf[t], s); }, work);
-#ifdef CH2
-    s += s1;
-#endif
-    asm volatile("" : "+v"(s));
+  auto mask = [&](int k0) __attribute__((always_inline)) {
     if (first + k0 + TK > min(end, least)) {
       const int lim = min(end, seen) - first - k0 - 4 * (lane >> 5);
 #pragma unroll
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
     }
   };
   frag p[2], pn[2];
-  auto quad = [&](int k) {  // four tokens' probabilities
+  auto quad = [&](int k) __attribute__((always_inline)) {  // four tokens' probabilities
     const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -147,19 +147,9 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
       pn[k / 2][4 * (k & 1) + j] = (bf16)e;
     }
   };
-  // A tile's probabilities times its latents; beside them `work`.
-  auto values = [&](int buf, auto work) {
-    uint32_t av = l0 + buf * STAGE + bc;
-    asm volatile("" : "+v"(av));
-    in_groups<2 * NT, YG, YL, YV, frag>([&](int j) { return LC::col(av, 16 * (j / NT), 32 * (j % NT)); },
-                                     [&](int j, frag a) { acc[j % NT] = M32<bf16>::mma(a, p[j / NT], acc[j % NT]); },
-                                     work);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) in_accum(acc[n]);
-  };
   // A new reference where a score is far above its row's: a whole number, so that what
   // fades, the last tile's probabilities among it, is scaled exactly.
-  auto settle = [&] {
+  auto settle = [&](auto fades) __attribute__((always_inline)) {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
@@ -168,6 +158,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m, ceilf(top)), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
       m = mn;
+      if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
       sum *= fade;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -185,18 +176,69 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
       asm volatile("s_nop 7" ::: "memory");
     }
   };
+  // The scores of tile i in buffer `kb` and the products of the tile before in `vb`, as one run
+  // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
+  // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
+  constexpr int G = 2, LA = 2, GS = KS / G, GV = 2 * NT / G;
+  auto tile = [&](auto with_k, auto with_v, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
+    constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
+    uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
+    asm volatile("" : "+v"(ac), "+v"(ar), "+v"(av));
+    auto load = [&](int j) {
+      return j < KC ? LC::row(ac, 0, 16 * j)
+                    : j < KS ? LR::row(ar, 0, 16 * (j - KC)) : LC::col(av, 16 * ((j - KS) / NT), 32 * ((j - KS) % NT));
+    };
+    frag f[LA + 1][G];
+    static_for<LA * G>([&](auto j) { f[(g0 + j.value / G) % (LA + 1)][j.value % G] = load(g0 * G + j.value); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<g1 - g0>([&](auto gr) __attribute__((always_inline)) {
+      constexpr int g = g0 + decltype(gr)::value;
+      static_for<G>([&](auto j) {
+        if constexpr (g + LA < g1) f[(g + LA) % (LA + 1)][j.value] = load((g + LA) * G + j.value);
+      });
+      if constexpr (g < GS) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+          if (decltype(with_v)::value && j * GS / NL == g) send(j, to);
+        if constexpr (g == 0) s = zero16();
+        static_for<G>([&](auto j) { s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[g * G + j.value], s); });
+        if constexpr (g == GS - 1) {
+          asm volatile("" : "+v"(s));
+          mask(k0);
+          settle(with_v);
+        }
+      } else {
+        if constexpr (decltype(with_k)::value && (g - GS) % (GV / 4) == 1) quad((g - GS) / (GV / 4));
+        static_for<G>([&](auto j) {
+          constexpr int v = (g - GS) * G + decltype(j)::value;
+          acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], p[v / NT], acc[v % NT]);
+        });
+        __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
+        static_for<G>([&](auto) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector
+        });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (decltype(with_v)::value) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) in_accum(acc[n]);
+    }
+  };
   const int tiles = (end - first + TK - 1) / TK;
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    aim(TK * k);
+    look(TK * k);
+    aim();
 #pragma unroll
-    for (int i = 0; i < NL; ++i) load(i, l0 + k * STAGE);
+    for (int i = 0; i < NL; ++i) send(i, l0 + k * STAGE);
   }
+  look(TK * 3);
   vm_wait<2 * NL>();
   bare_barrier();
-  p[0] = p[1] = zero_frag<bf16>();
-  scores(0, 0, [](int) {});
-  settle();
+  tile(IntC<1>(), IntC<0>(), 0, 0, 0, 0);
 #pragma unroll
   for (int k = 0; k < 4; ++k) quad(k);
   p[0] = pn[0];
@@ -204,42 +246,127 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   for (int i = 1; i < tiles; ++i) {
     vm_wait<NL>();   // tile i is there (of this wave's loads; behind the barrier, of all)
     bare_barrier();  // and nobody reads tile i - 2 any more
-    aim(TK * (i + 2));
-    const uint32_t to = l0 + (i + 2) % kPreBufs * STAGE;
-    scores(i % kPreBufs, TK * i, [&](int t) {
-#pragma unroll
-      for (int j = 0; j < NL; ++j)
-        if (j * KS / NL == t) load(j, to);
-    });
-    settle();
-    values((i - 1) % kPreBufs, [&](int j) {
-      if (j % 8 == 2) quad(j / 8);
-    });
+    aim();
+    look(TK * (i + 3));
+    tile(IntC<1>(), IntC<1>(), i % kPreBufs, (i - 1) % kPreBufs, TK * i, l0 + (i + 2) % kPreBufs * STAGE);
     p[0] = pn[0];
     p[1] = pn[1];
   }
-  values((tiles - 1) % kPreBufs, [](int) {});
+  tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % kPreBufs, 0, 0);
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
-  if (row >= rows) return;
   sum += __shfl_xor(sum, 32);
-  const int64_t to = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
+  float big = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int c = 32 * n + 8 * (r >> 2) + 4 * (lane >> 5);
-      if (c < d.dc) store4(part + to * d.dc + c, f32x4{acc[n][r], acc[n][r + 1], acc[n][r + 2], acc[n][r + 3]});
+    for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(acc[n][r]));
+  big = fmaxf(big, __shfl_xor(big, 32));
+  const int e = max((int)(__builtin_bit_cast(uint32_t, big) >> 23), 30) - 127;  // 2^e <= big < 2^(e + 1)
+  const float up = __builtin_bit_cast(float, (uint32_t)(14 - e + 127) << 23);
+  const int64_t group = ((int64_t)b * blocks + blk) * 4 + wv, tile_at = group * d.splits + sp;
+  Part* to = parts + tile_at * (2 * NT * 64) + lane;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      Part x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (_Float16)(acc[n][8 * k + j] * up);
+      if (32 * n < d.dc) to[(2 * n + k) * 64] = x;
     }
   if (lane < 32) {
-    stat[2 * to] = m;
-    stat[2 * to + 1] = sum;
+    scales[tile_at * 32 + lane] = __builtin_bit_cast(float, (uint32_t)(e - 14 + 127) << 23);
+    if (row < rows) {
+      const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
+      stat[2 * at] = m;
+      stat[2 * at + 1] = sum;
+    }
   }
 }
+
+// o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
+// tokens joined.  A workgroup takes 32 rows and four of the parts' blocks, one a wave, whose
+// 1 KB a split is one load.
+__global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
+                                                          const float* __restrict__ scales,
+                                                          const float* __restrict__ part,
+                                                          const float* __restrict__ stat,
+                                                          const int32_t* __restrict__ kv_lens,
+                                                          float* __restrict__ olat) {
+  constexpr int NT = 16;
+  __shared__ float refs[32], invs[32];
+  const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id(), lane = lane_id();
+  const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
+  if (r0 >= rows) return;
+  // a row's reference and sum: eight threads each
+  {
+    const int r = r0 + threadIdx.x / 8, seq = b * f.share + min(r, rows - 1) / each, place = min(r, rows - 1) % each;
+    const Parts ps(d, kv_lens, seq);
+    const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
+    float m = -INFINITY, sum = 0.f;
+    for (int s = threadIdx.x & 7; s < ps.all; s += 8) {
+      const float2 x = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * each);
+      const float mn = fmaxf(m, x.x);
+      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + x.y * fast_exp2(x.x - mn);
+      m = mn;
+    }
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) {
+      const float mo = __shfl_xor(m, i), so = __shfl_xor(sum, i), mn = fmaxf(m, mo);
+      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + so * fast_exp2(mo - mn);
+      m = mn;
+    }
+    if ((threadIdx.x & 7) == 0) {
+      refs[threadIdx.x / 8] = m == -INFINITY ? 0.f : m;
+      invs[threadIdx.x / 8] = sum == 0.f ? 0.f : 1.f / sum;
+    }
+  }
+  __syncthreads();
+  const int c = 16 * k + 4 * (lane >> 5), row = r0 + (lane & 31);  // columns c .. c + 3 and c + 8 .. c + 11
+  if (32 * (k / 2) >= d.dc) return;
+  const int seq = b * f.share + min(row, rows - 1) / each, place = min(row, rows - 1) % each;
+  const Parts ps(d, kv_lens, seq);
+  const float ref = refs[lane & 31], inv = invs[lane & 31];
+  const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
+  const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + k * 64 + lane;
+  const float* sc = scales + (int64_t)group * f.splits * 32 + (lane & 31);
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < ps.front; ++s) {
+    const Part y = from[(int64_t)s * (2 * NT * 64)];
+    const float w = fast_exp2(st[2 * (int64_t)s * each] - ref) * sc[(int64_t)s * 32];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] += w * (float)y[j];
+  }
+  const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc;
+  const bool lo = c < d.dc, hi = c + 8 < d.dc;
+#pragma unroll 4
+  for (int s = ps.front; s < ps.all; ++s) {
+    const float w = fast_exp2(st[2 * (int64_t)ps.slot(s) * each] - ref);
+    const float* y = own + (int64_t)(s - ps.front) * each * d.dc;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(y + (lo ? c : 0)), z = *reinterpret_cast<const f32x4*>(y + (hi ? c + 8 : 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] += w * a[j];
+      x[4 + j] += w * z[j];
+    }
+  }
+  if (row >= rows) return;
+  float* to = olat + ((int64_t)seq * each + place) * d.dc;
+  if (lo) store4(to + c, f32x4{x[0], x[1], x[2], x[3]} * inv);
+  if (hi) store4(to + c + 8, f32x4{x[4], x[5], x[6], x[7]} * inv);
+}
+
+static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
+// Rows of 32 times splits: each leaves 32 KB and 32 scales.
+static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units * prefix_blocks(d) * 4 * d.splits; }
 
 bool prefix_plan(DecDims& d, int units) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
   if (rows <= 32 || most < 256 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
-  const int64_t blocks = (rows + kPreRows - 1) / kPreRows * units;
+  const int64_t blocks = (int64_t)prefix_blocks(d) * units;
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
     const int64_t wg = blocks * ((most + chunk - 1) / chunk);
@@ -253,11 +380,22 @@ bool prefix_plan(DecDims& d, int units) {
   return blocks * d.splits <= INT32_MAX;
 }
 
+size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (32 * 512 * 2 + 32 * 4); }
+
 void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
-                   const int32_t* lens, const int32_t* own, int own_most, float* part, float* stat) {
-  const int blocks = (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows);
+                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat) {
+  const int blocks = prefix_blocks(d);
+  float* scales = (float*)((char*)parts + prefix_tiles(d, units) * (32 * 512 * 2));
   hipLaunchKernelGGL((latent_prefix<512>), dim3((unsigned)(d.splits * units * blocks)), dim3(256), 0, st, d, blocks,
-                     units, qa, (const bf16*)cache, table, lens, own, own_most, part, stat);
+                     units, qa, (const bf16*)cache, table, lens, own, own_most, (Part*)parts, scales, stat);
+}
+
+void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
+                        const float* part, const float* stat, const int32_t* kv_lens, float* olat) {
+  const int blocks = prefix_blocks(f);
+  const float* scales = (const float*)((const char*)parts + prefix_tiles(f, units) * (32 * 512 * 2));
+  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 8)), dim3(256), 0, st, f, d, blocks,
+                     (const Part*)parts, scales, part, stat, kv_lens, olat);
 }
 
 }  // namespace ah
