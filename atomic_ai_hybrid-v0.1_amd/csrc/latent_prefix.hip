@@ -294,7 +294,9 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
                                                           const int32_t* __restrict__ kv_lens,
                                                           float* __restrict__ olat) {
   constexpr int NT = 16;
+  constexpr int LD = 68;
   __shared__ float refs[32], invs[32];
+  __shared__ __attribute__((aligned(16))) float tile[32 * LD];
   const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id(), lane = lane_id();
   const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
   if (r0 >= rows) return;
@@ -322,41 +324,50 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
     }
   }
   __syncthreads();
-  const int c = 16 * k + 4 * (lane >> 5), row = r0 + (lane & 31);  // columns c .. c + 3 and c + 8 .. c + 11
-  if (32 * (k / 2) >= d.dc) return;
-  const int seq = b * f.share + min(row, rows - 1) / each, place = min(row, rows - 1) % each;
-  const Parts ps(d, kv_lens, seq);
-  const float ref = refs[lane & 31], inv = invs[lane & 31];
-  const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-  const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + k * 64 + lane;
-  const float* sc = scales + (int64_t)group * f.splits * 32 + (lane & 31);
-  float x[8];
+  {
+    const int row = min(r0 + (lane & 31), rows - 1), seq = b * f.share + row / each, place = row % each;
+    const Parts ps(d, kv_lens, seq);
+    const float ref = refs[lane & 31];
+    const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
+    const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + k * 64 + lane;
+    const float* sc = scales + (int64_t)group * f.splits * 32 + (lane & 31);
+    float x[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (32 * (k / 2) < d.dc) {
 #pragma unroll 8
-  for (int s = 0; s < ps.front; ++s) {
-    const Part y = from[(int64_t)s * (2 * NT * 64)];
-    const float w = fast_exp2(st[2 * (int64_t)s * each] - ref) * sc[(int64_t)s * 32];
+      for (int s = 0; s < ps.front; ++s) {
+        const Part y = from[(int64_t)s * (2 * NT * 64)];
+        const float w = fast_exp2(st[2 * (int64_t)s * each] - ref) * sc[(int64_t)s * 32];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] += w * (float)y[j];
+        for (int j = 0; j < 8; ++j) x[j] += w * (float)y[j];
+      }
+    }
+    float* to = tile + (lane & 31) * LD + 16 * wave_id() + 4 * (lane >> 5);
+    store4(to, f32x4{x[0], x[1], x[2], x[3]});
+    store4(to + 8, f32x4{x[4], x[5], x[6], x[7]});
   }
-  const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc;
-  const bool lo = c < d.dc, hi = c + 8 < d.dc;
+  __syncthreads();
+  // the own tokens' parts and the result: eight columns of a row a thread
+  const int r = threadIdx.x / 8, c = 64 * (blockIdx.x % 8) + 8 * (threadIdx.x & 7), row = r0 + r;
+  if (row >= rows || c >= d.dc) return;
+  const int seq = b * f.share + row / each, place = row % each;
+  const Parts ps(d, kv_lens, seq);
+  const float ref = refs[r], inv = invs[r];
+  const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
+  const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + c;
+  const float* x = tile + r * LD + (c & 63);
+  f32x4 lo = *reinterpret_cast<const f32x4*>(x), hi = *reinterpret_cast<const f32x4*>(x + 4);
 #pragma unroll 4
   for (int s = ps.front; s < ps.all; ++s) {
     const float w = fast_exp2(st[2 * (int64_t)ps.slot(s) * each] - ref);
     const float* y = own + (int64_t)(s - ps.front) * each * d.dc;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(y + (lo ? c : 0)), z = *reinterpret_cast<const f32x4*>(y + (hi ? c + 8 : 0));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] += w * a[j];
-      x[4 + j] += w * z[j];
-    }
+    lo += w * *reinterpret_cast<const f32x4*>(y);
+    hi += w * *reinterpret_cast<const f32x4*>(y + 4);
   }
-  if (row >= rows) return;
-  float* to = olat + ((int64_t)seq * each + place) * d.dc;
-  if (lo) store4(to + c, f32x4{x[0], x[1], x[2], x[3]} * inv);
-  if (hi) store4(to + c + 8, f32x4{x[4], x[5], x[6], x[7]} * inv);
+  float* to = olat + ((int64_t)seq * each + place) * d.dc + c;
+  store4(to, lo * inv);
+  store4(to + 4, hi * inv);
 }
 
 static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
@@ -370,7 +381,7 @@ bool prefix_plan(DecDims& d, int units) {
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
     const int64_t wg = blocks * ((most + chunk - 1) / chunk);
-    const double cost = (double)((wg + 255) / 256) * (0.034 * chunk + 4) + 0.13 * (double)wg;
+    const double cost = (double)((wg + 255) / 256) * (0.0713 * chunk + 4.4) + 0.035 * (double)wg;
     if (chunk == 64 || cost < best) {
       best = cost;
       d.chunk = chunk;
