@@ -589,6 +589,7 @@ constexpr int kWeighTiles = 16, kMostRows = 4096;
 struct Weigh {
   int row_tiles, first;  // row tiles of a sequence; latent_up's grid x where its workgroups begin
   const float* score;
+  const float* shift;  // corrections of the rows' sums over their prefixes (latent_prefix_join), or NULL
   float* weights;
   int64_t stride;
 };
@@ -605,8 +606,14 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
     float m = -INFINITY, sum = 0.f;
     if (r < rows) {
       const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r);
+      float shift = 0.f;
+      if (x.shift) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) shift += x.shift[((int64_t)b * rows + r) * 8 + k];
+      }
       for (int s = lane & 15; s < ps.all; s += 16) {
-        const float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
+        float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
+        if (s < ps.front) a.x += shift;
         const float mn = fmaxf(m, a.x);
         if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + a.y * fast_exp2(a.x - mn);
         m = mn;
@@ -826,7 +833,7 @@ struct DecPlan {
   bool many;                   // the prefixes' rows are many: latent_prefix takes them
   bool both;                   // one launch for both
 };
-static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, bool scored) {
+static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages) {
   DecPlan p{};
   p.own_tiles = dec_row_tiles((int64_t)a->tokens * a->heads, a->dtype);
   p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
@@ -835,7 +842,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
   p.front_tiles = dec_row_tiles((int64_t)share * a->tokens * a->heads, a->dtype);
   p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles);
   DecDims many = p.front;
-  p.many = !scored && a->dtype == ATOMIC_BF16 && a->dc > 256 && prefix_plan(many, prefixes) &&
+  p.many = a->dtype == ATOMIC_BF16 && a->dc > 256 && prefix_plan(many, prefixes) &&
            many.splits + p.own.splits > 1;
   if (p.many) p.front = many;
   // One launch costs less than what the own tokens lose by the prefix's row tiles while they
@@ -865,7 +872,7 @@ static bool dec_up_joins(const DecDims& d) {
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // What a call leaves in its workspace, part after part.
 struct DecSpace {
-  size_t qa, olat, stat, part, front, score, all;
+  size_t qa, olat, stat, part, front, shift, score, all;
 };
 static DecSpace dec_space(const DecPlan& p, int prefixes, int dtype, bool scored) {
   const DecDims& d = p.own;
@@ -878,7 +885,8 @@ static DecSpace dec_space(const DecPlan& p, int prefixes, int dtype, bool scored
   s.stat = s.olat + up256(rows * d.dc * sizeof(float));
   s.part = s.stat + up256((scored || d.slots > 1 ? rows * d.slots : 0) * 2 * sizeof(float));
   s.front = s.part + up256(parts * d.dc * sizeof(float));
-  s.score = s.front + (p.many ? up256(prefix_bytes(p.front, prefixes)) : 0);
+  s.shift = s.front + (p.many ? up256(prefix_bytes(p.front, prefixes)) : 0);
+  s.score = s.shift + (p.many && scored ? up256(rows * 8 * sizeof(float)) : 0);
   s.all = s.score + (scored ? (size_t)d.B * tiles * 256 * sizeof(float) : 0);
   return s;
 }
@@ -966,7 +974,7 @@ static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStrea
 template <typename T, bool SCORED>
 static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, const DecPtrs& p,
                    hipStream_t st) {
-  DecPlan plan = dec_plan(a, prefixes, prefix_pages, SCORED);
+  DecPlan plan = dec_plan(a, prefixes, prefix_pages);
   plan.own.pre_lens = p.prefix_lens;
   const DecDims& d = plan.own;
   const DecSpace at = dec_space(plan, prefixes, a->dtype, SCORED);
@@ -991,9 +999,9 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
   }
   if (plan.front.splits && !plan.both) {
     rc = L(plan.many ? "latent_prefix" : "latent_split (prefix)", [&] {
-      if constexpr (sizeof(T) == 2 && !SCORED) {
+      if constexpr (sizeof(T) == 2) {
         if (plan.many)
-          return launch_prefix(plan.front, prefixes, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
+          return launch_prefix(plan.front, prefixes, SCORED, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
                                d.table * d.page, ws + at.front, x.stat);
       }
       split(true);
@@ -1005,9 +1013,11 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     if (rc) return rc;
   }
   const bool joins = !plan.many && dec_up_joins(d);
+  float* shift = plan.many && SCORED ? (float*)(ws + at.shift) : nullptr;
   if (plan.many) {
     rc = L("latent_prefix_join", [&] {
-      launch_prefix_join(plan.front, d, prefixes, st, ws + at.front, x.part, x.stat, p.lens, x.olat);
+      launch_prefix_join(plan.front, d, prefixes, st, ws + at.front, x.part, x.stat, p.lens, x.olat,
+                         (const bf16*)x.qa, shift);
     });
     if (rc) return rc;
   } else if (d.slots > 1 && !joins) {
@@ -1020,7 +1030,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     });
     if (rc) return rc;
   }
-  const Weigh wx{d.groups * plan.own_tiles, d.H, x.score, p.weights, p.weights_stride};
+  const Weigh wx{d.groups * plan.own_tiles, d.H, x.score, shift, p.weights, p.weights_stride};
   unsigned more = 0;  // the weights' workgroups
   const unsigned gy = (unsigned)((d.dv + 63) / 64);
   if (SCORED && d.splits) {
@@ -1039,7 +1049,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
 
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(a, 0, 0, false), 0, a->dtype, false).all;
+  return dec_space(dec_plan(a, 0, 0), 0, a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -1060,7 +1070,7 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
 
 extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
   if (shared_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0), a->prefixes, a->dec.dtype, a->scored != 0)
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages), a->prefixes, a->dec.dtype, a->scored != 0)
       .all;
 }
 

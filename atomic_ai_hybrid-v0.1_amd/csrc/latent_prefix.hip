@@ -25,7 +25,7 @@ typedef _Float16 Part __attribute__((ext_vector_type(8)));
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
-template <int DC>
+template <int DC, bool SCORED>
 __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, int units,
                                                         const bf16* __restrict__ qa, const bf16* __restrict__ cache,
                                                         const int32_t* __restrict__ table,
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   // 9300 clocks.)
   const uint32_t l0 = lds_addr(lds), wb = 2 * d.dc, rb = 2 * d.dr;
   {
-    const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * wide);
+    const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * (SCORED ? 2 : 1) * wide);
     const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
@@ -87,6 +87,17 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
     const uint32_t ac = l0 + wv * STAGE + LC::row_base(), ar = l0 + wv * STAGE + SC + LR::row_base();
 #pragma unroll
     for (int t = 0; t < KS; ++t) qf[t] = t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC));
+  }
+  // What the rounding of the rotated queries left out enters the scores too where they have to
+  // be exact; that of q_lat is made good in the join.
+  frag ql[SCORED ? KS - KC : 1];
+  if constexpr (SCORED) {
+    const bf16* qr = qa + (((int64_t)seq * each + place) * 2 + 1) * wide + d.dc;
+#pragma unroll
+    for (int t = 0; t < KS - KC; ++t) {
+      const int k = 16 * t + 8 * (lane >> 5);
+      ql[t] = ld_frag(k < d.dr ? qr + k : (const bf16*)lat_zeros);
+    }
   }
   __syncthreads();  // the tokens' places are there, the buffers free
   // This wave's loads of the tile at k0 (from `first` on): eight latents, then their rotated keys.
@@ -122,6 +133,8 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   if (d.scale < 0.f) {
 #pragma unroll
     for (int t = 0; t < KS; ++t) qf[t] = -qf[t];
+#pragma unroll
+    for (int t = 0; t < (SCORED ? KS - KC : 0); ++t) ql[t] = -ql[t];
   }
   float m = -INFINITY, sum = 0.f;
   f32x16 s;
@@ -179,7 +192,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   // The scores of tile i in buffer `kb` and the products of the tile before in `vb`, as one run
   // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
   // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
-  constexpr int G = 2, LA = 2, GS = KS / G, GV = 2 * NT / G;
+  constexpr int G = SCORED ? 1 : 2, LA = 2, GS = KS / G, GV = 2 * NT / G;
   auto tile = [&](auto with_k, auto with_v, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
     constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
     uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
@@ -202,7 +215,11 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
         for (int j = 0; j < NL; ++j)
           if (decltype(with_v)::value && j * GS / NL == g) send(j, to);
         if constexpr (g == 0) s = zero16();
-        static_for<G>([&](auto j) { s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[g * G + j.value], s); });
+        static_for<G>([&](auto j) {
+          constexpr int t = g * G + decltype(j)::value;
+          s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[t], s);
+          if constexpr (SCORED && t >= KC) s = M32<bf16>::mma(f[g % (LA + 1)][j.value], ql[t - KC], s);
+        });
         if constexpr (g == GS - 1) {
           asm volatile("" : "+v"(s));
           mask(k0);
@@ -287,15 +304,23 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
 // tokens joined.  A workgroup takes 32 rows and four of the parts' blocks, one a wave, whose
 // 1 KB a split is one load.
+//
+// Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
+// to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
+// by c e . c_j, so the log by c e . (sum_j p_j c_j) and, what is left, half the variance of
+// c e . c_j (1.5e-6 for scores of unit spread; uncorrected, the sum was off by 5e-5).
+// Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
+// take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
 __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
                                                           const float* __restrict__ scales,
                                                           const float* __restrict__ part,
                                                           const float* __restrict__ stat,
                                                           const int32_t* __restrict__ kv_lens,
-                                                          float* __restrict__ olat) {
+                                                          float* __restrict__ olat, const bf16* __restrict__ qa,
+                                                          float* __restrict__ shift) {
   constexpr int NT = 16;
   constexpr int LD = 68;
-  __shared__ float refs[32], invs[32];
+  __shared__ float refs[32], invs[32], fronts[32];
   __shared__ __attribute__((aligned(16))) float tile[32 * LD];
   const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id(), lane = lane_id();
   const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
@@ -305,22 +330,31 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
     const int r = r0 + threadIdx.x / 8, seq = b * f.share + min(r, rows - 1) / each, place = min(r, rows - 1) % each;
     const Parts ps(d, kv_lens, seq);
     const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, sum = 0.f, front = 0.f;
     for (int s = threadIdx.x & 7; s < ps.all; s += 8) {
       const float2 x = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * each);
       const float mn = fmaxf(m, x.x);
-      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + x.y * fast_exp2(x.x - mn);
+      if (mn > -INFINITY) {
+        const float fade = fast_exp2(m - mn), add = x.y * fast_exp2(x.x - mn);
+        sum = sum * fade + add;
+        front = front * fade + (s < ps.front ? add : 0.f);
+      }
       m = mn;
     }
 #pragma unroll
     for (int i = 1; i < 8; i *= 2) {
-      const float mo = __shfl_xor(m, i), so = __shfl_xor(sum, i), mn = fmaxf(m, mo);
-      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + so * fast_exp2(mo - mn);
+      const float mo = __shfl_xor(m, i), so = __shfl_xor(sum, i), fo = __shfl_xor(front, i), mn = fmaxf(m, mo);
+      if (mn > -INFINITY) {
+        const float fade = fast_exp2(m - mn), other = fast_exp2(mo - mn);
+        sum = sum * fade + so * other;
+        front = front * fade + fo * other;
+      }
       m = mn;
     }
     if ((threadIdx.x & 7) == 0) {
       refs[threadIdx.x / 8] = m == -INFINITY ? 0.f : m;
       invs[threadIdx.x / 8] = sum == 0.f ? 0.f : 1.f / sum;
+      fronts[threadIdx.x / 8] = front == 0.f ? 0.f : 1.f / front;
     }
   }
   __syncthreads();
@@ -350,6 +384,21 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
   __syncthreads();
   // the own tokens' parts and the result: eight columns of a row a thread
   const int r = threadIdx.x / 8, c = 64 * (blockIdx.x % 8) + 8 * (threadIdx.x & 7), row = r0 + r;
+  if (shift) {
+    const float* x = tile + r * LD + (c & 63);
+    float dot = 0.f;
+    if (row < rows && c < d.dc) {
+      float lo[8];
+      load8(qa + (((int64_t)(b * f.share + row / each) * each + row % each) * 2 + 1) * (d.dc + d.dr) + c, lo);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot += lo[j] * x[j];
+    }
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) dot += __shfl_xor(dot, i);
+    if (row < rows && (threadIdx.x & 7) == 0)
+      shift[((int64_t)(b * f.share + row / each) * each + row % each) * 8 + blockIdx.x % 8] =
+          dot * fronts[r] * d.scale * kLog2e;
+  }
   if (row >= rows || c >= d.dc) return;
   const int seq = b * f.share + row / each, place = row % each;
   const Parts ps(d, kv_lens, seq);
@@ -393,20 +442,27 @@ bool prefix_plan(DecDims& d, int units) {
 
 size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (32 * 512 * 2 + 32 * 4); }
 
-void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
-                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat) {
+void launch_prefix(const DecDims& d, int units, bool scored, hipStream_t st, const bf16* qa, const void* cache,
+                   const int32_t* table, const int32_t* lens, const int32_t* own, int own_most, void* parts,
+                   float* stat) {
   const int blocks = prefix_blocks(d);
   float* scales = (float*)((char*)parts + prefix_tiles(d, units) * (32 * 512 * 2));
-  hipLaunchKernelGGL((latent_prefix<512>), dim3((unsigned)(d.splits * units * blocks)), dim3(256), 0, st, d, blocks,
-                     units, qa, (const bf16*)cache, table, lens, own, own_most, (Part*)parts, scales, stat);
+  auto go = [&](auto s) {
+    hipLaunchKernelGGL((latent_prefix<512, decltype(s)::value != 0>), dim3((unsigned)(d.splits * units * blocks)),
+                       dim3(256), 0, st, d, blocks, units, qa, (const bf16*)cache, table, lens, own, own_most,
+                       (Part*)parts, scales, stat);
+  };
+  if (scored) go(IntC<1>());
+  else go(IntC<0>());
 }
 
 void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
-                        const float* part, const float* stat, const int32_t* kv_lens, float* olat) {
+                        const float* part, const float* stat, const int32_t* kv_lens, float* olat, const bf16* qa,
+                        float* shift) {
   const int blocks = prefix_blocks(f);
   const float* scales = (const float*)((const char*)parts + prefix_tiles(f, units) * (32 * 512 * 2));
   hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 8)), dim3(256), 0, st, f, d, blocks,
-                     (const Part*)parts, scales, part, stat, kv_lens, olat);
+                     (const Part*)parts, scales, part, stat, kv_lens, olat, qa, shift);
 }
 
 }  // namespace ah
