@@ -290,7 +290,7 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, int b, const T* _
   int seen = len - d.n + place / d.H + 1;  // tokens that it sees
   if (own) seen += min(max(own[seq], 0), own_most);
   const int least = len - d.n + 1;  // and that every row sees
-  const T* qr = qa + ((int64_t)seq * each + place) * NQ * wide;
+  const T* qr = qa + ((int64_t)seq * each + place) * d.qn * wide;
   frag qf[NQ][KS];
 #pragma unroll
   for (int u = 0; u < NQ; ++u)
@@ -609,7 +609,7 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
       float shift = 0.f;
       if (x.shift) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) shift += x.shift[((int64_t)b * rows + r) * 8 + k];
+        for (int k = 0; k < 16; ++k) shift += x.shift[((int64_t)b * rows + r) * 16 + k];
       }
       for (int s = lane & 15; s < ps.all; s += 16) {
         float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
@@ -806,7 +806,7 @@ static int dec_row_tiles(int64_t rows, int dtype) {
 static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table, int mt) {
   DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, table,
             a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]},
-            share, 0, 0, 0, 0, 1, 0, 0, nullptr};
+            share, 0, 0, 1, 0, 0, 1, 0, 0, nullptr};
   const int64_t rows = (int64_t)share * d.n * d.H;
   const int rt = 16 * mt, tile = mt == 4 ? 64 : 32;
   d.groups = (int)((rows + rt - 1) / rt);
@@ -833,10 +833,12 @@ struct DecPlan {
   bool many;                   // the prefixes' rows are many: latent_prefix takes them
   bool both;                   // one launch for both
 };
-static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages) {
+static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, bool scored) {
   DecPlan p{};
   p.own_tiles = dec_row_tiles((int64_t)a->tokens * a->heads, a->dtype);
   p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
+  const int qn = scored && a->dtype == ATOMIC_BF16 ? 2 : 1;
+  p.own.qn = qn;
   if (!prefixes) return p;
   const int share = a->batch / prefixes;
   p.front_tiles = dec_row_tiles((int64_t)share * a->tokens * a->heads, a->dtype);
@@ -853,6 +855,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
     p.own_tiles = p.front_tiles;
     p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
   }
+  p.own.qn = p.front.qn = p.many ? 2 : qn;
   p.own.slot0 = p.front.splits;
   if (p.many) p.own.part0 = p.front.splits;
   p.own.slots = p.front.slots = p.own.splits + p.front.splits;
@@ -881,12 +884,12 @@ static DecSpace dec_space(const DecPlan& p, int prefixes, int dtype, bool scored
   const size_t tiles = (size_t)d.groups * p.own_tiles * (((size_t)d.table * d.page + 15) / 16);
   DecSpace s;
   s.qa = 0;
-  s.olat = s.qa + up256(rows * (d.dc + d.dr) * es * (scored && es == 2 ? 2 : 1));
+  s.olat = s.qa + up256(rows * (d.dc + d.dr) * es * d.qn);
   s.stat = s.olat + up256(rows * d.dc * sizeof(float));
   s.part = s.stat + up256((scored || d.slots > 1 ? rows * d.slots : 0) * 2 * sizeof(float));
   s.front = s.part + up256(parts * d.dc * sizeof(float));
   s.shift = s.front + (p.many ? up256(prefix_bytes(p.front, prefixes)) : 0);
-  s.score = s.shift + (p.many && scored ? up256(rows * 8 * sizeof(float)) : 0);
+  s.score = s.shift + (p.many && scored ? up256(rows * 16 * sizeof(float)) : 0);
   s.all = s.score + (scored ? (size_t)d.B * tiles * 256 * sizeof(float) : 0);
   return s;
 }
@@ -974,7 +977,7 @@ static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStrea
 template <typename T, bool SCORED>
 static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, const DecPtrs& p,
                    hipStream_t st) {
-  DecPlan plan = dec_plan(a, prefixes, prefix_pages);
+  DecPlan plan = dec_plan(a, prefixes, prefix_pages, SCORED);
   plan.own.pre_lens = p.prefix_lens;
   const DecDims& d = plan.own;
   const DecSpace at = dec_space(plan, prefixes, a->dtype, SCORED);
@@ -984,9 +987,16 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
                       SCORED ? (float*)(ws + at.score) : nullptr};
   const unsigned rt = (unsigned)((d.B * d.n + 15) / 16);
   int rc = L("latent_absorb", [&] {
-    hipLaunchKernelGGL((latent_absorb<T, SCORED && sizeof(T) == 2>),
-                       dim3((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt), dim3(256), 0, st, d, (const T*)p.q,
-                       (const T*)p.w_kv, p.lens, p.cos, p.sin, x.qa);
+    const dim3 grid((unsigned)d.H, (unsigned)((d.dc + 63) / 64 + 1), rt);
+    if constexpr (sizeof(T) == 2) {
+      if (d.qn == 2) {
+        hipLaunchKernelGGL((latent_absorb<T, true>), grid, dim3(256), 0, st, d, (const T*)p.q, (const T*)p.w_kv, p.lens,
+                           p.cos, p.sin, x.qa);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((latent_absorb<T, false>), grid, dim3(256), 0, st, d, (const T*)p.q, (const T*)p.w_kv, p.lens,
+                       p.cos, p.sin, x.qa);
   });
   if (rc) return rc;
   auto split = [&](bool front) {
@@ -1001,7 +1011,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     rc = L(plan.many ? "latent_prefix" : "latent_split (prefix)", [&] {
       if constexpr (sizeof(T) == 2) {
         if (plan.many)
-          return launch_prefix(plan.front, prefixes, SCORED, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
+          return launch_prefix(plan.front, prefixes, st, x.qa, p.cache, p.prefix_table, p.prefix_lens, p.lens,
                                d.table * d.page, ws + at.front, x.stat);
       }
       split(true);
@@ -1049,7 +1059,7 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
 
 extern "C" size_t atomic_latent_decode_workspace_size(const atomic_latent_decode_args* a) {
   if (dec_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(a, 0, 0), 0, a->dtype, false).all;
+  return dec_space(dec_plan(a, 0, 0, false), 0, a->dtype, false).all;
 }
 
 extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, const void* w_kv,
@@ -1070,7 +1080,7 @@ extern "C" int atomic_latent_decode(const atomic_latent_decode_args* a, const vo
 
 extern "C" size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a) {
   if (shared_check(a) != ATOMIC_OK) return 0;
-  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages), a->prefixes, a->dec.dtype, a->scored != 0)
+  return dec_space(dec_plan(&a->dec, a->prefixes, a->prefix_pages, a->scored != 0), a->prefixes, a->dec.dtype, a->scored != 0)
       .all;
 }
 

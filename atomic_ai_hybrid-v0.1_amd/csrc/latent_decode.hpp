@@ -12,6 +12,7 @@ struct DecDims {
   int64_t qs[3];
   int share;         // latent_split: sequences whose rows read the same tokens (those of a prefix, or one)
   int slot0, slots;  // its first slot among a row's parts, and all of them
+  int qn;            // rows that a query takes in q_lat: it, and where asked for what its rounding left out
   int part0;         // slots before the first whose part is fp32 (latent_prefix leaves its parts in its own way)
   // prefixes: sequences of each (0: there are none), tokens a split, slots, tokens their table holds, lengths
   int pre_share, pre_chunk, pre_splits, pre_most;
@@ -44,11 +45,10 @@ static __device__ __attribute__((aligned(16))) const uint32_t lat_zeros[8] = {0,
 bool prefix_plan(DecDims& d, int units);
 // Bytes of the parts that it leaves for the join.
 size_t prefix_bytes(const DecDims& d, int units);
-void launch_prefix(const DecDims& d, int units, bool scored, hipStream_t st, const bf16* qa, const void* cache,
-                   const int32_t* table, const int32_t* lens, const int32_t* own, int own_most, void* parts,
-                   float* stat);
+void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
+                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat);
 // Joins them with those of the own tokens (`d`).  `shift`, unless NULL: a correction of each
-// row's sum over the prefix (in its kernel's comment), in eight shares.
+// row's sum over the prefix (in its kernel's comment), in sixteen shares.
 void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
                         const float* part, const float* stat, const int32_t* kv_lens, float* olat, const bf16* qa,
                         float* shift);

@@ -25,7 +25,7 @@ typedef _Float16 Part __attribute__((ext_vector_type(8)));
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
-template <int DC, bool SCORED>
+template <int DC>
 __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, int units,
                                                         const bf16* __restrict__ qa, const bf16* __restrict__ cache,
                                                         const int32_t* __restrict__ table,
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   // 9300 clocks.)
   const uint32_t l0 = lds_addr(lds), wb = 2 * d.dc, rb = 2 * d.dr;
   {
-    const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * (SCORED ? 2 : 1) * wide);
+    const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * 2 * wide);
     const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
@@ -88,10 +88,9 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
 #pragma unroll
     for (int t = 0; t < KS; ++t) qf[t] = t < KC ? LC::row(ac, 0, 16 * t) : LR::row(ar, 0, 16 * (t - KC));
   }
-  // What the rounding of the rotated queries left out enters the scores too where they have to
-  // be exact; that of q_lat is made good in the join.
-  frag ql[SCORED ? KS - KC : 1];
-  if constexpr (SCORED) {
+  // What the rounding of the rotated queries left out enters the scores too.
+  frag ql[KS - KC];
+  {
     const bf16* qr = qa + (((int64_t)seq * each + place) * 2 + 1) * wide + d.dc;
 #pragma unroll
     for (int t = 0; t < KS - KC; ++t) {
@@ -134,7 +133,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
 #pragma unroll
     for (int t = 0; t < KS; ++t) qf[t] = -qf[t];
 #pragma unroll
-    for (int t = 0; t < (SCORED ? KS - KC : 0); ++t) ql[t] = -ql[t];
+    for (int t = 0; t < KS - KC; ++t) ql[t] = -ql[t];
   }
   float m = -INFINITY, sum = 0.f;
   f32x16 s;
@@ -192,7 +191,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   // The scores of tile i in buffer `kb` and the products of the tile before in `vb`, as one run
   // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
   // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
-  constexpr int G = SCORED ? 1 : 2, LA = 2, GS = KS / G, GV = 2 * NT / G;
+  constexpr int G = 1, LA = 2, GS = KS / G, GV = 2 * NT / G;
   auto tile = [&](auto with_k, auto with_v, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
     constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
     uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
@@ -218,7 +217,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
         static_for<G>([&](auto j) {
           constexpr int t = g * G + decltype(j)::value;
           s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[t], s);
-          if constexpr (SCORED && t >= KC) s = M32<bf16>::mma(f[g % (LA + 1)][j.value], ql[t - KC], s);
+          if constexpr (t >= KC) s = M32<bf16>::mma(f[g % (LA + 1)][j.value], ql[t - KC], s);
         });
         if constexpr (g == GS - 1) {
           asm volatile("" : "+v"(s));
@@ -302,14 +301,14 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
 }
 
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
-// tokens joined.  A workgroup takes 32 rows and four of the parts' blocks, one a wave, whose
-// 1 KB a split is one load.
+// tokens joined.  A workgroup takes 32 rows and 32 columns, two of the parts' blocks of 1 KB;
+// a wave has one of them and every other split.
 //
-// Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
+// Where the tokens' weights are gathered, `shift` [rows, 16] receives what q_lat's rounding did
 // to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
 // by c e . c_j, so the log by c e . (sum_j p_j c_j) and, what is left, half the variance of
 // c e . c_j (1.5e-6 for scores of unit spread; uncorrected, the sum was off by 5e-5).
-// Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
+// Each workgroup gives its 32 columns' share.  (As a second number in the scores it would
 // take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
 __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
                                                           const float* __restrict__ scales,
@@ -319,10 +318,10 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
                                                           float* __restrict__ olat, const bf16* __restrict__ qa,
                                                           float* __restrict__ shift) {
   constexpr int NT = 16;
-  constexpr int LD = 68;
+  constexpr int LD = 36;
   __shared__ float refs[32], invs[32], fronts[32];
-  __shared__ __attribute__((aligned(16))) float tile[32 * LD];
-  const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id(), lane = lane_id();
+  __shared__ __attribute__((aligned(16))) float tile[2][32 * LD];
+  const int group = blockIdx.x / 16, k = 2 * (blockIdx.x % 16) + wave_id() % 2, lane = lane_id();
   const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
   if (r0 >= rows) return;
   // a row's reference and sum: eight threads each
@@ -370,53 +369,45 @@ __global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, 
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
     if (32 * (k / 2) < d.dc) {
 #pragma unroll 8
-      for (int s = 0; s < ps.front; ++s) {
+      for (int s = wave_id() / 2; s < ps.front; s += 2) {
         const Part y = from[(int64_t)s * (2 * NT * 64)];
         const float w = fast_exp2(st[2 * (int64_t)s * each] - ref) * sc[(int64_t)s * 32];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += w * (float)y[j];
       }
     }
-    float* to = tile + (lane & 31) * LD + 16 * wave_id() + 4 * (lane >> 5);
+    float* to = tile[wave_id() / 2] + (lane & 31) * LD + 16 * (wave_id() % 2) + 4 * (lane >> 5);
     store4(to, f32x4{x[0], x[1], x[2], x[3]});
     store4(to + 8, f32x4{x[4], x[5], x[6], x[7]});
   }
   __syncthreads();
-  // the own tokens' parts and the result: eight columns of a row a thread
-  const int r = threadIdx.x / 8, c = 64 * (blockIdx.x % 8) + 8 * (threadIdx.x & 7), row = r0 + r;
+  // the own tokens' parts and the result: four columns of a row a thread
+  const int r = threadIdx.x / 8, c4 = 4 * (threadIdx.x & 7), c = 32 * (blockIdx.x % 16) + c4, row = min(r0 + r, rows - 1);
+  const int seq = b * f.share + row / each, place = row % each;
+  const bool here = r0 + r < rows && c < d.dc;
+  f32x4 x = *reinterpret_cast<const f32x4*>(tile[0] + r * LD + c4) + *reinterpret_cast<const f32x4*>(tile[1] + r * LD + c4);
   if (shift) {
-    const float* x = tile + r * LD + (c & 63);
     float dot = 0.f;
-    if (row < rows && c < d.dc) {
-      float lo[8];
-      load8(qa + (((int64_t)(b * f.share + row / each) * each + row % each) * 2 + 1) * (d.dc + d.dr) + c, lo);
+    if (here) {
+      const bf16x4 lo = *reinterpret_cast<const bf16x4*>(qa + (((int64_t)seq * each + place) * 2 + 1) * (d.dc + d.dr) + c);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot += lo[j] * x[j];
+      for (int j = 0; j < 4; ++j) dot += (float)lo[j] * x[j];
     }
 #pragma unroll
     for (int i = 1; i < 8; i *= 2) dot += __shfl_xor(dot, i);
-    if (row < rows && (threadIdx.x & 7) == 0)
-      shift[((int64_t)(b * f.share + row / each) * each + row % each) * 8 + blockIdx.x % 8] =
-          dot * fronts[r] * d.scale * kLog2e;
+    if (r0 + r < rows && (threadIdx.x & 7) == 0)
+      shift[((int64_t)seq * each + place) * 16 + blockIdx.x % 16] = dot * fronts[r] * d.scale * kLog2e;
   }
-  if (row >= rows || c >= d.dc) return;
-  const int seq = b * f.share + row / each, place = row % each;
+  if (!here) return;
   const Parts ps(d, kv_lens, seq);
-  const float ref = refs[r], inv = invs[r];
+  const float ref = refs[r];
   const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
   const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + c;
-  const float* x = tile + r * LD + (c & 63);
-  f32x4 lo = *reinterpret_cast<const f32x4*>(x), hi = *reinterpret_cast<const f32x4*>(x + 4);
-#pragma unroll 4
-  for (int s = ps.front; s < ps.all; ++s) {
-    const float w = fast_exp2(st[2 * (int64_t)ps.slot(s) * each] - ref);
-    const float* y = own + (int64_t)(s - ps.front) * each * d.dc;
-    lo += w * *reinterpret_cast<const f32x4*>(y);
-    hi += w * *reinterpret_cast<const f32x4*>(y + 4);
-  }
-  float* to = olat + ((int64_t)seq * each + place) * d.dc + c;
-  store4(to, lo * inv);
-  store4(to + 4, hi * inv);
+#pragma unroll 8
+  for (int s = ps.front; s < ps.all; ++s)
+    x += fast_exp2(st[2 * (int64_t)ps.slot(s) * each] - ref) *
+         *reinterpret_cast<const f32x4*>(own + (int64_t)(s - ps.front) * each * d.dc);
+  store4(olat + ((int64_t)seq * each + place) * d.dc + c, x * invs[r]);
 }
 
 static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
@@ -425,7 +416,7 @@ static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units *
 
 bool prefix_plan(DecDims& d, int units) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
-  if (rows <= 32 || most < 256 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
+  if (rows <= 32 || most < 2048 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
   const int64_t blocks = (int64_t)prefix_blocks(d) * units;
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
@@ -442,18 +433,12 @@ bool prefix_plan(DecDims& d, int units) {
 
 size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (32 * 512 * 2 + 32 * 4); }
 
-void launch_prefix(const DecDims& d, int units, bool scored, hipStream_t st, const bf16* qa, const void* cache,
-                   const int32_t* table, const int32_t* lens, const int32_t* own, int own_most, void* parts,
-                   float* stat) {
+void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
+                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat) {
   const int blocks = prefix_blocks(d);
   float* scales = (float*)((char*)parts + prefix_tiles(d, units) * (32 * 512 * 2));
-  auto go = [&](auto s) {
-    hipLaunchKernelGGL((latent_prefix<512, decltype(s)::value != 0>), dim3((unsigned)(d.splits * units * blocks)),
-                       dim3(256), 0, st, d, blocks, units, qa, (const bf16*)cache, table, lens, own, own_most,
-                       (Part*)parts, scales, stat);
-  };
-  if (scored) go(IntC<1>());
-  else go(IntC<0>());
+  hipLaunchKernelGGL((latent_prefix<512>), dim3((unsigned)(d.splits * units * blocks)), dim3(256), 0, st, d, blocks,
+                     units, qa, (const bf16*)cache, table, lens, own, own_most, (Part*)parts, scales, stat);
 }
 
 void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
@@ -461,7 +446,7 @@ void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream
                         float* shift) {
   const int blocks = prefix_blocks(f);
   const float* scales = (const float*)((const char*)parts + prefix_tiles(f, units) * (32 * 512 * 2));
-  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 8)), dim3(256), 0, st, f, d, blocks,
+  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 16)), dim3(256), 0, st, f, d, blocks,
                      (const Part*)parts, scales, part, stat, kv_lens, olat, qa, shift);
 }
 
