@@ -609,7 +609,7 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
       float shift = 0.f;
       if (x.shift) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) shift += x.shift[((int64_t)b * rows + r) * 16 + k];
+        for (int k = 0; k < 8; ++k) shift += x.shift[((int64_t)b * rows + r) * 8 + k];
       }
       for (int s = lane & 15; s < ps.all; s += 16) {
         float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
@@ -889,7 +889,7 @@ static DecSpace dec_space(const DecPlan& p, int prefixes, int dtype, bool scored
   s.part = s.stat + up256((scored || d.slots > 1 ? rows * d.slots : 0) * 2 * sizeof(float));
   s.front = s.part + up256(parts * d.dc * sizeof(float));
   s.shift = s.front + (p.many ? up256(prefix_bytes(p.front, prefixes)) : 0);
-  s.score = s.shift + (p.many && scored ? up256(rows * 16 * sizeof(float)) : 0);
+  s.score = s.shift + (p.many && scored ? up256(rows * 8 * sizeof(float)) : 0);
   s.all = s.score + (scored ? (size_t)d.B * tiles * 256 * sizeof(float) : 0);
   return s;
 }

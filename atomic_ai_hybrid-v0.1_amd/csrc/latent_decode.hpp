@@ -48,7 +48,7 @@ size_t prefix_bytes(const DecDims& d, int units);
 void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
                    const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat);
 // Joins them with those of the own tokens (`d`).  `shift`, unless NULL: a correction of each
-// row's sum over the prefix (in its kernel's comment), in sixteen shares.
+// row's sum over the prefix (in its kernel's comment), in eight shares.
 void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
                         const float* part, const float* stat, const int32_t* kv_lens, float* olat, const bf16* qa,
                         float* shift);

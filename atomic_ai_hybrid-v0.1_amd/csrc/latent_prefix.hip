@@ -301,113 +301,133 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
 }
 
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
-// tokens joined.  A workgroup takes 32 rows and 32 columns, two of the parts' blocks of 1 KB;
+// tokens joined.  A workgroup takes 32 rows and 64 columns, four of the parts' blocks of 1 KB;
 // a wave has one of them and every other split.
 //
-// Where the tokens' weights are gathered, `shift` [rows, 16] receives what q_lat's rounding did
+// Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
 // to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
 // by c e . c_j, so the log by c e . (sum_j p_j c_j) and, what is left, half the variance of
 // c e . c_j (1.5e-6 for scores of unit spread; uncorrected, the sum was off by 5e-5).
-// Each workgroup gives its 32 columns' share.  (As a second number in the scores it would
+// Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
 // take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
-__global__ __launch_bounds__(256) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
+__global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
                                                           const float* __restrict__ scales,
                                                           const float* __restrict__ part,
                                                           const float* __restrict__ stat,
                                                           const int32_t* __restrict__ kv_lens,
                                                           float* __restrict__ olat, const bf16* __restrict__ qa,
                                                           float* __restrict__ shift) {
-  constexpr int NT = 16;
-  constexpr int LD = 36;
-  __shared__ float refs[32], invs[32], fronts[32];
+  constexpr int NT = 16, LD = 68;
+  __shared__ float ms[2][32], ss[2][32];
   __shared__ __attribute__((aligned(16))) float tile[2][32 * LD];
-  const int group = blockIdx.x / 16, k = 2 * (blockIdx.x % 16) + wave_id() % 2, lane = lane_id();
+  const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id() % 4, half = wave_id() / 4, lane = lane_id();
   const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
   if (r0 >= rows) return;
-  // a row's reference and sum: eight threads each
-  {
-    const int r = r0 + threadIdx.x / 8, seq = b * f.share + min(r, rows - 1) / each, place = min(r, rows - 1) % each;
-    const Parts ps(d, kv_lens, seq);
-    const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-    float m = -INFINITY, sum = 0.f, front = 0.f;
-    for (int s = threadIdx.x & 7; s < ps.all; s += 8) {
-      const float2 x = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * each);
-      const float mn = fmaxf(m, x.x);
-      if (mn > -INFINITY) {
-        const float fade = fast_exp2(m - mn), add = x.y * fast_exp2(x.x - mn);
-        sum = sum * fade + add;
-        front = front * fade + (s < ps.front ? add : 0.f);
-      }
-      m = mn;
-    }
-#pragma unroll
-    for (int i = 1; i < 8; i *= 2) {
-      const float mo = __shfl_xor(m, i), so = __shfl_xor(sum, i), fo = __shfl_xor(front, i), mn = fmaxf(m, mo);
-      if (mn > -INFINITY) {
-        const float fade = fast_exp2(m - mn), other = fast_exp2(mo - mn);
-        sum = sum * fade + so * other;
-        front = front * fade + fo * other;
-      }
-      m = mn;
-    }
-    if ((threadIdx.x & 7) == 0) {
-      refs[threadIdx.x / 8] = m == -INFINITY ? 0.f : m;
-      invs[threadIdx.x / 8] = sum == 0.f ? 0.f : 1.f / sum;
-      fronts[threadIdx.x / 8] = front == 0.f ? 0.f : 1.f / front;
-    }
-  }
-  __syncthreads();
+  // Both kinds of parts with a reference of their own, so that nothing waits for the other's
+  // statistics: the prefix's, a row a lane,
   {
     const int row = min(r0 + (lane & 31), rows - 1), seq = b * f.share + row / each, place = row % each;
-    const Parts ps(d, kv_lens, seq);
-    const float ref = refs[lane & 31];
+    const int n = Parts(d, kv_lens, seq).front;
     const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-    const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + k * 64 + lane;
+    const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + (32 * (k / 2) < d.dc ? k : 0) * 64 + lane;
     const float* sc = scales + (int64_t)group * f.splits * 32 + (lane & 31);
-    float x[8];
+    float x[8], m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (32 * (k / 2) < d.dc) {
-#pragma unroll 8
-      for (int s = wave_id() / 2; s < ps.front; s += 2) {
-        const Part y = from[(int64_t)s * (2 * NT * 64)];
-        const float w = fast_exp2(st[2 * (int64_t)s * each] - ref) * sc[(int64_t)s * 32];
+    for (int s0 = half; s0 < n; s0 += 16) {
+      Part y[8];
+      float2 a[8];
+      float by[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += w * (float)y[j];
+      for (int i = 0; i < 8; ++i) {  // (splits past the last repeat it, with a weight of zero)
+        const int s = min(s0 + 2 * i, n - 1);
+        a[i] = *reinterpret_cast<const float2*>(st + 2 * (int64_t)s * each);
+        by[i] = sc[(int64_t)s * 32];
+        y[i] = from[(int64_t)s * (2 * NT * 64)];
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, s0 + 2 * i < n ? a[i].x : -INFINITY);
+      const float ref = mn == -INFINITY ? 0.f : mn, fade = fast_exp2(m - ref);
+      m = mn;
+      sum *= fade;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] *= fade;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = s0 + 2 * i < n ? fast_exp2(a[i].x - ref) : 0.f;
+        sum += w * a[i].y;
+        if (w != 0.f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] += w * by[i] * (float)y[i][j];
+        }
       }
     }
-    float* to = tile[wave_id() / 2] + (lane & 31) * LD + 16 * (wave_id() % 2) + 4 * (lane >> 5);
+    float* to = tile[half] + (lane & 31) * LD + 16 * (wave_id() % 4) + 4 * (lane >> 5);
     store4(to, f32x4{x[0], x[1], x[2], x[3]});
     store4(to + 8, f32x4{x[4], x[5], x[6], x[7]});
+    if (wave_id() % 4 == 0 && lane < 32) {
+      ms[half][lane] = m;
+      ss[half][lane] = sum;
+    }
   }
-  __syncthreads();
-  // the own tokens' parts and the result: four columns of a row a thread
-  const int r = threadIdx.x / 8, c4 = 4 * (threadIdx.x & 7), c = 32 * (blockIdx.x % 16) + c4, row = min(r0 + r, rows - 1);
+  // and the own tokens', four columns of a row a thread.
+  const int r = threadIdx.x / 16, c4 = 4 * (threadIdx.x & 15), c = 64 * (blockIdx.x % 8) + c4, row = min(r0 + r, rows - 1);
   const int seq = b * f.share + row / each, place = row % each;
   const bool here = r0 + r < rows && c < d.dc;
-  f32x4 x = *reinterpret_cast<const f32x4*>(tile[0] + r * LD + c4) + *reinterpret_cast<const f32x4*>(tile[1] + r * LD + c4);
+  f32x4 x = zero4();
+  float m = -INFINITY, sum = 0.f;
+  {
+    const Parts ps(d, kv_lens, seq);
+    const float* st = stat + 2 * (((int64_t)seq * d.slots + d.slot0) * each + place);
+    const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + min(c, d.dc - 4);
+    const int n = ps.all - ps.front;
+    for (int s0 = 0; s0 < n; s0 += 8) {
+      f32x4 y[8];
+      float2 a[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = min(s0 + i, n - 1);
+        a[i] = *reinterpret_cast<const float2*>(st + 2 * (int64_t)s * each);
+        y[i] = *reinterpret_cast<const f32x4*>(own + (int64_t)s * each * d.dc);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, s0 + i < n ? a[i].x : -INFINITY);
+      const float ref = mn == -INFINITY ? 0.f : mn, fade = fast_exp2(m - ref);
+      m = mn;
+      sum *= fade;
+      x *= fade;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = s0 + i < n ? fast_exp2(a[i].x - ref) : 0.f;
+        sum += w * a[i].y;
+        if (w != 0.f) x += w * y[i];
+      }
+    }
+  }
+  __syncthreads();
+  const float m0 = ms[0][r], m1 = ms[1][r], mf = fmaxf(m0, m1), all = fmaxf(m, mf);
+  const float rf = mf == -INFINITY ? 0.f : mf, w0 = fast_exp2(m0 - rf), w1 = fast_exp2(m1 - rf);
+  const f32x4 front = w0 * *reinterpret_cast<const f32x4*>(tile[0] + r * LD + c4) +
+                      w1 * *reinterpret_cast<const f32x4*>(tile[1] + r * LD + c4);
+  const float sf = w0 * ss[0][r] + w1 * ss[1][r];
   if (shift) {
     float dot = 0.f;
     if (here) {
       const bf16x4 lo = *reinterpret_cast<const bf16x4*>(qa + (((int64_t)seq * each + place) * 2 + 1) * (d.dc + d.dr) + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) dot += (float)lo[j] * x[j];
+      for (int j = 0; j < 4; ++j) dot += (float)lo[j] * front[j];
     }
 #pragma unroll
-    for (int i = 1; i < 8; i *= 2) dot += __shfl_xor(dot, i);
-    if (r0 + r < rows && (threadIdx.x & 7) == 0)
-      shift[((int64_t)seq * each + place) * 16 + blockIdx.x % 16] = dot * fronts[r] * d.scale * kLog2e;
+    for (int i = 1; i < 16; i *= 2) dot += __shfl_xor(dot, i);
+    if (r0 + r < rows && (threadIdx.x & 15) == 0)
+      shift[((int64_t)seq * each + place) * 8 + blockIdx.x % 8] = sf == 0.f ? 0.f : dot / sf * d.scale * kLog2e;
   }
   if (!here) return;
-  const Parts ps(d, kv_lens, seq);
-  const float ref = refs[r];
-  const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-  const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + c;
-#pragma unroll 8
-  for (int s = ps.front; s < ps.all; ++s)
-    x += fast_exp2(st[2 * (int64_t)ps.slot(s) * each] - ref) *
-         *reinterpret_cast<const f32x4*>(own + (int64_t)(s - ps.front) * each * d.dc);
-  store4(olat + ((int64_t)seq * each + place) * d.dc + c, x * invs[r]);
+  const float ref = all == -INFINITY ? 0.f : all, wf = fast_exp2(mf - ref), wo = fast_exp2(m - ref);
+  const float total = wf * sf + wo * sum;
+  store4(olat + ((int64_t)seq * each + place) * d.dc + c, (wf * front + wo * x) * (total == 0.f ? 0.f : 1.f / total));
 }
 
 static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
@@ -416,7 +436,7 @@ static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units *
 
 bool prefix_plan(DecDims& d, int units) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
-  if (rows <= 32 || most < 2048 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
+  if (rows <= 32 || most < 4096 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
   const int64_t blocks = (int64_t)prefix_blocks(d) * units;
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
@@ -446,7 +466,7 @@ void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream
                         float* shift) {
   const int blocks = prefix_blocks(f);
   const float* scales = (const float*)((const char*)parts + prefix_tiles(f, units) * (32 * 512 * 2));
-  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 16)), dim3(256), 0, st, f, d, blocks,
+  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 8)), dim3(512), 0, st, f, d, blocks,
                      (const Part*)parts, scales, part, stat, kv_lens, olat, qa, shift);
 }
 

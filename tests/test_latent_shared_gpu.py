@@ -96,7 +96,7 @@ CASES = [
 
 
 # rows enough that a prefix's tokens are bound by matrix instructions (wide latents in bf16,
-# tables of 2048 tokens or more, here wider than the prefixes)
+# tables of 4096 tokens or more, here wider than the prefixes)
 MANY = [
     ([256], [0] * 33, 1, 1, 128, 64, 128, 512, 64),                          # 33 rows of one head
     ([300], [0, 40, 2] * 5, 3, 6, 128, 64, 128, 512, 16),                    # queries that stand in the prefix
@@ -108,7 +108,7 @@ MANY = [
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page,most", [(*c, 0) for c in CASES] + [(*c, 2048) for c in MANY])
+@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page,most", [(*c, 0) for c in CASES] + [(*c, 4096) for c in MANY])
 def test_shared_matches_the_formula(pre, own, n, H, dn, dr, dv, dc, page, most, dtype):
     banner(f"latent shared {pre} {own} n{n} H{H} {dn}/{dr}/{dv}/{dc} page {page} {most} {dtype}")
     q, w, cache, pt, pl, table, ln = _case(pre, own, n, H, dn, dr, dv, dc, page, dtype, seed=H + n + pre[0])
@@ -177,7 +177,7 @@ def test_other_scales(scale, dc, H):
     pre, own = [300, 77], [40, 1, 0, 90]
     q, w, cache, pt, pl, table, ln = _case(pre, own, 2, H, 64, 32, 64, dc, 32, BF16, seed=31)
     if dc == 512:
-        pt = torch.cat((pt, pt.new_full((2, 60), 1 << 30)), 1)      # room for 2240 tokens
+        pt = torch.cat((pt, pt.new_full((2, 120), 1 << 30)), 1)     # room for 4160 tokens
     if scale == 3.0:
         o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), scale)
         want, _ = ol.decode_shared(q, w, cache, pt, pl, table, own, scale)
@@ -198,6 +198,7 @@ def test_many_rows_behind_one_prefix(dc):
     banner(f"latent shared many rows {dc}")
     pre, own = [2600], [3 + 5 * i % 40 for i in range(48)]
     q, w, cache, pt, pl, table, ln = _case(pre, own, 1, 32, 64, 32, 64, dc, 64, BF16, seed=32)
+    pt = torch.cat((pt, pt.new_full((1, 30), -7)), 1)
     o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), 0.1)
     want, _ = ol.decode_shared(q, w, cache, pt, pl, table, own, 0.1)
     _rows_within(o, want, U[BF16])
