@@ -42,7 +42,8 @@ def _ptr(t):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle.  (As torch.cuda.current_stream gives it, without the 1.7 us of a Stream object.)"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _strided(t, n):
@@ -430,6 +431,10 @@ def _per_token(what, name, t, B, least, dtype, device):
 def _decode(q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, cos, sin, interleaved, weights,
             workspace, timer):
     _operands("latent decode", ("q", q), ("w_kv", w_kv), ("cache", cache))
+    if q.get_device() != torch.cuda.current_device():      # the library launches on the current device
+        with torch.cuda.device(q.device):
+            return _decode(q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, cos, sin, interleaved,
+                           weights, workspace, timer)
     if q.dim() != 4 or w_kv.dim() != 3 or w_kv.shape[0] != q.shape[2]:
         raise ValueError("latent decode: q must be [B, n, H, dn + dr] and w_kv [H, dn + dv, dc]")
     B, n, H, d = q.shape
@@ -519,6 +524,10 @@ def evict(cache, page_table, kv_lens, weights, order, keep, *, sinks=0, recent=1
         raise ValueError(f"{what}: inputs must be HIP device tensors")
     if cache.dtype not in _DT:
         raise TypeError(f"{what}: cache must be bfloat16 or float32")
+    if cache.get_device() != torch.cuda.current_device():      # the library launches on the current device
+        with torch.cuda.device(cache.device):
+            return evict(cache, page_table, kv_lens, weights, order, keep, sinks=sinks, recent=recent, in_place=in_place,
+                         workspace=workspace, timer=timer)
     if cache.dim() != 3 or cache.requires_grad:
         raise ValueError(f"{what}: cache must be a dense [pages, page, dc + dr], without a gradient")
     _cache(what, cache, cache.shape[2])
