@@ -25,14 +25,17 @@ typedef _Float16 Part __attribute__((ext_vector_type(8)));
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
+struct PrefixLds {
+  char lds[kPreBufs * kPreTokens * (LTile<bf16, 512>::ROWB + LTile<bf16, 64>::ROWB)];
+  uint32_t slot[kPreChunk];
+};
+// Workgroup `id` of those over the prefixes.
 template <int DC>
-__global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, int units,
-                                                        const bf16* __restrict__ qa, const bf16* __restrict__ cache,
-                                                        const int32_t* __restrict__ table,
-                                                        const int32_t* __restrict__ lens,
-                                                        const int32_t* __restrict__ own, int own_most,
-                                                        Part* __restrict__ parts, float* __restrict__ scales,
-                                                        float* __restrict__ stat) {
+__device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, int id, int blocks, int units,
+                                              const bf16* __restrict__ qa, const bf16* __restrict__ cache,
+                                              const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
+                                              const int32_t* __restrict__ own, int own_most, Part* __restrict__ parts,
+                                              float* __restrict__ scales, float* __restrict__ stat) {
   constexpr int DR = 64, KS = (DC + DR) / 16, KC = DC / 16, NT = DC / 32, TK = kPreTokens;
   typedef LTile<bf16, DC> LC;
   typedef LTile<bf16, DR> LR;
@@ -40,11 +43,10 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   constexpr int SC = TK * LC::ROWB, SR = TK * LR::ROWB, STAGE = SC + SR;
   constexpr int PT = TK / 4, NL = PT + 1;  // a wave's tokens of a tile, and its loads
   static_assert(DC == 512, "a latent is one load of a wave");
-  __shared__ __attribute__((aligned(1024))) char lds[kPreBufs * STAGE];
-  __shared__ uint32_t slot[kPreChunk];
+  uint32_t* const slot = mem.slot;
   // the row blocks of a split on one XCD, whose L2 then holds the split's tokens
   int sp, blk;
-  xcd_group_map(blockIdx.x, d.splits * units, blocks, sp, blk);
+  xcd_group_map(id, d.splits * units, blocks, sp, blk);
   const int b = sp / d.splits, wv = wave_id(), lane = lane_id();
   sp %= d.splits;
   const int each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   // The queries of a wave go through the tile buffer of its number, row by row, while the
   // tokens' places are looked up.  (Loaded as fragments, 32 rows an instruction, they took
   // 9300 clocks.)
-  const uint32_t l0 = lds_addr(lds), wb = 2 * d.dc, rb = 2 * d.dr;
+  const uint32_t l0 = lds_addr(mem.lds), wb = 2 * d.dc, rb = 2 * d.dr;
   {
     const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * 2 * wide);
     const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
@@ -300,6 +302,26 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(DecDims d, int blocks, i
   }
 }
 
+// Both kinds of workgroups in one launch, the longer ones first: those over the own tokens
+// begin on each CU as its prefix's part ends.
+template <int MT, bool SCORED>
+__global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, Part* __restrict__ parts,
+                                                        float* __restrict__ scales) {
+  typedef SplitLds<bf16, 512, 4> OwnLds;
+  __shared__ __attribute__((aligned(1024))) char mem[sizeof(PrefixLds) > sizeof(OwnLds) ? sizeof(PrefixLds) : sizeof(OwnLds)];
+  const DecDims& d = c.d;
+  const int front = c.f.splits * c.units * blocks;
+  if ((int)blockIdx.x < front) {
+    prefix_tokens<512>(c.f, *reinterpret_cast<PrefixLds*>(mem), blockIdx.x, blocks, c.units, c.qa, c.cache, c.prefix_table,
+                       c.prefix_lens, c.lens, d.table * d.page, parts, scales, c.stat);
+  } else {
+    const int id = blockIdx.x - front;
+    split_tokens<bf16, 512, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
+                                           id / d.splits / d.groups, c.qa, c.cache, c.table, c.lens, nullptr, 0, c.part,
+                                           c.stat, c.olat, c.score);
+  }
+}
+
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
 // tokens joined.  A workgroup takes 32 rows and 64 columns, four of the parts' blocks of 1 KB;
 // a wave has one of them and every other split.
@@ -448,26 +470,33 @@ bool prefix_plan(DecDims& d, int units) {
     }
   }
   d.splits = (int)((most + d.chunk - 1) / d.chunk);
-  return blocks * d.splits <= INT32_MAX;
+  return blocks * d.splits <= (1 << 30);
 }
 
 size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (32 * 512 * 2 + 32 * 4); }
 
-void launch_prefix(const DecDims& d, int units, hipStream_t st, const bf16* qa, const void* cache, const int32_t* table,
-                   const int32_t* lens, const int32_t* own, int own_most, void* parts, float* stat) {
-  const int blocks = prefix_blocks(d);
-  float* scales = (float*)((char*)parts + prefix_tiles(d, units) * (32 * 512 * 2));
-  hipLaunchKernelGGL((latent_prefix<512>), dim3((unsigned)(d.splits * units * blocks)), dim3(256), 0, st, d, blocks,
-                     units, qa, (const bf16*)cache, table, lens, own, own_most, (Part*)parts, scales, stat);
+void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
+  const int blocks = prefix_blocks(c.f);
+  float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * (32 * 512 * 2));
+  const unsigned grid = (unsigned)(c.d.splits * c.d.groups * c.d.B + c.f.splits * c.units * blocks);
+  auto go = [&](auto m, auto s) {
+    hipLaunchKernelGGL((latent_prefix<decltype(m)::value, decltype(s)::value != 0>), dim3(grid), dim3(256), 0, st, c,
+                       blocks, (Part*)c.parts, scales);
+  };
+  auto rows = [&](auto s) {
+    if (c.own_tiles == 1) go(IntC<1>(), s);
+    else if (c.own_tiles == 2) go(IntC<2>(), s);
+    else go(IntC<4>(), s);
+  };
+  if (scored) rows(IntC<1>());
+  else rows(IntC<0>());
 }
 
-void launch_prefix_join(const DecDims& f, const DecDims& d, int units, hipStream_t st, const void* parts,
-                        const float* part, const float* stat, const int32_t* kv_lens, float* olat, const bf16* qa,
-                        float* shift) {
-  const int blocks = prefix_blocks(f);
-  const float* scales = (const float*)((const char*)parts + prefix_tiles(f, units) * (32 * 512 * 2));
-  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(units * blocks * 4 * 8)), dim3(512), 0, st, f, d, blocks,
-                     (const Part*)parts, scales, part, stat, kv_lens, olat, qa, shift);
+void launch_prefix_join(const PrefixCall& c, hipStream_t st, float* shift) {
+  const int blocks = prefix_blocks(c.f);
+  const float* scales = (const float*)((const char*)c.parts + prefix_tiles(c.f, c.units) * (32 * 512 * 2));
+  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(c.units * blocks * 4 * 8)), dim3(512), 0, st, c.f, c.d, blocks,
+                     (const Part*)c.parts, scales, c.part, c.stat, c.lens, c.olat, c.qa, shift);
 }
 
 }  // namespace ah
