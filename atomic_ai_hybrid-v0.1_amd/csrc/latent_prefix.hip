@@ -302,20 +302,22 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
   }
 }
 
-// Both kinds of workgroups in one launch, the longer ones first: those over the own tokens
-// begin on each CU as its prefix's part ends.
+// Both kinds of workgroups in one launch: `early` of those over the own tokens, up to half a
+// card of them, then those over the prefixes, then the rest of the former.  So half of the CUs
+// begin with the one and end with the other, and what is bound by memory runs beside what is
+// bound by matrix instructions.
 template <int MT, bool SCORED>
-__global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, Part* __restrict__ parts,
+__global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, Part* __restrict__ parts,
                                                         float* __restrict__ scales) {
   typedef SplitLds<bf16, 512, 4> OwnLds;
   __shared__ __attribute__((aligned(1024))) char mem[sizeof(PrefixLds) > sizeof(OwnLds) ? sizeof(PrefixLds) : sizeof(OwnLds)];
   const DecDims& d = c.d;
-  const int front = c.f.splits * c.units * blocks;
-  if ((int)blockIdx.x < front) {
-    prefix_tokens<512>(c.f, *reinterpret_cast<PrefixLds*>(mem), blockIdx.x, blocks, c.units, c.qa, c.cache, c.prefix_table,
+  const int front = c.f.splits * c.units * blocks, at = (int)blockIdx.x - early;
+  if (at >= 0 && at < front) {
+    prefix_tokens<512>(c.f, *reinterpret_cast<PrefixLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
                        c.prefix_lens, c.lens, d.table * d.page, parts, scales, c.stat);
   } else {
-    const int id = blockIdx.x - front;
+    const int id = at < 0 ? (int)blockIdx.x : (int)blockIdx.x - front;
     split_tokens<bf16, 512, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
                                            id / d.splits / d.groups, c.qa, c.cache, c.table, c.lens, nullptr, 0, c.part,
                                            c.stat, c.olat, c.score);
@@ -478,10 +480,11 @@ size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units)
 void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
   const int blocks = prefix_blocks(c.f);
   float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * (32 * 512 * 2));
-  const unsigned grid = (unsigned)(c.d.splits * c.d.groups * c.d.B + c.f.splits * c.units * blocks);
+  const int own = c.d.splits * c.d.groups * c.d.B, early = (own / 2 < 128 ? own / 2 : 128) & ~7;  // (whole rounds of the XCDs)
+  const unsigned grid = (unsigned)(own + c.f.splits * c.units * blocks);
   auto go = [&](auto m, auto s) {
     hipLaunchKernelGGL((latent_prefix<decltype(m)::value, decltype(s)::value != 0>), dim3(grid), dim3(256), 0, st, c,
-                       blocks, (Part*)c.parts, scales);
+                       blocks, early, (Part*)c.parts, scales);
   };
   auto rows = [&](auto s) {
     if (c.own_tiles == 1) go(IntC<1>(), s);
