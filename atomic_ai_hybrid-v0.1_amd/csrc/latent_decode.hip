@@ -254,6 +254,14 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
 // a tile is padded with, and those that see nothing, get infinity), and goes over
 // kWeighTiles tiles.  Reads 4 bytes a row and token, where latent_split read 1152 a token.
 constexpr int kWeighTiles = 16, kMostRows = 4096;
+// Sum over the sixteen lanes of a row, in each of them, by rotations within it (through LDS, as __shfl_xor goes, a
+// tile's 16 of them took as long as its scores).
+template <int CTRL> __device__ __forceinline__ float row_turn(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_sum16(float v) {
+  return row_turn<0x121>(row_turn<0x122>(row_turn<0x124>(row_turn<0x128>(v))));
+}
 struct Weigh {
   int row_tiles, first;  // row tiles of a sequence; latent_up's grid x where its workgroups begin
   const float* score;
@@ -318,9 +326,7 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
 #pragma unroll
   for (int i = 0; i < kWeighTiles / 4; ++i) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int k = 1; k < 16; k *= 2) w[i][r] += __shfl_xor(w[i][r], k);
+    for (int r = 0; r < 4; ++r) w[i][r] = row_sum16(w[i][r]);
     const int j = 16 * (t0 + 4 * i) + tile_row(lane & 3);
     const float add = (lane & 2) ? ((lane & 1) ? w[i][3] : w[i][2]) : ((lane & 1) ? w[i][1] : w[i][0]);
     float* to = x.weights + b * x.stride + j;
