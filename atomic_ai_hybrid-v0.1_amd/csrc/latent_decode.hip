@@ -180,8 +180,9 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
   split_tokens<T, DC, MT, NW, SCORED>(d, lds, blockIdx.x, blockIdx.y, blockIdx.z, qa, cache, table, kv_lens, own,
                                       own_most, part, stat, olat, score);
 }
-// Prefixes and own tokens in one launch, where both are small (a launch less): grid z
-// below `units` are prefixes.
+// Prefixes and own tokens in one launch, where both are small (a launch less): the
+// prefixes' workgroups, then the others.  (One grid with the larger of both in each dimension has
+// empty workgroups; 6000 of them, each of which waits for a CU's LDS, took 45 us.)
 template <typename T, int DC, int MT, int NW, bool SCORED>
 __global__ __launch_bounds__(64 * NW) void latent_split_both(DecDims f, DecDims d, int units, const T* __restrict__ qa,
                                                              const T* __restrict__ cache,
@@ -191,12 +192,12 @@ __global__ __launch_bounds__(64 * NW) void latent_split_both(DecDims f, DecDims 
                                                              const int32_t* __restrict__ kv_lens,
                                                              float* __restrict__ part, float* __restrict__ stat,
                                                              float* __restrict__ olat, float* __restrict__ score) {
-  const bool front = (int)blockIdx.z < units;
-  const int own_most = d.table * d.page;
+  const int of_front = f.splits * f.groups * units;
+  const bool front = (int)blockIdx.x < of_front;
+  const int own_most = d.table * d.page, id = blockIdx.x - (front ? 0 : of_front);
   if (front) d = f;
-  if ((int)blockIdx.x >= d.splits || (int)blockIdx.y >= d.groups) return;
   __shared__ __attribute__((aligned(1024))) SplitLds<T, DC, NW> lds;
-  split_tokens<T, DC, MT, NW, SCORED>(d, lds, blockIdx.x, blockIdx.y, front ? blockIdx.z : blockIdx.z - units, qa,
+  split_tokens<T, DC, MT, NW, SCORED>(d, lds, id % d.splits, id / d.splits % d.groups, id / d.splits / d.groups, qa,
                                       cache, front ? prefix_table : table, front ? prefix_lens : kv_lens,
                                       front ? kv_lens : nullptr, own_most, part, stat, olat, front ? nullptr : score);
 }
@@ -517,6 +518,12 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
   if (!prefixes) return p;
   const int share = a->batch / prefixes;
   p.front_tiles = dec_row_tiles((int64_t)share * a->tokens * a->heads, a->dtype);
+  // (float32, whose matrix instructions are the bound: four waves, with one tile in LDS, where there are tokens
+  // enough to use them.  Us: 624 rows over 2952 tokens 63, with two tiles and waves 151; 931 rows over 2 tokens and
+  // the own tokens of 49 sequences 50, with two, then in one launch, 34.)
+  if (a->dtype != ATOMIC_BF16 && p.front_tiles == 2 && (int64_t)share * a->tokens * a->heads > 32 &&
+      (int64_t)prefix_pages * a->page >= 512)
+    p.front_tiles = 4;
   p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles);
   DecDims many = p.front;
   if (a->dtype == ATOMIC_BF16 && a->dc > 256 && prefix_plan(many, prefixes)) {
@@ -530,7 +537,8 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
   }
   // One launch costs less than what the own tokens lose by the prefix's row tiles while they
   // are few.
-  p.both = !p.many && p.front_tiles <= 2 && p.front.splits && p.own.splits && a->batch + prefixes <= 65535 &&
+  p.both = !p.many && p.front_tiles <= 2 && p.front.splits && p.own.splits &&
+           (int64_t)p.front.splits * p.front.groups * prefixes <= (1 << 29) &&
            (int64_t)a->batch * a->table_pages * a->page <= 32768;
   if (p.both && p.own_tiles != p.front_tiles) {
     p.own_tiles = p.front_tiles;
@@ -631,8 +639,7 @@ static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStrea
     constexpr int MT = decltype(m)::value, NW = MT == 4 ? 4 : 2;
     if constexpr (MT <= 2) {
       if (plan.both) {
-        const dim3 grid((unsigned)(d.splits > f.splits ? d.splits : f.splits),
-                        (unsigned)(d.groups > f.groups ? d.groups : f.groups), (unsigned)(prefixes + d.B));
+        const dim3 grid((unsigned)(d.splits * d.groups * d.B + f.splits * f.groups * prefixes));
         hipLaunchKernelGGL((latent_split_both<T, DC, MT, NW, SCORED>), grid, dim3(64 * NW), 0, st, f, d, prefixes, x.qa,
                            (const T*)p.cache, p.prefix_table, p.prefix_lens, p.table, p.lens, x.part, x.stat, x.olat,
                            x.score);
@@ -652,7 +659,7 @@ static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStrea
   const int mt = front ? plan.front_tiles : plan.own_tiles;
   if (mt == 1) go(IntC<1>());
   else if (mt == 2) go(IntC<2>());
-  else if constexpr (sizeof(T) == 2) go(IntC<4>());
+  else go(IntC<4>());
 }
 
 template <typename T, bool SCORED>

@@ -131,7 +131,9 @@ struct DTile : LTile<T, W, 16> {
 // two are left there for latent_weigh, a wave's 16 x 16 of them as they lie in its registers.
 template <typename T, int DC, int NW> struct SplitLds {
   static constexpr int SC = 16 * DTile<T, DC>::ROWB, SR = 16 * DTile<T, 64>::ROWB;  // one wave's tokens of a tile
-  char sk[2 * NW * (SC + SR)];
+  // two tiles, or one where they do not fit (float32 with four waves, bound by its matrix instructions)
+  static constexpr int NB = sizeof(T) * NW <= 8 ? 2 : 1;
+  char sk[NB * NW * (SC + SR)];
   int32_t spt[kDecPages];
   float sm[NW][16], ss[NW][16];
 };
@@ -152,7 +154,7 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, N
   typedef DTile<T, DR> LR;
   typedef typename M16<T>::frag frag;
   typedef typename M16<T>::half half;
-  constexpr int SC = SplitLds<T, DC, NW>::SC, SR = SplitLds<T, DC, NW>::SR;
+  constexpr int SC = SplitLds<T, DC, NW>::SC, SR = SplitLds<T, DC, NW>::SR, NB = SplitLds<T, DC, NW>::NB;
   char* const sk = lds.sk;
   int32_t* const spt = lds.spt;
   float(*const sm)[16] = lds.sm;
@@ -228,10 +230,10 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, N
   float m = -INFINITY, sum = 0.f;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // the query fragments: no later wait for them drains the tiles
   if (first < end) load(first, 0);
-  if (first + TK < end) load(first + TK, 1);
+  if (NB == 2 && first + TK < end) load(first + TK, 1);
   int buf = 0;
-  for (int k0 = first; k0 < end; k0 += TK, buf ^= 1) {
-    if (k0 + TK < end) vm_wait<IC + IR>();  // this tile is there, the next one in flight
+  for (int k0 = first; k0 < end; k0 += TK, buf ^= NB - 1) {
+    if (NB == 2 && k0 + TK < end) vm_wait<IC + IR>();  // this tile is there, the next one in flight
     else vm_wait<0>();
     if constexpr (MT > 1) bare_barrier();
     f32x4 s[MT];
@@ -327,7 +329,7 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, N
     // every read of this buffer has returned before it is loaded again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if constexpr (MT > 1) bare_barrier();
-    if (k0 + 2 * TK < end) load(k0 + 2 * TK, buf);
+    if (k0 + NB * TK < end) load(k0 + NB * TK, buf);
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);

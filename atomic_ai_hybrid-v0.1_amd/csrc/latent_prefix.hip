@@ -76,7 +76,10 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
   }
   const int len = dec_len(d, lens, b);
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
-  if (first >= end) return;
+  if (first >= end) {
+    vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
+    return;
+  }
   for (int i = threadIdx.x; i < end - first; i += 256) {
     const int j = first + i, pg = j / d.page;
     slot[i] = (uint32_t)min(max(table[(int64_t)b * d.table + pg], 0), d.pages - 1) * d.page + (j - pg * d.page);
@@ -465,7 +468,7 @@ bool prefix_plan(DecDims& d, int units) {
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
     const int64_t wg = blocks * ((most + chunk - 1) / chunk);
-    const double cost = (double)((wg + 255) / 256) * (0.0713 * chunk + 4.4) + 0.035 * (double)wg;
+    const double cost = (double)((wg + 255) / 256) * (0.0713 * chunk + 4.4) + 0.11 * (double)((most + chunk - 1) / chunk);
     if (chunk == 64 || cost < best) {
       best = cost;
       d.chunk = chunk;
