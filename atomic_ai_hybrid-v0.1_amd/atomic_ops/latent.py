@@ -419,8 +419,8 @@ class LatentDecode(torch.autograd.Function):
 
 def _per_token(what, name, t, B, least, dtype, device):
     """Checks a [B, tokens] state whose rows the library reads or writes in place; its row stride."""
-    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or t.shape[1] < least or t.get_device() != device or \
-            t.requires_grad:
+    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or not least <= t.shape[1] < 1 << 31 or \
+            t.get_device() != device or t.requires_grad:
         raise ValueError(f"{what}: {name} must be {str(dtype)[6:]} [{B}, {least} or more] on the inputs' device, "
                          "without a gradient")
     if t.shape[1] > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < t.shape[1]:
@@ -539,8 +539,8 @@ def evict(cache, page_table, kv_lens, weights, order, keep, *, sinks=0, recent=1
     lens = _index(what, "kv_lens", kv_lens, (B,), torch.int32, dev)
     if in_place and lens is not kv_lens:
         raise ValueError(f"{what}: kv_lens must be dense to be written in place")
-    if not 0 <= sinks <= keep or not 0 <= recent <= keep - sinks or keep < 1:
-        raise ValueError(f"{what}: sinks and recent must be 0 or more and together at most keep")
+    if not 1 <= keep <= 1 << 30 or not 0 <= sinks <= keep or not 0 <= recent <= keep - sinks:
+        raise ValueError(f"{what}: keep must be 1 .. 2^30, sinks and recent 0 or more and together at most keep")
     pages, page, row = cache.shape
     ws = _per_token(what, "weights", weights, B, per * page, torch.float32, dev)
     os = _per_token(what, "order", order, B, per * page, torch.int32, dev)

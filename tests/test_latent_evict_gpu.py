@@ -271,6 +271,40 @@ def test_serving_loop():
         assert torch.equal(dev[0].cpu()[table[b].long()[at // page], at % page][:, :dc], torch.stack(held[b])[:, :dc])
 
 
+def test_serving_step_in_a_graph():
+    """The step of the loop above as a captured graph, replayed with new tokens and eager work in between."""
+    banner("latent serving graph")
+    g = torch.Generator().manual_seed(21)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+    B, H, dn, dr, dv, dc, page, keep, per = 6, 20, 64, 32, 64, 512, 16, 40, 3
+    cos, sin = (t.cuda() for t in _tables(6000, dr))
+    w_kv = (torch.randn(H, dn + dv, dc, generator=g) * dc ** -0.5).to(BF16).cuda()
+    front = 4096 // page
+    ids = torch.randperm(front + B * per, generator=g).to(torch.int32).cuda()
+    pt, table = ids[:front].view(1, front), ids[front:].view(B, per)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    state = [r(len(ids), page, dc + dr), table, pt, i32(4090), i32(*[keep] * B), torch.rand(B, per * page, generator=g).cuda(),
+             torch.full((B, per * page), -1, dtype=torch.int32, device="cuda")]
+    tokens = [r(B, dc), r(B, dr), r(B, H, dn + dr)]
+    pos = i32(*[4090 + keep] * B)
+    rest = (keep, w_kv, cos, sin, pos, 8, 2)
+    step = lambda s: _serve(*s, tokens, *rest)
+    twin = [t.clone() for t in state]
+    step([t.clone() for t in state])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(state)
+    for k in range(4):
+        for t in tokens:
+            t.copy_(torch.randn(t.shape, generator=g))
+        pos += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(twin)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(state, twin))
+
+
 def test_nothing_to_do():
     banner("latent evict empty dimensions")
     z = lambda *s, dt=F32: torch.ones(*s, dtype=dt, device="cuda")
@@ -286,7 +320,7 @@ def test_refusals():
     banner("latent evict refusals")
     cache, table, lens, w, o = (t.cuda() for t in _state([50, 20], 16, 96, BF16, seed=12))
     W = w.shape[1]
-    for keep, sinks, recent in ((0, 0, 0), (-1, 0, 0), (5, 6, 0), (5, 0, 6), (5, 3, 3), (5, -1, 0), (5, 0, -1)):
+    for keep, sinks, recent in ((0, 0, 0), (-1, 0, 0), ((1 << 32) + 10, 0, 0), (5, 6, 0), (5, 0, 6), (5, 3, 3), (5, -1, 0), (5, 0, -1)):
         with pytest.raises(ValueError, match="sinks and recent"):
             L.evict(cache, table, lens, w, o, keep, sinks=sinks, recent=recent)
     for bad in (w[:1], w.double(), w[:, :-4], w.cpu(), w[0], w.t().contiguous().t(), w[:1].expand(2, W)):

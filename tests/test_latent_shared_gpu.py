@@ -129,6 +129,9 @@ def test_shared_matches_the_formula(pre, own, n, H, dn, dr, dv, dc, page, most, 
         _rows_within(o, want, U[dtype])
         _rows_within(o2, want, U[dtype])
         _weights_within(got, before, add, own, n, UW[dtype])
+    again, twice = before.cuda(), L.decode_shared(*d, scale, **kw)       # the same bits
+    assert torch.equal(L.decode_shared(*d, scale, weights=again, **kw), o2) and torch.equal(again, got)
+    assert torch.equal(twice, o)
 
 
 DECODES = [
