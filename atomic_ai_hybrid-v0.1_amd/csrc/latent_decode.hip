@@ -775,7 +775,8 @@ extern "C" int atomic_latent_decode_shared(const atomic_latent_shared_args* a, c
                                            size_t workspace_bytes, void* stream) {
   if (int rc = shared_check(a)) return rc;
   if (!q || !w_kv || !cache || !kv_lens || !o || !cos != !sin || (a->dec.table_pages && !page_table) ||
-      (a->prefixes && (!prefix_lens || (a->prefix_pages && !prefix_table))) || (a->scored && !weights))
+      (a->prefixes && (!prefix_lens || (a->prefix_pages && !prefix_table))) || 
+      (a->scored && a->dec.table_pages && !weights))
     return ATOMIC_ERR_NULL;
   if (cos && a->dec.rope_rows < 1) return ATOMIC_ERR_SHAPE;
   if (!aligned16({q, w_kv, cache, cos, sin, o})) return ATOMIC_ERR_SHAPE;

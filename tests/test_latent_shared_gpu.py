@@ -229,6 +229,23 @@ def test_wider_tables_and_lengths_past_them():
     assert (L.decode_shared(q, w, cache, pt[:, :0], pl, none, ln, 0.1) == 0).all()
 
 
+@pytest.mark.parametrize("most", [96, 4096])
+def test_weights_of_no_own_pages(most):
+    """A prefix by itself where weights are asked for: there are none to gather, and o is that of the call
+    whose sequences have pages without tokens."""
+    banner(f"latent shared weights of nothing {most}")
+    q, w, cache, pt, pl, table, ln = (t.cuda() for t in _case([90], [0] * 5, 1, 8, 64, 32, 64, 512, 32, BF16, seed=39))
+    pt = torch.cat((pt, pt.new_full((1, most // 32 - 3), -7)), 1)
+    some = torch.ones(5, 32, device="cuda")
+    want = L.decode_shared(q, w, cache, pt, pl, table, ln, 0.1, weights=some)
+    for wide in (0, 7):
+        weights = torch.ones(5, wide, device="cuda")
+        o = L.decode_shared(q, w, cache, pt, pl, table[:, :0], ln, 0.1, weights=weights)
+        assert ((o.float() - want.float()).norm() <= 4 * U[BF16] * want.float().norm()).item()
+        assert (weights == 1).all()
+    assert (some == 1).all()
+
+
 def test_strided_queries_and_another_stream():
     banner("latent shared strides and streams")
     d = [t.cuda() for t in _case([150], [40, 9, 0], 2, 4, 64, 32, 64, 128, 16, BF16, seed=34)]
