@@ -25,13 +25,21 @@ typedef _Float16 Part __attribute__((ext_vector_type(8)));
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
-struct PrefixLds {
-  char lds[kPreBufs * kPreTokens * (LTile<bf16, 512>::ROWB + LTile<bf16, 64>::ROWB)];
+template <int DC> struct PrefixLds {
+  // (seven tiles of 256 latents, for which there is room, were no faster)
+  char lds[kPreBufs * kPreTokens * (LTile<bf16, DC>::ROWB + LTile<bf16, 64>::ROWB)];
   uint32_t slot[kPreChunk];
 };
+// The address that lane r holds, and those of lanes r and r + 1 in the lower and upper half of a wave.
+__device__ __forceinline__ uint64_t row_at(uint32_t lo, uint32_t hi, int r) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, r) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, r);
+}
+__device__ __forceinline__ uint64_t pair_at(uint32_t lo, uint32_t hi, int r) {
+  return lane_id() < 32 ? row_at(lo, hi, r) : row_at(lo, hi, r + 1);
+}
 // Workgroup `id` of those over the prefixes.
 template <int DC>
-__device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, int id, int blocks, int units,
+__device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& mem, int id, int blocks, int units,
                                               const bf16* __restrict__ qa, const bf16* __restrict__ cache,
                                               const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
                                               const int32_t* __restrict__ own, int own_most, Part* __restrict__ parts,
@@ -41,8 +49,10 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
   typedef LTile<bf16, DR> LR;
   typedef bf16x8 frag;
   constexpr int SC = TK * LC::ROWB, SR = TK * LR::ROWB, STAGE = SC + SR;
-  constexpr int PT = TK / 4, NL = PT + 1;  // a wave's tokens of a tile, and its loads
-  static_assert(DC == 512, "a latent is one load of a wave");
+  constexpr int PL = DC / 8, RL = 64 / PL;      // lanes that load a latent, latents of a load
+  constexpr int NB = kPreBufs;
+  constexpr int PT = TK / 4, NL = PT / RL + 1;  // a wave's tokens of a tile, and its loads
+  static_assert(DC == 512 || DC == 256, "a latent, or two, are one load of a wave");
   uint32_t* const slot = mem.slot;
   // the row blocks of a split on one XCD, whose L2 then holds the split's tokens
   int sp, blk;
@@ -60,11 +70,11 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
     const uint64_t a = (uint64_t)(qa + ((int64_t)seq * each + place) * 2 * wide);
     const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) {
-      const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, r) << 32 |
-                            (uint32_t)__builtin_amdgcn_readlane(lo, r);
-      const uint32_t off = 16 * lane ^ 16 * LC::swz(r);
-      dma16_raw((const void*)(off < wb ? base + off : (uint64_t)lat_zeros), to + r * LC::ROWB);
+    for (int i = 0; i < 32 / RL; ++i) {
+      const int r = RL * i + lane / PL;
+      const uint64_t base = RL == 1 ? row_at(lo, hi, i) : pair_at(lo, hi, 2 * i);
+      const uint32_t off = 16 * (lane % PL) ^ 16 * LC::swz(r);
+      dma16_raw((const void*)(off < wb ? base + off : (uint64_t)lat_zeros), to + RL * i * LC::ROWB);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -114,13 +124,12 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
     hi = (uint32_t)(a >> 32);
   };
   auto send = [&](int i, uint32_t to) __attribute__((always_inline)) {
-    if (i < PT) {
-      const int r = PT * wv + i;
-      const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32 |
-                            (uint32_t)__builtin_amdgcn_readlane(lo, i);
-      uint32_t off = 16 * lane ^ 16 * LC::swz(r);
+    if (i < PT / RL) {
+      const int r = PT * wv + RL * i;
+      uint32_t off = 16 * (lane % PL) ^ 16 * LC::swz(r + lane / PL);
       if (off >= wb) off = 0;  // the padding of a width: the query has zeros there
-      dma16_raw_s(base, off, to + r * LC::ROWB);
+      if constexpr (RL == 1) dma16_raw_s(row_at(lo, hi, i), off, to + r * LC::ROWB);
+      else dma16_raw((const void*)(pair_at(lo, hi, 2 * i) + off), to + r * LC::ROWB);
     } else {
       const int r = PT * wv + lane / 8;
       const uint64_t base = (uint64_t)__shfl(hi, lane / 8) << 32 | (uint32_t)__shfl(lo, lane / 8);
@@ -250,14 +259,14 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
   };
   const int tiles = (end - first + TK - 1) / TK;
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
+  for (int k = 0; k < NB - 1; ++k) {
     look(TK * k);
     aim();
 #pragma unroll
     for (int i = 0; i < NL; ++i) send(i, l0 + k * STAGE);
   }
-  look(TK * 3);
-  vm_wait<2 * NL>();
+  look(TK * (NB - 1));
+  vm_wait<(NB - 2) * NL>();
   bare_barrier();
   tile(IntC<1>(), IntC<0>(), 0, 0, 0, 0);
 #pragma unroll
@@ -265,16 +274,17 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
   p[0] = pn[0];
   p[1] = pn[1];
   for (int i = 1; i < tiles; ++i) {
-    vm_wait<NL>();   // tile i is there (of this wave's loads; behind the barrier, of all)
-    bare_barrier();  // and nobody reads tile i - 2 any more
+    vm_wait<(NB - 3) * NL>();  // tile i is there (of this wave's loads; behind the barrier, of all)
+    bare_barrier();            // and nobody reads tile i - 2 any more
     aim();
-    look(TK * (i + 3));
-    tile(IntC<1>(), IntC<1>(), i % kPreBufs, (i - 1) % kPreBufs, TK * i, l0 + (i + 2) % kPreBufs * STAGE);
+    look(TK * (i + NB - 1));
+    tile(IntC<1>(), IntC<1>(), i % NB, (i - 1) % NB, TK * i, l0 + (i + NB - 2) % NB * STAGE);
     p[0] = pn[0];
     p[1] = pn[1];
   }
-  tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % kPreBufs, 0, 0);
+  tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % NB, 0, 0);
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
+  if (kPreRows * blk + 32 * wv >= rows) return;
   sum += __shfl_xor(sum, 32);
   float big = 0.f;
 #pragma unroll
@@ -309,27 +319,28 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds& mem, 
 // card of them, then those over the prefixes, then the rest of the former.  So half of the CUs
 // begin with the one and end with the other, and what is bound by memory runs beside what is
 // bound by matrix instructions.
-template <int MT, bool SCORED>
+template <int DC, int MT, bool SCORED>
 __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, Part* __restrict__ parts,
                                                         float* __restrict__ scales) {
-  typedef SplitLds<bf16, 512, 4> OwnLds;
-  __shared__ __attribute__((aligned(1024))) char mem[sizeof(PrefixLds) > sizeof(OwnLds) ? sizeof(PrefixLds) : sizeof(OwnLds)];
+  typedef SplitLds<bf16, DC, 4> OwnLds;
+  typedef PrefixLds<DC> PreLds;
+  __shared__ __attribute__((aligned(1024))) char mem[sizeof(PreLds) > sizeof(OwnLds) ? sizeof(PreLds) : sizeof(OwnLds)];
   const DecDims& d = c.d;
   const int front = c.f.splits * c.units * blocks, at = (int)blockIdx.x - early;
   if (at >= 0 && at < front) {
-    prefix_tokens<512>(c.f, *reinterpret_cast<PrefixLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
+    prefix_tokens<DC>(c.f, *reinterpret_cast<PreLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
                        c.prefix_lens, c.lens, d.table * d.page, parts, scales, c.stat);
   } else {
     const int id = at < 0 ? (int)blockIdx.x : (int)blockIdx.x - front;
-    split_tokens<bf16, 512, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
+    split_tokens<bf16, DC, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
                                            id / d.splits / d.groups, c.qa, c.cache, c.table, c.lens, nullptr, 0, c.part,
                                            c.stat, c.olat, c.score);
   }
 }
 
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
-// tokens joined.  A workgroup takes 32 rows and 64 columns, four of the parts' blocks of 1 KB;
-// a wave has one of them and every other split.
+// tokens joined.  A workgroup takes 32 rows and 64 (or 16) columns, four (one) of the parts'
+// blocks of 1 KB; a wave has one of them and every WAYS-th split.
 //
 // Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
 // to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
@@ -337,17 +348,18 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
 // c e . c_j (1.5e-6 for scores of unit spread; uncorrected, the sum was off by 5e-5).
 // Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
 // take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
-__global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
+template <int DC, int COLS, int WAYS>
+__global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
                                                           const float* __restrict__ scales,
                                                           const float* __restrict__ part,
                                                           const float* __restrict__ stat,
                                                           const int32_t* __restrict__ kv_lens,
                                                           float* __restrict__ olat, const bf16* __restrict__ qa,
                                                           float* __restrict__ shift) {
-  constexpr int NT = 16, LD = 68;
-  __shared__ float ms[2][32], ss[2][32];
-  __shared__ __attribute__((aligned(16))) float tile[2][32 * LD];
-  const int group = blockIdx.x / 8, k = 4 * (blockIdx.x % 8) + wave_id() % 4, half = wave_id() / 4, lane = lane_id();
+  constexpr int NT = DC / 32, CB = DC / COLS, NB = COLS / 16, LD = COLS + 4;
+  __shared__ float ms[WAYS][32], ss[WAYS][32];
+  __shared__ __attribute__((aligned(16))) float tile[WAYS][32 * LD];
+  const int group = blockIdx.x / CB, cb = blockIdx.x % CB, k = NB * cb + wave_id() % NB, way = wave_id() / NB, lane = lane_id();
   const int each = d.n * d.H, rows = f.share * each, b = group / (4 * blocks), r0 = 32 * (group % (4 * blocks));
   if (r0 >= rows) return;
   // Both kinds of parts with a reference of their own, so that nothing waits for the other's
@@ -361,20 +373,20 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
     float x[8], m = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    for (int s0 = half; s0 < n; s0 += 16) {
+    for (int s0 = way; s0 < n; s0 += 8 * WAYS) {
       Part y[8];
       float2 a[8];
       float by[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {  // (splits past the last repeat it, with a weight of zero)
-        const int s = min(s0 + 2 * i, n - 1);
+        const int s = min(s0 + WAYS * i, n - 1);
         a[i] = *reinterpret_cast<const float2*>(st + 2 * (int64_t)s * each);
         by[i] = sc[(int64_t)s * 32];
         y[i] = from[(int64_t)s * (2 * NT * 64)];
       }
       float mn = m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, s0 + 2 * i < n ? a[i].x : -INFINITY);
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, s0 + WAYS * i < n ? a[i].x : -INFINITY);
       const float ref = mn == -INFINITY ? 0.f : mn, fade = fast_exp2(m - ref);
       m = mn;
       sum *= fade;
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
       for (int j = 0; j < 8; ++j) x[j] *= fade;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float w = s0 + 2 * i < n ? fast_exp2(a[i].x - ref) : 0.f;
+        const float w = s0 + WAYS * i < n ? fast_exp2(a[i].x - ref) : 0.f;
         sum += w * a[i].y;
         if (w != 0.f) {
 #pragma unroll
@@ -390,16 +402,18 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
         }
       }
     }
-    float* to = tile[half] + (lane & 31) * LD + 16 * (wave_id() % 4) + 4 * (lane >> 5);
+    float* to = tile[way] + (lane & 31) * LD + 16 * (wave_id() % NB) + 4 * (lane >> 5);
     store4(to, f32x4{x[0], x[1], x[2], x[3]});
     store4(to + 8, f32x4{x[4], x[5], x[6], x[7]});
-    if (wave_id() % 4 == 0 && lane < 32) {
-      ms[half][lane] = m;
-      ss[half][lane] = sum;
+    if (wave_id() % NB == 0 && lane < 32) {
+      ms[way][lane] = m;
+      ss[way][lane] = sum;
     }
   }
   // and the own tokens', four columns of a row a thread.
-  const int r = threadIdx.x / 16, c4 = 4 * (threadIdx.x & 15), c = 64 * (blockIdx.x % 8) + c4, row = min(r0 + r, rows - 1);
+  constexpr int RT = COLS / 4;  // threads of a row
+  const bool mine = threadIdx.x < 32 * RT;
+  const int r = threadIdx.x / RT % 32, c4 = 4 * (threadIdx.x % RT), c = COLS * cb + c4, row = min(r0 + r, rows - 1);
   const int seq = b * f.share + row / each, place = row % each;
   const bool here = r0 + r < rows && c < d.dc;
   f32x4 x = zero4();
@@ -408,7 +422,7 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
     const Parts ps(d, kv_lens, seq);
     const float* st = stat + 2 * (((int64_t)seq * d.slots + d.slot0) * each + place);
     const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + min(c, d.dc - 4);
-    const int n = ps.all - ps.front;
+    const int n = mine ? ps.all - ps.front : 0;
     for (int s0 = 0; s0 < n; s0 += 8) {
       f32x4 y[8];
       float2 a[8];
@@ -434,12 +448,19 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
     }
   }
   __syncthreads();
-  const float m0 = ms[0][r], m1 = ms[1][r], mf = fmaxf(m0, m1), all = fmaxf(m, mf);
-  const float rf = mf == -INFINITY ? 0.f : mf, w0 = fast_exp2(m0 - rf), w1 = fast_exp2(m1 - rf);
-  const f32x4 front = w0 * *reinterpret_cast<const f32x4*>(tile[0] + r * LD + c4) +
-                      w1 * *reinterpret_cast<const f32x4*>(tile[1] + r * LD + c4);
-  const float sf = w0 * ss[0][r] + w1 * ss[1][r];
-  if (shift) {
+  if (!mine) return;
+  float mf = ms[0][r], sf = 0.f;
+#pragma unroll
+  for (int i = 1; i < WAYS; ++i) mf = fmaxf(mf, ms[i][r]);
+  const float rf = mf == -INFINITY ? 0.f : mf, all = fmaxf(m, mf);
+  f32x4 front = zero4();
+#pragma unroll
+  for (int i = 0; i < WAYS; ++i) {
+    const float w = fast_exp2(ms[i][r] - rf);
+    front += w * *reinterpret_cast<const f32x4*>(tile[i] + r * LD + c4);
+    sf += w * ss[i][r];
+  }
+  if (COLS == 64 && shift) {
     float dot = 0.f;
     if (here) {
       const bf16x4 lo = *reinterpret_cast<const bf16x4*>(qa + (((int64_t)seq * each + place) * 2 + 1) * (d.dc + d.dr) + c);
@@ -447,9 +468,12 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
       for (int j = 0; j < 4; ++j) dot += (float)lo[j] * front[j];
     }
 #pragma unroll
-    for (int i = 1; i < 16; i *= 2) dot += __shfl_xor(dot, i);
-    if (r0 + r < rows && (threadIdx.x & 15) == 0)
-      shift[((int64_t)seq * each + place) * 8 + blockIdx.x % 8] = sf == 0.f ? 0.f : dot / sf * d.scale * kLog2e;
+    for (int i = 1; i < RT; i *= 2) dot += __shfl_xor(dot, i);
+    float* to = shift + ((int64_t)seq * each + place) * 8;
+    if (r0 + r < rows && c4 == 0) {
+      to[cb] = sf == 0.f ? 0.f : dot / sf * d.scale * kLog2e;
+      if constexpr (CB < 8) to[CB + cb] = 0.f;
+    }
   }
   if (!here) return;
   const float ref = all == -INFINITY ? 0.f : all, wf = fast_exp2(mf - ref), wo = fast_exp2(m - ref);
@@ -458,8 +482,9 @@ __global__ __launch_bounds__(512) void latent_prefix_join(DecDims f, DecDims d, 
 }
 
 static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
-// Rows of 32 times splits: each leaves 32 KB and 32 scales.
+// Rows of 32 times splits: each leaves 32 or 16 KB and 32 scales.
 static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units * prefix_blocks(d) * 4 * d.splits; }
+static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(_Float16); }
 
 bool prefix_plan(DecDims& d, int units) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
@@ -478,16 +503,22 @@ bool prefix_plan(DecDims& d, int units) {
   return blocks * d.splits <= (1 << 30);
 }
 
-size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (32 * 512 * 2 + 32 * 4); }
+size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (tile_bytes(d) + 32 * 4); }
 
 void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
   const int blocks = prefix_blocks(c.f);
-  float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * (32 * 512 * 2));
+  float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * tile_bytes(c.f));
   const int own = c.d.splits * c.d.groups * c.d.B, early = (own / 2 < 128 ? own / 2 : 128) & ~7;  // (whole rounds of the XCDs)
   const unsigned grid = (unsigned)(own + c.f.splits * c.units * blocks);
   auto go = [&](auto m, auto s) {
-    hipLaunchKernelGGL((latent_prefix<decltype(m)::value, decltype(s)::value != 0>), dim3(grid), dim3(256), 0, st, c,
-                       blocks, early, (Part*)c.parts, scales);
+    constexpr int MT = decltype(m)::value;
+    constexpr bool SCORED = decltype(s)::value != 0;
+    if (c.f.dc > 256)
+      hipLaunchKernelGGL((latent_prefix<512, MT, SCORED>), dim3(grid), dim3(256), 0, st, c, blocks, early,
+                         (Part*)c.parts, scales);
+    else
+      hipLaunchKernelGGL((latent_prefix<256, MT, SCORED>), dim3(grid), dim3(256), 0, st, c, blocks, early,
+                         (Part*)c.parts, scales);
   };
   auto rows = [&](auto s) {
     if (c.own_tiles == 1) go(IntC<1>(), s);
@@ -500,9 +531,23 @@ void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
 
 void launch_prefix_join(const PrefixCall& c, hipStream_t st, float* shift) {
   const int blocks = prefix_blocks(c.f);
-  const float* scales = (const float*)((const char*)c.parts + prefix_tiles(c.f, c.units) * (32 * 512 * 2));
-  hipLaunchKernelGGL(latent_prefix_join, dim3((unsigned)(c.units * blocks * 4 * 8)), dim3(512), 0, st, c.f, c.d, blocks,
-                     (const Part*)c.parts, scales, c.part, c.stat, c.lens, c.olat, c.qa, shift);
+  const float* scales = (const float*)((const char*)c.parts + prefix_tiles(c.f, c.units) * tile_bytes(c.f));
+  auto run = [&](auto dc, auto cols, auto ways) {
+    constexpr int DC = decltype(dc)::value, COLS = decltype(cols)::value, WAYS = decltype(ways)::value;
+    hipLaunchKernelGGL((latent_prefix_join<DC, COLS, WAYS>), dim3((unsigned)(c.units * blocks * 4 * (DC / COLS))),
+                       dim3(4 * COLS * WAYS), 0, st, c.f, c.d, blocks, (const Part*)c.parts, scales, c.part, c.stat, c.lens,
+                       c.olat, c.qa, shift);
+  };
+  // Where 64 columns a workgroup leave half of the CUs without one, 16: a CU takes in about 10 bytes a clock.  (Us, 64
+  // rows of 256 latents in 128 splits: 17 and 7; 1024 rows of 512 in 32 splits, 256 workgroups: 11 and 14.)
+  const int64_t rows = (int64_t)c.f.share * c.f.n * c.f.H;
+  const bool few = c.units * ((rows + 31) / 32) * ((c.f.dc + 63) / 64) <= 128 && !shift;
+  auto go = [&](auto dc) {
+    if (few) run(dc, IntC<16>(), IntC<8>());
+    else run(dc, IntC<64>(), IntC<2>());
+  };
+  if (c.f.dc > 256) go(IntC<512>());
+  else go(IntC<256>());
 }
 
 }  // namespace ah

@@ -104,6 +104,10 @@ MANY = [
     ([2049], [17 * i % 50 for i in range(9)], 2, 15, 64, 32, 64, 264, 1),    # 270 rows; a token past a split
     ([33, 500], [20] * 8, 4, 40, 128, 32, 96, 320, 128),
     ([256], [3, 0], 19, 16, 64, 32, 64, 512, 256),                           # more queries than own tokens
+    ([300], [0, 40, 2] * 5, 3, 6, 64, 32, 64, 256, 16),                      # the same with narrow latents
+    ([1, 700, 0, 257], [5, 0, 33, 64] * 3, 1, 20, 56, 24, 72, 200, 24),
+    ([33, 500], [20] * 8, 4, 40, 128, 64, 96, 128, 128),
+    ([256], [70] * 33, 1, 1, 128, 64, 128, 8, 64),
 ]
 
 
@@ -171,7 +175,7 @@ def test_decode_gathers_the_weights(lens, n, H, dn, dr, dv, dc, page, dtype):
     _weights_within(a, torch.zeros_like(before), add, lens, n, UW[dtype])
 
 
-@pytest.mark.parametrize("dc,H", [(128, 4), (512, 18)])
+@pytest.mark.parametrize("dc,H", [(128, 4), (512, 18), (128, 18)])
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
 def test_other_scales(scale, dc, H):
     """Negative, zero, and large enough that single tokens carry a row and its reference moves often
@@ -179,7 +183,7 @@ def test_other_scales(scale, dc, H):
     banner(f"latent shared scale {scale} {dc} {H}")
     pre, own = [300, 77], [40, 1, 0, 90]
     q, w, cache, pt, pl, table, ln = _case(pre, own, 2, H, 64, 32, 64, dc, 32, BF16, seed=31)
-    if dc == 512:
+    if H == 18:
         pt = torch.cat((pt, pt.new_full((2, 120), 1 << 30)), 1)     # room for 4160 tokens
     if scale == 3.0:
         o = L.decode_shared(*(t.cuda() for t in (q, w, cache, pt, pl, table, ln)), scale)
