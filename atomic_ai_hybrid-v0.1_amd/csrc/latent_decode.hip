@@ -220,16 +220,21 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
   if (ok) {
     const int b = (int)(row / rows);
     const Parts ps(d, kv_lens, b);
-    const int64_t at = (int64_t)b * d.slots * rows + row % rows;
-    for (int s = g; s < ps.all; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)ps.slot(s) * rows)]);
+    const int64_t at = (int64_t)b * d.slots * rows + row % rows, own = at + (int64_t)ps.skip * rows;
+    int s = g;
+    for (; s < ps.front; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)s * rows)]);
+    for (; s < ps.all; s += ways) m = fmaxf(m, stat[2 * (own + (int64_t)s * rows)]);
     const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-    for (int s = g; s < ps.all; s += ways) {
-      const int64_t a = at + (int64_t)ps.slot(s) * rows;
+    auto take = [&](int64_t a) {
       const float w = fast_exp2(stat[2 * a] - ref);
       sum += w * stat[2 * a + 1];
       x += w * *reinterpret_cast<const f32x4*>(part + a * d.dc + c);
-    }
+    };
+    s = g;
+#pragma unroll 4
+    for (; s < ps.front; s += ways) take(at + (int64_t)s * rows);
+#pragma unroll 4
+    for (; s < ps.all; s += ways) take(own + (int64_t)s * rows);
   }
   sa[tid] = x;
   sm[tid] = m;
@@ -395,9 +400,13 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
         const int b = (r0 + r) / d.n;
         const Parts ps(d, kv_lens, b);
         const float* p = part + ((int64_t)b * d.slots * rows + (r0 + r) % d.n * d.H + h) * d.dc + c;
+        // (a loop for each kind of parts: with their slots chosen in one the loads were not sent eight at a time)
+        int s = 0;
 #pragma unroll 8
-        for (int s = 0; s < ps.all; ++s)
-          x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)ps.slot(s) * rows * d.dc);
+        for (; s < ps.front; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
+        p += (int64_t)ps.skip * rows * d.dc;
+#pragma unroll 8
+        for (; s < ps.all; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
       } else {
         x = *reinterpret_cast<const f32x4*>(olat + ((int64_t)(r0 + r) * d.H + h) * d.dc + c);
       }
