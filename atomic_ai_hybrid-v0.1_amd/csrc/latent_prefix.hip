@@ -58,6 +58,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   int sp, blk;
   xcd_group_map(id, d.splits * units, blocks, sp, blk);
   const int b = sp / d.splits, wv = wave_id(), lane = lane_id();
+  const int pl = RL == 1 ? lane : lane % PL, lr = RL == 1 ? 0 : lane / PL;  // this lane's piece and latent of a load
   sp %= d.splits;
   const int each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
   const int row = kPreRows * blk + 32 * wv + (lane & 31), at = min(row, rows - 1);
@@ -71,9 +72,9 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
     const uint32_t lo = (uint32_t)a, hi = (uint32_t)(a >> 32), to = l0 + wv * STAGE;
 #pragma unroll
     for (int i = 0; i < 32 / RL; ++i) {
-      const int r = RL * i + lane / PL;
+      const int r = RL * i + lr;
       const uint64_t base = RL == 1 ? row_at(lo, hi, i) : pair_at(lo, hi, 2 * i);
-      const uint32_t off = 16 * (lane % PL) ^ 16 * LC::swz(r);
+      const uint32_t off = 16 * pl ^ 16 * LC::swz(r);
       dma16_raw((const void*)(off < wb ? base + off : (uint64_t)lat_zeros), to + RL * i * LC::ROWB);
     }
 #pragma unroll
@@ -126,7 +127,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   auto send = [&](int i, uint32_t to) __attribute__((always_inline)) {
     if (i < PT / RL) {
       const int r = PT * wv + RL * i;
-      uint32_t off = 16 * (lane % PL) ^ 16 * LC::swz(r + lane / PL);
+      uint32_t off = 16 * pl ^ 16 * LC::swz(r + lr);
       if (off >= wb) off = 0;  // the padding of a width: the query has zeros there
       if constexpr (RL == 1) dma16_raw_s(row_at(lo, hi, i), off, to + r * LC::ROWB);
       else dma16_raw((const void*)(pair_at(lo, hi, 2 * i) + off), to + r * LC::ROWB);
@@ -284,7 +285,6 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   }
   tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % NB, 0, 0);
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
-  if (kPreRows * blk + 32 * wv >= rows) return;
   sum += __shfl_xor(sum, 32);
   float big = 0.f;
 #pragma unroll
@@ -296,6 +296,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   const float up = __builtin_bit_cast(float, (uint32_t)(14 - e + 127) << 23);
   const int64_t group = ((int64_t)b * blocks + blk) * 4 + wv, tile_at = group * d.splits + sp;
   Part* to = parts + tile_at * (2 * NT * 64) + lane;
+  const int columns = kPreRows * blk + 32 * wv < rows ? d.dc : 0;  // (nobody reads a part without rows)
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -303,7 +304,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       Part x;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (_Float16)(acc[n][8 * k + j] * up);
-      if (32 * n < d.dc) to[(2 * n + k) * 64] = x;
+      if (32 * n < columns) to[(2 * n + k) * 64] = x;
     }
   if (lane < 32) {
     scales[tile_at * 32 + lane] = __builtin_bit_cast(float, (uint32_t)(e - 14 + 127) << 23);
