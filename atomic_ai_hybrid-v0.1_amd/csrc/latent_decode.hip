@@ -8,11 +8,12 @@
 //
 // All heads of a sequence read the same cache row, once, as key and as value.
 // Sequences that share a prefix read it together: its rows are then those of all of them
-// (latent_split over the prefix first, then over each sequence's own tokens; the parts of
-// both are joined alike).  Where the tokens' weights are gathered, latent_weigh forms them
-// from the scores, once the rows' sums are known.
+// (latent_split over the prefix and over each sequence's own tokens, in one launch or two, or
+// latent_prefix for both; the parts are joined alike).  Where the tokens' weights are gathered,
+// latent_weigh forms them from the scores, once the rows' sums are known.
 //
-// q_lat is rounded to the operand type, as the MFMA takes it; the probabilities
+// q_lat is rounded to the operand type, as the MFMA takes it (with weights it enters as two
+// such numbers: a score's rounding is one of its weight); the probabilities
 // and o_lat, fp32, enter their products as the sum of two bf16 numbers (the cache's
 // bytes leave the matrix instructions idle; with probabilities of eight bits o was off
 // by 0.0025 of its norm at 64 sequences of up to 8192 tokens, now by 0.0023, of which
@@ -258,7 +259,8 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
 // wave in a fixed order: over the row tiles, then across the 16 rows of a tile.  A
 // workgroup forms the rows' lse from the parts' statistics, sixteen lanes a row (the rows that
 // a tile is padded with, and those that see nothing, get infinity), and goes over
-// kWeighTiles tiles.  Reads 4 bytes a row and token, where latent_split read 1152 a token.
+// kWeighTiles tiles.  Reads 4 bytes a row and token, where latent_split read 1152 a token (64
+// sequences of 8192 tokens, 16 heads: 25 MB, 7 us beside the up-projection's 8).
 constexpr int kWeighTiles = 16, kMostRows = 4096;
 // Sum over the sixteen lanes of a row, in each of them, by rotations within it (through LDS, as __shfl_xor goes, a
 // tile's 16 of them took as long as its scores).
@@ -544,11 +546,14 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
       p.own = own;
     }
   }
-  // One launch costs less than what the own tokens lose by the prefix's row tiles while they
-  // are few.
+  // One launch for both costs less than what the own tokens lose by the prefix's row tiles while they are few: in bf16
+  // up to some 262144 of them (32 rows over 4000 tokens, 32 sequences of own tokens, us, in one launch and in two: 22.9
+  // and 29 of 1024, 42 and 47 of 4096, 69 and 73 of 8192, 126 and 126 of 16384), in float32, bound by the products that an empty row tile has too,
+  // up to some 4096 (32 rows over 777, 16 of 4096: 192 and 76; 24 rows over 1501, 6 of 130: 21 and 34).
   p.both = !p.many && p.front_tiles <= 2 && p.front.splits && p.own.splits &&
            (int64_t)p.front.splits * p.front.groups * prefixes <= (1 << 29) &&
-           (int64_t)a->batch * a->table_pages * a->page <= 32768;
+           (int64_t)a->batch * a->table_pages * a->page <=
+               (a->dtype != ATOMIC_BF16 && p.own_tiles != p.front_tiles ? 4096 : 262144);
   if (p.both && p.own_tiles != p.front_tiles) {
     p.own_tiles = p.front_tiles;
     p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);

@@ -122,8 +122,9 @@ struct DTile : LTile<T, W, 16> {
 // in flight.  64 sequences of up to 8192 tokens, 16 heads: 95 to 97 us for 440 MB,
 // 4.6 TB/s; 4 of 32768: 33 us, 4.6 TB/s; both where a copy reaches 5.0.
 //
-// (float32 with 512 latents: the query's fragments take 144 registers and the
-// accumulators 128; 3 registers lie in scratch memory with MT = 1, 54 with MT = 2.)
+// (With 512 latents the accumulators take 128 registers and the query's fragments 144 in
+// float32 and 144 in bf16 where it enters as two numbers: in scratch memory lie 9 registers with
+// MT = 1 and 60 with more, and 2, 83 and 97 with MT = 1, 2 and 4.)
 //
 // The rows of a launch are those of `share` sequences after one another: one, or all that
 // follow the same prefix (`own`, then, are the lengths of what follows it).  With SCORED the
@@ -131,7 +132,8 @@ struct DTile : LTile<T, W, 16> {
 // two are left there for latent_weigh, a wave's 16 x 16 of them as they lie in its registers.
 template <typename T, int DC, int NW> struct SplitLds {
   static constexpr int SC = 16 * DTile<T, DC>::ROWB, SR = 16 * DTile<T, 64>::ROWB;  // one wave's tokens of a tile
-  // two tiles, or one where they do not fit (float32 with four waves, bound by its matrix instructions)
+  // two tiles, or one where they do not fit (float32 with four waves, bound by its matrix instructions: 624 rows over
+  // 2952 tokens 63 us, with two waves and two tiles 151)
   static constexpr int NB = sizeof(T) * NW <= 8 ? 2 : 1;
   char sk[NB * NW * (SC + SR)];
   int32_t spt[kDecPages];

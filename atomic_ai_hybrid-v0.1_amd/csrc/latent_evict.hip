@@ -10,9 +10,9 @@
 // order of its atomics.  What moves are the kept rows past `keep` only.
 //
 // A table of up to 8192 tokens is selected from by one workgroup a sequence, its keys in
-// registers; a longer one by many (one CU takes in about 10 bytes a clock of what is not in
-// its cache: 131072 tokens took 200 us), with a launch between the steps that need each
-// other's sums.
+// registers (32 sequences of 8192: 13.6 us, in the other way 30); a longer one by many (one
+// CU takes in about 10 bytes a clock of what is not in its cache: 131072 tokens took 200 us,
+// in six launches 27), with a launch between the steps that need each other's sums.
 #include "latent.hpp"
 
 namespace ah {
@@ -182,8 +182,8 @@ __device__ __forceinline__ int64_t cache_piece(const EvictDims& d, const int32_t
 }
 
 // ------------------------------------------------------------------ short tables
-// One sequence, its rows in runs of a wave each.  The loads of all rows are sent before
-// the length is known.  Where few rows can move (`fused`: the step of a full cache) it
+// One sequence, its rows in runs of a wave each: bound by the latency of its steps (10 us with
+// 2048 rows, 14 with 8192).  The loads of all rows are sent before the length is known.  Where few rows can move (`fused`: the step of a full cache) it
 // moves them too, which saves a launch; else it leaves them in `movers` [moves] and `count`.
 template <int NT>
 __global__ __launch_bounds__(NT) void evict_small(EvictDims d, EvictIn in, EvictOut out,
@@ -316,7 +316,9 @@ __global__ __launch_bounds__(NT) void evict_small(EvictDims d, EvictIn in, Evict
     }
   }
 }
-constexpr int kFused = 128;  // rows that evict_small moves itself
+// Rows that evict_small moves itself.  (64 sequences of 2048 tokens and more, us: 9.8 of 1 row each, 22 of 128, 34 of
+// 256; with evict_move 9.8 + 4, 9.7 + 8.7 and 9.4 + 9.6, and a launch's gap.)
+constexpr int kFused = 96;
 
 // ------------------------------------------------------------------ long tables
 // 2048 rows a workgroup; those below `keep` and those from it on are divided apart.  Each
@@ -549,8 +551,8 @@ __global__ __launch_bounds__(256) void evict_emit(EvictDims d, EvictIn in, Evict
   }
 }
 
-// Cache rows, 64 that move a workgroup.  With STATE the moved rows' weights and order
-// as well, and what lies past the length.
+// Cache rows, 64 that move a workgroup: bound by their bytes, read and written in rows that lie
+// scattered (32 sequences of 4100 to 8192 tokens to 2048: 25 us for 107 MB, 4.2 TB/s).  With STATE the moved rows' weights and order as well, and what lies past the length.
 constexpr int kMoveRows = 64;
 template <bool STATE>
 __global__ __launch_bounds__(256) void evict_move(EvictDims d, const int32_t* __restrict__ table,

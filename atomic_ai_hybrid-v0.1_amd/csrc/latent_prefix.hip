@@ -1,6 +1,26 @@
 // The absorbed form over a prefix that many query rows share, for gfx950: with 64
 // sequences of 16 heads a prefix token is read once for 1024 rows, so that matrix
 // instructions bound it (1900 operations a byte), not the cache's bytes.
+//
+// A workgroup takes 128 rows, 32 a wave, and a split of the prefix in tiles of 32 tokens:
+//   s = K q^T      tokens x rows: a lane holds 16 tokens' scores of its row
+//   p = 2^(s - m)  in registers, which are the B operand of the next product as they stand
+//   o^T += C^T p   latents x rows, in the accumulator half of the register file
+// Each MFMA reads 1 KB of LDS, so a tile costs a wave 36 + 32 of them (and 4 for the rest of
+// the rotated queries) and as many reads; all four waves read the same tile, four tiles are
+// in LDS, and loads, reads and MFMAs are spread over each other by hand (`tile`).  The scores of
+// tile i and the products of tile i - 1 are one run, so that the softmax of one lies under
+// the products of the other.  A tile takes 1.95 us, of whose clocks its 72 MFMAs are two
+// thirds.  64 sequences of 16 heads over 32768 tokens and their 512 own ones: 91 us, 0.82
+// PFLOP/s (latent_split took 150 for the prefix alone); over 8192 and up to 1024: 47 us.  What is
+// not tiles is the queries, which have to be there before the first product (128 KB a
+// workgroup), the parts and the own tokens.  More operands read ahead, two chains of scores
+// and, with 256 latents, seven tiles in LDS changed nothing.
+//
+// p enters as one bf16 number: o is off by 0.0024 of its norm instead of 0.0023, as
+// latent_split has it with two (those 32 MFMAs more a tile).  Behind a prefix of 256
+// tokens it would be 0.0027, 1.7 times what the rounding of o alone leaves, of 4096 1.5
+// times: hence prefix_plan's limit.
 #include "latent_decode.hpp"
 
 namespace ah {
@@ -319,7 +339,9 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
 // Both kinds of workgroups in one launch: `early` of those over the own tokens, up to half a
 // card of them, then those over the prefixes, then the rest of the former.  So half of the CUs
 // begin with the one and end with the other, and what is bound by memory runs beside what is
-// bound by matrix instructions.
+// bound by matrix instructions (64 sequences of 16 heads over 8192 tokens and up to 1024 own
+// ones, 47 us.  Whole calls: 32 sequences over 8192 and 2048 tokens with weights 77 us in two
+// launches and 71 in one; 64 over 32768 and 512 132 with the two kinds by turns and 109 so).
 template <int DC, int MT, bool SCORED>
 __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, Part* __restrict__ parts,
                                                         float* __restrict__ scales) {
@@ -487,6 +509,10 @@ static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.
 static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units * prefix_blocks(d) * 4 * d.splits; }
 static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(_Float16); }
 
+// Rows from 33 on (40 rows over 4096 tokens, us with the join: 21, latent_split and its join 30; 32 rows: 20 and 22),
+// prefixes whose table has 4096 tokens or more (above), 32-bit row numbers in LDS.  The tokens are divided by what was
+// measured, in us: 0.0713 a token and 4.4 a workgroup, as many rounds as there are workgroups for 256 CUs, and 0.11 a
+// split in the join.
 bool prefix_plan(DecDims& d, int units) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
   if (rows <= 32 || most < 4096 || (int64_t)d.pages * d.page > UINT32_MAX) return false;

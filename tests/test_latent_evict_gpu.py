@@ -77,6 +77,7 @@ def test_evict_keeps_what_the_oracle_keeps(lens, page, row, keep, sinks, recent,
 
 
 @pytest.mark.parametrize("most,keep", [(2048, 1900), (2049, 1900), (4096, 3000), (4097, 4000), (8192, 8063), (8192, 8064),
+                                       (8192, 8095), (8192, 8096),
                                        (8193, 5000), (8193, 8100), (10240, 2048), (10240, 6144), (12000, 11999), (9000, 1)])
 def test_around_the_limits_of_table_and_budget(most, keep):
     """Tables that one workgroup takes and longer ones, few and many rows to move, budgets that end at a chunk's end."""

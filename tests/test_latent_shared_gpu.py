@@ -111,8 +111,18 @@ MANY = [
 ]
 
 
+# prefixes and own tokens in one launch and in two: up to some 262144 own tokens, in float32, where
+# the two kinds differ in their row tiles, up to 4096
+BOTH = [
+    ([90], [1024, 3, 700, 0], 1, 6, 64, 32, 64, 64, 128),
+    ([90], [1030, 3, 700, 0], 1, 6, 64, 32, 64, 64, 1),
+    ([40], [16384] + [7] * 15, 1, 2, 64, 32, 64, 32, 256),
+    ([40], [16390] + [7] * 15, 1, 2, 64, 32, 64, 32, 1),
+]
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page,most", [(*c, 0) for c in CASES] + [(*c, 4096) for c in MANY])
+@pytest.mark.parametrize("pre,own,n,H,dn,dr,dv,dc,page,most", [(*c, 0) for c in CASES + BOTH] + [(*c, 4096) for c in MANY])
 def test_shared_matches_the_formula(pre, own, n, H, dn, dr, dv, dc, page, most, dtype):
     banner(f"latent shared {pre} {own} n{n} H{H} {dn}/{dr}/{dv}/{dc} page {page} {most} {dtype}")
     q, w, cache, pt, pl, table, ln = _case(pre, own, n, H, dn, dr, dv, dc, page, dtype, seed=H + n + pre[0])
