@@ -537,8 +537,8 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
     p.front_tiles = 4;
   p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles);
   DecDims many = p.front;
-  if (a->dtype == ATOMIC_BF16 && prefix_plan(many, prefixes)) {
-    const DecDims own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, true);
+  const DecDims own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, true);
+  if (a->dtype == ATOMIC_BF16 && prefix_plan(many, prefixes, own)) {
     const int64_t wgs = (int64_t)own.splits * own.groups * a->batch;  // one grid dimension for both
     p.many = many.splits + own.splits > 1 && wgs <= (1 << 30);
     if (p.many) {

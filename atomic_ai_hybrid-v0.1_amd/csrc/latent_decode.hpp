@@ -399,8 +399,8 @@ struct PrefixCall {
   float *part, *stat, *olat, *score;
   void* parts;   // of the prefixes, prefix_bytes
 };
-// Whether it takes the rows of `units` prefixes; divides their tokens for it, if so.
-bool prefix_plan(DecDims& d, int units);
+// Whether it takes the rows of `units` prefixes, beside the own tokens `own`; divides their tokens for it, if so.
+bool prefix_plan(DecDims& d, int units, const DecDims& own);
 // Bytes of the parts that it leaves for the join.
 size_t prefix_bytes(const DecDims& d, int units);
 void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st);

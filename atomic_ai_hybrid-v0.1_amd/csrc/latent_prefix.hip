@@ -12,7 +12,7 @@
 // tile i and the products of tile i - 1 are one run, so that the softmax of one lies under
 // the products of the other.  A tile takes 1.95 us, of whose clocks its 72 MFMAs are two
 // thirds.  64 sequences of 16 heads over 32768 tokens and their 512 own ones: 91 us, 0.82
-// PFLOP/s (latent_split took 150 for the prefix alone); over 8192 and up to 1024: 47 us.  What is
+// PFLOP/s (latent_split took 150 for the prefix alone); over 8192 and up to 1024: 45 us.  What is
 // not tiles is the queries, which have to be there before the first product (128 KB a
 // workgroup), the parts and the own tokens.  More operands read ahead, two chains of scores
 // and, with 256 latents, seven tiles in LDS changed nothing.
@@ -336,11 +336,12 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   }
 }
 
-// Both kinds of workgroups in one launch: `early` of those over the own tokens, up to half a
-// card of them, then those over the prefixes, then the rest of the former.  So half of the CUs
-// begin with the one and end with the other, and what is bound by memory runs beside what is
-// bound by matrix instructions (64 sequences of 16 heads over 8192 tokens and up to 1024 own
-// ones, 47 us.  Whole calls: 32 sequences over 8192 and 2048 tokens with weights 77 us in two
+// Both kinds of workgroups in one launch: those over the prefixes and, on the CUs that they
+// leave and behind them, those over the own tokens.  Where there is a prefix workgroup for every CU,
+// `early` of the others, up to half a card of them, go first: half of the CUs then begin with
+// the one kind and end with the other.  What is bound by memory so runs beside what is bound by
+// matrix instructions (64 sequences of 16 heads over 8192 tokens and up to 1024 own
+// ones, 45 us.  Whole calls: 32 sequences over 8192 and 2048 tokens with weights 77 us in two
 // launches and 71 in one; 64 over 32768 and 512 132 with the two kinds by turns and 109 so).
 template <int DC, int MT, bool SCORED>
 __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, Part* __restrict__ parts,
@@ -510,17 +511,28 @@ static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units *
 static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(_Float16); }
 
 // Rows from 33 on (40 rows over 4096 tokens, us with the join: 21, latent_split and its join 30; 32 rows: 20 and 22),
-// prefixes whose table has 4096 tokens or more (above), 32-bit row numbers in LDS.  The tokens are divided by what was
-// measured, in us: 0.0713 a token and 4.4 a workgroup, as many rounds as there are workgroups for 256 CUs, and 0.11 a
-// split in the join.
-bool prefix_plan(DecDims& d, int units) {
+// prefixes whose table has 4096 tokens or more (above), 32-bit row numbers in LDS.
+//
+// The tokens are divided by what was measured, in us: a workgroup takes 10.5 and 0.061 a token, one over own tokens 7.5
+// and 0.065, the join 0.11 a split.  With fewer than 256 the own tokens fill the other CUs.  `least` is what a perfect
+// division of all of it would take; `longest` what it takes if every own workgroup is as long as its share of the table:
+// CUs without a prefix run own ones meanwhile, what is left follows in rounds.  (64 sequences of 16 heads, 8192 and up to
+// 1024 tokens, launch and join: 59 in splits of 256, 51 of 512, 74 of 1024, 63 of 384; 32768 and 512: 102 of 1024, 108 of
+// 1184, 112 of 1280, 133 of 896; 4 prefixes of 4096, 512 rows each: 55 of 256, 49 of 384, 50 of 512.)
+bool prefix_plan(DecDims& d, int units, const DecDims& own) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
   if (rows <= 32 || most < 4096 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
   const int64_t blocks = (int64_t)prefix_blocks(d) * units;
+  const int64_t others = (int64_t)own.splits * own.groups * own.B;
+  const double other = 0.065 * own.chunk + 7.5;
   double best = 0;
   for (int chunk = 64; chunk <= kPreChunk; chunk += 32) {
-    const int64_t wg = blocks * ((most + chunk - 1) / chunk);
-    const double cost = (double)((wg + 255) / 256) * (0.0713 * chunk + 4.4) + 0.11 * (double)((most + chunk - 1) / chunk);
+    const int64_t splits = (most + chunk - 1) / chunk, wg = blocks * splits;
+    const double each = 0.061 * chunk + 10.5, rounds = (double)((wg + 255) / 256) * each;
+    const double all = ((double)wg * each + (double)others * other) / 256, least = rounds > all ? rounds : all;
+    const int64_t meanwhile = wg % 256 ? (256 - wg % 256) * (int64_t)(each / other + 0.15) : 0;
+    const double longest = rounds + (double)(((others > meanwhile ? others - meanwhile : 0) + 255) / 256) * other;
+    const double cost = 0.7 * least + 0.3 * longest + 0.11 * (double)splits;
     if (chunk == 64 || cost < best) {
       best = cost;
       d.chunk = chunk;
@@ -535,8 +547,9 @@ size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units)
 void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
   const int blocks = prefix_blocks(c.f);
   float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * tile_bytes(c.f));
-  const int own = c.d.splits * c.d.groups * c.d.B, early = (own / 2 < 128 ? own / 2 : 128) & ~7;  // (whole rounds of the XCDs)
-  const unsigned grid = (unsigned)(own + c.f.splits * c.units * blocks);
+  const int own = c.d.splits * c.d.groups * c.d.B, front = c.f.splits * c.units * blocks;
+  const int early = front < 256 ? 0 : (own / 2 < 128 ? own / 2 : 128) & ~7;  // (whole rounds of the XCDs)
+  const unsigned grid = (unsigned)(own + front);
   auto go = [&](auto m, auto s) {
     constexpr int MT = decltype(m)::value;
     constexpr bool SCORED = decltype(s)::value != 0;
