@@ -937,7 +937,8 @@ typedef struct atomic_latent_shared_args {
 size_t atomic_latent_decode_shared_workspace_size(const atomic_latent_shared_args* a);
 
 /* prefix_table int32 [prefixes, prefix_pages], prefix_lens int32 [prefixes] (both NULL
- * without prefixes); weights float32, NULL unless scored. */
+ * without prefixes); weights float32, NULL unless scored (or where no sequence has own
+ * pages: there is nothing to gather then). */
 int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* q, const void* w_kv,
                                 const void* cache, const int32_t* prefix_table, const int32_t* prefix_lens,
                                 const int32_t* page_table, const int32_t* kv_lens, const float* cos,
