@@ -489,8 +489,10 @@ static int dec_row_tiles(int64_t rows, int dtype) {
   return rows <= 16 ? 1 : rows <= 32 || dtype != ATOMIC_BF16 ? 2 : 4;
 }
 
-// (`wide`: four waves a workgroup whatever its row tiles, as in latent_prefix.)
-static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table, int mt, bool wide = false) {
+// (`wide`: four waves a workgroup whatever its row tiles, as in latent_prefix.  `fit`: no second round for a few
+// workgroups.)
+static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share, int table, int mt, bool wide = false,
+                        bool fit = false) {
   DecDims d{a->batch, a->tokens, a->heads, a->dn, a->dr, a->dv, a->dc, a->page, a->pages, table,
             a->rope_rows, a->interleaved, 0, 0, 0, a->scale, {a->q_stride[0], a->q_stride[1], a->q_stride[2]},
             share, 0, 0, 1, 0, 0, 1, 0, 0, nullptr};
@@ -509,6 +511,19 @@ static DecDims dec_dims(const atomic_latent_decode_args* a, int units, int share
   const int64_t chunk = want < tile ? tile : want > kDecChunk ? kDecChunk : want;
   d.chunk = (int)((chunk + tile - 1) / tile * tile);
   d.splits = (int)((most + d.chunk - 1) / d.chunk);
+  // Whole tiles can make a few workgroups more than the card holds, and those a second round: longer splits then.
+  // (Us: 625 float32 rows over 3211 tokens, in 260 workgroups 117, in 170 90; five prefixes of 3445 tokens, 525 rows each,
+  // in 270 70, in 225 54; 94 sequences of 500 tokens, 36 heads, with weights, in 282 74, in 188 54.)
+  const int64_t wg = (int64_t)d.splits * units * d.groups;
+  if (fit && wg > slots && 2 * wg < 3 * slots) {
+    for (int c = d.chunk + tile; c <= kDecChunk; c += tile) {
+      const int64_t s = (most + c - 1) / c;
+      if (s * units * d.groups > slots) continue;
+      d.chunk = c;
+      d.splits = (int)s;
+      break;
+    }
+  }
   d.slots = d.splits;
   return d;
 }
@@ -523,7 +538,8 @@ struct DecPlan {
 static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int prefix_pages, bool scored) {
   DecPlan p{};
   p.own_tiles = dec_row_tiles((int64_t)a->tokens * a->heads, a->dtype);
-  p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
+  // (without prefixes and weights as it always was: a sum's bits follow its splits)
+  p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, false, prefixes || scored);
   const int qn = scored && a->dtype == ATOMIC_BF16 ? 2 : 1;
   p.own.qn = qn;
   if (!prefixes) return p;
@@ -535,7 +551,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
   if (a->dtype != ATOMIC_BF16 && p.front_tiles == 2 && (int64_t)share * a->tokens * a->heads > 32 &&
       (int64_t)prefix_pages * a->page >= 512)
     p.front_tiles = 4;
-  p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles);
+  p.front = dec_dims(a, prefixes, share, prefix_pages, p.front_tiles, false, true);
   DecDims many = p.front;
   const DecDims own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, true);
   if (a->dtype == ATOMIC_BF16 && prefix_plan(many, prefixes, own)) {
@@ -556,7 +572,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
                (a->dtype != ATOMIC_BF16 && p.own_tiles != p.front_tiles ? 4096 : 262144);
   if (p.both && p.own_tiles != p.front_tiles) {
     p.own_tiles = p.front_tiles;
-    p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles);
+    p.own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, false, true);
   }
   p.own.qn = p.front.qn = p.many ? 2 : qn;
   p.own.slot0 = p.front.splits;
