@@ -299,17 +299,17 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
         float2 a = *reinterpret_cast<const float2*>(st + 2 * (int64_t)ps.slot(s) * rows);
         if (s < ps.front) a.x += shift;
         const float mn = fmaxf(m, a.x);
-        if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + a.y * fast_exp2(a.x - mn);
+        sum = mn > -INFINITY ? sum * fast_exp2(m - mn) + a.y * fast_exp2(a.x - mn) : sum + a.y;
         m = mn;
       }
     }
 #pragma unroll
     for (int k = 1; k < 16; k *= 2) {
       const float mo = __shfl_xor(m, k), so = __shfl_xor(sum, k), mn = fmaxf(m, mo);
-      if (mn > -INFINITY) sum = sum * fast_exp2(m - mn) + so * fast_exp2(mo - mn);
+      sum = mn > -INFINITY ? sum * fast_exp2(m - mn) + so * fast_exp2(mo - mn) : sum + so;
       m = mn;
     }
-    // (a NaN among a row's scores stays one)
+    // (a NaN among a row's scores stays one, also where a part has no other: its maximum is -inf then, its sum NaN)
     if ((lane & 15) == 0) lse[r] = sum == 0.f ? INFINITY : m + fast_log2(sum);
   }
   __syncthreads();
