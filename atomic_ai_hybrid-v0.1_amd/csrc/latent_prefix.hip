@@ -58,7 +58,12 @@ __device__ __forceinline__ uint64_t pair_at(uint32_t lo, uint32_t hi, int r) {
   return lane_id() < 32 ? row_at(lo, hi, r) : row_at(lo, hi, r + 1);
 }
 // Workgroup `id` of those over the prefixes.
-template <int DC>
+//
+// p enters its products as one bf16 number, so a row's average of the latents is theirs by the
+// sum of those numbers, `held`.  (By the sum of p itself a row that looks at one token was off
+// by that one's rounding, up to 2^-8.)  Where the tokens' weights are gathered the row's sum has to
+// be that of p, and the products are scaled to it.
+template <int DC, bool SCORED>
 __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& mem, int id, int blocks, int units,
                                               const bf16* __restrict__ qa, const bf16* __restrict__ cache,
                                               const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
@@ -170,7 +175,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
 #pragma unroll
     for (int t = 0; t < KS - KC; ++t) ql[t] = -ql[t];
   }
-  float m = -INFINITY, sum = 0.f;
+  float m = -INFINITY, sum = 0.f, held = 0.f;
   f32x16 s;
   const uint32_t br = LC::row_base(), bp = LR::row_base(), bc = LC::col_base();
   auto mask = [&](int k0) __attribute__((always_inline)) {
@@ -184,15 +189,20 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       }
     }
   };
+  typedef bf16 pair __attribute__((ext_vector_type(2)));
   frag p[2], pn[2];
   auto quad = [&](int k) __attribute__((always_inline)) {  // four tokens' probabilities
     const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float e = fast_exp2(__builtin_fmaf(s[4 * k + j], c2, ref));
-      sum += e;
+      if constexpr (SCORED) sum += e;
       pn[k / 2][4 * (k & 1) + j] = (bf16)e;
     }
+    const pair one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int j = 0; j < 4; j += 2)
+      held = __builtin_amdgcn_fdot2_f32_bf16(pair{pn[k / 2][4 * (k & 1) + j], pn[k / 2][4 * (k & 1) + j + 1]}, one, held, false);
   };
   // A new reference where a score is far above its row's: a whole number, so that what
   // fades, the last tile's probabilities among it, is scaled exactly.
@@ -206,7 +216,8 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       const float mn = fmaxf(m, ceilf(top)), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
       m = mn;
       if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
-      sum *= fade;
+      if constexpr (SCORED) sum *= fade;
+      held *= fade;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -305,12 +316,16 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   }
   tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % NB, 0, 0);
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
-  sum += __shfl_xor(sum, 32);
+  held += __shfl_xor(held, 32);
+  if constexpr (SCORED) sum += __shfl_xor(sum, 32);
+  else sum = held;
+  const float even = SCORED && held != 0.f ? sum / held : 1.f;
   float big = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(acc[n][r]));
+  big *= even;
   big = fmaxf(big, __shfl_xor(big, 32));
   const int e = max((int)(__builtin_bit_cast(uint32_t, big) >> 23), 30) - 127;  // 2^e <= big < 2^(e + 1)
   const float up = __builtin_bit_cast(float, (uint32_t)(14 - e + 127) << 23);
@@ -323,7 +338,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
     for (int k = 0; k < 2; ++k) {
       Part x;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (_Float16)(acc[n][8 * k + j] * up);
+      for (int j = 0; j < 8; ++j) x[j] = (_Float16)(acc[n][8 * k + j] * even * up);
       if (32 * n < columns) to[(2 * n + k) * 64] = x;
     }
   if (lane < 32) {
@@ -352,7 +367,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
   const DecDims& d = c.d;
   const int front = c.f.splits * c.units * blocks, at = (int)blockIdx.x - early;
   if (at >= 0 && at < front) {
-    prefix_tokens<DC>(c.f, *reinterpret_cast<PreLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
+    prefix_tokens<DC, SCORED>(c.f, *reinterpret_cast<PreLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
                        c.prefix_lens, c.lens, d.table * d.page, parts, scales, c.stat);
   } else {
     const int id = at < 0 ? (int)blockIdx.x : (int)blockIdx.x - front;
