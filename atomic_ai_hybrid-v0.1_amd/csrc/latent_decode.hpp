@@ -13,7 +13,7 @@ struct DecDims {
   int share;         // latent_split: sequences whose rows read the same tokens (those of a prefix, or one)
   int slot0, slots;  // its first slot among a row's parts, and all of them
   int qn;            // rows that a query takes in q_lat: it, and where asked for what its rounding left out
-  int part0;         // slots before the first whose part is fp32 (latent_prefix leaves its parts in its own way)
+  int part0;         // slots before the first whose part lies row by row (latent_prefix leaves its parts in its own order)
   // prefixes: sequences of each (0: there are none), tokens a split, slots, tokens their table holds, lengths
   int pre_share, pre_chunk, pre_splits, pre_most;
   const int32_t* pre_lens;

@@ -37,12 +37,6 @@ __device__ __forceinline__ void accum_mul(float& x, float f) {
                : "v"(f));
 }
 
-// Eight numbers of a part: of a lane's query and a block of 32 latent columns those that
-// registers 8 k .. 8 k + 7 of its accumulator hold, as fp16 times a power of two of the row
-// (rounded to 2^-11, a quarter of a bf16's step: 0.0003 of what is off by 0.0024 anyway;
-// in fp32 the parts of 1024 rows were 67 MB, 9 us to write and 25 to join).
-typedef _Float16 Part __attribute__((ext_vector_type(8)));
-
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 
 template <int DC> struct PrefixLds {
@@ -67,8 +61,8 @@ template <int DC, bool SCORED>
 __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& mem, int id, int blocks, int units,
                                               const bf16* __restrict__ qa, const bf16* __restrict__ cache,
                                               const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
-                                              const int32_t* __restrict__ own, int own_most, Part* __restrict__ parts,
-                                              float* __restrict__ scales, float* __restrict__ stat) {
+                                              const int32_t* __restrict__ own, int own_most, f32x4* __restrict__ parts,
+                                              float* __restrict__ stat) {
   constexpr int DR = 64, KS = (DC + DR) / 16, KC = DC / 16, NT = DC / 32, TK = kPreTokens;
   typedef LTile<bf16, DC> LC;
   typedef LTile<bf16, DR> LR;
@@ -320,34 +314,22 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   if constexpr (SCORED) sum += __shfl_xor(sum, 32);
   else sum = held;
   const float even = SCORED && held != 0.f ? sum / held : 1.f;
-  float big = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(acc[n][r]));
-  big *= even;
-  big = fmaxf(big, __shfl_xor(big, 32));
-  const int e = max((int)(__builtin_bit_cast(uint32_t, big) >> 23), 30) - 127;  // 2^e <= big < 2^(e + 1)
-  const float up = __builtin_bit_cast(float, (uint32_t)(14 - e + 127) << 23);
-  const int64_t group = ((int64_t)b * blocks + blk) * 4 + wv, tile_at = group * d.splits + sp;
-  Part* to = parts + tile_at * (2 * NT * 64) + lane;
+  // A part: a lane's accumulators four by four, in the order that they have.
+  const int64_t group = ((int64_t)b * blocks + blk) * 4 + wv;
+  f32x4* to = parts + (group * d.splits + sp) * (4 * NT * 64) + lane;
   const int columns = kPreRows * blk + 32 * wv < rows ? d.dc : 0;  // (nobody reads a part without rows)
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      Part x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (_Float16)(acc[n][8 * k + j] * even * up);
-      if (32 * n < columns) to[(2 * n + k) * 64] = x;
+    for (int k = 0; k < 4; ++k) {
+      f32x4 x = {acc[n][4 * k], acc[n][4 * k + 1], acc[n][4 * k + 2], acc[n][4 * k + 3]};
+      if constexpr (SCORED) x *= even;
+      if (32 * n < columns) to[(4 * n + k) * 64] = x;
     }
-  if (lane < 32) {
-    scales[tile_at * 32 + lane] = __builtin_bit_cast(float, (uint32_t)(e - 14 + 127) << 23);
-    if (row < rows) {
-      const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
-      stat[2 * at] = m;
-      stat[2 * at + 1] = sum;
-    }
+  if (lane < 32 && row < rows) {
+    const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
+    stat[2 * at] = m;
+    stat[2 * at + 1] = sum;
   }
 }
 
@@ -359,8 +341,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
 // ones, 45 us.  Whole calls: 32 sequences over 8192 and 2048 tokens with weights 77 us in two
 // launches and 71 in one; 64 over 32768 and 512 132 with the two kinds by turns and 109 so).
 template <int DC, int MT, bool SCORED>
-__global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, Part* __restrict__ parts,
-                                                        float* __restrict__ scales) {
+__global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, f32x4* __restrict__ parts) {
   typedef SplitLds<bf16, DC, 4> OwnLds;
   typedef PrefixLds<DC> PreLds;
   __shared__ __attribute__((aligned(1024))) char mem[sizeof(PreLds) > sizeof(OwnLds) ? sizeof(PreLds) : sizeof(OwnLds)];
@@ -368,7 +349,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
   const int front = c.f.splits * c.units * blocks, at = (int)blockIdx.x - early;
   if (at >= 0 && at < front) {
     prefix_tokens<DC, SCORED>(c.f, *reinterpret_cast<PreLds*>(mem), at, blocks, c.units, c.qa, c.cache, c.prefix_table,
-                       c.prefix_lens, c.lens, d.table * d.page, parts, scales, c.stat);
+                       c.prefix_lens, c.lens, d.table * d.page, parts, c.stat);
   } else {
     const int id = at < 0 ? (int)blockIdx.x : (int)blockIdx.x - front;
     split_tokens<bf16, DC, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
@@ -378,8 +359,8 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
 }
 
 // o_lat of the rows behind a prefix: latent_prefix's parts and those of the sequences' own
-// tokens joined.  A workgroup takes 32 rows and 64 (or 16) columns, four (one) of the parts'
-// blocks of 1 KB; a wave has one of them and every WAYS-th split.
+// tokens joined.  A workgroup takes 32 rows and 64 (or 16) columns, eight (two) of the parts'
+// blocks of 1 KB; a wave has two of them and every WAYS-th split.
 //
 // Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
 // to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
@@ -388,8 +369,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
 // Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
 // take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
 template <int DC, int COLS, int WAYS>
-__global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f, DecDims d, int blocks, const Part* __restrict__ parts,
-                                                          const float* __restrict__ scales,
+__global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f, DecDims d, int blocks, const f32x4* __restrict__ parts,
                                                           const float* __restrict__ part,
                                                           const float* __restrict__ stat,
                                                           const int32_t* __restrict__ kv_lens,
@@ -407,21 +387,18 @@ __global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f,
     const int row = min(r0 + (lane & 31), rows - 1), seq = b * f.share + row / each, place = row % each;
     const int n = Parts(d, kv_lens, seq).front;
     const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
-    const Part* from = parts + (int64_t)group * f.splits * (2 * NT * 64) + (32 * (k / 2) < d.dc ? k : 0) * 64 + lane;
-    const float* sc = scales + (int64_t)group * f.splits * 32 + (lane & 31);
-    float x[8], m = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    const f32x4* from = parts + (int64_t)group * f.splits * (4 * NT * 64) + (32 * (k / 2) < d.dc ? k : 0) * 128 + lane;
+    f32x4 x[2] = {zero4(), zero4()};
+    float m = -INFINITY, sum = 0.f;
     for (int s0 = way; s0 < n; s0 += 8 * WAYS) {
-      Part y[8];
+      f32x4 y[8][2];
       float2 a[8];
-      float by[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {  // (splits past the last repeat it, with a weight of zero)
         const int s = min(s0 + WAYS * i, n - 1);
         a[i] = *reinterpret_cast<const float2*>(st + 2 * (int64_t)s * each);
-        by[i] = sc[(int64_t)s * 32];
-        y[i] = from[(int64_t)s * (2 * NT * 64)];
+        y[i][0] = from[(int64_t)s * (4 * NT * 64)];
+        y[i][1] = from[(int64_t)s * (4 * NT * 64) + 64];
       }
       float mn = m;
 #pragma unroll
@@ -429,21 +406,21 @@ __global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f,
       const float ref = mn == -INFINITY ? 0.f : mn, fade = fast_exp2(m - ref);
       m = mn;
       sum *= fade;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= fade;
+      x[0] *= fade;
+      x[1] *= fade;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float w = s0 + WAYS * i < n ? fast_exp2(a[i].x - ref) : 0.f;
         sum += w * a[i].y;
         if (w != 0.f) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] += w * by[i] * (float)y[i][j];
+          x[0] += w * y[i][0];
+          x[1] += w * y[i][1];
         }
       }
     }
     float* to = tile[way] + (lane & 31) * LD + 16 * (wave_id() % NB) + 4 * (lane >> 5);
-    store4(to, f32x4{x[0], x[1], x[2], x[3]});
-    store4(to + 8, f32x4{x[4], x[5], x[6], x[7]});
+    store4(to, x[0]);
+    store4(to + 8, x[1]);
     if (wave_id() % NB == 0 && lane < 32) {
       ms[way][lane] = m;
       ss[way][lane] = sum;
@@ -521,9 +498,9 @@ __global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f,
 }
 
 static int prefix_blocks(const DecDims& d) { return (int)(((int64_t)d.share * d.n * d.H + kPreRows - 1) / kPreRows); }
-// Rows of 32 times splits: each leaves 32 or 16 KB and 32 scales.
+// Rows of 32 times splits: each leaves 64 or 32 KB.
 static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units * prefix_blocks(d) * 4 * d.splits; }
-static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(_Float16); }
+static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(float); }
 
 // Rows from 33 on (40 rows over 4096 tokens, us with the join: 21, latent_split and its join 30; 32 rows: 20 and 22),
 // prefixes whose table has 4096 tokens or more (above), 32-bit row numbers in LDS.
@@ -557,11 +534,10 @@ bool prefix_plan(DecDims& d, int units, const DecDims& own) {
   return blocks * d.splits <= (1 << 30);
 }
 
-size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * (tile_bytes(d) + 32 * 4); }
+size_t prefix_bytes(const DecDims& d, int units) { return prefix_tiles(d, units) * tile_bytes(d); }
 
 void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
   const int blocks = prefix_blocks(c.f);
-  float* scales = (float*)((char*)c.parts + prefix_tiles(c.f, c.units) * tile_bytes(c.f));
   const int own = c.d.splits * c.d.groups * c.d.B, front = c.f.splits * c.units * blocks;
   const int early = front < 256 ? 0 : (own / 2 < 128 ? own / 2 : 128) & ~7;  // (whole rounds of the XCDs)
   const unsigned grid = (unsigned)(own + front);
@@ -570,10 +546,10 @@ void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
     constexpr bool SCORED = decltype(s)::value != 0;
     if (c.f.dc > 256)
       hipLaunchKernelGGL((latent_prefix<512, MT, SCORED>), dim3(grid), dim3(256), 0, st, c, blocks, early,
-                         (Part*)c.parts, scales);
+                         (f32x4*)c.parts);
     else
       hipLaunchKernelGGL((latent_prefix<256, MT, SCORED>), dim3(grid), dim3(256), 0, st, c, blocks, early,
-                         (Part*)c.parts, scales);
+                         (f32x4*)c.parts);
   };
   auto rows = [&](auto s) {
     if (c.own_tiles == 1) go(IntC<1>(), s);
@@ -586,11 +562,10 @@ void launch_prefix(const PrefixCall& c, bool scored, hipStream_t st) {
 
 void launch_prefix_join(const PrefixCall& c, hipStream_t st, float* shift) {
   const int blocks = prefix_blocks(c.f);
-  const float* scales = (const float*)((const char*)c.parts + prefix_tiles(c.f, c.units) * tile_bytes(c.f));
   auto run = [&](auto dc, auto cols, auto ways) {
     constexpr int DC = decltype(dc)::value, COLS = decltype(cols)::value, WAYS = decltype(ways)::value;
     hipLaunchKernelGGL((latent_prefix_join<DC, COLS, WAYS>), dim3((unsigned)(c.units * blocks * 4 * (DC / COLS))),
-                       dim3(4 * COLS * WAYS), 0, st, c.f, c.d, blocks, (const Part*)c.parts, scales, c.part, c.stat, c.lens,
+                       dim3(4 * COLS * WAYS), 0, st, c.f, c.d, blocks, (const f32x4*)c.parts, c.part, c.stat, c.lens,
                        c.olat, c.qa, shift);
   };
   // Where 64 columns a workgroup leave half of the CUs without one, 16: a CU takes in about 10 bytes a clock.  (Us, 64

@@ -36,3 +36,30 @@ def test_a_row_that_looks_at_one_token_has_its_length(P, dc, dr, scored):
     want, _ = ol.decode_shared(*d[:5], d[5], [0] * 40, scale)
     along = (o * want).sum(-1) / (want * want).sum(-1)
     assert ((along - 1).abs() <= 4 * 2.0 ** -8 * 128 ** -0.5).all(), (along - 1).abs().max()
+
+
+def _rounded_once(o, want, share=0.03):
+    """All but a share of o are the bf16 numbers nearest to the exact ones.
+
+    An error of e times an output's terms moves its rounding in a share of e / ulp of the
+    cases, ulp at least 2^-8 of an output; over outputs that are normal numbers of the
+    terms' size the mean of their inverses, as far as the error is the smaller one, is
+    0.8 * 2 ln(2^-8 / e).  float32 sums and the two bf16 numbers that p and o_lat each enter
+    as leave e below 2^-16: a share of 0.8 * 2^-8 * 0.8 * 2 * ln(2^8) = 0.03."""
+    assert torch.isfinite(o).all()
+    other = (o.cpu() != want.to(BF16)).double().mean().item()
+    assert other <= share, other
+
+
+@pytest.mark.parametrize("dc,dr", [(512, 64), (256, 32)])
+@pytest.mark.parametrize("P", [1, 40, 4200])
+def test_tokens_of_one_latent(P, dc, dr):
+    """Every token of the prefix carries one latent and a key of its own: whatever the
+    probabilities, o is that latent's value.  So nothing but the parts' sums and o's
+    rounding is left, at any length."""
+    banner(f"latent prefix of one latent {P} {dc}")
+    d = _exact_queries([P], [0] * 40, 1, 2, 64, dr, 128, dc, 64, 51, 4096)
+    cache = d[2]
+    cache[..., :dc] = torch.randn(dc, generator=torch.Generator().manual_seed(P)).to(BF16)
+    o = L.decode_shared(*(t.cuda() for t in d), 0.1)
+    _rounded_once(o, ol.decode_shared(*d[:5], d[5], [0] * 40, 0.1)[0])
