@@ -17,10 +17,12 @@
 // workgroup), the parts and the own tokens.  More operands read ahead, two chains of scores
 // and, with 256 latents, seven tiles in LDS changed nothing.
 //
-// p enters as one bf16 number: o is off by 0.0024 of its norm instead of 0.0023, as
-// latent_split has it with two (those 32 MFMAs more a tile).  Behind a prefix of 256
-// tokens it would be 0.0027, 1.7 times what the rounding of o alone leaves, of 4096 1.5
-// times: hence prefix_plan's limit.
+// From 2048 tokens of a prefix on p enters as one bf16 number: o is off by 0.0025 of its norm
+// behind 2048 to 4096 of them and 0.0024 behind 8192, where latent_split, which has two, is at
+// 0.0023 to 0.0024 and o's own rounding at 0.0017 (the rest is q_lat's).  Behind 64 to 1024 it
+// was 0.0025 to 0.0027; there p is two numbers here too, whatever the table's width, and o off
+// by 0.0022 (with one, 32 of 104 MFMAs a tile less: four prefixes of 2049 to 4096 tokens, 512
+// rows each, 61 us a call, and 68 with two).
 #include "latent_decode.hpp"
 
 namespace ah {
@@ -38,6 +40,7 @@ __device__ __forceinline__ void accum_mul(float& x, float f) {
 }
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
+constexpr int kPreOne = 2048;  // tokens of a prefix from which on p enters as one bf16 number
 
 template <int DC> struct PrefixLds {
   // (seven tiles of 256 latents, for which there is room, were no faster)
@@ -183,20 +186,32 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       }
     }
   };
+  // All tiles, with p as NP bf16 numbers.
   typedef bf16 pair __attribute__((ext_vector_type(2)));
-  frag p[2], pn[2];
+  auto walk = [&](auto numbers) __attribute__((always_inline)) {
+  constexpr int NP = decltype(numbers)::value;
+  frag p[2], pn[NP][2];  // the last tile's, and this one's
   auto quad = [&](int k) __attribute__((always_inline)) {  // four tokens' probabilities
     const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float e = fast_exp2(__builtin_fmaf(s[4 * k + j], c2, ref));
+      float e = fast_exp2(__builtin_fmaf(s[4 * k + j], c2, ref));
       if constexpr (SCORED) sum += e;
-      pn[k / 2][4 * (k & 1) + j] = (bf16)e;
+#pragma unroll
+      for (int u = 0; u < NP; ++u) {
+        const bf16 h = (bf16)e;
+        pn[u][k / 2][4 * (k & 1) + j] = h;
+        e -= (float)h;
+      }
     }
     const pair one = {(bf16)1.f, (bf16)1.f};
 #pragma unroll
-    for (int j = 0; j < 4; j += 2)
-      held = __builtin_amdgcn_fdot2_f32_bf16(pair{pn[k / 2][4 * (k & 1) + j], pn[k / 2][4 * (k & 1) + j + 1]}, one, held, false);
+    for (int u = 0; u < NP; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const int at = 4 * (k & 1) + j;
+        held = __builtin_amdgcn_fdot2_f32_bf16(pair{pn[u][k / 2][at], pn[u][k / 2][at + 1]}, one, held, false);
+      }
   };
   // A new reference where a score is far above its row's: a whole number, so that what
   // fades, the last tile's probabilities among it, is scaled exactly.
@@ -212,10 +227,12 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
       if constexpr (SCORED) sum *= fade;
       held *= fade;
+      if constexpr (NP == 1) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[k][j] = (bf16)((float)p[k][j] * fade);
+          for (int j = 0; j < 8; ++j) p[k][j] = (bf16)((float)p[k][j] * fade);
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -232,7 +249,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
   // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
   constexpr int G = 1, LA = 2, GS = KS / G, GV = 2 * NT / G;
-  auto tile = [&](auto with_k, auto with_v, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
+  auto tile = [&](auto with_k, auto with_v, auto sends, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
     constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
     uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
     asm volatile("" : "+v"(ac), "+v"(ar), "+v"(av));
@@ -252,7 +269,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < NL; ++j)
-          if (decltype(with_v)::value && j * GS / NL == g) send(j, to);
+          if (decltype(sends)::value && j * GS / NL == g) send(j, to);
         if constexpr (g == 0) s = zero16();
         static_for<G>([&](auto j) {
           constexpr int t = g * G + decltype(j)::value;
@@ -262,16 +279,19 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
         if constexpr (g == GS - 1) {
           asm volatile("" : "+v"(s));
           mask(k0);
-          settle(with_v);
+          settle(sends);  // (the first tile sends no other)
         }
       } else {
         if constexpr (decltype(with_k)::value && (g - GS) % (GV / 4) == 1) quad((g - GS) / (GV / 4));
         static_for<G>([&](auto j) {
           constexpr int v = (g - GS) * G + decltype(j)::value;
-          acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], p[v / NT], acc[v % NT]);
+          if constexpr (NP == 1) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], p[v / NT], acc[v % NT]);
+          else
+#pragma unroll
+            for (int u = 0; u < NP; ++u) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], pn[u][v / NT], acc[v % NT]);
         });
         __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
-        static_for<G>([&](auto) {
+        static_for<NP * G>([&](auto) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
           __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector
         });
@@ -294,21 +314,38 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   look(TK * (NB - 1));
   vm_wait<(NB - 2) * NL>();
   bare_barrier();
-  tile(IntC<1>(), IntC<0>(), 0, 0, 0, 0);
+  const IntC<0> no;
+  const IntC<1> yes;
+  tile(yes, no, no, 0, 0, 0, 0);
 #pragma unroll
   for (int k = 0; k < 4; ++k) quad(k);
-  p[0] = pn[0];
-  p[1] = pn[1];
+  if constexpr (NP == 1) {
+    p[0] = pn[0][0];
+    p[1] = pn[0][1];
+  } else {
+    tile(no, yes, no, 0, 0, 0, 0);
+  }
   for (int i = 1; i < tiles; ++i) {
     vm_wait<(NB - 3) * NL>();  // tile i is there (of this wave's loads; behind the barrier, of all)
     bare_barrier();            // and nobody reads tile i - 2 any more
     aim();
     look(TK * (i + NB - 1));
-    tile(IntC<1>(), IntC<1>(), i % NB, (i - 1) % NB, TK * i, l0 + (i + NB - 2) % NB * STAGE);
-    p[0] = pn[0];
-    p[1] = pn[1];
+    const uint32_t to = l0 + (i + NB - 2) % NB * STAGE;
+    if constexpr (NP == 1) {
+      tile(yes, yes, yes, i % NB, (i - 1) % NB, TK * i, to);
+      p[0] = pn[0][0];
+      p[1] = pn[0][1];
+    } else {  // (the products of the same tile: two numbers of two tiles would be 16 registers more)
+      tile(yes, no, yes, i % NB, 0, TK * i, to);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) quad(k);
+      tile(no, yes, no, 0, i % NB, 0, 0);
+    }
   }
-  tile(IntC<0>(), IntC<1>(), 0, (tiles - 1) % NB, 0, 0);
+  if constexpr (NP == 1) tile(no, yes, no, 0, (tiles - 1) % NB, 0, 0);
+  };
+  if (len < kPreOne) walk(IntC<2>());
+  else walk(IntC<1>());
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
   held += __shfl_xor(held, 32);
   if constexpr (SCORED) sum += __shfl_xor(sum, 32);
@@ -503,7 +540,7 @@ static size_t prefix_tiles(const DecDims& d, int units) { return (size_t)units *
 static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256) * sizeof(float); }
 
 // Rows from 33 on (40 rows over 4096 tokens, us with the join: 21, latent_split and its join 30; 32 rows: 20 and 22),
-// prefixes whose table has 4096 tokens or more (above), 32-bit row numbers in LDS.
+// prefixes whose table has 4096 tokens or more (the host does not know their lengths), 32-bit row numbers in LDS.
 //
 // The tokens are divided by what was measured, in us: a workgroup takes 10.5 and 0.061 a token, one over own tokens 7.5
 // and 0.065, the join 0.11 a split.  With fewer than 256 the own tokens fill the other CUs.  `least` is what a perfect

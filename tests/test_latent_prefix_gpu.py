@@ -63,3 +63,17 @@ def test_tokens_of_one_latent(P, dc, dr):
     cache[..., :dc] = torch.randn(dc, generator=torch.Generator().manual_seed(P)).to(BF16)
     o = L.decode_shared(*(t.cuda() for t in d), 0.1)
     _rounded_once(o, ol.decode_shared(*d[:5], d[5], [0] * 40, 0.1)[0])
+
+
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("dc,dr", [(512, 64), (256, 32), (72, 24)])
+@pytest.mark.parametrize("most", [0, 4096])
+def test_a_short_prefix_in_a_wide_table(most, dc, dr, scored):
+    """p enters as two bf16 numbers behind a prefix of fewer than 2048 tokens, however many its table has
+    room for, so o has no other rounding than its own in either table (the queries having none)."""
+    banner(f"latent prefix short in a table of {most} {dc} {scored}")
+    pre, own = [33, 64, 1, 300, 0, 700], [17 * i % 50 for i in range(30)]
+    d = _exact_queries(pre, own, 1, 8, 64, dr, 128, dc, 16, 52, most)
+    weights = torch.zeros(30, d[5].shape[1] * 16, device="cuda") if scored else None
+    o = L.decode_shared(*(t.cuda() for t in d), 0.1, weights=weights)
+    _rounded_once(o, ol.decode_shared(*d[:5], d[5], own, 0.1)[0])
