@@ -530,6 +530,8 @@ def evict(cache, page_table, kv_lens, weights, order, keep, *, sinks=0, recent=1
                          workspace=workspace, timer=timer)
     if cache.dim() != 3 or cache.requires_grad:
         raise ValueError(f"{what}: cache must be a dense [pages, page, dc + dr], without a gradient")
+    if _tangents(cache, weights):
+        raise NotImplementedError(f"{what}: no tangents in forward mode: cache and weights must have none")
     _cache(what, cache, cache.shape[2])
     dev = cache.get_device()
     if page_table.dim() != 2:

@@ -2,6 +2,7 @@
 have: what a part holds that has nothing else in it, and calls that reach few of the paths."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from _util import banner
 from atomic_ops import latent as L
@@ -35,3 +36,21 @@ def test_a_nan_that_is_alone_in_its_part_stays_one(where, at, most, dtype):
     assert torch.equal(torch.isnan(o.cpu()), torch.isnan(want))
     assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want_w))
     assert torch.isnan(want_w[0, :own[0]]).all() and not torch.isnan(want_w[0, own[0]:]).any()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("which", ["cache", "weights"])
+def test_evict_refuses_tangents(which, in_place):
+    """A row that moves would leave its tangent with another token's row."""
+    banner(f"latent evict tangents {which} {in_place}")
+    state = {"cache": torch.randn(4, 16, 96, device="cuda"),
+             "table": torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2),
+             "lens": torch.tensor([32, 20], dtype=torch.int32, device="cuda"), "weights": torch.rand(2, 32, device="cuda"),
+             "order": torch.full((2, 32), -1, dtype=torch.int32, device="cuda")}
+    before = {k: t.clone() for k, t in state.items()}
+    with forward_ad.dual_level():
+        given = {**state, which: forward_ad.make_dual(state[which], torch.ones_like(state[which]))}
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            L.evict(*given.values(), 8, in_place=in_place)
+    assert all(torch.equal(state[k], before[k]) for k in state)
+    assert L.evict(*state.values(), 8, in_place=in_place)[0].tolist() == [8, 8]
