@@ -164,6 +164,10 @@ def forward(q, kv, k_pe, scale, *, causal=True, q_lens=None, kv_lens=None, save=
     weight of zero times it).  Inputs of any batch, token and head strides are
     read in place."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
+    if q.get_device() != torch.cuda.current_device():      # the library launches on the current device
+        with torch.cuda.device(q.device):
+            return forward(q, kv, k_pe, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens, save=save,
+                           workspace=workspace, timer=timer)
     lib = _lib.load()
     if not (q.numel() and kv.numel()):      # no queries, or none that sees a key
         o = q.new_zeros(*q.shape[:3], kv.shape[3] - (q.shape[3] - k_pe.shape[2]))
@@ -196,6 +200,10 @@ def backward(q, kv, k_pe, o, lse, dout, scale, *, causal=True, q_lens=None, kv_l
     single key gives its score a gradient of exactly zero.  The same inputs give the
     same bits."""
     q_lens, kv_lens = _check(q, kv, k_pe, q_lens, kv_lens)
+    if q.get_device() != torch.cuda.current_device():      # the library launches on the current device
+        with torch.cuda.device(q.device):
+            return backward(q, kv, k_pe, o, lse, dout, scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens, rest=rest,
+                            workspace=workspace, timer=timer)
     B, T, H, d = q.shape
     dv = kv.shape[3] - (d - k_pe.shape[2])
     _operands("latent attention", ("q", q), ("o", o), ("dout", dout))
@@ -318,6 +326,9 @@ class LatentAppend(torch.autograd.Function):
 def _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer):
     named = [("k_pe", k_pe)] + [(n, t) for n, t in (("c_kv", c_kv), ("cache", cache), ("q", q)) if t is not None]
     _operands("latent append", *named)
+    if k_pe.get_device() != torch.cuda.current_device():      # the library launches on the current device
+        with torch.cuda.device(k_pe.device):
+            return _append(cache, c_kv, k_pe, slots, positions, cos, sin, q, interleaved, timer)
     if k_pe.dim() != 2:
         raise ValueError("latent append: k_pe must be [N, dr]")
     N, dr = k_pe.shape

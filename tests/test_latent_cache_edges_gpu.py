@@ -54,3 +54,46 @@ def test_evict_refuses_tangents(which, in_place):
             L.evict(*given.values(), 8, in_place=in_place)
     assert all(torch.equal(state[k], before[k]) for k in state)
     assert L.evict(*state.values(), 8, in_place=in_place)[0].tolist() == [8, 8]
+
+
+@pytest.mark.parametrize("call", ["forward", "backward", "attention", "append", "decode", "decode_shared", "evict"])
+def test_tensors_of_another_device_than_the_current_one(call, monkeypatch):
+    """The library launches on the current device: each call makes the tensors' device it for that
+    long.  (With one card the current one is said to be another.)"""
+    banner(f"latent on another device {call}")
+    r = lambda *s: torch.randn(*s, dtype=BF16, device="cuda")
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    qkv = r(1, 5, 2, 96), r(1, 5, 2, 128), r(1, 5, 32)
+    q, w, cache, table, lens = r(1, 1, 2, 96), r(2, 128, 64), r(4, 16, 96), i(0, 1)[None], i(20)
+    o, lse, rest = L.forward(*qkv, 0.1, save=True)
+    dout = r(1, 5, 2, 64)
+    cos, sin = torch.rand(9, 16, device="cuda"), torch.rand(9, 16, device="cuda")
+    calls = {
+        "forward": lambda: L.forward(*qkv, 0.1),
+        "backward": lambda: L.backward(*qkv, o, lse, dout, 0.1, rest=rest),
+        "attention": lambda: torch.autograd.grad(L.attention(*[t.requires_grad_(True) for t in qkv], 0.1), qkv, dout),
+        "append": lambda: L.append(cache, r(3, 64) * 0, r(3, 32) * 0, i(2, 3, 4).long(), i(0, 1, 2), cos, sin),
+        "decode": lambda: (L.decode(q, w, cache, table, lens, 0.1),),
+        "decode_shared": lambda: (L.decode_shared(q, w, cache, table, lens, table + 2, lens, 0.1),),
+        "evict": lambda: L.evict(cache.clone(), table, lens, torch.ones(1, 32, device="cuda"), i(*[-1] * 32)[None], 9),
+    }
+    want = calls[call]()
+    current, entered = [7], []
+
+    class Device:
+        def __init__(self, device):
+            self.to = torch.device(device).index
+
+        def __enter__(self):
+            entered.append(self.to)
+            self.was, current[0] = current[0], self.to
+
+        def __exit__(self, *_):
+            current[0] = self.was
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "current_device", lambda: current[0])
+        m.setattr(torch.cuda, "device", Device)
+        got = calls[call]()
+    assert entered and set(entered) == {0} and current == [7]
+    assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
