@@ -476,6 +476,8 @@ static int shared_check(const atomic_latent_shared_args* a) {
       (int64_t)a->prefix_pages * c->page > (1 << 30) ||
       (c->table_pages < 1 && (a->prefixes == 0 || a->prefix_pages < 1)))  // no token at all
     return ATOMIC_ERR_SHAPE;
+  // positions behind a prefix are 32-bit
+  if ((int64_t)a->prefix_pages * c->page + (int64_t)c->table_pages * c->page > INT32_MAX) return ATOMIC_ERR_SHAPE;
   // the rows that read a prefix are one grid dimension
   if (a->prefixes && (c->batch % a->prefixes ||
                       (int64_t)(c->batch / a->prefixes) * c->tokens * c->heads > (1 << 20)))

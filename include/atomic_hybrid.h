@@ -928,7 +928,8 @@ typedef struct atomic_latent_shared_args {
   atomic_latent_decode_args dec; /* as above; table_pages may be 0 with prefixes      */
   int32_t prefixes;              /* 0 (none), or a divisor of dec.batch; at most 2^20
                                     query rows (tokens and heads) follow one          */
-  int32_t prefix_pages;          /* entries of a prefix_table row, 0 or more          */
+  int32_t prefix_pages;          /* entries of a prefix_table row, 0 or more; both
+                                    tables together hold fewer than 2^31 tokens       */
   int32_t scored;                /* 0 or 1                                            */
   int64_t weights_stride;        /* of weights: sequence; at least table_pages * page */
 } atomic_latent_shared_args;
