@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void latent_absorb(DecDims d, const T* __restr
   }
 }
 
-template <typename T, int DC, int MT, int NW, bool SCORED>
+template <typename T, int DC, int MT, int NW, bool SCORED, bool FRONT>
 __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __restrict__ qa,
                                                         const T* __restrict__ cache, const int32_t* __restrict__ table,
                                                         const int32_t* __restrict__ kv_lens,
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split(DecDims d, const T* __re
                                                         float* __restrict__ part, float* __restrict__ stat,
                                                         float* __restrict__ olat, float* __restrict__ score) {
   __shared__ __attribute__((aligned(1024))) SplitLds<T, DC, NW> lds;
-  split_tokens<T, DC, MT, NW, SCORED>(d, lds, blockIdx.x, blockIdx.y, blockIdx.z, qa, cache, table, kv_lens, own,
+  split_tokens<T, DC, MT, NW, SCORED, FRONT>(d, lds, blockIdx.x, blockIdx.y, blockIdx.z, qa, cache, table, kv_lens, own,
                                       own_most, part, stat, olat, score);
 }
 // Prefixes and own tokens in one launch, where both are small (a launch less): the
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split_both(DecDims f, DecDims 
   const int own_most = d.table * d.page, id = blockIdx.x - (front ? 0 : of_front);
   if (front) d = f;
   __shared__ __attribute__((aligned(1024))) SplitLds<T, DC, NW> lds;
-  split_tokens<T, DC, MT, NW, SCORED>(d, lds, id % d.splits, id / d.splits % d.groups, id / d.splits / d.groups, qa,
+  split_tokens<T, DC, MT, NW, SCORED, true>(d, lds, id % d.splits, id / d.splits % d.groups, id / d.splits / d.groups, qa,
                                       cache, front ? prefix_table : table, front ? prefix_lens : kv_lens,
                                       front ? kv_lens : nullptr, own_most, part, stat, olat, front ? nullptr : score);
 }
@@ -206,6 +206,7 @@ __global__ __launch_bounds__(64 * NW) void latent_split_both(DecDims f, DecDims 
 // columns of a row, thread group g the splits g, g + ways, ...; the groups join
 // through LDS.  (With few rows and many splits the parts are spread over the card
 // this way: 4 sequences of 32768 tokens, 16 heads: 16 MB of parts.)
+template <bool FRONT>
 __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const float* __restrict__ part,
                                                    const float* __restrict__ stat,
                                                    const int32_t* __restrict__ kv_lens, float* __restrict__ olat) {
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(256) void latent_join(DecDims d, int ways, const fl
   f32x4 x = zero4();
   if (ok) {
     const int b = (int)(row / rows);
-    const Parts ps(d, kv_lens, b);
+    const Parts<FRONT> ps(d, kv_lens, b);
     const int64_t at = (int64_t)b * d.slots * rows + row % rows, own = at + (int64_t)ps.skip * rows;
     int s = g;
     for (; s < ps.front; s += ways) m = fmaxf(m, stat[2 * (at + (int64_t)s * rows)]);
@@ -277,6 +278,7 @@ struct Weigh {
   float* weights;
   int64_t stride;
 };
+template <bool FRONT>
 __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, const float* __restrict__ stat,
                                              const int32_t* __restrict__ kv_lens, float* lse) {
   const int per = (int)(((int64_t)d.table * d.page + 16 * kWeighTiles - 1) / (16 * kWeighTiles));
@@ -285,7 +287,7 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
   if (b >= d.B) return;
   const int len = dec_len(d, kv_lens, b);
   if (16 * kWeighTiles * chunk >= len) return;
-  const Parts ps(d, kv_lens, b);
+  const Parts<FRONT> ps(d, kv_lens, b);
   for (int r = threadIdx.x >> 4; r < 16 * x.row_tiles; r += 16) {
     float m = -INFINITY, sum = 0.f;
     if (r < rows) {
@@ -348,7 +350,7 @@ __device__ __forceinline__ void latent_weigh(const DecDims& d, const Weigh& x, c
 // the same parts read once instead of dv / 64 times.  Latency: 5 to 8 us without the join.
 // With SCORED the workgroups from grid x `x.first` on gather the tokens' weights instead.
 constexpr int kUpSplits = 64;
-template <typename T, bool JOIN, bool SCORED>
+template <typename T, bool JOIN, bool SCORED, bool FRONT>
 __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict__ w_kv, const float* __restrict__ olat,
                                                  const float* __restrict__ part, const float* __restrict__ stat,
                                                  const int32_t* __restrict__ kv_lens, T* __restrict__ o, Weigh x) {
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
   __shared__ __attribute__((aligned(16))) T so[PARTS][16 * LD];
   __shared__ float sw[JOIN ? 16 : 1][kUpSplits];
   static_assert(sizeof(so) >= (kMostRows + 64) * sizeof(float), "a float for each row of a sequence's row tiles");
-  if (SCORED && (int)blockIdx.x >= x.first) return latent_weigh(d, x, stat, kv_lens, reinterpret_cast<float*>(so));
+  if (SCORED && (int)blockIdx.x >= x.first) return latent_weigh<FRONT>(d, x, stat, kv_lens, reinterpret_cast<float*>(so));
   const int h = blockIdx.x, v0 = 64 * blockIdx.y, r0 = 16 * blockIdx.z, R = d.B * d.n, KP = (d.dc + 31) / 32 * 32;
   const int vr = v0 + 16 * wave_id(), rows = d.n * d.H;
   const T* w = w_kv + ((int64_t)h * (d.dn + d.dv) + d.dn + min(vr + (lane_id() & 15), d.dv - 1)) * d.dc;
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
   }
   if constexpr (JOIN) {  // the splits' weights: sixteen threads a row
     const int r = min(r0 + (int)(threadIdx.x >> 4), R - 1), b = r / d.n, g = threadIdx.x & 15;
-    const Parts ps(d, kv_lens, b);
+    const Parts<FRONT> ps(d, kv_lens, b);
     const float* st = stat + 2 * ((int64_t)b * d.slots * rows + r % d.n * d.H + h);
     float m = -INFINITY, sum = 0.f, ms[kUpSplits / 16], ls[kUpSplits / 16];
 #pragma unroll
@@ -400,13 +402,15 @@ __global__ __launch_bounds__(256) void latent_up(DecDims d, const T* __restrict_
     if (c < d.dc && r0 + r < R) {
       if constexpr (JOIN) {
         const int b = (r0 + r) / d.n;
-        const Parts ps(d, kv_lens, b);
+        const Parts<FRONT> ps(d, kv_lens, b);
         const float* p = part + ((int64_t)b * d.slots * rows + (r0 + r) % d.n * d.H + h) * d.dc + c;
         // (a loop for each kind of parts: with their slots chosen in one the loads were not sent eight at a time)
         int s = 0;
+        if constexpr (FRONT) {
 #pragma unroll 8
-        for (; s < ps.front; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
-        p += (int64_t)ps.skip * rows * d.dc;
+          for (; s < ps.front; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
+          p += (int64_t)ps.skip * rows * d.dc;
+        }
 #pragma unroll 8
         for (; s < ps.all; ++s) x += sw[r][s] * *reinterpret_cast<const f32x4*>(p + (int64_t)s * rows * d.dc);
       } else {
@@ -679,12 +683,12 @@ static void launch_split(const DecPlan& plan, int prefixes, bool front, hipStrea
       }
     }
     if (front)
-      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED>),
+      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED, true>),
                          dim3((unsigned)f.splits, (unsigned)f.groups, (unsigned)prefixes), dim3(64 * NW), 0, st, f, x.qa,
                          (const T*)p.cache, p.prefix_table, p.prefix_lens, p.lens, own_most, x.part, x.stat, x.olat,
                          (float*)nullptr);
     else
-      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED>),
+      hipLaunchKernelGGL((latent_split<T, DC, MT, NW, SCORED, false>),
                          dim3((unsigned)d.splits, (unsigned)d.groups, (unsigned)d.B), dim3(64 * NW), 0, st, d, x.qa,
                          (const T*)p.cache, p.table, p.lens, (const int32_t*)nullptr, 0, x.part, x.stat, x.olat, x.score);
   };
@@ -751,8 +755,12 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     while (ways < 16 && 4 * ways < d.slots) ways *= 2;
     const int64_t units = (int64_t)d.B * d.n * d.H * ((d.dc + 63) / 64);
     rc = L("latent_join", [&] {
-      hipLaunchKernelGGL(latent_join, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0, st, d, ways, x.part,
-                         x.stat, p.lens, x.olat);
+      auto go = [&](auto f) {
+        hipLaunchKernelGGL(latent_join<decltype(f)::value != 0>, dim3((unsigned)((units * ways + 15) / 16)), dim3(256), 0,
+                           st, d, ways, x.part, x.stat, p.lens, x.olat);
+      };
+      if (prefixes) go(IntC<1>());
+      else go(IntC<0>());
     });
     if (rc) return rc;
   }
@@ -764,12 +772,15 @@ static int dec_run(const atomic_latent_decode_args* a, int prefixes, int prefix_
     more = (unsigned)((per * d.B + gy * rt - 1) / (gy * rt));
   }
   return L("latent_up", [&] {
-    auto go = [&](auto j) {
-      hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0, SCORED>), dim3((unsigned)d.H + more, gy, rt), dim3(256),
-                         0, st, d, (const T*)p.w_kv, x.olat, x.part, x.stat, p.lens, (T*)p.o, wx);
+    auto go = [&](auto j, auto f) {
+      hipLaunchKernelGGL((latent_up<T, decltype(j)::value != 0, SCORED, decltype(f)::value != 0>),
+                         dim3((unsigned)d.H + more, gy, rt), dim3(256), 0, st, d, (const T*)p.w_kv, x.olat, x.part,
+                         x.stat, p.lens, (T*)p.o, wx);
     };
-    if (joins) go(IntC<1>());
-    else go(IntC<0>());
+    if (!joins && (!SCORED || !prefixes)) go(IntC<0>(), IntC<0>());
+    else if (!joins) go(IntC<0>(), IntC<SCORED>());
+    else if (prefixes) go(IntC<1>(), IntC<1>());
+    else go(IntC<1>(), IntC<0>());
   });
 }
 

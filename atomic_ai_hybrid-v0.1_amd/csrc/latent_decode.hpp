@@ -26,13 +26,16 @@ __device__ __forceinline__ int dec_len(const DecDims& d, const int32_t* kv_lens,
 __device__ __forceinline__ int pre_len(const DecDims& d, int b) {
   return d.pre_share ? min(max(d.pre_lens[b / d.pre_share], 0), d.pre_most) : 0;
 }
-// The parts of sequence b's rows: those of the prefix's splits, then those of its own.
+// The parts of sequence b's rows: those of the prefix's splits, then those of its own.  (Whether there are
+// prefixes is known when a kernel is compiled: with the question asked in it, latent_up's join of 16 rows was
+// 1 us longer in the calls that have none.)
+template <bool FRONT>
 struct Parts {
   int front, all, skip;  // splits of the prefix, of both, slots to leave out between them
   __device__ __forceinline__ Parts(const DecDims& d, const int32_t* kv_lens, int b) {
-    front = d.pre_share ? (pre_len(d, b) + d.pre_chunk - 1) / d.pre_chunk : 0;
-    all = front + (d.splits ? (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk : 0);
-    skip = d.pre_splits - front;
+    front = FRONT ? (pre_len(d, b) + d.pre_chunk - 1) / d.pre_chunk : 0;
+    all = front + (!FRONT || d.splits ? (dec_len(d, kv_lens, b) + d.chunk - 1) / d.chunk : 0);
+    skip = FRONT ? d.pre_splits - front : 0;
   }
   __device__ __forceinline__ int slot(int s) const { return s < front ? s : s + skip; }
 };
@@ -123,8 +126,9 @@ struct DTile : LTile<T, W, 16> {
 // 4.6 TB/s; 4 of 32768: 33 us, 4.6 TB/s; both where a copy reaches 5.0.
 //
 // (With 512 latents the accumulators take 128 registers and the query's fragments 144 in
-// float32 and 144 in bf16 where it enters as two numbers: in scratch memory lie 9 registers with
-// MT = 1 and 60 with more, and 2, 83 and 97 with MT = 1, 2 and 4.)
+// float32 and 144 in bf16 where it enters as two numbers.  In scratch memory lie 6 registers with MT = 1
+// and 58 with more in float32, and 0, 81 and 97 with MT = 1, 2 and 4 where there are two numbers, with FRONT
+// up to 3 more; with 3 and 54 float32 calls took the same time to 2 %.)
 //
 // The rows of a launch are those of `share` sequences after one another: one, or all that
 // follow the same prefix (`own`, then, are the lengths of what follows it).  With SCORED the
@@ -139,8 +143,8 @@ template <typename T, int DC, int NW> struct SplitLds {
   int32_t spt[kDecPages];
   float sm[NW][16], ss[NW][16];
 };
-// Split `sp` of unit b (a sequence, or a prefix) against row group `rg` of its rows.
-template <typename T, int DC, int MT, int NW, bool SCORED>
+// Split `sp` of unit b (a sequence, or with FRONT a prefix too) against row group `rg` of its rows.
+template <typename T, int DC, int MT, int NW, bool SCORED, bool FRONT>
 __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, NW>& lds, int sp, int rg, int b,
                                              const T* __restrict__ qa,
                                              const T* __restrict__ cache, const int32_t* __restrict__ table,
@@ -162,17 +166,20 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, N
   float(*const sm)[16] = lds.sm;
   float(*const ss)[16] = lds.ss;
   const int wv = wave_id(), lane = lane_id(), rw = wv % MT, tw = wv / MT;
-  const int len = dec_len(d, kv_lens, b), each = d.n * d.H, rows = d.share * each, wide = d.dc + d.dr;
+  const int len = dec_len(d, kv_lens, b), each = d.n * d.H, rows = (FRONT ? d.share : 1) * each, wide = d.dc + d.dr;
   const int first = sp * d.chunk, end = min(len, first + d.chunk);
   if (first >= len && (sp > 0 || d.slots > 1)) return;  // (one split only: it writes the empty sequence's zeros)
   const int page0 = first / d.page;
   for (int i = threadIdx.x; first < end && i <= (end - 1) / d.page - page0; i += 64 * NW)
     spt[i] = min(max(table[(int64_t)b * d.table + page0 + i], 0), d.pages - 1);
   const int row = 16 * (rg * MT + rw) + (lane & 15);
-  const int seq = b * d.share + min(row, rows - 1) / each;  // this lane's row: its sequence, and its place there
-  const int place = min(row, rows - 1) % each;
+  int seq = b, place = min(row, rows - 1);  // this lane's row: its sequence, and its place there
+  if (FRONT && d.share > 1) {
+    seq = b * d.share + place / each;
+    place %= each;
+  }
   int seen = len - d.n + place / d.H + 1;  // tokens that it sees
-  if (own) seen += min(max(own[seq], 0), own_most);
+  if (FRONT && own) seen += min(max(own[seq], 0), own_most);
   const int least = len - d.n + 1;  // and that every row sees
   const T* qr = qa + ((int64_t)seq * each + place) * d.qn * wide;
   frag qf[NQ][KS];

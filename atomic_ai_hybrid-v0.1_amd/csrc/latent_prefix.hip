@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
                        c.prefix_lens, c.lens, d.table * d.page, parts, c.stat);
   } else {
     const int id = at < 0 ? (int)blockIdx.x : (int)blockIdx.x - front;
-    split_tokens<bf16, DC, MT, 4, SCORED>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
+    split_tokens<bf16, DC, MT, 4, SCORED, false>(d, *reinterpret_cast<OwnLds*>(mem), id % d.splits, id / d.splits % d.groups,
                                            id / d.splits / d.groups, c.qa, c.cache, c.table, c.lens, nullptr, 0, c.part,
                                            c.stat, c.olat, c.score);
   }
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f,
   // statistics: the prefix's, a row a lane,
   {
     const int row = min(r0 + (lane & 31), rows - 1), seq = b * f.share + row / each, place = row % each;
-    const int n = Parts(d, kv_lens, seq).front;
+    const int n = Parts<true>(d, kv_lens, seq).front;
     const float* st = stat + 2 * ((int64_t)seq * d.slots * each + place);
     const f32x4* from = parts + (int64_t)group * f.splits * (4 * NT * 64) + (32 * (k / 2) < d.dc ? k : 0) * 128 + lane;
     f32x4 x[2] = {zero4(), zero4()};
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(4 * COLS * WAYS) void latent_prefix_join(DecDims f,
   f32x4 x = zero4();
   float m = -INFINITY, sum = 0.f;
   {
-    const Parts ps(d, kv_lens, seq);
+    const Parts<true> ps(d, kv_lens, seq);
     const float* st = stat + 2 * (((int64_t)seq * d.slots + d.slot0) * each + place);
     const float* own = part + ((int64_t)seq * (d.slots - d.part0) * each + place) * d.dc + min(c, d.dc - 4);
     const int n = mine ? ps.all - ps.front : 0;
