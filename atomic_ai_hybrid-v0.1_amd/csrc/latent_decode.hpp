@@ -5,6 +5,9 @@
 
 namespace ah {
 
+// Keep a value in the accumulator half of the register file.
+template <typename F> __device__ __forceinline__ void in_accum(F& x) { asm volatile("" : "+a"(x)); }
+
 struct DecDims {
   int B, n, H, dn, dr, dv, dc, page, pages, table, rope, inter;
   int chunk, splits, groups;  // tokens a split (whole tiles), splits of the longest sequence, row groups
@@ -126,9 +129,9 @@ struct DTile : LTile<T, W, 16> {
 // 4.6 TB/s; 4 of 32768: 33 us, 4.6 TB/s; both where a copy reaches 5.0.
 //
 // (With 512 latents the accumulators take 128 registers and the query's fragments 144 in
-// float32 and 144 in bf16 where it enters as two numbers.  In scratch memory lie 6 registers with MT = 1
-// and 58 with more in float32, and 0, 81 and 97 with MT = 1, 2 and 4 where there are two numbers, with FRONT
-// up to 3 more; with 3 and 54 float32 calls took the same time to 2 %.)
+// float32 and 144 in bf16 where it enters as two numbers.  The accumulators are held where they are while
+// they fade: else the compiler copies all of them ahead of that, and puts up to 97 registers into
+// scratch memory, which it did not always get back whole.)
 //
 // The rows of a launch are those of `share` sequences after one another: one, or all that
 // follow the same prefix (`own`, then, are the lengths of what follows it).  With SCORED the
@@ -293,7 +296,11 @@ __device__ __forceinline__ void split_tokens(const DecDims& d, SplitLds<T, DC, N
       m = mn;
       sum *= fade;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n] *= fade;
+      for (int n = 0; n < NT; ++n) {
+        in_accum(acc[n]);
+        acc[n] *= fade;
+        in_accum(acc[n]);
+      }
     }
     const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
     half p[NP][MT];

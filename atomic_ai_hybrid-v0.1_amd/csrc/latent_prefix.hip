@@ -27,9 +27,6 @@
 
 namespace ah {
 
-// Keep a value in the accumulator half of the register file.
-template <typename F> __device__ __forceinline__ void in_accum(F& x) { asm volatile("" : "+a"(x)); }
-
 // x *= f for an x there.  (Written as a product, the compiler reads all accumulators ahead of the
 // branch that this is in, into registers that are not there.)
 __device__ __forceinline__ void accum_mul(float& x, float f) {
@@ -53,6 +50,10 @@ __device__ __forceinline__ uint64_t row_at(uint32_t lo, uint32_t hi, int r) {
 }
 __device__ __forceinline__ uint64_t pair_at(uint32_t lo, uint32_t hi, int r) {
   return lane_id() < 32 ? row_at(lo, hi, r) : row_at(lo, hi, r + 1);
+}
+// What lane r holds.  (__shfl keeps two registers more.)
+template <typename X> __device__ __forceinline__ X lane_at(X x, int r) {
+  return __builtin_bit_cast(X, __builtin_amdgcn_ds_bpermute(4 * r, __builtin_bit_cast(int, x)));
 }
 // Workgroup `id` of those over the prefixes.
 //
@@ -102,7 +103,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 8 * i + lane / 8;
-      const uint64_t base = (uint64_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r);
+      const uint64_t base = (uint64_t)lane_at(hi, r) << 32 | lane_at(lo, r);
       const uint32_t off = 16 * (lane % 8) ^ 16 * LR::swz(r);
       dma16_raw((const void*)(off < rb ? base + wb + off : (uint64_t)lat_zeros), to + SC + 8 * i * LR::ROWB);
     }
@@ -139,24 +140,28 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   __syncthreads();  // the tokens' places are there, the buffers free
   // This wave's loads of the tile at k0 (from `first` on): eight latents, then their rotated keys.
   // (Their places are read a tile ahead.)
-  uint32_t lo, hi, next;
+  uint32_t lo, hi, next, off0;  // (off0: each load's offset from it when it is sent, not eight of them kept over the tiles)
   auto look = [&](int k0) { next = slot[min(k0 + PT * wv + (lane & 7), end - first - 1)]; };
   auto aim = [&] {
     const uint64_t a = (uint64_t)cache + (uint64_t)next * (2 * wide);
     lo = (uint32_t)a;
     hi = (uint32_t)(a >> 32);
+    off0 = 16 * pl;
+    asm volatile("" : "+v"(off0));
   };
   auto send = [&](int i, uint32_t to) __attribute__((always_inline)) {
     if (i < PT / RL) {
       const int r = PT * wv + RL * i;
-      uint32_t off = 16 * pl ^ 16 * LC::swz(r + lr);
+      uint32_t off = off0 ^ 16 * LC::swz(r + lr);
       if (off >= wb) off = 0;  // the padding of a width: the query has zeros there
       if constexpr (RL == 1) dma16_raw_s(row_at(lo, hi, i), off, to + r * LC::ROWB);
       else dma16_raw((const void*)(pair_at(lo, hi, 2 * i) + off), to + r * LC::ROWB);
     } else {
-      const int r = PT * wv + lane / 8;
-      const uint64_t base = (uint64_t)__shfl(hi, lane / 8) << 32 | (uint32_t)__shfl(lo, lane / 8);
-      uint32_t off = 16 * (lane % 8) ^ 16 * LR::swz(r);
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      const int r = PT * wv + ln / 8;
+      const uint64_t base = (uint64_t)lane_at(hi, ln / 8) << 32 | lane_at(lo, ln / 8);
+      uint32_t off = 16 * (ln % 8) ^ 16 * LR::swz(r);
       if (off >= rb) off = 0;
       dma16_raw((const void*)(base + wb + off), to + SC + PT * wv * LR::ROWB);
     }
@@ -221,7 +226,7 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top *= c2;
     if (__any(top > m + kLag)) {
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fmaxf(top, lane_at(top, lane ^ 32));
       const float mn = fmaxf(m, ceilf(top)), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
       m = mn;
       if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
@@ -347,13 +352,16 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
   if (len < kPreOne) walk(IntC<2>());
   else walk(IntC<1>());
   vm_wait<0>();  // nothing is on its way to LDS when the workgroup ends
-  held += __shfl_xor(held, 32);
-  if constexpr (SCORED) sum += __shfl_xor(sum, 32);
+  held += lane_at(held, lane ^ 32);
+  if constexpr (SCORED) sum += lane_at(sum, lane ^ 32);
   else sum = held;
   const float even = SCORED && held != 0.f ? sum / held : 1.f;
   // A part: a lane's accumulators four by four, in the order that they have.
   const int64_t group = ((int64_t)b * blocks + blk) * 4 + wv;
-  f32x4* to = parts + (group * d.splits + sp) * (4 * NT * 64) + lane;
+  // (this lane and its row once more, so that they are not kept over the tiles)
+  const int row0 = kPreRows * blk + 32 * wv + opaque_zero();
+  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, opaque_zero()));
+  f32x4* to = parts + (group * d.splits + sp) * (4 * NT * 64) + ln;
   const int columns = kPreRows * blk + 32 * wv < rows ? d.dc : 0;  // (nobody reads a part without rows)
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -363,8 +371,9 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       if constexpr (SCORED) x *= even;
       if (32 * n < columns) to[(4 * n + k) * 64] = x;
     }
-  if (lane < 32 && row < rows) {
-    const int64_t at = ((int64_t)seq * d.slots + d.slot0 + sp) * each + place;
+  if (ln < 32 && row0 + ln < rows) {
+    const int of = each + opaque_zero(), own_seq = b * d.share + (row0 + ln) / of;
+    const int64_t at = ((int64_t)own_seq * d.slots + d.slot0 + sp) * of + (row0 + ln) % of;
     stat[2 * at] = m;
     stat[2 * at + 1] = sum;
   }
