@@ -275,13 +275,15 @@ __device__ __forceinline__ void dma_touch(const void* src, void* dst) {
 __device__ __forceinline__ void dma16_raw(const void* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }
-// The same from a wave-uniform base and a 32-bit byte offset a lane.
+// The same from a wave-uniform base and a 32-bit byte offset a lane.  (A scalar register that a vector
+// instruction wrote, as a lane read does, may be read by a load five wait states later; the
+// compiler does not see the load, so they stand here: one for m0's write and four.)
 __device__ __forceinline__ void dma16_raw_s(uint64_t base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst)
                : "memory", "m0");
 }
 // The same through a buffer descriptor (buffer_of) at the lane's byte offset plus
-// a uniform one; what lies past the descriptor's bytes is written as zeros.
+// a uniform one; what lies past the descriptor's bytes is written as zeros.  (Wait states as above.)
 typedef uint32_t buffer_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ buffer_t buffer_of(uint64_t base, uint32_t bytes) {
   buffer_t d;
@@ -292,7 +294,7 @@ __device__ __forceinline__ buffer_t buffer_of(uint64_t base, uint32_t bytes) {
   return d;
 }
 __device__ __forceinline__ void dma16_buf(buffer_t d, uint32_t lane_off, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_off), "s"(d),
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_off), "s"(d),
                "s"(off), "s"(dst)
                : "memory", "m0");
 }

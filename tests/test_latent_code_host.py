@@ -58,3 +58,39 @@ def test_no_registers_in_scratch_memory(latent_objects):
             assert get("vgpr_spill_count") == get("private_segment_fixed_size") == 0, name
             seen += 1
     assert seen > 50
+
+
+def _sgprs(operand):
+    m = re.fullmatch(r"s\[(\d+):(\d+)\]|s(\d+)", operand)
+    if not m:
+        return set()
+    return {int(m[3])} if m[3] else set(range(int(m[1]), int(m[2]) + 1))
+
+
+def test_scalar_addresses_are_there_when_a_load_reads_them(latent_objects):
+    """A memory instruction may read a scalar register five wait states after a vector instruction has written
+    it, and nothing in the card waits for that.  The compiler does not look into inline assembly, so what
+    stands there has to wait by itself."""
+    loads = 0
+    for path, _ in latent_objects:
+        wrote = {}                                  # scalar register: wait states since a vector instruction wrote it
+        for line in _tool("llvm-objdump", "-d", path).splitlines():
+            if line.endswith(">:"):
+                wrote, where = {}, line
+                continue
+            op, _, rest = line.split("//")[0].strip().partition(" ")
+            if not re.match(r"[vs]_|ds_|global_|buffer_|scratch_|flat_", op):
+                continue
+            operands = [x.strip() for x in re.split(r",|\s(?!\s)", rest) if x.strip()]
+            if op.startswith(("global_", "buffer_", "scratch_", "flat_")):
+                loads += 1
+                for x in operands:
+                    assert not _sgprs(x) & wrote.keys(), (where, line)
+            states = int(operands[0]) + 1 if op == "s_nop" else 1
+            wrote = {r: n + states for r, n in wrote.items() if n + states < 5}
+            if op.startswith("v_"):
+                wrote.update((r, 0) for x in operands[:2 if "_co_" in op or "div_scale" in op else 1] for r in _sgprs(x))
+            elif op.startswith("s_") and operands:
+                for r in _sgprs(operands[0]):
+                    wrote.pop(r, None)
+    assert loads > 1000
