@@ -283,7 +283,9 @@ __device__ __forceinline__ void dma16_raw_s(uint64_t base, uint32_t off, uint32_
                : "memory", "m0");
 }
 // The same through a buffer descriptor (buffer_of) at the lane's byte offset plus
-// a uniform one; what lies past the descriptor's bytes is written as zeros.  (Wait states as above.)
+// a uniform one; what lies past the descriptor's bytes is written as zeros.  (No wait
+// states here, 1 % of the latent backward: descriptors are made long before the loops that use them; a test
+// goes through the built code for it.)
 typedef uint32_t buffer_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ buffer_t buffer_of(uint64_t base, uint32_t bytes) {
   buffer_t d;
@@ -294,7 +296,7 @@ __device__ __forceinline__ buffer_t buffer_of(uint64_t base, uint32_t bytes) {
   return d;
 }
 __device__ __forceinline__ void dma16_buf(buffer_t d, uint32_t lane_off, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_off), "s"(d),
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_off), "s"(d),
                "s"(off), "s"(dst)
                : "memory", "m0");
 }
