@@ -7,6 +7,7 @@ from torch.autograd import forward_ad
 from _util import banner
 from atomic_ops import latent as L
 from oracle import latent as ol
+from test_latent_evict_gpu import _state
 from test_latent_shared_gpu import BF16, F32, _case
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +98,56 @@ def test_tensors_of_another_device_than_the_current_one(call, monkeypatch):
         got = calls[call]()
     assert entered and set(entered) == {0} and current == [7]
     assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+
+
+def _evict_in_place(lens, page, keep, sinks, recent, seed, settled=0, strided=False, per=None):
+    state = [t.cuda() for t in _state(lens, page, 16, BF16, seed=seed, settled=settled, per=per)]
+    other = [t.clone() for t in state]
+    if strided:      # rows of wider buffers
+        wide = torch.full((len(lens), state[3].shape[1] + 9), 7.0, device="cuda")
+        ages = torch.full((len(lens), state[4].shape[1] + 4), 77, dtype=torch.int32, device="cuda")
+        wide[:, 2:-7], ages[:, 4:] = state[3], state[4]
+        other[3], other[4] = wide[:, 2:-7], ages[:, 4:]
+    want = L.evict(*state, keep, sinks=sinks, recent=recent)
+    got = L.evict(*other, keep, sinks=sinks, recent=recent, in_place=True)
+    assert all(a is b for a, b in zip(got, other[2:]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(other[0], state[0])
+    if strided:
+        assert (wide[:, :2] == 7).all() and (wide[:, -7:] == 7).all() and (ages[:, :4] == 77).all()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("lens,page,keep,sinks,recent,settled,per", [
+    ([40000, 33000, 500], 128, 20000, 4, 700, 2000, None),       # movers and holes of many workgroups
+    ([32768, 100, 0], 128, 32000, 4, 700, 0, None),
+    ([9000, 8193], 1, 1, 0, 0, 30, None),
+    ([12000, 12000], 24, 11999, 0, 11000, 500, None),
+    ([300, 100], 64, 70000, 4, 70, 0, 1000),                     # more than the table holds
+])
+def test_long_tables_in_place(lens, page, keep, sinks, recent, settled, per, strided):
+    """The launches after the selection read the state that the call writes over."""
+    banner(f"latent evict long in place {lens} page {page} keep {keep} {strided}")
+    _evict_in_place(lens, page, keep, sinks, recent, 14, settled, strided, per)
+
+
+def test_a_long_table_as_a_replayed_graph():
+    """A captured eviction of long tables in place, replayed on new states with eager work between."""
+    banner("latent evict long graph")
+    states = [[t.cuda() for t in _state([30000, 20001, 123], 64, 16, BF16, seed=s, settled=100 * s)] for s in range(4)]
+    held = [t.clone() for t in states[0]]
+    kw = dict(sinks=4, recent=500)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        L.evict(*[t.clone() for t in held], 9000, **kw)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        source = L.evict(*held, 9000, **kw, in_place=True)[3]
+    for state in states[1:] + states:
+        for a, b in zip(held, state):
+            a.copy_(b)
+        graph.replay()
+        cache = state[0].clone()
+        want = L.evict(cache, *state[1:], 9000, **kw)
+        assert all(torch.equal(a, b) for a, b in zip((*held[2:], source, held[0]), (*want, cache)))
