@@ -562,7 +562,7 @@ static DecPlan dec_plan(const atomic_latent_decode_args* a, int prefixes, int pr
   const DecDims own = dec_dims(a, a->batch, 1, a->table_pages, p.own_tiles, true);
   if (a->dtype == ATOMIC_BF16 && prefix_plan(many, prefixes, own)) {
     const int64_t wgs = (int64_t)own.splits * own.groups * a->batch;  // one grid dimension for both
-    p.many = many.splits + own.splits > 1 && wgs <= (1 << 30);
+    p.many = wgs <= (1 << 30);
     if (p.many) {
       p.front = many;
       p.own = own;

@@ -38,6 +38,8 @@ __device__ __forceinline__ void accum_mul(float& x, float f) {
 
 constexpr int kPreRows = 128, kPreTokens = 32, kPreBufs = 4, kPreChunk = 2048;
 constexpr int kPreOne = 2048;  // tokens of a prefix from which on p enters as one bf16 number
+constexpr int kPreTable = 4096;  // tokens that a prefix's table has at least
+static_assert(kPreTable >= 2 * kPreChunk, "two splits or more: a row's parts are always joined");
 
 template <int DC> struct PrefixLds {
   // (seven tiles of 256 latents, for which there is room, were no faster)
@@ -559,7 +561,7 @@ static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256
 // 1184, 112 of 1280, 133 of 896; 4 prefixes of 4096, 512 rows each: 55 of 256, 49 of 384, 50 of 512.)
 bool prefix_plan(DecDims& d, int units, const DecDims& own) {
   const int64_t rows = (int64_t)d.share * d.n * d.H, most = (int64_t)d.table * d.page;
-  if (rows <= 32 || most < 4096 || (int64_t)d.pages * d.page > UINT32_MAX) return false;
+  if (rows <= 32 || most < kPreTable || (int64_t)d.pages * d.page > UINT32_MAX) return false;
   const int64_t blocks = (int64_t)prefix_blocks(d) * units;
   const int64_t others = (int64_t)own.splits * own.groups * own.B;
   const double other = 0.065 * own.chunk + 7.5;
