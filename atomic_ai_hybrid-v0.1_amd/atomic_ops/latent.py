@@ -410,6 +410,8 @@ def decode_shared(q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens
     stands at position prefix_lens[g] + kv_lens[b] - n + t and sees the tokens up to and
     with its own: what ``decode`` gives for the two tables as one, up to rounding.
     ``weights`` are those of the own tokens; a prefix's are not gathered."""
+    if (prefix_table is None) != (prefix_lens is None):
+        raise ValueError("latent decode: prefix_table and prefix_lens come together")
     given = (q, w_kv, cache, cos, sin, weights)
     args = (q, w_kv, cache, prefix_table, prefix_lens, page_table, kv_lens, scale, cos, sin, interleaved, weights,
             workspace, timer)
