@@ -299,8 +299,8 @@ __global__ __launch_bounds__(NT) void evict_small(EvictDims d, EvictIn in, Evict
       if (!d.fused) movers[(int64_t)b * d.moves + r] = m;
     }
   }
-  // past the length (every row has been read)
-  for (int j = left + tid; j < d.width; j += NT) {
+  // past the length (every row has been read; a state may end within a step of 2^31)
+  for (int64_t j = left + tid; j < d.width; j += NT) {
     w_out[j] = 0.f;
     o_out[j] = -1;
   }
@@ -564,12 +564,13 @@ __global__ __launch_bounds__(256) void evict_move(EvictDims d, const int32_t* __
   int32_t* o_out = out.o + b * d.oos;
   int* source = out.source + (int64_t)b * d.keep;
   if constexpr (STATE) {
-    const int left = left_of[b], step = 256 * gridDim.x;
-    for (int j = left + 256 * blockIdx.x + threadIdx.x; j < d.width; j += step) {
+    const int left = left_of[b];
+    const int64_t first = left + 256 * (int64_t)blockIdx.x + threadIdx.x, step = 256 * (int64_t)gridDim.x;
+    for (int64_t j = first; j < d.width; j += step) {
       w_out[j] = 0.f;
       o_out[j] = -1;
     }
-    for (int j = left + 256 * blockIdx.x + threadIdx.x; j < d.keep; j += step) source[j] = -1;
+    for (int64_t j = first; j < d.keep; j += step) source[j] = -1;
     if (blockIdx.x == 0 && threadIdx.x == 0) out.lens[b] = left;
   }
   if (n <= 0) return;

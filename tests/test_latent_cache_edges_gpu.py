@@ -151,3 +151,21 @@ def test_a_long_table_as_a_replayed_graph():
         cache = state[0].clone()
         want = L.evict(cache, *state[1:], 9000, **kw)
         assert all(torch.equal(a, b) for a, b in zip((*held[2:], source, held[0]), (*want, cache)))
+
+
+@pytest.mark.parametrize("rows", [100, 9000])
+def test_evict_with_a_state_of_nearly_2_to_the_31(rows):
+    """What lies past the length is cleared up to the last element, by steps that would not fit 32 bits."""
+    banner(f"latent evict wide state {rows}")
+    W = (1 << 31) - 1
+    cache = torch.randn(-(-rows // 64), 64, 16, device="cuda").to(BF16)
+    table = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    weights = torch.ones(1, W, device="cuda")
+    order = torch.full((1, W), -1, dtype=torch.int32, device="cuda")
+    order[0, rows:] = 5
+    got = L.evict(cache, table, lens, weights, order, rows // 2, sinks=3, recent=7, in_place=True)
+    assert got[0].tolist() == [rows // 2]
+    assert (weights[0, :rows // 2] == 1).all() and (order[0, :rows // 2] >= 0).all()
+    for i in range(rows // 2, W, 1 << 28):
+        assert not weights[0, i:i + (1 << 28)].any() and (order[0, i:i + (1 << 28)] == -1).all()
