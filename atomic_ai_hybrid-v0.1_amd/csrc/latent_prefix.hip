@@ -10,12 +10,12 @@
 // the rotated queries) and as many reads; all four waves read the same tile, four tiles are
 // in LDS, and loads, reads and MFMAs are spread over each other by hand (`tile`).  The scores of
 // tile i and the products of tile i - 1 are one run, so that the softmax of one lies under
-// the products of the other.  A tile takes 1.95 us, of whose clocks its 72 MFMAs are two
-// thirds.  64 sequences of 16 heads over 32768 tokens and their 512 own ones: 91 us, 0.82
-// PFLOP/s (latent_split took 150 for the prefix alone); over 8192 and up to 1024: 45 us.  What is
-// not tiles is the queries, which have to be there before the first product (128 KB a
-// workgroup), the parts and the own tokens.  More operands read ahead, two chains of scores
-// and, with 256 latents, seven tiles in LDS changed nothing.
+// the products of the other.  A tile takes 4000 clocks (2.2 us), 2304 of them its 72
+// MFMAs.  64 sequences of 16 heads over 32768 tokens and their 512 own ones: 97 us, 0.77
+// PFLOP/s (latent_split took 150 for the prefix alone); over 8192 and up to 1024: 47 us.  What is
+// not tiles, 38 % of the clocks of the first, is the queries, which have to be there before the first
+// product (128 KB a workgroup), the parts (67 MB there) and the own tokens.  More operands
+// read ahead, two chains of scores and, with 256 latents, seven tiles in LDS changed nothing.
 //
 // From 2048 tokens of a prefix on p enters as one bf16 number: o is off by 0.0025 of its norm
 // behind 2048 to 4096 of them and 0.0024 behind 8192, where latent_split, which has two, is at
@@ -386,8 +386,8 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
 // `early` of the others, up to half a card of them, go first: half of the CUs then begin with
 // the one kind and end with the other.  What is bound by memory so runs beside what is bound by
 // matrix instructions (64 sequences of 16 heads over 8192 tokens and up to 1024 own
-// ones, 45 us.  Whole calls: 32 sequences over 8192 and 2048 tokens with weights 77 us in two
-// launches and 71 in one; 64 over 32768 and 512 132 with the two kinds by turns and 109 so).
+// ones, 47 us.  Whole calls, measured with parts of half the bytes: 32 sequences over 8192 and 2048 tokens with
+// weights 77 us in two launches and 71 in one; 64 over 32768 and 512 132 with the two kinds by turns and 109 so).
 template <int DC, int MT, bool SCORED>
 __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks, int early, f32x4* __restrict__ parts) {
   typedef SplitLds<bf16, DC, 4> OwnLds;
@@ -413,7 +413,9 @@ __global__ __launch_bounds__(256, 1) void latent_prefix(PrefixCall c, int blocks
 // Where the tokens' weights are gathered, `shift` [rows, 8] receives what q_lat's rounding did
 // to the log (base 2) of a row's sum over the prefix: with e = q_lat - its bf16, a score is off
 // by c e . c_j, so the log by c e . (sum_j p_j c_j) and, what is left, half the variance of
-// c e . c_j (1.5e-6 for scores of unit spread; uncorrected, the sum was off by 5e-5).
+// c e . c_j, which grows with the scores: gathered weights are off by 1.5e-6 of their norm where
+// scores have unit spread, 9e-6 at a spread of 3 and 2e-5 to 3e-5 at 10; with the second number in every
+// score, as latent_split has it, by 1e-6, 4e-6 and 8e-6.  (Uncorrected 5e-5 at unit spread.)
 // Each workgroup gives its 64 columns' share.  (As a second number in the scores it would
 // take another 32 of 36 matrix instructions a tile and 128 registers that are not there.)
 template <int DC, int COLS, int WAYS>
@@ -554,7 +556,8 @@ static size_t tile_bytes(const DecDims& d) { return 32 * (d.dc > 256 ? 512 : 256
 // prefixes whose table has 4096 tokens or more (the host does not know their lengths), 32-bit row numbers in LDS.
 //
 // The tokens are divided by what was measured, in us: a workgroup takes 10.5 and 0.061 a token, one over own tokens 7.5
-// and 0.065, the join 0.11 a split.  With fewer than 256 the own tokens fill the other CUs.  `least` is what a perfect
+// and 0.065, the join 0.11 a split (measured with parts of half the bytes; with 0.2 four of ten shapes were 1 to 2 us
+// shorter and four as much longer).  With fewer than 256 the own tokens fill the other CUs.  `least` is what a perfect
 // division of all of it would take; `longest` what it takes if every own workgroup is as long as its share of the table:
 // CUs without a prefix run own ones meanwhile, what is left follows in rounds.  (64 sequences of 16 heads, 8192 and up to
 // 1024 tokens, launch and join: 59 in splits of 256, 51 of 512, 74 of 1024, 63 of 384; 32768 and 512: 102 of 1024, 108 of
@@ -617,7 +620,8 @@ void launch_prefix_join(const PrefixCall& c, hipStream_t st, float* shift) {
                        c.olat, c.qa, shift);
   };
   // Where 64 columns a workgroup leave half of the CUs without one, 16: a CU takes in about 10 bytes a clock.  (Us, 64
-  // rows of 256 latents in 128 splits: 17 and 7; 1024 rows of 512 in 32 splits, 256 workgroups: 11 and 14.)
+  // rows of 512 latents in 64 splits: 11.3 and 5.9; 512 rows, 128 workgroups: 14.5 and 12.1; 1024 rows in 32 splits, 256
+  // workgroups: 15.0 and 16.5.)
   const int64_t rows = (int64_t)c.f.share * c.f.n * c.f.H;
   const bool few = c.units * ((rows + 31) / 32) * ((c.f.dc + 63) / 64) <= 128 && !shift;
   auto go = [&](auto dc) {

@@ -922,7 +922,9 @@ int atomic_latent_decode(const atomic_latent_decode_args* a, const void* q, cons
  * j < kv_lens[b], the sum of its softmax weights over the heads and query tokens:
  * added to what stands there, except for the n newest tokens (j >= kv_lens[b] - n),
  * whose sums begin with this call.  What lies past the length stays as it is.  Each sum
- * is made in a fixed order.  The workspace then holds the scores: 4 bytes a query row
+ * is made in a fixed order and float32's in either type (in bf16, with more than 32 query
+ * rows behind a prefix table of 4096 tokens or more, to half the variance of what the
+ * query's rounding to bf16 adds to a row's scores over the prefix).  The workspace then holds the scores: 4 bytes a query row
  * (of whole tiles of 16 to 64 rows a sequence) and token of the table. */
 typedef struct atomic_latent_shared_args {
   atomic_latent_decode_args dec; /* as above; table_pages may be 0 with prefixes      */
@@ -950,10 +952,10 @@ int atomic_latent_decode_shared(const atomic_latent_shared_args* a, const void* 
  *
  * order[b, j] says how old the token in row j of sequence b is: its place among all the
  * sequence's tokens.  A row that no eviction has seen holds -1; such rows are taken as the
- * newest, in the order of their rows.  The first `sinks` tokens (order < sinks) and the
- * `recent` newest stay; of the others those with the largest weights, among equal ones
- * the lowest rows (a NaN counts as less than every number).  Kept tokens from rows >= keep
- * move into the rows below keep that became free, the k-th into the k-th, with their cache
+ * newest, in the order of their rows.  The first `sinks` tokens (order < sinks) and those
+ * of the `recent` last places (order above the newest one's less recent) stay; of the
+ * others those with the largest weights, among equal ones the lowest rows (a NaN counts as
+ * less than every number).  Kept tokens from rows >= keep move into the rows below keep that became free, the k-th into the k-th, with their cache
  * rows, weights and order; nothing else moves.
  *
  * kv_lens_out [batch] (at most keep), weights_out and order_out [batch, width] receive
