@@ -193,163 +193,163 @@ __device__ __forceinline__ void prefix_tokens(const DecDims& d, PrefixLds<DC>& m
       }
     }
   };
-  // All tiles, with p as NP bf16 numbers.
   typedef bf16 pair __attribute__((ext_vector_type(2)));
+  // All tiles, with p as NP bf16 numbers.
   auto walk = [&](auto numbers) __attribute__((always_inline)) {
-  constexpr int NP = decltype(numbers)::value;
-  frag p[2], pn[NP][2];  // the last tile's, and this one's
-  auto quad = [&](int k) __attribute__((always_inline)) {  // four tokens' probabilities
-    const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
+    constexpr int NP = decltype(numbers)::value;
+    frag p[2], pn[NP][2];  // the last tile's, and this one's
+    auto quad = [&](int k) __attribute__((always_inline)) {  // four tokens' probabilities
+      const float ref = m == -INFINITY ? 0.f : -m;  // a row that has seen nothing yet: every p is exp2(-inf) = 0
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float e = fast_exp2(__builtin_fmaf(s[4 * k + j], c2, ref));
-      if constexpr (SCORED) sum += e;
+      for (int j = 0; j < 4; ++j) {
+        float e = fast_exp2(__builtin_fmaf(s[4 * k + j], c2, ref));
+        if constexpr (SCORED) sum += e;
 #pragma unroll
-      for (int u = 0; u < NP; ++u) {
-        const bf16 h = (bf16)e;
-        pn[u][k / 2][4 * (k & 1) + j] = h;
-        e -= (float)h;
-      }
-    }
-    const pair one = {(bf16)1.f, (bf16)1.f};
-#pragma unroll
-    for (int u = 0; u < NP; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const int at = 4 * (k & 1) + j;
-        held = __builtin_amdgcn_fdot2_f32_bf16(pair{pn[u][k / 2][at], pn[u][k / 2][at + 1]}, one, held, false);
-      }
-  };
-  // A new reference where a score is far above its row's: a whole number, so that what
-  // fades, the last tile's probabilities among it, is scaled exactly.
-  auto settle = [&](auto fades) __attribute__((always_inline)) {
-    float top = s[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-    top *= c2;
-    if (__any(top > m + kLag)) {
-      top = fmaxf(top, lane_at(top, lane ^ 32));
-      const float mn = fmaxf(m, ceilf(top)), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
-      m = mn;
-      if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
-      if constexpr (SCORED) sum *= fade;
-      held *= fade;
-      if constexpr (NP == 1) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) p[k][j] = (bf16)((float)p[k][j] * fade);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float z = acc[n][r];
-          accum_mul(z, fade);
-          acc[n][r] = z;
+        for (int u = 0; u < NP; ++u) {
+          const bf16 h = (bf16)e;
+          pn[u][k / 2][4 * (k & 1) + j] = h;
+          e -= (float)h;
         }
       }
-      asm volatile("s_nop 7" ::: "memory");
-    }
-  };
-  // The scores of tile i in buffer `kb` and the products of the tile before in `vb`, as one run
-  // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
-  // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
-  constexpr int G = 1, LA = 2, GS = KS / G, GV = 2 * NT / G;
-  auto tile = [&](auto with_k, auto with_v, auto sends, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
-    constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
-    uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
-    asm volatile("" : "+v"(ac), "+v"(ar), "+v"(av));
-    auto load = [&](int j) {
-      return j < KC ? LC::row(ac, 0, 16 * j)
-                    : j < KS ? LR::row(ar, 0, 16 * (j - KC)) : LC::col(av, 16 * ((j - KS) / NT), 32 * ((j - KS) % NT));
+      const pair one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+      for (int u = 0; u < NP; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const int at = 4 * (k & 1) + j;
+          held = __builtin_amdgcn_fdot2_f32_bf16(pair{pn[u][k / 2][at], pn[u][k / 2][at + 1]}, one, held, false);
+        }
     };
-    frag f[LA + 1][G];
-    static_for<LA * G>([&](auto j) { f[(g0 + j.value / G) % (LA + 1)][j.value % G] = load(g0 * G + j.value); });
-    __builtin_amdgcn_sched_barrier(0);
-    static_for<g1 - g0>([&](auto gr) __attribute__((always_inline)) {
-      constexpr int g = g0 + decltype(gr)::value;
-      static_for<G>([&](auto j) {
-        if constexpr (g + LA < g1) f[(g + LA) % (LA + 1)][j.value] = load((g + LA) * G + j.value);
-      });
-      if constexpr (g < GS) {
-        __builtin_amdgcn_sched_barrier(0);
+    // A new reference where a score is far above its row's: a whole number, so that what
+    // fades, the last tile's probabilities among it, is scaled exactly.
+    auto settle = [&](auto fades) __attribute__((always_inline)) {
+      float top = s[0];
 #pragma unroll
-        for (int j = 0; j < NL; ++j)
-          if (decltype(sends)::value && j * GS / NL == g) send(j, to);
-        if constexpr (g == 0) s = zero16();
-        static_for<G>([&](auto j) {
-          constexpr int t = g * G + decltype(j)::value;
-          s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[t], s);
-          if constexpr (t >= KC) s = M32<bf16>::mma(f[g % (LA + 1)][j.value], ql[t - KC], s);
-        });
-        if constexpr (g == GS - 1) {
-          asm volatile("" : "+v"(s));
-          mask(k0);
-          settle(sends);  // (the first tile sends no other)
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      top *= c2;
+      if (__any(top > m + kLag)) {
+        top = fmaxf(top, lane_at(top, lane ^ 32));
+        const float mn = fmaxf(m, ceilf(top)), fade = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+        m = mn;
+        if constexpr (!decltype(fades)::value) return;  // (the first tile: nothing is there yet)
+        if constexpr (SCORED) sum *= fade;
+        held *= fade;
+        if constexpr (NP == 1) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[k][j] = (bf16)((float)p[k][j] * fade);
         }
-      } else {
-        if constexpr (decltype(with_k)::value && (g - GS) % (GV / 4) == 1) quad((g - GS) / (GV / 4));
-        static_for<G>([&](auto j) {
-          constexpr int v = (g - GS) * G + decltype(j)::value;
-          if constexpr (NP == 1) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], p[v / NT], acc[v % NT]);
-          else
 #pragma unroll
-            for (int u = 0; u < NP; ++u) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], pn[u][v / NT], acc[v % NT]);
-        });
-        __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
-        static_for<NP * G>([&](auto) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector
-        });
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float z = acc[n][r];
+            accum_mul(z, fade);
+            acc[n][r] = z;
+          }
+        }
+        asm volatile("s_nop 7" ::: "memory");
       }
+    };
+    // The scores of tile i in buffer `kb` and the products of the tile before in `vb`, as one run
+    // of groups of G MFMAs whose operands are read LA groups ahead, so that the second part
+    // does not begin with a wait.  Either part may be left out (`kb`, `vb` below zero).
+    constexpr int G = 1, LA = 2, GS = KS / G, GV = 2 * NT / G;
+    auto tile = [&](auto with_k, auto with_v, auto sends, int kb, int vb, int k0, uint32_t to) __attribute__((always_inline)) {
+      constexpr int g0 = decltype(with_k)::value ? 0 : GS, g1 = decltype(with_v)::value ? GS + GV : GS;
+      uint32_t ac = l0 + kb * STAGE + br, ar = l0 + kb * STAGE + SC + bp, av = l0 + vb * STAGE + bc;
+      asm volatile("" : "+v"(ac), "+v"(ar), "+v"(av));
+      auto load = [&](int j) {
+        return j < KC ? LC::row(ac, 0, 16 * j)
+                      : j < KS ? LR::row(ar, 0, 16 * (j - KC)) : LC::col(av, 16 * ((j - KS) / NT), 32 * ((j - KS) % NT));
+      };
+      frag f[LA + 1][G];
+      static_for<LA * G>([&](auto j) { f[(g0 + j.value / G) % (LA + 1)][j.value % G] = load(g0 * G + j.value); });
       __builtin_amdgcn_sched_barrier(0);
-    });
-    if constexpr (decltype(with_v)::value) {
+      static_for<g1 - g0>([&](auto gr) __attribute__((always_inline)) {
+        constexpr int g = g0 + decltype(gr)::value;
+        static_for<G>([&](auto j) {
+          if constexpr (g + LA < g1) f[(g + LA) % (LA + 1)][j.value] = load((g + LA) * G + j.value);
+        });
+        if constexpr (g < GS) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) in_accum(acc[n]);
+          for (int j = 0; j < NL; ++j)
+            if (decltype(sends)::value && j * GS / NL == g) send(j, to);
+          if constexpr (g == 0) s = zero16();
+          static_for<G>([&](auto j) {
+            constexpr int t = g * G + decltype(j)::value;
+            s = M32<bf16>::mma(f[g % (LA + 1)][j.value], qf[t], s);
+            if constexpr (t >= KC) s = M32<bf16>::mma(f[g % (LA + 1)][j.value], ql[t - KC], s);
+          });
+          if constexpr (g == GS - 1) {
+            asm volatile("" : "+v"(s));
+            mask(k0);
+            settle(sends);  // (the first tile sends no other)
+          }
+        } else {
+          if constexpr (decltype(with_k)::value && (g - GS) % (GV / 4) == 1) quad((g - GS) / (GV / 4));
+          static_for<G>([&](auto j) {
+            constexpr int v = (g - GS) * G + decltype(j)::value;
+            if constexpr (NP == 1) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], p[v / NT], acc[v % NT]);
+            else
+#pragma unroll
+              for (int u = 0; u < NP; ++u) acc[v % NT] = M32<bf16>::mma(f[g % (LA + 1)][j.value], pn[u][v / NT], acc[v % NT]);
+          });
+          __builtin_amdgcn_sched_group_barrier(0x100, 4 * G, 0);  // LDS reads
+          static_for<NP * G>([&](auto) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // vector
+          });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (decltype(with_v)::value) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) in_accum(acc[n]);
+      }
+    };
+    const int tiles = (end - first + TK - 1) / TK;
+#pragma unroll
+    for (int k = 0; k < NB - 1; ++k) {
+      look(TK * k);
+      aim();
+#pragma unroll
+      for (int i = 0; i < NL; ++i) send(i, l0 + k * STAGE);
     }
-  };
-  const int tiles = (end - first + TK - 1) / TK;
+    look(TK * (NB - 1));
+    vm_wait<(NB - 2) * NL>();
+    bare_barrier();
+    const IntC<0> no;
+    const IntC<1> yes;
+    tile(yes, no, no, 0, 0, 0, 0);
 #pragma unroll
-  for (int k = 0; k < NB - 1; ++k) {
-    look(TK * k);
-    aim();
-#pragma unroll
-    for (int i = 0; i < NL; ++i) send(i, l0 + k * STAGE);
-  }
-  look(TK * (NB - 1));
-  vm_wait<(NB - 2) * NL>();
-  bare_barrier();
-  const IntC<0> no;
-  const IntC<1> yes;
-  tile(yes, no, no, 0, 0, 0, 0);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) quad(k);
-  if constexpr (NP == 1) {
-    p[0] = pn[0][0];
-    p[1] = pn[0][1];
-  } else {
-    tile(no, yes, no, 0, 0, 0, 0);
-  }
-  for (int i = 1; i < tiles; ++i) {
-    vm_wait<(NB - 3) * NL>();  // tile i is there (of this wave's loads; behind the barrier, of all)
-    bare_barrier();            // and nobody reads tile i - 2 any more
-    aim();
-    look(TK * (i + NB - 1));
-    const uint32_t to = l0 + (i + NB - 2) % NB * STAGE;
+    for (int k = 0; k < 4; ++k) quad(k);
     if constexpr (NP == 1) {
-      tile(yes, yes, yes, i % NB, (i - 1) % NB, TK * i, to);
       p[0] = pn[0][0];
       p[1] = pn[0][1];
-    } else {  // (the products of the same tile: two numbers of two tiles would be 16 registers more)
-      tile(yes, no, yes, i % NB, 0, TK * i, to);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) quad(k);
-      tile(no, yes, no, 0, i % NB, 0, 0);
+    } else {
+      tile(no, yes, no, 0, 0, 0, 0);
     }
-  }
-  if constexpr (NP == 1) tile(no, yes, no, 0, (tiles - 1) % NB, 0, 0);
+    for (int i = 1; i < tiles; ++i) {
+      vm_wait<(NB - 3) * NL>();  // tile i is there (of this wave's loads; behind the barrier, of all)
+      bare_barrier();            // and nobody reads tile i - 2 any more
+      aim();
+      look(TK * (i + NB - 1));
+      const uint32_t to = l0 + (i + NB - 2) % NB * STAGE;
+      if constexpr (NP == 1) {
+        tile(yes, yes, yes, i % NB, (i - 1) % NB, TK * i, to);
+        p[0] = pn[0][0];
+        p[1] = pn[0][1];
+      } else {  // (the products of the same tile: two numbers of two tiles would be 16 registers more)
+        tile(yes, no, yes, i % NB, 0, TK * i, to);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) quad(k);
+        tile(no, yes, no, 0, i % NB, 0, 0);
+      }
+    }
+    if constexpr (NP == 1) tile(no, yes, no, 0, (tiles - 1) % NB, 0, 0);
   };
   if (len < kPreOne) walk(IntC<2>());
   else walk(IntC<1>());
